@@ -538,6 +538,146 @@ typedef struct stark_qmm_gated_act_mul_args {
 STARK_QMM_API stark_qmm_status stark_qmm_gated_act_mul(const stark_qmm_gated_act_mul_args* args, void* stream);
 
 /* ------------------------------------------------------------------ */
+/* 4-bit paged key/value cache, and attention over it                  */
+/* ------------------------------------------------------------------ */
+
+/* No counterpart in the reference, whose caches hold 16-bit rows of one
+ * session (src/encodable_block/mixer/attention/). For serving loops around the
+ * products: keys and values by the affine rule of the weights (group of
+ * group_size values: f16 scale s = (max - min) / 15, f16 bias b = min, codes
+ * round-half-even((x - b) / s) clamped to 0..15, values s * code + b; computed
+ * in 64 bits, s and b rounded to f32 and then to f16), in pages of page_size tokens shared by all
+ * sequences. A group with a value outside +-32768 or not a number reads as NaN.
+ *
+ * The cache is one buffer per layer, opaque to the caller (records of 16
+ * tokens of a head: see stark_qmm_kv_read to take rows out); it needs no
+ * initialisation: rows never written are never used by a call that is given
+ * correct lengths. Token slot = page * page_size + position in the page. */
+typedef struct stark_qmm_kv_cache {
+    void* data;              /* 128-byte aligned, >= stark_qmm_kv_cache_size() bytes */
+    uint64_t data_size;
+    uint32_t page_count;     /* page_count * page_size < 2^31 */
+    uint32_t page_size;      /* power of two, 16 .. 1024 */
+    uint32_t kv_heads;       /* 1 .. 1024 */
+    uint32_t head_dim;       /* 64, 128 or 256 */
+    uint32_t group_size;     /* 32, 64 or 128, dividing head_dim */
+} stark_qmm_kv_cache;
+
+/* Bytes that the geometry in `cache` needs (data and data_size are ignored). */
+STARK_QMM_API stark_qmm_status stark_qmm_kv_cache_size(const stark_qmm_kv_cache* cache, uint64_t* bytes);
+
+/* Bits of stark_qmm_kv_plan_args.status. */
+enum { STARK_QMM_KV_OUT_OF_PAGES = 1,   /* the free list is too short */
+       STARK_QMM_KV_TABLE_FULL = 2,     /* a request needs more pages than its table row holds */
+       STARK_QMM_KV_BAD_LENGTH = 4,     /* a negative length (taken as 0) */
+       STARK_QMM_KV_TOO_MANY_TOKENS = 8 /* more new tokens than token_capacity (the rest is dropped) */ };
+
+typedef struct stark_qmm_kv_plan_args {
+    uint32_t struct_size;
+    const int32_t* cached;       /* [batch] tokens each request has in the cache */
+    const int32_t* added;        /* [batch] new tokens of the step (0 for an idle row) */
+    const int32_t* free_pages;   /* [free_capacity] ids of free pages; taken from the end */
+    const int32_t* free_count;   /* [1] ids in use of free_pages */
+    int32_t* block_table;        /* [batch, table_stride]: entries of the pages in use are read, those of
+                                    new pages written (-1: none left); the others stay as they were */
+    int32_t* query_start;        /* [batch + 1] running sum of added */
+    int32_t* kv_lengths;         /* [batch] cached + added */
+    int32_t* slots;              /* [token_capacity] cache slot of each new token; -1 without a page, and
+                                    behind the last token */
+    int32_t* positions;          /* [token_capacity] position in its request; 0 behind the last token */
+    int32_t* free_left;          /* [1] ids left in free_pages (may be free_count of the next call, not of this) */
+    int32_t* status;             /* [1] STARK_QMM_KV_* bits */
+    uint32_t batch, token_capacity, free_capacity, table_stride, page_size;
+} stark_qmm_kv_plan_args;
+
+/* Plan of a serving step from request lengths, on the device: new pages for the
+ * new tokens (request by request, in order), the slot and position of each of
+ * them, and the lengths that stark_qmm_kv_attention reads. One launch; outputs
+ * must not overlap inputs or each other. */
+STARK_QMM_API stark_qmm_status stark_qmm_kv_plan(const stark_qmm_kv_plan_args* args, void* stream);
+
+/* Rotary embedding of query and key rows: pair i is values (i, i + rotary_dim / 2),
+ * or (2 i, 2 i + 1) when interleaved; it turns by the table's row
+ * positions[axis_of_pair[i]][token]. Several axes serve image and video
+ * positions (time, height, width). A position outside the table gives NaN. */
+typedef struct stark_qmm_rotary {
+    const float* table;          /* [table_rows, rotary_dim / 2] pairs (cos, sin), 8-byte aligned */
+    const int32_t* positions;    /* [axes] rows of position_stride */
+    uint64_t position_stride;
+    uint32_t table_rows;
+    uint32_t rotary_dim;         /* multiple of 16, <= head_dim; 0: no rotation */
+    uint32_t axes;               /* 1 .. 4 */
+    uint32_t interleaved;
+    uint8_t axis_of_pair[128];   /* < axes, the first rotary_dim / 2 */
+} stark_qmm_rotary;
+
+typedef struct stark_qmm_kv_append_args {
+    uint32_t struct_size;
+    stark_qmm_kv_cache cache;
+    uint32_t data_type;          /* of q, k, v and q_out: F32, F16 or BF16 */
+    const void* q;               /* [tokens, heads, head_dim], or NULL (then q_out is NULL too) */
+    void* q_out;                 /* rotated rows; may be q itself with the same strides */
+    const void* k;               /* [tokens, kv_heads, head_dim] */
+    const void* v;
+    const int32_t* slots;        /* [tokens]; a token whose slot is outside the cache writes no row */
+    /* strides in elements; the values of a head are contiguous */
+    uint64_t q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride;
+    uint64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    uint32_t tokens, heads;
+    stark_qmm_rotary rotary;
+} stark_qmm_kv_append_args;
+
+/* Rotates the query and key rows of new tokens and writes their keys (rotated,
+ * not rounded in between) and values to the cache. Slots must be distinct: of
+ * two rows for one slot each group keeps one or the other. */
+STARK_QMM_API stark_qmm_status stark_qmm_kv_append(const stark_qmm_kv_append_args* args, void* stream);
+
+typedef struct stark_qmm_kv_read_args {
+    uint32_t struct_size;
+    stark_qmm_kv_cache cache;
+    const int32_t* slots;        /* [tokens]; rows of a slot outside the cache stay as they were */
+    uint32_t data_type;          /* of k and v: F32, F16 or BF16 */
+    void* k;                     /* [tokens, kv_heads, head_dim], or NULL */
+    void* v;                     /* likewise */
+    uint64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    uint32_t tokens;
+} stark_qmm_kv_read_args;
+
+/* Reads rows back as the values that their 4 bits stand for. */
+STARK_QMM_API stark_qmm_status stark_qmm_kv_read(const stark_qmm_kv_read_args* args, void* stream);
+
+typedef struct stark_qmm_kv_attention_args {
+    uint32_t struct_size;
+    stark_qmm_kv_cache cache;
+    uint32_t data_type;          /* of q and out: F16 or BF16 */
+    const void* q;               /* [tokens, heads, head_dim] */
+    void* out;                   /* likewise; may not overlap q */
+    float* lse;                  /* [tokens, heads] log of the softmax's sum (-inf for an empty row), or NULL */
+    uint64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride; /* elements */
+    const int32_t* block_table;  /* [batch, table_stride] page ids; tokens of an id outside the cache are not seen */
+    const int32_t* query_start;  /* [batch + 1]: request b's rows are query_start[b] .. query_start[b + 1] - 1 */
+    const int32_t* kv_lengths;   /* [batch] tokens in the cache, the new ones among them */
+    uint32_t batch, tokens, heads, table_stride;
+    uint32_t max_query;          /* bounds on the lengths of any request; what is longer is cut */
+    uint32_t max_kv;
+    float scale;                 /* of the scores */
+    float soft_cap;              /* 0, or scores become soft_cap * tanh(score / soft_cap) */
+    uint32_t causal;             /* query i of n sees keys up to kv_length - n + i */
+    uint32_t window;             /* 0, or only the last `window` of those */
+    void* workspace;             /* device, 16-byte aligned, >= stark_qmm_kv_attention_workspace_size() bytes */
+    uint64_t workspace_size;     /* its contents do not survive the call; calls that may overlap need their own */
+} stark_qmm_kv_attention_args;
+
+/* 0 where the call needs none (workspace may then be NULL). */
+STARK_QMM_API stark_qmm_status stark_qmm_kv_attention_workspace_size(const stark_qmm_kv_attention_args* args,
+                                                                     uint64_t* bytes);
+
+/* Attention of new query rows over the cache: decode, verify and prompt rows in
+ * one call, heads / kv_heads query heads to a key head. An empty row gives
+ * zeros; rows that no request has stay as they were. */
+STARK_QMM_API stark_qmm_status stark_qmm_kv_attention(const stark_qmm_kv_attention_args* args, void* stream);
+
+/* ------------------------------------------------------------------ */
 /* Weight files: Stark's converted artifact (model.safetensors) and      */
 /* GGUF v3 checkpoints                                                    */
 /* ------------------------------------------------------------------ */

@@ -231,6 +231,13 @@ SIGNATURES = {
     "stark_qmm_unified_sampling": (C.c_uint32, [C.POINTER(_SamplingArgs), C.c_void_p]),
     "stark_qmm_activation_transform": (C.c_uint32, [C.POINTER(_TransformArgs), C.c_void_p]),
     "stark_qmm_gated_act_mul": (C.c_uint32, [C.POINTER(_GatedArgs), C.c_void_p]),
+    # the key/value cache's structs are in stark_amd/kv.py
+    "stark_qmm_kv_cache_size": (C.c_uint32, [C.c_void_p, C.POINTER(C.c_uint64)]),
+    "stark_qmm_kv_plan": (C.c_uint32, [C.c_void_p, C.c_void_p]),
+    "stark_qmm_kv_append": (C.c_uint32, [C.c_void_p, C.c_void_p]),
+    "stark_qmm_kv_read": (C.c_uint32, [C.c_void_p, C.c_void_p]),
+    "stark_qmm_kv_attention_workspace_size": (C.c_uint32, [C.c_void_p, C.POINTER(C.c_uint64)]),
+    "stark_qmm_kv_attention": (C.c_uint32, [C.c_void_p, C.c_void_p]),
 }
 
 _lib = None
