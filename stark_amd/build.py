@@ -26,11 +26,19 @@ FLAGS = [
     "-Wall", "-Wno-unused-function",
 ]
 
+# flags of one source
+FILE_FLAGS = {
+    # matrix-core accumulators that vector instructions read and write every step stay in VGPRs (without it each step
+    # copied them from and to the accumulation registers: 64 of about 370 instructions)
+    "kv_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+}
+
 
 def _compile(src: str) -> str:
     obj = os.path.join(OBJ, os.path.basename(src) + ".o")
     # the drop-in library exports only the entry points its header marks STARK_QMM_API
     extra = ["-fvisibility=hidden", "-fvisibility-inlines-hidden"] if os.path.dirname(src) == CSRC else []
+    extra += FILE_FLAGS.get(os.path.basename(src), [])
     cmd = [HIPCC, *FLAGS, *extra, "-c", src, "-o", obj]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

@@ -38,23 +38,25 @@ QMM_DEVICE kv::Request request_of(const AttendArgs& a, uint32_t b) {
     return kv::request(a.query_start[b], a.query_start[b + 1], a.kv_lengths[b], a.tokens, a.max_query, a.max_kv);
 }
 
-// 16-bit pair of f32 values in the output type.
-QMM_DEVICE uint32_t pack_out(float lo, float hi, uint32_t is_bf16) {
-    if (is_bf16) return __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)lo, (__bf16)hi});
-    return __builtin_bit_cast(uint32_t, f16x2{(_Float16)lo, (_Float16)hi});
-}
-
-// Eight neighbouring values of an output row.
-QMM_DEVICE void store_out8(const AttendArgs& a, uint32_t token, uint32_t head, uint32_t d, const float* x) {
-    uint16_t* p = (uint16_t*)a.out.p + (token * a.out.token + head * a.out.head + d);
-    u32x4 w;
+// N neighbouring output values, times f, at p; vec: 2 N bytes aligned.
+template <int N>
+QMM_DEVICE void store_out(uint16_t* p, uint32_t vec, uint32_t is_bf16, const float* x, float f) {
+    uint32_t w[N / 2];
+    if (is_bf16) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = pack_out(x[2 * e], x[2 * e + 1], a.is_bf16);
-    if (a.out.vec) {
-        *(u32x4*)p = w;
+        for (int e = 0; e < N / 2; ++e)
+            w[e] = __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)(x[2 * e] * f), (__bf16)(x[2 * e + 1] * f)});
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) p[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+        for (int e = 0; e < N / 2; ++e)
+            w[e] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)(x[2 * e] * f), (_Float16)(x[2 * e + 1] * f)});
+    }
+    if (vec) {
+        if (N == 8) *(u32x4*)p = u32x4{w[0], w[1], w[2 % (N / 2)], w[3 % (N / 2)]};
+        else *(u32x2*)p = u32x2{w[0], w[1]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) p[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
     }
 }
 
@@ -65,19 +67,14 @@ struct Step {
     u32x4 kp[2][G], vp[2][G];
     bool ok[2];  // the record's page is inside the cache
 
-    QMM_DEVICE void load(const AttendArgs& a, const int32_t* row, uint32_t head, uint32_t t0, uint32_t lane) {
-        const uint32_t c = lane & 15, g = lane >> 4;
+    // page: the two records' page ids; t0: first key
+    QMM_DEVICE void load(const AttendArgs& a, const uint32_t (&page)[2], uint32_t head, uint32_t t0, uint32_t lane) {
+        const uint32_t c = lane & 15, g = lane >> 4, mask = (1u << a.cache.page_shift) - 1;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            const uint32_t t = t0 + 16 * i;
-            // a step may reach past the last key: its second record may have no table entry
-            const uint32_t entry = min(t >> a.cache.page_shift, a.stride - 1);
-            const uint32_t id = (uint32_t)__builtin_amdgcn_readfirstlane(row[entry]);
-            ok[i] = id < a.cache.page_count;
-            const uint8_t* rec = a.cache.data + kv::record_index(ok[i] ? id : 0, a.cache.kv_heads, head,
-                                                                  1u << a.cache.page_shift,
-                                                                  t & ((1u << a.cache.page_shift) - 1)) *
-                                                    (uint64_t)a.cache.record;
+            ok[i] = page[i] < a.cache.page_count;
+            const uint8_t* rec = a.cache.data + kv::record_index(ok[i] ? page[i] : 0, a.cache.kv_heads, head, mask + 1,
+                                                                  (t0 + 16 * i) & mask) * (uint64_t)a.cache.record;
             const uint8_t* kq = rec + (DIM == 64 ? c * 32 + g * 8 : c * 64 + g * 16);
             const uint8_t* vq = rec + 8 * DIM + 64 * G + lane * (DIM == 64 ? 8 : 16);
             if (DIM == 64) {
@@ -99,6 +96,45 @@ struct Step {
     }
 };
 
+// Page ids of a wave's records: lane 2 n + i holds that of record i of step base + n, 32 steps to a load, and a step
+// reads its two with v_readlane.
+struct PageIds {
+    const int32_t* row;
+    int32_t from, stride;  // first key of step 0; keys from a wave's step to its next
+    uint32_t shift, last;  // last entry of the table row
+    uint32_t ids, base;
+
+    QMM_DEVICE void fill(uint32_t n, uint32_t lane) {
+        base = n;
+        const uint32_t t = (uint32_t)(from + stride * (int32_t)(n + lane / 2)) + 16 * (lane & 1);
+        ids = (uint32_t)row[min(t >> shift, last)];  // a step may reach past the last key: past the table too
+        asm volatile("" : "+v"(ids));  // the wait for it is here, not before every v_readlane (for all loads in flight)
+    }
+    QMM_DEVICE void get(uint32_t n, uint32_t lane, uint32_t (&page)[2]) {
+        if (n - base >= 32) fill(n, lane);
+        page[0] = (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)(2 * (n - base)));
+        page[1] = (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)(2 * (n - base) + 1));
+    }
+};
+
+// Running state of 16 query rows: lane (c, g) holds row c.
+template <int DIM, int G>
+struct Running {
+    static constexpr int J = DIM / 32, JG = J / G;
+    f32x4 o[2 * J];          // [32-value block, parity]: codes times p s, values 32 i + 2 (4 g + e) + parity
+    float beta[G], l, m, mf; // sum p b and sum p over the lane's keys; reference; reference - exponent
+    int fexp;
+
+    QMM_DEVICE void start(int exponent) {
+        fexp = exponent;
+        m = kNone, mf = kNone - (float)exponent, l = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2 * J; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) beta[gr] = 0.0f;
+    }
+};
+
 // Rows of a tile by 32-key steps, the steps dealt to four waves, each with its own running maximum and sums, joined
 // at the end. Keys and values stay codes: with C the codes,
 //   q . k = sum over groups (s_g C_g . q + b_g sum q),   out = sum over tokens (p s_g) C + sum p b_g,
@@ -109,7 +145,7 @@ struct Step {
 // record, which is the B operand of the second product as it stands, with no lane exchange.
 // q is scaled per row by a power of two into f16's range, exact but for values 2^-24 below the row's largest.
 template <int DIM, int G>
-__global__ __launch_bounds__(256) void kv_attend_rows(AttendArgs a) {
+__global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(AttendArgs a) {
     constexpr int J = DIM / 32;       // k blocks of a score product, and 32-value blocks of the output
     constexpr int JG = J / G;         // of one scale group
     constexpr int kRow = DIM + 4;     // padded row of the joining buffers, floats
@@ -144,27 +180,39 @@ __global__ __launch_bounds__(256) void kv_attend_rows(AttendArgs a) {
     float qsum[G];
     float c1;
     {
+        // a row past the tile's last reads the request's first one, as zeros
+        u32x4 w[J];
+        const uint16_t* p = (const uint16_t*)a.q.p + (token * a.q.token + qh * a.q.head + 8 * g);
+        if (a.q.vec) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) w[j] = *(const u32x4*)(p + 32 * j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[j][e] = p[32 * j + 2 * e] | (uint32_t)p[32 * j + 2 * e + 1] << 16;
+        }
         float x[J][8];
+        if (a.is_bf16) {
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[j][e] = __uint_as_float(e & 1 ? w[j][e / 2] & 0xffff0000u : w[j][e / 2] << 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[j][e] = (float)__builtin_bit_cast(f16x2, (uint32_t)w[j][e / 2])[e & 1];
+        }
         float top = 0.0f;
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            const uint16_t* p = (const uint16_t*)a.q.p + (token * a.q.token + qh * a.q.head + 8 * (4 * j + g));
-            u32x4 w = {0, 0, 0, 0};
-            if (live) {
-                if (a.q.vec) {
-                    w = *(const u32x4*)p;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = p[2 * e] | (uint32_t)p[2 * e + 1] << 16;
-                }
-            }
+        for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const uint32_t h = e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
-                x[j][e] = a.is_bf16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+                x[j][e] = live ? x[j][e] : 0.0f;
                 top = fmaxf(top, fabsf(x[j][e]));
             }
-        }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const int k = 13 - (top > 0.0f && top < INFINITY ? ilogbf(top) : 0);  // the largest in [2^13, 2^14)
@@ -191,150 +239,175 @@ __global__ __launch_bounds__(256) void kv_attend_rows(AttendArgs a) {
         c1 = ldexp_f32(a.scale, 24 - k);
     }
 
-    const int32_t* row = a.table + (size_t)b * a.stride;
-    const int32_t steps = from < to ? (to - from + 31) / 32 : 0;
-    // steps from which no row masks anything: [inner_lo, inner_hi) in keys
+    // this wave's 32-key steps: wave, wave + 4, ...
+    const int32_t all_steps = from < to ? (to - from + 31) / 32 : 0;
+    const uint32_t steps = (int32_t)wave < all_steps ? (uint32_t)(all_steps - (int32_t)wave + 3) / 4 : 0;
+    // keys that every row of the tile sees: [inner_lo, inner_hi)
     const kv::Range first = kv::visible((int32_t)(tile * kv::kRows / a.ratio), r.q_len, r.kv_len, a.causal, a.window);
     const kv::Range last = kv::visible((int32_t)(min(tile * kv::kRows + kv::kRows, rows) - 1) / (int32_t)a.ratio,
                                        r.q_len, r.kv_len, a.causal, a.window);
     const int32_t inner_lo = last.lo, inner_hi = min(first.hi, last.hi);
+    PageIds pages{a.table + (size_t)b * a.stride, from + 32 * (int32_t)wave, 128, a.cache.page_shift, a.stride - 1, 0, 0};
 
-    f32x4 o[2 * J];
-    float beta[G], m, l, mf;
-    int fexp = 0;
-    Step<DIM, G> st;
+    Running<DIM, G> run;
+    run.start(0);
+
+    const auto load = [&](Step<DIM, G>& st, uint32_t n) {
+        uint32_t page[2];
+        pages.get(n, lane, page);
+        st.load(a, page, head, (uint32_t)(from + 32 * (int32_t)wave + 128 * (int32_t)n), lane);
+    };
+    // largest value scale (f16 bits) of the step's keys before `to`
+    const auto scale_max = [&](const Step<DIM, G>& st, uint32_t n, uint32_t smax) {
+        const int32_t t0 = from + 32 * (int32_t)wave + 128 * (int32_t)n;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t h = st.vp[i][gr][e] & 0xffffu;
+                    if (t0 + 16 * i + 4 * (int32_t)g + e < to && h < 0x7c00u && st.ok[i]) smax = max(smax, h);
+                }
+        return smax;
+    };
+    const auto exponent = [&](uint32_t smax) {
+        smax = group_max<16>(smax);
+        smax = max(smax, (uint32_t)__shfl_xor((int)smax, 16, 64));
+        smax = max(smax, (uint32_t)__shfl_xor((int)smax, 32, 64));
+        return smax ? 8 - ilogbf(f16_bits_to_f32(smax)) : 0;
+    };
+    const auto step = [&](Step<DIM, G>& st, uint32_t n) {
+        const int32_t t0 = from + 32 * (int32_t)wave + 128 * (int32_t)n;
+        float x[2][4];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            f32x4 acc[G];
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) acc[gr] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const uint32_t w = st.kc[i][j], v = w >> 8;
+                const f16x8 k = operand(w & 0x000f000fu, w & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u);
+                acc[j / JG] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qb[j], acc[j / JG], 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                float y = 0.0f, z = 0.0f;
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    y = fmaf(plane_scale(st.kp[i][gr][e]), acc[gr][e], y);
+                    z = fmaf(plane_bias(st.kp[i][gr][e]), qsum[gr], z);
+                }
+                x[i][e] = fmaf(y, c1, z);
+            }
+        }
+        if (a.cap != 0.0f) {  // cap tanh(s / cap) = cap (1 - 2 / (1 + e^(2 s / cap)))
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    x[i][e] = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[i][e]));
+        }
+        if (t0 < inner_lo || t0 + 32 > inner_hi || !st.ok[0] || !st.ok[1]) {
+            // keys that a row does not see: score -inf, and planes 0, so that nothing of theirs (a NaN) gets through
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int32_t t = t0 + 16 * i + 4 * (int32_t)g + e;
+                    const bool seen = t >= see.lo && t < see.hi && t < to && st.ok[i];
+                    x[i][e] = seen ? x[i][e] : -INFINITY;
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) st.vp[i][gr][e] = seen ? st.vp[i][gr][e] : 0u;
+                }
+        }
+        float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                          fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+        // the reference moves only when a score passes it by 2^6: rescaling is then rare
+        if (__any(top > run.m + 6.0f)) {
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            const float mn = fmaxf(run.m, top), f = __builtin_amdgcn_exp2f(run.m - mn);
+            run.m = mn;
+            run.mf = mn - (float)run.fexp;
+            run.l *= f;
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) run.beta[gr] *= f;
+#pragma unroll
+            for (int j = 0; j < 2 * J; ++j) run.o[j] *= f;
+        }
+        f16x8 ps[G];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = __builtin_amdgcn_exp2f(x[i][e] - run.mf);
+                run.l += p;
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    // p s to f16, half a unit of 2^-11: the codes it multiplies are exact
+                    ps[gr][4 * i + e] = (_Float16)(p * plane_scale(st.vp[i][gr][e]));
+                    run.beta[gr] = fmaf(p, plane_bias(st.vp[i][gr][e]), run.beta[gr]);
+                }
+            }
+#pragma unroll
+        for (int i = 0; i < J; ++i) {  // 32-value blocks; byte i of a lane's value words
+            uint32_t w[4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (DIM == 64) {
+                    const uint32_t sel = 0x0c000c00u | (uint32_t)(2 + i) << 16 | (uint32_t)i;
+                    w[2 * u] = permb(0, st.vc[u][0], sel);
+                    w[2 * u + 1] = permb(0, st.vc[u][1], sel);
+                } else {
+                    const uint32_t sel = 0x0c000c00u | (uint32_t)(4 + i % 4) << 16 | (uint32_t)(i % 4);
+                    const uint32_t* v = &st.vc[u][i / 4 * 4];
+                    w[2 * u] = permb(v[1], v[0], sel);
+                    w[2 * u + 1] = permb(v[3], v[2], sel);
+                }
+            }
+            const f16x8 lo = operand(w[0] & 0x000f000fu, w[1] & 0x000f000fu, w[2] & 0x000f000fu, w[3] & 0x000f000fu);
+            const f16x8 hi = operand(w[0] & 0x00f000f0u, w[1] & 0x00f000f0u, w[2] & 0x00f000f0u, w[3] & 0x00f000f0u);
+            run.o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, ps[i / JG], run.o[2 * i], 0, 0, 0);
+            run.o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ps[i / JG], run.o[2 * i + 1], 0, 0, 0);
+        }
+    };
+
     // Power of two on the probabilities: p s below 2^15 while p < 2^6, taken from the scales of the wave's first step.
     // Should a later scale be far larger, the products overflow to infinity, which shows in the sums at the end:
     // then the wave starts again with the largest scale of all its steps.
-    for (int attempt = 0; attempt < 2; ++attempt) {
+    for (int attempt = 0; attempt < 2 && steps; ++attempt) {
+        Step<DIM, G> st[2];
         uint32_t smax = 0;
-        for (int32_t s = (int32_t)wave; s < steps; s += 4) {
-            const uint32_t t0 = (uint32_t)(from + 32 * s);
-            st.load(a, row, head, t0, lane);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int gr = 0; gr < G; ++gr)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const uint32_t h = st.vp[i][gr][e] & 0xffffu;
-                        if ((int32_t)(t0 + 16 * i + 4 * g + e) < to && h < 0x7c00u && st.ok[i]) smax = max(smax, h);
-                    }
-            if (attempt == 0) break;
+        if (attempt) {
+            for (uint32_t n = 0; n < steps; ++n) {
+                load(st[0], n);
+                smax = scale_max(st[0], n, smax);
+            }
         }
-#pragma unroll
-        for (int off = 32; off >= 1; off >>= 1) smax = max(smax, (uint32_t)__shfl_xor((int)smax, off, 64));
-        fexp = smax ? 8 - ilogbf(f16_bits_to_f32(smax)) : 0;
-        m = kNone, mf = kNone - (float)fexp, l = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 2 * J; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int gr = 0; gr < G; ++gr) beta[gr] = 0.0f;
-
-        for (int32_t s = (int32_t)wave; s < steps; s += 4) {
-            const int32_t t0 = from + 32 * s;
-            st.load(a, row, head, (uint32_t)t0, lane);
-            float x[2][4];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                f32x4 acc[G];
-#pragma unroll
-                for (int gr = 0; gr < G; ++gr) acc[gr] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    const uint32_t w = st.kc[i][j], v = w >> 8;
-                    const f16x8 k = operand(w & 0x000f000fu, w & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u);
-                    acc[j / JG] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qb[j], acc[j / JG], 0, 0, 0);
-                }
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float y = 0.0f, z = 0.0f;
-#pragma unroll
-                    for (int gr = 0; gr < G; ++gr) {
-                        y = fmaf(plane_scale(st.kp[i][gr][e]), acc[gr][e], y);
-                        z = fmaf(plane_bias(st.kp[i][gr][e]), qsum[gr], z);
-                    }
-                    x[i][e] = fmaf(y, c1, z);
-                }
-            }
-            if (a.cap != 0.0f) {  // cap tanh(s / cap) = cap (1 - 2 / (1 + e^(2 s / cap)))
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        x[i][e] = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[i][e]));
-            }
-            if (t0 < inner_lo || t0 + 32 > inner_hi || !st.ok[0] || !st.ok[1]) {
-                // keys that a row does not see: score -inf, and planes 0, so that nothing of theirs (a NaN) gets through
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int32_t t = t0 + 16 * i + 4 * (int32_t)g + e;
-                        const bool seen = t >= see.lo && t < see.hi && t < to && st.ok[i];
-                        x[i][e] = seen ? x[i][e] : -INFINITY;
-#pragma unroll
-                        for (int gr = 0; gr < G; ++gr) st.vp[i][gr][e] = seen ? st.vp[i][gr][e] : 0u;
-                    }
-            }
-            float top = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
-                              fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-            // the reference moves only when a score passes it by 2^6: rescaling is then rare
-            if (__any(top > m + 6.0f)) {
-                top = fmaxf(top, __shfl_xor(top, 16, 64));
-                top = fmaxf(top, __shfl_xor(top, 32, 64));
-                const float mn = fmaxf(m, top), f = __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
-                mf = m - (float)fexp;
-                l *= f;
-#pragma unroll
-                for (int gr = 0; gr < G; ++gr) beta[gr] *= f;
-#pragma unroll
-                for (int j = 0; j < 2 * J; ++j) o[j] *= f;
-            }
-            f16x8 ps[G];
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float p = __builtin_amdgcn_exp2f(x[i][e] - mf);
-                    l += p;
-#pragma unroll
-                    for (int gr = 0; gr < G; ++gr) {
-                        // p s to f16, half a unit of 2^-11: the codes it multiplies are exact
-                        ps[gr][4 * i + e] = (_Float16)(p * plane_scale(st.vp[i][gr][e]));
-                        beta[gr] = fmaf(p, plane_bias(st.vp[i][gr][e]), beta[gr]);
-                    }
-                }
-#pragma unroll
-            for (int i = 0; i < J; ++i) {  // 32-value blocks; byte i of a lane's value words
-                uint32_t w[4];
-#pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    if (DIM == 64) {
-                        const uint32_t sel = 0x0c000c00u | (uint32_t)(2 + i) << 16 | (uint32_t)i;
-                        w[2 * u] = permb(0, st.vc[u][0], sel);
-                        w[2 * u + 1] = permb(0, st.vc[u][1], sel);
-                    } else {
-                        const uint32_t sel = 0x0c000c00u | (uint32_t)(4 + i % 4) << 16 | (uint32_t)(i % 4);
-                        const uint32_t* v = &st.vc[u][i / 4 * 4];
-                        w[2 * u] = permb(v[1], v[0], sel);
-                        w[2 * u + 1] = permb(v[3], v[2], sel);
-                    }
-                }
-                const f16x8 lo = operand(w[0] & 0x000f000fu, w[1] & 0x000f000fu, w[2] & 0x000f000fu, w[3] & 0x000f000fu);
-                const f16x8 hi = operand(w[0] & 0x00f000f0u, w[1] & 0x00f000f0u, w[2] & 0x00f000f0u, w[3] & 0x00f000f0u);
-                o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, ps[i / JG], o[2 * i], 0, 0, 0);
-                o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, ps[i / JG], o[2 * i + 1], 0, 0, 0);
-            }
+        // the next step's loads go out before a step is computed (past the last step: the last again)
+        pages.fill(0, lane);
+        load(st[0], 0);
+        if (!attempt) smax = scale_max(st[0], 0, 0);
+        run.start(exponent(smax));
+        for (uint32_t n = 0; n < steps; n += 2) {
+            load(st[1], min(n + 1, steps - 1));
+            step(st[0], n);
+            if (n + 1 >= steps) break;
+            load(st[0], min(n + 2, steps - 1));
+            step(st[1], n + 1);
         }
         float bad = 0.0f;
 #pragma unroll
         for (int j = 0; j < 2 * J; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) bad = fmaf(o[j][e], 0.0f, bad);
+            for (int e = 0; e < 4; ++e) bad = fmaf(run.o[j][e], 0.0f, bad);
         if (!__any(bad != 0.0f)) break;  // 0 but where a sum is not finite
     }
+    float l = run.l, mf = run.mf;
+    auto& o = run.o;
+    auto& beta = run.beta;
 
     // the four lane groups hold different keys of one row
     l += __shfl_xor(l, 16, 64);
@@ -383,12 +456,9 @@ __global__ __launch_bounds__(256) void kv_attend_rows(AttendArgs a) {
     const float sum = (wave_sum_l[0][c] + wave_sum_l[1][c]) + (wave_sum_l[2][c] + wave_sum_l[3][c]);
     if (a.chunks == 1) {
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        uint16_t* p = (uint16_t*)a.out.p + (token * a.out.token + qh * a.out.head + 8 * g);
 #pragma unroll
-        for (int i = 0; i < J; ++i) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) y[i][e] *= inv;
-            store_out8(a, token, qh, 32 * i + 8 * g, y[i]);
-        }
+        for (int i = 0; i < J; ++i) store_out<8>(p + 32 * i, a.out.vec, a.is_bf16, y[i], inv);
         if (a.lse && g == 0)
             a.lse[(size_t)token * a.heads + qh] = sum == 0.0f ? -INFINITY : (ref + __builtin_amdgcn_logf(sum)) * kLn2;
     } else {
@@ -450,13 +520,8 @@ __global__ __launch_bounds__(256) void kv_attend_join(AttendArgs a) {
         for (uint32_t s = 1; s < SUBS; ++s) sum += acc[s][col];
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         uint16_t* p = (uint16_t*)a.out.p + (token * a.out.token + qh * a.out.head + 4 * col);
-        const u32x2 w = {pack_out(sum[0] * inv, sum[1] * inv, a.is_bf16), pack_out(sum[2] * inv, sum[3] * inv, a.is_bf16)};
-        if (a.out.vec) {
-            *(u32x2*)p = w;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) p[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
-        }
+        const float y[4] = {sum[0], sum[1], sum[2], sum[3]};
+        store_out<4>(p, a.out.vec, a.is_bf16, y, inv);
         if (a.lse && col == 0)
             a.lse[(size_t)token * a.heads + qh] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
     }

@@ -187,7 +187,6 @@ QMM_DEVICE double shfl_xor_f64(double v, int mask) { return __shfl_xor(v, mask, 
 // heads, then value heads. Arithmetic in f64: a rotated value a c - b s of f32 factors has exact products and one
 // rounding there, and codes, scales and biases come out as from exact arithmetic (an f32 quotient beside a half way
 // point would take the wrong code, one step of the group's range / 15). Decode steps are bound by the launch.
-// figures in the design notes), decode steps by the launch.
 template <int DIM>
 __global__ __launch_bounds__(256) void kv_append(AppendArgs a) {
     constexpr uint32_t L = DIM / 8;  // lanes of a row
