@@ -660,8 +660,8 @@ typedef struct stark_qmm_kv_attention_args {
     uint32_t batch, tokens, heads, table_stride;
     uint32_t max_query;          /* bounds on the lengths of any request; what is longer is cut */
     uint32_t max_kv;
-    float scale;                 /* of the scores */
-    float soft_cap;              /* 0, or scores become soft_cap * tanh(score / soft_cap) */
+    float scale;                 /* of the scores: 0, or 2^-64 <= |scale| <= 2^64 */
+    float soft_cap;              /* 0, or 2^-20 .. 2^20: scores become soft_cap * tanh(score / soft_cap) */
     uint32_t causal;             /* query i of n sees keys up to kv_length - n + i */
     uint32_t window;             /* 0, or only the last `window` of those */
     void* workspace;             /* device, 16-byte aligned, >= stark_qmm_kv_attention_workspace_size() bytes */

@@ -30,7 +30,8 @@ FLAGS = [
 FILE_FLAGS = {
     # matrix-core accumulators that vector instructions read and write every step stay in VGPRs (without it each step
     # copied them from and to the accumulation registers: 64 of about 370 instructions)
-    "kv_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "kv_attend_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "kv_attend_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 

@@ -1,0 +1,93 @@
+// Shared by the attention kernels over the 4-bit paged key/value cache.
+#pragma once
+
+#include "kv_common.h"
+
+namespace qmm {
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kNone = -1e30f;  // running maximum before any key
+constexpr uint32_t kRows = 16;   // query rows of a matrix-core column block
+
+struct AttendArgs {
+    KvCache cache;
+    KvRows q, out;
+    float* lse;
+    const int32_t *table, *query_start, *kv_lengths;
+    uint32_t batch, tokens, heads, ratio, stride, max_query, max_kv;
+    float scale;    // of q . k: log2(e) * |scale|, or 2 log2(e) * |scale| / soft_cap; 1 for a scale of 0
+    float sign;     // of the scale: 1, -1 or 0; it goes to q
+    float cap;      // soft_cap * log2(e), or 0
+    uint32_t causal, is_bf16;
+    int32_t window;
+    // decode rows (kv_attend_rows)
+    uint32_t row_limit;      // requests with more rows to a kv head are kv_attend_tiles's; 0: all are
+    uint32_t ratio_inverse;  // ceil(65536 / ratio): x / ratio for x < 16
+    uint32_t whole;          // a unit to a workgroup, no partial results
+    uint32_t grid, inverse;  // else the workgroups that share the steps, and 2^32 / grid
+    float* po;               // [2 grid][16 rows][dim] unnormalised partial outputs
+    float2* pml;             // [2 grid][16 rows] (reference exponent, sum)
+    int4* begun;             // [grid] unit that begins in a workgroup and goes on in later ones: request (-1: none), head, how many
+    // rows of prompts (kv_attend_tiles)
+    uint32_t tile_rows, tiles;  // rows of a tile; tiles that the longest request may have
+    uint32_t chunk, chunks;     // keys of a workgroup, a multiple of 64, and how many such chunks the longest request may have
+    float* tile_po;             // [token][head][chunk][dim] unnormalised partial outputs
+    float2* tile_pml;           // [token][head][chunk] (reference exponent, sum)
+};
+
+QMM_DEVICE float plane_scale(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[0]; }
+QMM_DEVICE float plane_bias(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[1]; }
+// bias + 8 scale: the value of code 8
+QMM_DEVICE float plane_middle(uint32_t w) { return fmaf(plane_scale(w), 8.0f, plane_bias(w)); }
+
+QMM_DEVICE f16x8 operand(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_bit_cast(f16x8, u32x4{a, b, c, d});
+}
+
+QMM_DEVICE kv::Request request_of(const AttendArgs& a, uint32_t b) {
+    return kv::request(a.query_start[b], a.query_start[b + 1], a.kv_lengths[b], a.tokens, a.max_query, a.max_kv);
+}
+
+// Eight values of a q row as f32.
+QMM_DEVICE void widen8(const u32x4& w, uint32_t is_bf16, float* x) {
+    if (is_bf16) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = (float)__builtin_bit_cast(f16x2, (uint32_t)w[e / 2])[e & 1];
+    }
+}
+
+// N neighbouring output values, times f, at p; vec: 2 N bytes aligned.
+template <int N>
+QMM_DEVICE void store_out(uint16_t* p, uint32_t vec, uint32_t is_bf16, const float* x, float f) {
+    uint32_t w[N / 2];
+    if (is_bf16) {
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e)
+            w[e] = __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)(x[2 * e] * f), (__bf16)(x[2 * e + 1] * f)});
+    } else {
+#pragma unroll
+        for (int e = 0; e < N / 2; ++e)
+            w[e] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)(x[2 * e] * f), (_Float16)(x[2 * e + 1] * f)});
+    }
+    if (vec) {
+        if (N == 8) *(u32x4*)p = u32x4{w[0], w[1], w[2 % (N / 2)], w[3 % (N / 2)]};
+        else *(u32x2*)p = u32x2{w[0], w[1]};
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) p[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+    }
+}
+
+// Launchers (kv_attend_rows.hip, kv_attend_tiles.hip).
+stark_qmm_status launch_attend_rows(const AttendArgs& a, hipStream_t stream);
+stark_qmm_status launch_attend_tiles(const AttendArgs& a, hipStream_t stream);
+
+}  // namespace qmm

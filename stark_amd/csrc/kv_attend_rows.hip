@@ -1,0 +1,711 @@
+// Attention over the 4-bit paged key/value cache for requests of few rows: decode and short verify.
+#include "kv_attend.h"
+
+namespace {
+
+using namespace qmm;
+
+// Records of a step and how they are packed. PACK: records whose scores share one 16 x 16 block.
+template <int PACK>
+struct Shape {
+    static constexpr int R = 16 / PACK;            // rows of a request
+    static constexpr int T = PACK == 4 ? 4 : 2;    // records of a step
+    static constexpr int KEYS = 16 * T;            // keys of a step
+    static constexpr int B = T / PACK;             // score blocks of a step
+};
+
+// The keys of a step of one kv head as a wave's loads leave them: code words, and of the planes each word in one lane
+// only (lane 32 i + 16 v + t of pair h: record 2 h + i, keys' planes (v = 0) or values', token t).
+template <int DIM, int G, int T>
+struct Step {
+    uint32_t kc[T][DIM / 32], vc[T][DIM / 32], plane[T / 2][G];
+    uint32_t absent;  // bit i: record i's page is not in the cache
+
+    // base: the head's first record in page 0; page: the records' page ids; t0: first key
+    QMM_DEVICE void load(const KvCache& cache, const uint8_t* base, const uint32_t (&page)[T], uint32_t t0, uint32_t lane) {
+        const uint32_t c = lane & 15, g = lane >> 4, mask = (1u << cache.page_shift) - 1;
+        uint64_t rec[T];  // the records' offsets from base
+        absent = 0;
+#pragma unroll
+        for (int i = 0; i < T; ++i) {
+            const bool out = page[i] >= cache.page_count;
+            absent |= out ? 1u << i : 0u;
+            rec[i] = (uint64_t)(out ? 0 : page[i]) * cache.page_bytes + ((t0 + 16 * i) & mask) / 16 * cache.record;
+            const uint8_t* kq = base + rec[i] + (DIM == 64 ? c * 32 + g * 8 : c * 64 + g * 16);
+            const uint8_t* vq = base + rec[i] + 8 * DIM + 64 * G + lane * (DIM == 64 ? 8 : 16);
+            if (DIM == 64) {
+                *(u32x2*)&kc[i][0] = __builtin_nontemporal_load((const u32x2*)kq);
+                *(u32x2*)&vc[i][0] = __builtin_nontemporal_load((const u32x2*)vq);
+            } else {
+#pragma unroll
+                for (int h = 0; h < DIM / 128; ++h) {
+                    *(u32x4*)&kc[i][4 * h] = load_stream(kq + 1024 * h);
+                    *(u32x4*)&vc[i][4 * h] = load_stream(vq + 1024 * h);
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < T / 2; ++h) {
+            const uint64_t even = rec[2 * h], odd = rec[2 * h + 1];
+            const uint8_t* p = base + (lane & 32 ? odd : even) + (lane & 16 ? 16 * DIM + 64 * G : 8 * DIM) + 4 * c;
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) plane[h][gr] = *(const uint32_t*)(p + 64 * gr);
+        }
+    }
+};
+
+// A wave's planes of one step in LDS, [record][key or value][group][scale or middle][token] in f32: each word is
+// converted once, and the 16 lanes that need the same four tokens' read them with one 16-byte read.
+template <int G, int T>
+struct PlaneBuffer {
+    float v[T][2][G][2][16];
+};
+
+// Page ids of a wave's records: lane T n + i holds that of record i of step base + n, 64 / T steps to a load, and a step
+// reads its own with v_readlane.
+template <int T>
+struct PageIds {
+    const int32_t* row;
+    uint32_t from;         // first key of step 0
+    uint32_t stride;       // keys from a wave's step to its next
+    uint32_t shift, last;  // last entry of the table row
+    uint32_t ids, base;
+
+    QMM_DEVICE void fill(uint32_t n, uint32_t lane) {
+        base = n;
+        const uint32_t t = from + stride * (n + lane / T) + 16 * (lane % T);
+        ids = (uint32_t)row[min(t >> shift, last)];  // steps past the last key may be past the table too
+        asm volatile("" : "+v"(ids));  // the wait for it is here, not before every v_readlane (for all loads in flight)
+    }
+    QMM_DEVICE void get(uint32_t n, uint32_t lane, uint32_t (&page)[T]) {
+        if (n - base >= 64 / T) fill(n, lane);
+#pragma unroll
+        for (int i = 0; i < T; ++i) page[i] = (uint32_t)__builtin_amdgcn_readlane((int)ids, (int)(T * (n - base)) + i);
+    }
+};
+
+// Running state of 16 columns: lane (c, g) holds column c.
+template <int DIM, int G>
+struct Running {
+    static constexpr int J = DIM / 32;
+    f32x4 o[2 * J];          // [32-value block, parity]: codes times p s, values 32 i + 2 (4 g + e) + parity
+    f32x4 rounded[G];        // 8 sum p s, of the same roundings
+    float beta[G], l, m, mf; // sum p (b + 8 s) and sum p over the lane's keys; reference; reference - exponent
+    int fexp;
+
+    QMM_DEVICE void start(int exponent) {
+        fexp = exponent;
+        m = kNone, mf = kNone - (float)exponent, l = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 2 * J; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) beta[gr] = 0.0f, rounded[gr] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+};
+
+// A unit of work: the rows of a request (row_limit at most) that share a kv head, over its keys.
+struct Unit {
+    kv::Request r;
+    kv::Range span;  // keys that some row sees
+    int32_t from;    // span.lo, aligned to a step
+    uint32_t rows, steps;
+    uint32_t cost;   // steps, and what a unit costs to begin
+};
+
+// steps: at least one where there are rows (they are written in any case); 0 (and no cost) without rows, or with too many.
+template <int KEYS>
+QMM_DEVICE Unit unit_of(const AttendArgs& a, const kv::Request& r) {
+    Unit u;
+    u.r = r;
+    u.rows = (uint32_t)r.q_len * a.ratio;
+    u.span = kv::request_range(r.q_len, r.kv_len, a.causal, a.window);
+    u.from = u.span.lo & ~(KEYS - 1);
+    u.steps = (uint32_t)max((u.span.hi - u.from + KEYS - 1) / KEYS, 1);
+    if (u.rows == 0 || u.rows > a.row_limit) u.steps = 0;
+    u.cost = u.steps ? u.steps + kv::kUnitKeys / KEYS : 0;
+    return u;
+}
+
+// Lengths of 64 requests, one to a lane of the wave, so that a wave finds its way through the batch without LDS,
+// barriers or a second read.
+template <int KEYS>
+struct Requests {
+    kv::Request mine;
+    uint32_t b0;
+
+    QMM_DEVICE void load(const AttendArgs& a, uint32_t first, uint32_t lane) {
+        b0 = first;
+        mine = {0, 0, 0};
+        if (b0 + lane < a.batch) mine = request_of(a, b0 + lane);
+    }
+    QMM_DEVICE uint32_t cost(const AttendArgs& a) const { return unit_of<KEYS>(a, mine).cost * a.cache.kv_heads; }
+    QMM_DEVICE Unit unit(const AttendArgs& a, uint32_t b, uint32_t lane) {
+        if (b - b0 >= 64) load(a, b & ~63u, lane);
+        const int l = (int)(b - b0);
+        return unit_of<KEYS>(a, kv::Request{__builtin_amdgcn_readlane(mine.first, l), __builtin_amdgcn_readlane(mine.q_len, l),
+                                            __builtin_amdgcn_readlane(mine.kv_len, l)});
+    }
+};
+
+// Inclusive sum over the lanes of a wave.
+template <int CTRL, int ROWS>
+QMM_DEVICE uint32_t shifted(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+QMM_DEVICE uint32_t wave_scan(uint32_t v) {
+    v += shifted<0x111, 0xf>(v);  // one, two, four and eight lanes to the right inside rows of 16
+    v += shifted<0x112, 0xf>(v);
+    v += shifted<0x114, 0xf>(v);
+    v += shifted<0x118, 0xf>(v);
+    v += shifted<0x142, 0xa>(v);  // the last lane of rows 0 and 2 to rows 1 and 3
+    v += shifted<0x143, 0xc>(v);  // lane 31 to rows 2 and 3
+    return v;
+}
+
+// Decode and short verify: requests of up to R = 16 / PACK rows (a kv head's query heads times the new tokens).
+//
+// The work of a call is the steps (32 or 64 keys) of all (request, kv head) units, in that order; each workgroup takes
+// an equal run of them, so unlike lengths leave no CU idle and a workgroup pays its start once or twice, not once a
+// chunk. A unit inside one run is finished there; of the others each workgroup leaves partial results, which
+// kv_attend_join adds. Within a run the steps of a unit are dealt to four waves, each with its own running maximum and
+// sums, joined in LDS.
+//
+// Keys and values stay codes. With C the codes less 8,
+//   q . k = sum over groups (s_g C_g . q + (b_g + 8 s_g) sum q),   out = sum over tokens (p s_g) C + sum p (b_g + 8 s_g),
+// so a key's planes are a few fma per score and group, a value's scale goes into the probability (f16, p s_g scaled by a
+// power of two that keeps it in f16's normal range), and a code becomes an f16 operand by a mask: the bits of c in the
+// low (or 4 bits higher) end of an f16 are the subnormal c 2^-24 (c 2^-20), exact. The 8 is taken off by the score
+// accumulator's start value, and for the outputs by 8 sum (p s_g), summed as it was rounded: f32 sums and f16 roundings
+// then stand beside codes of either sign instead of 0 .. 15 (2.7 times less rounding error).
+//
+// Scores come out transposed (A rows = 16 keys, B columns = query rows): a lane holds four keys of one column in each
+// block, which is the B operand of the second product as it stands, with no lane exchange. With few rows most of a
+// block's 16 columns would be idle, and with them most of the vector work (planes, exponentials): so PACK records share a
+// block. Record i's product takes a B operand with the rows in columns R i .. R i + R - 1 and zeros elsewhere, and all
+// add into one block; column R i + r is then row r against record i's keys, and the columns of one row are joined at the
+// end like the waves. In the second product each record's columns are the others' zeros.
+// q is scaled per row by a power of two into f16's range, exact but for values 2^-24 below the row's largest.
+template <int DIM, int G, int PACK>
+__global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(AttendArgs a) {
+    using S = Shape<PACK>;
+    constexpr int R = S::R, T = S::T, KEYS = S::KEYS, B = S::B;
+    constexpr int J = DIM / 32;       // k blocks of a score product, and 32-value blocks of the output
+    constexpr int JG = J / G;         // of one scale group
+    constexpr int kRow = DIM + 4;     // padded row of the joining buffers, floats
+    __shared__ union {
+        u32x4 q[J + 1][64];           // score products' B operands; the last row is zeros
+        float join[4][R * kRow];
+    } sh;
+    __shared__ PlaneBuffer<G, T> plane_buffers[4];
+    __shared__ float wave_ref[4][16], wave_sum_l[4][16];
+    const uint32_t lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, row = c % R, pack = c / R;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+    // this workgroup's run of steps [at, end), and the request and step in it where the run begins; all steps of a
+    // call are below 2^31
+    uint32_t at = 0, end, per = 0, b = 0, offset;
+    Requests<KEYS> batch;
+    if (a.whole) {  // a unit to a workgroup
+        b = blockIdx.x / a.cache.kv_heads;
+        batch.load(a, b & ~63u, lane);
+        end = batch.unit(a, b, lane).cost;
+        offset = (blockIdx.x - b * a.cache.kv_heads) * end;
+    } else {
+        uint32_t total = 0, cost = 0, sum = 0;
+        for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
+            batch.load(a, b0, lane);
+            cost = batch.cost(a);
+            sum = wave_scan(cost);
+            total += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+        }
+        per = kv::share_of(total, a.grid, a.inverse, KEYS);
+        at = min(blockIdx.x * per, total), end = min(at + per, total);
+        if (threadIdx.x == 0) a.begun[blockIdx.x] = int4{-1, 0, 0, 0};
+        if (at == end) return;
+        uint32_t done = 0;
+        for (uint32_t b0 = 0;; b0 += 64) {  // at < total: some lane of some pass has it
+            if (a.batch > 64) {  // else the pass above was this one
+                batch.load(a, b0, lane);
+                cost = batch.cost(a);
+                sum = wave_scan(cost);
+            }
+            const uint32_t before = done + sum - cost;
+            const uint64_t here = __ballot(at >= before && at - before < cost);
+            if (here) {
+                const int l = __ffsll((unsigned long long)here) - 1;
+                b = b0 + (uint32_t)l;
+                offset = at - (uint32_t)__builtin_amdgcn_readlane((int)before, l);
+                break;
+            }
+            done += (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+        }
+    }
+    if (threadIdx.x < 64) sh.q[J][threadIdx.x] = u32x4{0, 0, 0, 0};
+
+    while (at < end) {
+        Unit u;
+        for (;; ++b, offset = 0) {  // at < total: a later request has steps
+            u = batch.unit(a, b, lane);
+            if (offset < u.cost * a.cache.kv_heads) break;
+        }
+        const uint32_t head = offset / u.cost, o0 = offset - head * u.cost, taken = min(u.cost - o0, end - at);
+        // a unit's first steps are its cost to begin: no work
+        const uint32_t idle = u.cost - u.steps, s0 = max(o0, idle) - idle, s1 = max(o0 + taken, idle) - idle;
+        const uint32_t unit_end = at + u.cost - o0;  // where the unit ends in the call's steps
+        offset += taken;
+        at += taken;
+        if (s0 == s1) continue;
+
+        const bool live = row < u.rows;
+        const uint32_t qi = live ? row * a.ratio_inverse >> 16 : 0;
+        const uint32_t qh = head * a.ratio + (live ? row - qi * a.ratio : 0), token = (uint32_t)u.r.first + qi;
+        kv::Range see = kv::visible((int32_t)qi, u.r.q_len, u.r.kv_len, a.causal, a.window);
+        if (!live) see = {0, 0x7fffffff};
+        const int32_t from = u.from + KEYS * (int32_t)s0;
+        const int32_t to = min(u.span.hi, u.from + KEYS * (int32_t)s1);
+
+        // loads of the query rows (a row past the last reads the request's first one, as zeros), then the page ids and
+        // the first step, and only then the use of the query rows
+        u32x4 w[J];
+        {
+            const uint16_t* p = (const uint16_t*)a.q.p + (token * a.q.token + qh * a.q.head + 8 * g);
+            if (a.q.vec) {
+#pragma unroll
+                for (int j = 0; j < J; ++j) w[j] = *(const u32x4*)(p + 32 * j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[j][e] = p[32 * j + 2 * e] | (uint32_t)p[32 * j + 2 * e + 1] << 16;
+            }
+        }
+        // this wave's steps: s0 + wave, s0 + wave + 4, ...
+        const uint32_t steps = s0 + wave < s1 ? (s1 - s0 - wave + 3) / 4 : 0, mine = (uint32_t)from + KEYS * wave;
+        PageIds<T> pages{a.table + (size_t)b * a.stride, mine, 4 * KEYS, a.cache.page_shift, a.stride - 1, 0, 0};
+        const uint8_t* base = a.cache.data + (uint64_t)head * a.cache.head_bytes;
+        const auto load = [&](Step<DIM, G, T>& st, uint32_t n) {
+            uint32_t page[T];
+            pages.get(n, lane, page);
+            st.load(a.cache, base, page, mine + 4 * KEYS * n, lane);
+        };
+        Step<DIM, G, T> st[2];
+        if (steps) {
+            pages.fill(0, lane);
+            load(st[0], 0);
+        }
+
+        // B operands of the score products: lane group g holds dims 8 (4 j + g) .. + 7, in the order of the code pairs
+        float qsum[G], c1;
+        f32x4 less8[G];
+        {
+            float x[J][8], top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                widen8(w[j], a.is_bf16, x[j]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[j][e] *= a.sign;
+                    top = fmaxf(top, fabsf(x[j][e]));
+                }
+            }
+            top = fmaxf(top, __shfl_xor(top, 16, 64));
+            top = fmaxf(top, __shfl_xor(top, 32, 64));
+            // 2^k puts the largest in [2^13, 2^14)
+            const int k = live ? 13 - (top > 0.0f && top < INFINITY ? ilogbf(top) : 0) : 0;
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+                float s = 0.0f;
+#pragma unroll
+                for (int j = gr * JG; j < (gr + 1) * JG; ++j)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s += x[j][e];
+                s += __shfl_xor(s, 16, 64);
+                s += __shfl_xor(s, 32, 64);
+                s = live ? s : 0.0f;
+                qsum[gr] = s * a.scale;
+                const float v = -ldexp_f32(s, k - 21);  // -8 sum q, in the accumulator's scale
+                less8[gr] = f32x4{v, v, v, v};
+            }
+            c1 = ldexp_f32(a.scale, 24 - k);
+            // every wave has the same rows: wave w writes the blocks w, w + 4, ...
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                // code pairs of a word: nibbles (0, 4), (1, 5) sixteenfold, (2, 6), (3, 7) sixteenfold
+                f16x8 h;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[e] = (_Float16)ldexp_f32(x[j][e / 2 + 4 * (e & 1)], (e / 2) & 1 ? k - 4 : k);
+                const u32x4 bits = __builtin_bit_cast(u32x4, h);
+                if (j % 4 == (int)wave) sh.q[j][lane] = live ? bits : u32x4{0, 0, 0, 0};
+            }
+        }
+        __syncthreads();
+        // record i's operand: the rows where this lane's column is of record i, zeros elsewhere
+        const auto q_operand = [&](int i, int j) {
+            const u32x4* p = PACK == 1 ? &sh.q[j][lane] : &sh.q[(int)pack == i % PACK ? j : J][lane];
+            return __builtin_bit_cast(f16x8, *p);
+        };
+
+        // keys that every row sees: [inner_lo, inner_hi)
+        const int32_t inner_lo = kv::visible(u.r.q_len - 1, u.r.q_len, u.r.kv_len, a.causal, a.window).lo;
+        const int32_t inner_hi = min(kv::visible(0, u.r.q_len, u.r.kv_len, a.causal, a.window).hi, to);
+
+        Running<DIM, G> run;
+        run.start(0);
+        PlaneBuffer<G, T>& planes = plane_buffers[wave];
+        // largest value scale (f16 bits) of plane words of a record's keys before `to`; t: this lane's key
+        const auto scale_max = [&](const uint32_t (&plane)[G], int32_t t, bool ok, uint32_t smax) {
+            if ((lane & 16) && t < to && ok) {
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    const uint32_t h = plane[gr] & 0xffffu;
+                    if (h < 0x7c00u) smax = max(smax, h);
+                }
+            }
+            return smax;
+        };
+        const int32_t t_lane = (int32_t)mine + 16 * (int32_t)(lane >> 5) + (int32_t)c;  // of step 0's first plane words
+        const auto exponent = [&](uint32_t smax) {
+            smax = group_max<16>(smax);
+            smax = max(smax, (uint32_t)__shfl_xor((int)smax, 16, 64));
+            smax = max(smax, (uint32_t)__shfl_xor((int)smax, 32, 64));
+            return smax ? 8 - ilogbf(f16_bits_to_f32(smax)) : 0;
+        };
+        const auto step = [&](Step<DIM, G, T>& st, uint32_t n) {
+            const int32_t t0 = (int32_t)(mine + 4 * KEYS * n);
+#pragma unroll
+            for (int h = 0; h < T / 2; ++h)
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    float* p = &planes.v[2 * h + (lane >> 5)][(lane >> 4) & 1][gr][0][c];
+                    p[0] = plane_scale(st.plane[h][gr]);
+                    p[16] = plane_middle(st.plane[h][gr]);
+                }
+            // the reads are of other lanes' words: a wave's LDS operations run in order, and this keeps the compiler's too
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            // block u holds records PACK u .. PACK u + PACK - 1; this lane's is PACK u + pack
+            float x[B][4];
+#pragma unroll
+            for (int u = 0; u < B; ++u) {
+                f32x4 acc[G];
+#pragma unroll
+                for (int i = 0; i < PACK; ++i)
+#pragma unroll
+                    for (int j = 0; j < J; ++j) {
+                        const uint32_t w = st.kc[PACK * u + i][j], v = w >> 8;
+                        const f16x8 k = operand(w & 0x000f000fu, w & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u);
+                        acc[j / JG] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                            k, q_operand(i, j), i == 0 && j % JG == 0 ? less8[j / JG] : acc[j / JG], 0, 0, 0);
+                    }
+                f32x4 y, z;
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    const float* p = &planes.v[PACK * u + (PACK == 1 ? 0 : pack)][0][gr][0][4 * g];
+                    const f32x4 s = *(const f32x4*)p, mid = *(const f32x4*)(p + 16);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        y[e] = gr ? fmaf(s[e], acc[gr][e], y[e]) : s[e] * acc[gr][e];
+                        z[e] = gr ? fmaf(mid[e], qsum[gr], z[e]) : mid[e] * qsum[gr];
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[u][e] = fmaf(y[e], c1, z[e]);
+            }
+            if (a.cap != 0.0f) {  // cap tanh(s / cap) = cap (1 - 2 / (1 + e^(2 s / cap)))
+#pragma unroll
+                for (int u = 0; u < B; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        x[u][e] = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[u][e]));
+            }
+            const bool masked = t0 < inner_lo || t0 + KEYS > inner_hi || st.absent;
+            if (masked) {
+#pragma unroll
+                for (int u = 0; u < B; ++u)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t rec = PACK * u + pack;
+                        const int32_t t = t0 + 16 * (int32_t)rec + 4 * (int32_t)g + e;
+                        x[u][e] = t >= see.lo && t < see.hi && t < to && !(st.absent >> rec & 1) ? x[u][e] : -INFINITY;
+                    }
+            }
+            float top = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3]));
+            if (B == 2) top = fmaxf(top, fmaxf(fmaxf(x[B - 1][0], x[B - 1][1]), fmaxf(x[B - 1][2], x[B - 1][3])));
+            // the reference moves only when a score passes it by 2^6: rescaling is then rare
+            if (__any(top > run.m + 6.0f)) {
+                top = fmaxf(top, __shfl_xor(top, 16, 64));
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float mn = fmaxf(run.m, top), f = __builtin_amdgcn_exp2f(run.m - mn);
+                run.m = mn;
+                run.mf = mn - (float)run.fexp;
+                run.l *= f;
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) run.beta[gr] *= f, run.rounded[gr] *= f;
+#pragma unroll
+                for (int j = 0; j < 2 * J; ++j) run.o[j] *= f;
+            }
+            // p s to f16, half a unit of 2^-11: the codes it multiplies are exact
+            u32x2 ps[B][G];
+#pragma unroll
+            for (int u = 0; u < B; ++u) {
+                float p[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f(x[u][e] - run.mf);
+                    run.l += p[e];
+                }
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    const float* q = &planes.v[PACK * u + (PACK == 1 ? 0 : pack)][1][gr][0][4 * g];
+                    f32x4 s = *(const f32x4*)q, mid = *(const f32x4*)(q + 16);
+                    if (masked) {
+                        // nothing of a key that a row does not see gets through, be it not a number
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const bool none = x[u][e] == -INFINITY;
+                            s[e] = none ? 0.0f : s[e];
+                            mid[e] = none ? 0.0f : mid[e];
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) run.beta[gr] = fmaf(p[e], mid[e], run.beta[gr]);
+                    ps[u][gr][0] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)(p[0] * s[0]), (_Float16)(p[1] * s[1])});
+                    ps[u][gr][1] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)(p[2] * s[2]), (_Float16)(p[3] * s[3])});
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // before the next step's planes are written
+            const f16x8 eights = operand(0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u);  // 8 2^-24
+#pragma unroll
+            for (int h = 0; h < T / 2; ++h) {  // records 2 h and 2 h + 1
+                f16x8 pb[G];
+#pragma unroll
+                for (int gr = 0; gr < G; ++gr) {
+                    if (PACK == 1) {
+                        pb[gr] = operand(ps[0][gr][0], ps[0][gr][1], ps[B - 1][gr][0], ps[B - 1][gr][1]);
+                    } else {
+                        const bool lo = (int)pack == 2 * h, hi = (int)pack == 2 * h + 1;
+                        pb[gr] = operand(lo ? ps[0][gr][0] : 0, lo ? ps[0][gr][1] : 0, hi ? ps[0][gr][0] : 0,
+                                         hi ? ps[0][gr][1] : 0);
+                    }
+                    run.rounded[gr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eights, pb[gr], run.rounded[gr], 0, 0, 0);
+                }
+#pragma unroll
+                for (int i = 0; i < J; ++i) {  // 32-value blocks; byte i of a lane's value words
+                    uint32_t w[4];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t* v = st.vc[2 * h + u];
+                        if (DIM == 64) {
+                            const uint32_t sel = 0x0c000c00u | (uint32_t)(2 + i) << 16 | (uint32_t)i;
+                            w[2 * u] = permb(0, v[0], sel);
+                            w[2 * u + 1] = permb(0, v[1], sel);
+                        } else {
+                            const uint32_t sel = 0x0c000c00u | (uint32_t)(4 + i % 4) << 16 | (uint32_t)(i % 4);
+                            v += i / 4 * 4;
+                            w[2 * u] = permb(v[1], v[0], sel);
+                            w[2 * u + 1] = permb(v[3], v[2], sel);
+                        }
+                    }
+                    const f16x8 lo = operand(w[0] & 0x000f000fu, w[1] & 0x000f000fu, w[2] & 0x000f000fu, w[3] & 0x000f000fu);
+                    const f16x8 hi = operand(w[0] & 0x00f000f0u, w[1] & 0x00f000f0u, w[2] & 0x00f000f0u, w[3] & 0x00f000f0u);
+                    run.o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, pb[i / JG], run.o[2 * i], 0, 0, 0);
+                    run.o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, pb[i / JG], run.o[2 * i + 1], 0, 0, 0);
+                }
+            }
+        };
+
+        // Power of two on the probabilities: p s below 2^15 while p < 2^6, taken from the scales of the wave's first
+        // records. Should a later scale be far larger, the products overflow to infinity, which shows in the sums at the
+        // end: then the wave starts again with the largest scale of all its keys.
+        for (int attempt = 0; attempt < 2 && steps; ++attempt) {
+            uint32_t smax = 0;
+            if (attempt) {
+                for (uint32_t n = 0; n < steps * (T / 2); ++n) {
+                    const int32_t t = t_lane + 4 * KEYS * (int32_t)(n / (T / 2)) + 32 * (int32_t)(n % (T / 2));
+                    const uint32_t id = (uint32_t)pages.row[min((uint32_t)t >> a.cache.page_shift, pages.last)];
+                    const bool ok = id < a.cache.page_count;
+                    const uint8_t* p = base + (uint64_t)(ok ? id : 0) * a.cache.page_bytes + 16 * DIM + 64 * G + 4 * c +
+                                       ((uint32_t)t & ((1u << a.cache.page_shift) - 1)) / 16 * a.cache.record;
+                    uint32_t plane[G];
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) plane[gr] = *(const uint32_t*)(p + 64 * gr);
+                    smax = scale_max(plane, t, ok, smax);
+                }
+                pages.fill(0, lane);
+                load(st[0], 0);
+            } else {
+                smax = scale_max(st[0].plane[0], t_lane, !(st[0].absent >> (lane >> 5) & 1), 0);
+            }
+            run.start(exponent(smax));
+            // The next step's loads go out before a step is computed (past the last step: of the last again). Two copies
+            // of the body, so that each register of a step stays where it was loaded: a copy would wait for the loads.
+            for (uint32_t n = 0; n < steps; n += 2) {
+                load(st[1], min(n + 1, steps - 1));
+                step(st[0], n);
+                load(st[0], min(n + 2, steps - 1));
+                if (n + 1 < steps) step(st[1], n + 1);
+            }
+            float bad = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 2 * J; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) bad = fmaf(run.o[j][e], 0.0f, bad);
+            if (!__any(bad != 0.0f)) break;  // 0 but where a sum is not finite
+        }
+
+        // the four lane groups hold different keys of one column
+        float l = run.l, mf = run.mf;
+        l += __shfl_xor(l, 16, 64);
+        l += __shfl_xor(l, 32, 64);
+        if (l == 0.0f) mf = kNone;
+        if (g == 0) wave_ref[wave][c] = mf;
+        __syncthreads();
+        // a row's reference: over the waves and its columns
+        float ref = kNone;
+#pragma unroll
+        for (int k = 0; k < 4 * PACK; ++k) ref = fmaxf(ref, wave_ref[k / PACK][k % PACK * R + row]);
+        const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mf - ref);
+        if (g == 0) wave_sum_l[wave][c] = l == 0.0f ? 0.0f : l * f;
+        // lane: values 32 i + 8 g + 0 .. 7 of its column
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            float s = run.beta[gr];
+            s += __shfl_xor(s, 16, 64);
+            s += __shfl_xor(s, 32, 64);
+#pragma unroll
+            for (int i = gr * JG; i < (gr + 1) * JG; ++i) {
+                float y[8];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float even = run.o[2 * i][e] - run.rounded[gr][e];
+                    const float odd = fmaf(run.o[2 * i + 1][e], 0.0625f, -run.rounded[gr][e]);
+                    y[2 * e] = l == 0.0f ? 0.0f : fmaf(even, 0x1p24f, s) * f;
+                    y[2 * e + 1] = l == 0.0f ? 0.0f : fmaf(odd, 0x1p24f, s) * f;
+                }
+                // the columns of a row: rotations of the 16-lane row by R, 2 R, ...
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    if (PACK >= 2) y[e] += dpp_f32<0x128>(y[e]);
+                    if (PACK >= 4) y[e] += dpp_f32<0x124>(y[e]);
+                }
+                if (pack == 0) {
+                    float* dst = &sh.join[wave][row * kRow + 32 * i + 8 * g];
+                    *(f32x4*)dst = f32x4{y[0], y[1], y[2], y[3]};
+                    *(f32x4*)(dst + 4) = f32x4{y[4], y[5], y[6], y[7]};
+                }
+            }
+        }
+        __syncthreads();
+        // the rows' values, N neighbouring ones to a thread
+        constexpr int N = DIM * R / 256 < 4 ? 4 : DIM * R / 256;
+        const uint32_t rr = threadIdx.x / (DIM / N), d = threadIdx.x % (DIM / N) * N;
+        if (rr < R && rr < u.rows) {
+            float v[N], sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < N; e += 4) {
+                f32x4 s = *(const f32x4*)&sh.join[0][rr * kRow + d + e];
+#pragma unroll
+                for (int k = 1; k < 4; ++k) s += *(const f32x4*)&sh.join[k][rr * kRow + d + e];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[e + k] = s[k];
+            }
+            float rref = kNone;
+#pragma unroll
+            for (int k = 0; k < 4 * PACK; ++k) {
+                sum += wave_sum_l[k / PACK][k % PACK * R + rr];
+                rref = fmaxf(rref, wave_ref[k / PACK][k % PACK * R + rr]);
+            }
+            const uint32_t ti = rr * a.ratio_inverse >> 16, hh = head * a.ratio + rr - ti * a.ratio;
+            const uint32_t tok = (uint32_t)u.r.first + ti;
+            if (s0 == 0 && s1 == u.steps) {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                uint16_t* p = (uint16_t*)a.out.p + (tok * a.out.token + hh * a.out.head + d);
+#pragma unroll
+                for (int e = 0; e < N; e += 4) store_out<4>(p + e, a.out.vec, a.is_bf16, v + e, inv);
+                if (a.lse && d == 0)
+                    a.lse[(size_t)tok * a.heads + hh] =
+                        sum == 0.0f ? -INFINITY : (rref + __builtin_amdgcn_logf(sum)) * kLn2;
+            } else {
+                const size_t slot = (2 * (size_t)blockIdx.x + (s0 == 0)) * kRows + rr;
+#pragma unroll
+                for (int e = 0; e < N; e += 4) *(f32x4*)(a.po + slot * DIM + d + e) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
+                if (d == 0) a.pml[slot] = float2{rref, sum};
+                if (s0 == 0 && threadIdx.x == 0)  // goes on in the workgroups up to the one that holds its last step
+                    a.begun[blockIdx.x] = int4{(int)b, (int)head, (int)((unit_end - 1) / per - blockIdx.x), 0};
+            }
+        }
+        __syncthreads();  // the LDS buffers are free again
+        if (threadIdx.x < 64) sh.q[J][threadIdx.x] = u32x4{0, 0, 0, 0};
+    }
+}
+
+// A row of a unit that several workgroups share, by one wave: out = sum_w o_w 2^(m_w - m) / sum_w l_w 2^(m_w - m), in
+// the order of the workgroups. Four rows a workgroup.
+template <int DIM>
+__global__ __launch_bounds__(256) void kv_attend_join(AttendArgs a) {
+    constexpr int V = DIM / 64;  // values of a lane
+    typedef float vec __attribute__((ext_vector_type(V)));
+    const uint32_t w = blockIdx.x / 4, lane = threadIdx.x & 63, row = blockIdx.x % 4 * 4 + (threadIdx.x >> 6);
+    const int4 u = a.begun[w];
+    if (u.x < 0) return;
+    const kv::Request r = request_of(a, (uint32_t)u.x);
+    if (row >= (uint32_t)r.q_len * a.ratio) return;
+    const uint32_t token = (uint32_t)r.first + row / a.ratio, qh = (uint32_t)u.y * a.ratio + row % a.ratio;
+    const uint32_t parts = (uint32_t)u.z + 1;
+    // part 0 is the workgroup's last segment, part i the first of workgroup w + i
+    const auto slot = [&](uint32_t i) { return (size_t)(i ? 2 * (w + i) : 2 * w + 1) * 16 + row; };
+    float m = kNone;
+    for (uint32_t i = lane; i < parts; i += 64) m = fmaxf(m, a.pml[slot(i)].x);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    vec sum = 0.0f;
+    float l = 0.0f;
+#pragma unroll 8
+    for (uint32_t i = 0; i < parts; ++i) {
+        const float2 v = a.pml[slot(i)];
+        const float f = __builtin_amdgcn_exp2f(v.x - m);
+        l = fmaf(v.y, f, l);
+        sum += *(const vec*)(a.po + slot(i) * DIM + V * lane) * f;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* p = (uint16_t*)a.out.p + (token * a.out.token + qh * a.out.head + V * lane);
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+        p[e] = a.is_bf16 ? f32_to_bf16_bits(sum[e] * inv) : f32_to_f16_bits(sum[e] * inv);
+    if (a.lse && lane == 0) a.lse[(size_t)token * a.heads + qh] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+template <int DIM, int G, int PACK>
+stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
+    hipLaunchKernelGGL((kv_attend_rows<DIM, G, PACK>), dim3(a.whole ? a.batch * a.cache.kv_heads : a.grid), dim3(256), 0, s, a);
+    QMM_HIP_CHECK(hipGetLastError());
+    if (!a.whole) {
+        hipLaunchKernelGGL((kv_attend_join<DIM>), dim3(4 * a.grid), dim3(256), 0, s, a);
+        QMM_HIP_CHECK(hipGetLastError());
+    }
+    return STARK_QMM_OK;
+}
+
+template <int DIM, int G>
+stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
+    if (a.row_limit <= 4) return launch<DIM, G, 4>(a, s);
+    return a.row_limit <= 8 ? launch<DIM, G, 2>(a, s) : launch<DIM, G, 1>(a, s);
+}
+
+}  // namespace
+
+namespace qmm {
+
+stark_qmm_status launch_attend_rows(const AttendArgs& a, hipStream_t s) {
+    switch (a.cache.dim * 16 + a.cache.groups) {
+    case 64 * 16 + 1: return launch<64, 1>(a, s);
+    case 64 * 16 + 2: return launch<64, 2>(a, s);
+    case 128 * 16 + 1: return launch<128, 1>(a, s);
+    case 128 * 16 + 2: return launch<128, 2>(a, s);
+    case 128 * 16 + 4: return launch<128, 4>(a, s);
+    case 256 * 16 + 2: return launch<256, 2>(a, s);
+    case 256 * 16 + 4: return launch<256, 4>(a, s);
+    default: return launch<256, 8>(a, s);
+    }
+}
+
+}  // namespace qmm

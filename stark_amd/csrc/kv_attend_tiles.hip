@@ -1,0 +1,480 @@
+// Attention over the 4-bit paged key/value cache for requests of many rows: prompts, and verify of long drafts.
+#include "kv_attend.h"
+
+namespace {
+
+using namespace qmm;
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kKeys = 64;  // keys of a tile: four records
+
+// LDS of one tile: keys [key][value of the head], values transposed [value of the head][key], both f16 in 16-byte pieces
+// whose place in a row is swizzled by the row, so that 16 lanes that read the same piece of 16 rows meet no bank twice.
+// not_finite: keys (bits) whose values' planes are not finite, for each group; they stand as zeros in v.
+template <int DIM, int G>
+struct Tile {
+    u32x4 k[kKeys][DIM / 8];
+    u32x4 v[DIM][kKeys / 8];
+    unsigned long long not_finite[G];
+    alignas(16) uint32_t absent[4];  // records whose page is not in the cache
+    static QMM_DEVICE uint32_t key_piece(uint32_t key, uint32_t piece) {
+        return piece ^ (DIM >= 128 ? key & 15 : key >> 1 & 7);
+    }
+    static QMM_DEVICE uint32_t value_piece(uint32_t dim, uint32_t piece) { return piece ^ (dim >> 1 & 7); }
+};
+
+QMM_DEVICE f16x2 half2_of(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
+QMM_DEVICE uint32_t bits_of(f16x2 h) { return __builtin_bit_cast(uint32_t, h); }
+
+// Two codes (bits 0-3 and 16-19 of w) as values: 1024 + c by its bits, less 1024 exactly, then one rounding of s c + b.
+QMM_DEVICE uint32_t two_values(uint32_t w, f16x2 s, f16x2 b) {
+    const f16x2 c = half2_of(and_or(w, 0x000f000fu, 0x64006400u)) - (f16x2){(_Float16)1024.0f, (_Float16)1024.0f};
+    return bits_of(__builtin_elementwise_fma(c, s, b));
+}
+
+// What one thread brings of a tile: of one record, a lane's key words and value words, and their planes.
+template <int DIM, int G>
+struct Codes {
+    static constexpr int N = DIM / 32;  // words of a lane
+    uint32_t kc[N], vc[N], kp[G];
+    u32x4 vp[G];
+
+    QMM_DEVICE void load_keys(const uint8_t* rec, uint32_t lane) {
+        const uint32_t c = lane & 15, g = lane >> 4;
+        const uint8_t* p = rec + (DIM == 64 ? c * 32 + g * 8 : c * 64 + g * 16);
+        if (DIM == 64) {
+            *(u32x2*)kc = *(const u32x2*)p;
+        } else {
+#pragma unroll
+            for (int h = 0; h < DIM / 128; ++h) *(u32x4*)&kc[4 * h] = *(const u32x4*)(p + 1024 * h);
+        }
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) kp[gr] = *(const uint32_t*)(rec + 8 * DIM + 64 * gr + 4 * c);
+    }
+    QMM_DEVICE void load_values(const uint8_t* rec, uint32_t lane) {
+        const uint8_t* p = rec + 8 * DIM + 64 * G + lane * (DIM == 64 ? 8 : 16);
+        if (DIM == 64) {
+            *(u32x2*)vc = *(const u32x2*)p;
+        } else {
+#pragma unroll
+            for (int h = 0; h < DIM / 128; ++h) *(u32x4*)&vc[4 * h] = *(const u32x4*)(p + 1024 * h);
+        }
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) vp[gr] = *(const u32x4*)(rec + 16 * DIM + 64 * G + 64 * gr + 16 * (lane >> 4));
+    }
+    // record: 0 .. 3 in the tile
+    QMM_DEVICE void write_keys(Tile<DIM, G>& t, uint32_t record, uint32_t lane) const {
+        const uint32_t key = 16 * record + (lane & 15), g = lane >> 4;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {  // word 4 j + g: values 8 (4 j + g) .. + 7, of group j G / N
+            const f16x2 plane = half2_of(kp[j * G / N]), s = {plane[0], plane[0]}, b = {plane[1], plane[1]};
+            const uint32_t w = kc[j];
+            t.k[key][t.key_piece(key, 4 * j + g)] = u32x4{two_values(w, s, b), two_values(w >> 4, s, b),
+                                                          two_values(w >> 8, s, b), two_values(w >> 12, s, b)};
+        }
+    }
+    // live: bit e: the lane's token 4 (lane / 16) + e is a key of the request, in a page of the cache
+    QMM_DEVICE void write_values(Tile<DIM, G>& t, uint32_t record, uint32_t lane, uint32_t live) {
+        const uint32_t r = lane & 15, quad = lane >> 4;
+        uint32_t top = 0;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                vp[gr][e] = live >> e & 1 ? vp[gr][e] : 0u;
+                const uint32_t x = vp[gr][e] & 0x7c007c00u;
+                top = max(top & 0x7c00u, x & 0x7c00u) | max(top & 0x7c000000u, x & 0x7c000000u);
+            }
+        if ((top & 0x7c00u) == 0x7c00u || top >> 16 == 0x7c00u) {
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if ((vp[gr][e] & 0x7c00u) == 0x7c00u || (vp[gr][e] >> 16 & 0x7c00u) == 0x7c00u) {
+                        vp[gr][e] = 0;
+                        if (r == 0) atomicOr(&t.not_finite[gr], 1ull << (16 * record + 4 * quad + e));
+                    }
+        }
+        // quads 0 and 2 of a record share a piece, and 1 and 3: the order of the probabilities in their operand
+        const uint32_t piece = 2 * record + (quad & 1), half = quad >> 1;
+#pragma unroll
+        for (int i = 0; i < DIM / 32; ++i) {  // byte i of the lane's value words: values 32 i + 2 r and the next
+            constexpr int M = DIM / 32;
+            const u32x4 p = vp[i * G / M];
+            const f16x2 s01 = half2_of(permb(p[1], p[0], 0x05040100u)), b01 = half2_of(permb(p[1], p[0], 0x07060302u));
+            const f16x2 s23 = half2_of(permb(p[3], p[2], 0x05040100u)), b23 = half2_of(permb(p[3], p[2], 0x07060302u));
+            uint32_t w01, w23;
+            if (DIM == 64) {
+                const uint32_t sel = 0x0c000c00u | (uint32_t)(2 + i) << 16 | (uint32_t)i;
+                w01 = permb(0, vc[0], sel), w23 = permb(0, vc[1], sel);
+            } else {
+                const uint32_t sel = 0x0c000c00u | (uint32_t)(4 + i % 4) << 16 | (uint32_t)(i % 4);
+                const int o = i / 4 * 4;
+                w01 = permb(vc[o + 1], vc[o], sel), w23 = permb(vc[o + 3], vc[o + 2], sel);
+            }
+            const uint32_t d = 32 * i + 2 * r;
+            u32x2* lo = (u32x2*)&t.v[d][t.value_piece(d, piece)];
+            u32x2* hi = (u32x2*)&t.v[d + 1][t.value_piece(d + 1, piece)];
+            lo[half] = u32x2{two_values(w01, s01, b01), two_values(w23, s23, b23)};
+            hi[half] = u32x2{two_values(w01 >> 4, s01, b01), two_values(w23 >> 4, s23, b23)};
+        }
+    }
+};
+
+// Prompts: tiles of 32 W rows (a kv head's query heads times tokens, W waves of 32 rows) against tiles of 64 keys.
+//
+// The keys and values of a tile are made f16 values in LDS once for all W waves (2 packed operations a value); what that
+// rounds, 2^-12 of a value, is of the size of the probabilities' own rounding to f16. Scores come out transposed, from
+// v_mfma_f32_32x32x16_f16 with keys as rows and query rows as columns: a lane holds, of one row, 16 of each 32 keys, and
+// those are the second product's B operand as they stand: the order of the keys in the transposed values is chosen to
+// match. One pass over the keys, running maximum and sum; a lane's maximum moves only when a score passes it by 2^6.
+// Two tiles of LDS: the next tile is unpacked while this one is multiplied, and the one after that is in flight.
+// Bound by vector work beside the matrix cores: per 64 keys and 32 rows 64 products of 32x32x16 (1024 clocks) stand
+// against 32 exponentials (512 clocks), the maximum, conversion and sum (about 300), and the unpacking's share.
+template <int DIM, int G, int W>
+__global__ __launch_bounds__(64 * W, 1) void kv_attend_tiles(AttendArgs a) {
+    constexpr int J = DIM / 16;   // k blocks of a score product
+    constexpr int O = DIM / 32;   // blocks of the output
+    __shared__ Tile<DIM, G> tiles[2];
+    const uint32_t lane = threadIdx.x & 63, col = lane & 31, hf = lane >> 5;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // workgroup: kv head first (workgroups are dealt to the XCDs in turn: a head's row tiles meet in one L2), then the
+    // row tile, longest first, then the shortest of the rest (with two workgroups to a CU a long one meets a short one)
+    uint32_t id = blockIdx.x;
+    const uint32_t head = id % a.cache.kv_heads;
+    id /= a.cache.kv_heads;
+    const uint32_t turn = id % a.tiles;
+    id /= a.tiles;
+    const uint32_t b = id % a.batch, part = id / a.batch;
+    const kv::Request r = request_of(a, b);
+    const uint32_t rows = (uint32_t)r.q_len * a.ratio;
+    if (rows <= a.row_limit) return;
+    const uint32_t mine = (rows + 32 * W - 1) / (32 * W);  // row tiles of this request
+    if (turn >= mine) return;
+    const uint32_t tile = turn < (mine + 1) / 2 ? mine - 1 - turn : turn - (mine + 1) / 2;
+
+    const uint32_t row0 = tile * 32 * W, row_end = min(row0 + 32 * W, rows);
+    const kv::Range top_row = kv::visible((int32_t)(row0 / a.ratio), r.q_len, r.kv_len, a.causal, a.window);
+    const kv::Range last_row = kv::visible((int32_t)((row_end - 1) / a.ratio), r.q_len, r.kv_len, a.causal, a.window);
+    // this workgroup's keys: its chunk of those that the tile's rows see
+    const uint32_t cut0 = part * a.chunk;
+    const int32_t from = max(top_row.lo & ~(kKeys - 1), (int32_t)cut0);
+    const int32_t to = a.chunks > 1 ? (int32_t)min((uint32_t)last_row.hi, cut0 + a.chunk) : last_row.hi;
+    if (from >= to && a.chunks > 1) return;  // the join leaves it out as well
+    const int32_t steps = from < to ? (to - from + kKeys - 1) / kKeys : 0;
+
+    const uint32_t first = row0 + 32 * wave;  // this wave's rows
+    const bool any_row = first < row_end;
+    const uint32_t rho = first + col;
+    const bool live = rho < row_end;
+    const uint32_t qi = live ? rho / a.ratio : row0 / a.ratio, qh = head * a.ratio + (live ? rho - qi * a.ratio : 0);
+    const uint32_t token = (uint32_t)r.first + qi;
+    const kv::Range see = kv::visible((int32_t)qi, r.q_len, r.kv_len, a.causal, a.window);
+    // of the wave's rows: keys that all see, and that some sees
+    const kv::Range wave_top = kv::visible((int32_t)(min(first, row_end - 1) / a.ratio), r.q_len, r.kv_len, a.causal, a.window);
+    const kv::Range wave_last = kv::visible((int32_t)((min(first + 32, row_end) - 1) / a.ratio), r.q_len, r.kv_len, a.causal,
+                                            a.window);
+    const int32_t inner_lo = __builtin_amdgcn_readfirstlane(wave_last.lo), outer_lo = __builtin_amdgcn_readfirstlane(wave_top.lo);
+    const int32_t inner_hi = __builtin_amdgcn_readfirstlane(min(wave_top.hi, to));
+    const int32_t outer_hi = __builtin_amdgcn_readfirstlane(any_row ? min(wave_last.hi, to) : 0);
+
+    // unpacking: eight waves: one half keys, the other values, a record to a wave; four waves: both, a record to a wave
+    const uint32_t record = wave % 4;
+    const bool keys_mine = W == 4 || wave < 4, values_mine = W == 4 || wave >= 4;
+    const int32_t* table = a.table + (size_t)b * a.stride;
+    const uint32_t page_mask = (1u << a.cache.page_shift) - 1;
+    const uint8_t* base = a.cache.data + (uint64_t)head * a.cache.head_bytes;
+    Codes<DIM, G> codes;
+    const auto page_of = [&](int32_t n) {  // a tile may reach past the last key: past the table too
+        const uint32_t t = (uint32_t)(from + kKeys * n) + 16 * record;
+        return (uint32_t)table[min(t >> a.cache.page_shift, a.stride - 1)];
+    };
+    // of the codes in hand: the lane's tokens of its record that are keys, and whether the record's page is in the cache
+    uint32_t live_keys = 0;
+    bool in_cache = false;
+    const auto fetch = [&](int32_t n, uint32_t page) {
+        const uint32_t t = (uint32_t)(from + kKeys * n) + 16 * record;
+        in_cache = page < a.cache.page_count;
+        const uint8_t* rec = base + (uint64_t)(in_cache ? page : 0) * a.cache.page_bytes + (t & page_mask) / 16 * a.cache.record;
+        if (keys_mine) codes.load_keys(rec, lane);
+        if (values_mine) {
+            codes.load_values(rec, lane);
+            const int32_t left = r.kv_len - (int32_t)(t + 4 * (lane >> 4));
+            live_keys = !in_cache || left <= 0 ? 0 : left >= 4 ? 15 : (1u << left) - 1;
+        }
+    };
+    const auto unpack = [&](Tile<DIM, G>& t) {
+        if (keys_mine) {
+            codes.write_keys(t, record, lane);
+            if (lane == 0) t.absent[record] = !in_cache;
+        }
+        if (values_mine) codes.write_values(t, record, lane, live_keys);
+    };
+    if (threadIdx.x < 2 * G) tiles[threadIdx.x / G].not_finite[threadIdx.x % G] = 0;
+    uint32_t page = 0;  // of the tile to fetch next
+    if (steps) {
+        fetch(0, page_of(0));
+        page = page_of(1);
+    }
+
+    // B operands of the score products: lane half hf holds values 8 (2 j + hf) .. + 7 of its row, in the pieces' order
+    f16x8 qb[J];
+    float c1;
+    {
+        const uint16_t* p = (const uint16_t*)a.q.p + (token * a.q.token + qh * a.q.head + 8 * hf);
+        u32x4 w[J];
+        if (a.q.vec) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) w[j] = *(const u32x4*)(p + 16 * j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[j][e] = p[16 * j + 2 * e] | (uint32_t)p[16 * j + 2 * e + 1] << 16;
+        }
+        float top = 0.0f;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            float x[8];
+            widen8(w[j], a.is_bf16, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+        }
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        // 2^k puts the largest in [2^3, 2^4): scores of keys up to 2^15 stay far inside f32
+        // (and rows of nothing but tiny values as they are, so that c1 stays a normal number)
+        const int k = min(3 - (top > 0.0f && top < INFINITY ? ilogbf(top) : 0), 48);
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            float x[8];
+            widen8(w[j], a.is_bf16, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) qb[j][e] = (_Float16)(ldexp_f32(x[e / 2 + 4 * (e & 1)], k) * a.sign);
+        }
+        c1 = ldexp_f32(a.scale, -k);  // positive: the sign is q's
+    }
+
+    f32x16 o[O];
+#pragma unroll
+    for (int i = 0; i < O; ++i) o[i] = f32x16{};
+    float m = kNone, l = 0.0f;
+    __syncthreads();  // not_finite is clear
+    if (steps) unpack(tiles[0]);
+    if (steps > 1) {
+        fetch(1, page);
+        page = page_of(2);
+    }
+    for (int32_t n = 0; n < steps; ++n) {
+        __syncthreads();
+        Tile<DIM, G>& t = tiles[n & 1];
+        const int32_t t0 = from + kKeys * n;
+        const u32x4 out = *(const u32x4*)t.absent;
+        if (t0 < outer_hi && t0 + kKeys > outer_lo) {
+            f32x16 s[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                s[h] = f32x16{};
+                const uint32_t key = 32 * h + col;
+#pragma unroll
+                for (int j = 0; j < J; ++j) {
+                    const f16x8 k = __builtin_bit_cast(f16x8, t.k[key][t.key_piece(key, 2 * j + hf)]);
+                    s[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[j], s[h], 0, 0, 0);
+                }
+            }
+            // value i of block h: key 32 h + 8 (i / 4) + 4 hf + i % 4
+            if (a.cap != 0.0f) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        s[h][i] = a.cap - 2.0f * a.cap *
+                                              __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s[h][i] * c1));
+            }
+            const float scale = a.cap != 0.0f ? 1.0f : c1;
+            if (t0 < inner_lo || t0 + kKeys > inner_hi || (out[0] | out[1] | out[2] | out[3])) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const uint32_t at = 32 * h + 8 * (i / 4) + 4 * hf + i % 4;
+                        const int32_t key = t0 + (int32_t)at;
+                        s[h][i] = key >= see.lo && key < see.hi && key < to && !out[2 * h + i / 8] ? s[h][i] : -INFINITY;
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(s[h][i], s[h][i + 1]));
+            top = top == -INFINITY ? top : top * scale;
+            if (__any(top > m + 6.0f)) {
+                const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64))), f = __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int i = 0; i < O; ++i) o[i] *= f;
+            }
+            // probabilities to f16 (2^-11 of each); the sum is of the same rounded values
+            uint32_t p[2][8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const f16x2 v = {(_Float16)__builtin_amdgcn_exp2f(fmaf(s[h][2 * i], scale, -m)),
+                                     (_Float16)__builtin_amdgcn_exp2f(fmaf(s[h][2 * i + 1], scale, -m))};
+                    p[h][i] = bits_of(v);
+                    l = __builtin_amdgcn_fdot2(v, (f16x2){(_Float16)1.0f, (_Float16)1.0f}, l, false);
+                }
+#pragma unroll
+            for (int i = 0; i < O; ++i) {
+                const uint32_t d = 32 * i + col;
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    const f16x8 v = __builtin_bit_cast(f16x8, t.v[d][t.value_piece(d, 2 * h + hf)]);
+                    const uint32_t* q = &p[h / 2][h % 2 * 4];
+                    o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, operand(q[0], q[1], q[2], q[3]), o[i], 0, 0, 0);
+                }
+            }
+            // values that are not finite, of keys that the row sees
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) {
+                const uint64_t bad = t.not_finite[gr];
+                if (bad) {
+                    const int32_t lo = min(max(see.lo - t0, 0), 64), hi = min(max(see.hi - t0, 0), 64);
+                    const uint64_t below_hi = hi >= 64 ? ~0ull : (1ull << hi) - 1, below_lo = lo >= 64 ? ~0ull : (1ull << lo) - 1;
+                    if (bad & below_hi & ~below_lo) {
+#pragma unroll
+                        for (int i = gr * O / G; i < (gr + 1) * O / G; ++i) o[i] += __builtin_nanf("");
+                    }
+                }
+            }
+        }
+        if (n + 1 < steps) {
+            Tile<DIM, G>& next = tiles[(n + 1) & 1];
+            unpack(next);
+            if (n + 2 < steps) {
+                fetch(n + 2, page);
+                page = page_of(n + 3);
+            }
+        }
+        // this tile's flags are clear again before the tile after the next sets them
+        if (n + 2 < steps) {
+            bool any = false;
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr) any |= t.not_finite[gr] != 0;
+            if (any) {
+                __syncthreads();
+                if (threadIdx.x < G) t.not_finite[threadIdx.x] = 0;
+            }
+        }
+    }
+
+    l += __shfl_xor(l, 32, 64);
+    if (!live) return;
+    // value 4 q + e of block i: 32 i + 8 q + 4 hf + e
+    if (a.chunks == 1) {
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        uint16_t* p = (uint16_t*)a.out.p + (token * a.out.token + qh * a.out.head + 4 * hf);
+#pragma unroll
+        for (int i = 0; i < O; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const float v[4] = {o[i][4 * q], o[i][4 * q + 1], o[i][4 * q + 2], o[i][4 * q + 3]};
+                store_out<4>(p + 32 * i + 8 * q, a.out.vec, a.is_bf16, v, inv);
+            }
+        if (a.lse && hf == 0)
+            a.lse[(size_t)token * a.heads + qh] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+    } else {
+        const size_t at = ((size_t)token * a.heads + qh) * a.chunks + part;
+        float* dst = a.tile_po + at * DIM + 4 * hf;
+#pragma unroll
+        for (int i = 0; i < O; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                *(f32x4*)(dst + 32 * i + 8 * q) = f32x4{o[i][4 * q], o[i][4 * q + 1], o[i][4 * q + 2], o[i][4 * q + 3]};
+        if (hf == 0) a.tile_pml[at] = float2{l == 0.0f ? kNone : m, l};
+    }
+}
+
+// The chunks of one row, by one wave: out = sum_c o_c 2^(m_c - m) / sum_c l_c 2^(m_c - m), in the order of the chunks.
+template <int DIM>
+__global__ __launch_bounds__(256) void kv_attend_tiles_join(AttendArgs a) {
+    constexpr int V = DIM / 64;
+    typedef float vec __attribute__((ext_vector_type(V)));
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t qh = id % a.heads;
+    id /= a.heads;
+    const uint32_t qi = id % a.max_query, b = id / a.max_query;
+    if (b >= a.batch) return;
+    const kv::Request r = request_of(a, b);
+    const uint32_t rows = (uint32_t)r.q_len * a.ratio;
+    if ((int32_t)qi >= r.q_len || rows <= a.row_limit) return;
+    const uint32_t token = (uint32_t)r.first + qi, row0 = (qi * a.ratio + qh % a.ratio) / a.tile_rows * a.tile_rows;
+    // the chunks that hold a key of the row's tile: exactly those its workgroups wrote
+    const kv::Range top_row = kv::visible((int32_t)(row0 / a.ratio), r.q_len, r.kv_len, a.causal, a.window);
+    const kv::Range last_row = kv::visible((int32_t)((min(row0 + a.tile_rows, rows) - 1) / a.ratio), r.q_len, r.kv_len, a.causal,
+                                           a.window);
+    const uint32_t c0 = (uint32_t)(top_row.lo & ~(kKeys - 1)) / a.chunk;
+    const uint32_t c1 = last_row.hi > (top_row.lo & ~(kKeys - 1)) ? ((uint32_t)last_row.hi + a.chunk - 1) / a.chunk : c0;
+    const size_t base = ((size_t)token * a.heads + qh) * a.chunks;
+    float m = kNone;
+    for (uint32_t c = c0 + lane; c < c1; c += 64) m = fmaxf(m, a.tile_pml[base + c].x);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    vec sum = 0.0f;
+    float l = 0.0f;
+#pragma unroll 4
+    for (uint32_t c = c0; c < c1; ++c) {
+        const float2 v = a.tile_pml[base + c];
+        const float f = __builtin_amdgcn_exp2f(v.x - m);
+        l = fmaf(v.y, f, l);
+        sum += *(const vec*)(a.tile_po + (base + c) * DIM + V * lane) * f;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* p = (uint16_t*)a.out.p + (token * a.out.token + qh * a.out.head + V * lane);
+#pragma unroll
+    for (int e = 0; e < V; ++e) p[e] = a.is_bf16 ? f32_to_bf16_bits(sum[e] * inv) : f32_to_f16_bits(sum[e] * inv);
+    if (a.lse && lane == 0) a.lse[(size_t)token * a.heads + qh] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+template <int DIM, int G, int W>
+stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
+    const uint64_t blocks = (uint64_t)a.cache.kv_heads * a.tiles * a.batch * a.chunks;
+    if (blocks >= 1ull << 22) return STARK_QMM_UNSUPPORTED;
+    hipLaunchKernelGGL((kv_attend_tiles<DIM, G, W>), dim3((uint32_t)blocks), dim3(64 * W), 0, s, a);
+    QMM_HIP_CHECK(hipGetLastError());
+    if (a.chunks > 1) {
+        const uint64_t joins = ((uint64_t)a.heads * a.max_query * a.batch + 3) / 4;
+        if (joins >= 1ull << 24) return STARK_QMM_UNSUPPORTED;
+        hipLaunchKernelGGL((kv_attend_tiles_join<DIM>), dim3((uint32_t)joins), dim3(256), 0, s, a);
+        QMM_HIP_CHECK(hipGetLastError());
+    }
+    return STARK_QMM_OK;
+}
+
+template <int DIM, int G>
+stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
+    if (DIM != 256 && a.tile_rows == 256) return launch<DIM, G, DIM == 256 ? 4 : 8>(a, s);
+    return launch<DIM, G, 4>(a, s);
+}
+
+}  // namespace
+
+namespace qmm {
+
+stark_qmm_status launch_attend_tiles(const AttendArgs& a, hipStream_t s) {
+    switch (a.cache.dim * 16 + a.cache.groups) {
+    case 64 * 16 + 1: return launch<64, 1>(a, s);
+    case 64 * 16 + 2: return launch<64, 2>(a, s);
+    case 128 * 16 + 1: return launch<128, 1>(a, s);
+    case 128 * 16 + 2: return launch<128, 2>(a, s);
+    case 128 * 16 + 4: return launch<128, 4>(a, s);
+    case 256 * 16 + 2: return launch<256, 2>(a, s);
+    case 256 * 16 + 4: return launch<256, 4>(a, s);
+    default: return launch<256, 8>(a, s);
+    }
+}
+
+}  // namespace qmm

@@ -11,6 +11,7 @@ namespace qmm {
 struct KvCache {
     uint8_t* data;
     uint32_t page_count, page_shift, kv_heads, dim, groups, record;
+    uint32_t head_bytes, page_bytes;  // of one head's records in a page, and of a page
 };
 
 inline bool kv_aligned(const void* p, uint64_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
@@ -26,8 +27,10 @@ inline stark_qmm_status kv_geometry(const stark_qmm_kv_cache& c, KvCache* out, u
     const uint32_t groups = c.head_dim / c.group_size;
     uint32_t shift = 4;
     while ((1u << shift) < c.page_size) ++shift;
-    *out = KvCache{nullptr, c.page_count, shift, c.kv_heads, c.head_dim, groups, kv::record_bytes(c.head_dim, groups)};
-    *bytes = (uint64_t)c.page_count * (c.page_size / kv::kTile) * c.kv_heads * out->record;
+    const uint32_t record = kv::record_bytes(c.head_dim, groups), head = c.page_size / kv::kTile * record;
+    // a page is at most 1024 heads * 64 records * 5120 bytes, below 2^32
+    *out = KvCache{nullptr, c.page_count, shift, c.kv_heads, c.head_dim, groups, record, head, c.kv_heads * head};
+    *bytes = (uint64_t)c.page_count * out->page_bytes;
     return STARK_QMM_OK;
 }
 

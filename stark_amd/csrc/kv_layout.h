@@ -56,17 +56,17 @@ KV_HD uint64_t record_index(uint64_t page, uint32_t kv_heads, uint32_t head, uin
     return (page * kv_heads + head) * (page_size / kTile) + at / kTile;
 }
 
-// Keys that query token i (0 .. q_len - 1) of a request sees: [lo, hi). Its position is kv_len - q_len + i.
+// Keys that query token i (0 .. q_len - 1) of a request sees: [lo, hi). Its position is kv_len - q_len + i, so none sees
+// past kv_len; the position may be before the first key. window: 0, or below 2^31.
 struct Range {
     int32_t lo, hi;
 };
-KV_HD Range visible(int32_t i, int32_t q_len, int32_t kv_len, bool causal, uint32_t window) {
-    const int64_t pos = (int64_t)kv_len - q_len + i;
-    int64_t hi = causal && pos + 1 < kv_len ? pos + 1 : kv_len;
-    int64_t lo = window && pos + 1 > (int64_t)window ? pos + 1 - (int64_t)window : 0;
-    if (hi < 0) hi = 0;
-    if (lo > hi) lo = hi;
-    return {(int32_t)lo, (int32_t)hi};
+KV_HD Range visible(int32_t i, int32_t q_len, int32_t kv_len, bool causal, int32_t window) {
+    const int32_t end = kv_len - q_len + i + 1;  // at most kv_len
+    int32_t hi = causal ? end : kv_len, lo = window && end > window ? end - window : 0;
+    hi = hi < 0 ? 0 : hi;
+    lo = lo > hi ? hi : lo;
+    return {lo, hi};
 }
 
 // A request of an attention call, with lengths that no device value can push past what was checked.
@@ -93,29 +93,66 @@ KV_HD PagePlan page_plan(int64_t cached, int64_t added, uint32_t page_shift, uin
     return {(int32_t)before, (int32_t)(after - before)};
 }
 
-// Rows of a tile: query rows (token i, query head h of the kv head's `ratio`) numbered i * ratio + h.
-constexpr uint32_t kRows = 16;
-
-// Keys that any row of a tile sees.
-KV_HD Range tile_range(uint32_t tile, uint32_t ratio, int32_t q_len, int32_t kv_len, bool causal, uint32_t window) {
-    const uint32_t last = tile * kRows + kRows - 1, rows = (uint32_t)q_len * ratio;
-    const Range a = visible((int32_t)(tile * kRows / ratio), q_len, kv_len, causal, window);
-    const Range b = visible((int32_t)((last < rows ? last : rows - 1) / ratio), q_len, kv_len, causal, window);
-    return {a.lo, b.hi};
+// Keys that any row of a request sees (its q_len is not 0).
+KV_HD Range request_range(int32_t q_len, int32_t kv_len, bool causal, int32_t window) {
+    return {visible(0, q_len, kv_len, causal, window).lo, visible(q_len - 1, q_len, kv_len, causal, window).hi};
 }
 
-// Keys of one workgroup where `units` (requests x kv heads x row tiles) do not fill the GPU, and how many such
-// chunks a request has at most. A multiple of 128, so that the four waves' 32-key steps come out even.
-struct Split {
-    uint32_t chunk, chunks;
+// Most rows (a kv head's query heads times new tokens) of a request that the decode kernel takes in a call: 4, 8 or 16, by
+// what the bounds say that any request has; in a call of longer requests, what one new token has (decode rows among
+// prompts), or 0 where there is one request. The others go to the tile kernel.
+KV_HD uint32_t row_limit(uint32_t batch, uint32_t max_query, uint32_t ratio) {
+    const uint64_t most = (uint64_t)max_query * ratio;
+    const uint64_t rows = most <= 16 ? most : batch > 1 ? ratio : 17;
+    return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 0;
+}
+
+// Keys of a workgroup's least share of a decode call: one 64-key or two 32-key steps for each of its four waves.
+constexpr uint32_t kLeastKeys = 256;
+
+// What beginning a unit costs a workgroup, in keys: its steps are counted as so many more.
+constexpr uint32_t kUnitKeys = 512;
+
+// Steps of each of `grid` workgroups that share `total` (below 2^31): a multiple of four, one for each wave.
+// inverse: 2^32 / grid, rounded down (2^32 - 1 for 1).
+KV_HD uint32_t share_of(uint32_t total, uint32_t grid, uint32_t inverse, uint32_t step_keys) {
+    uint32_t per = (uint32_t)((uint64_t)total * inverse >> 32);
+    while (per * grid < total) ++per;  // the quotient was up to two short
+    per = (per + 3) / 4 * 4;
+    const uint32_t least = kLeastKeys / step_keys;
+    return per < least ? least : per;
+}
+
+// How a decode call's work is dealt: whole units (a request's rows on one kv head) to a workgroup where no unit has more
+// keys than twice the least share; else `grid` workgroups share all steps (no more workgroups than shares).
+struct Share {
+    uint32_t whole, grid;
 };
-KV_HD Split split(uint64_t units, uint32_t max_kv, uint32_t cus) {
-    const uint64_t want = 4ull * cus;
-    if (units >= want || max_kv <= 256) return {max_kv < 128 ? 128 : (max_kv + 127) / 128 * 128, 1};
-    const uint32_t parts = (uint32_t)((want + units - 1) / units);
-    uint32_t chunk = ((max_kv + parts - 1) / parts + 127) / 128 * 128;
-    if (chunk < 256) chunk = 256;
-    return {chunk, (max_kv + chunk - 1) / chunk};
+KV_HD Share share(uint32_t batch, uint32_t kv_heads, uint32_t max_kv, uint32_t slots) {
+    if (max_kv <= 2 * kLeastKeys) return {1, 0};
+    const uint64_t keys = (uint64_t)batch * kv_heads * (max_kv + 128ull + kUnitKeys), most = (keys + kLeastKeys - 1) / kLeastKeys;
+    return {0, most < slots ? (uint32_t)(most ? most : 1) : slots};
+}
+
+// Tiles of the tile kernel: 256 rows (eight waves) where a request may have as many and such tiles fill the GPU, else 128;
+// and chunks of the keys where the tiles do not fill it (two workgroups of four waves to a CU), of 512 keys at least.
+struct Tiling {
+    uint32_t rows, tiles, chunk, chunks;
+};
+KV_HD Tiling tiling(uint32_t batch, uint32_t kv_heads, uint64_t most_rows, uint32_t max_kv, uint32_t cus, bool eight) {
+    const uint64_t units = (uint64_t)batch * kv_heads, wide = units * ((most_rows + 255) / 256);
+    Tiling t;
+    t.rows = eight && wide >= cus ? 256 : 128;
+    t.tiles = (uint32_t)((most_rows + t.rows - 1) / t.rows);
+    const uint64_t have = units * t.tiles, slots = 2ull * cus;
+    uint64_t parts = t.rows == 256 || have >= slots ? 1 : (slots + have - 1) / have;
+    const uint64_t longest = (max_kv + 511) / 512;
+    if (parts > longest) parts = longest ? longest : 1;
+    t.chunk = (uint32_t)((max_kv + parts - 1) / parts + 63) / 64 * 64;
+    if (t.chunk == 0) t.chunk = 64;
+    t.chunks = (uint32_t)(((uint64_t)max_kv + t.chunk - 1) / t.chunk);
+    if (t.chunks == 0) t.chunks = 1;
+    return t;
 }
 
 }  // namespace kv

@@ -22,11 +22,11 @@ uint32_t key_word(uint32_t dim, uint32_t t, uint32_t d) { return kv::key_word(di
 uint32_t value_byte(uint32_t dim, uint32_t t, uint32_t h, uint32_t r, uint32_t i) { return kv::value_byte(dim, t, h, r, i); }
 uint32_t plane_word(uint32_t t, uint32_t g) { return kv::plane_word(t, g); }
 uint64_t record_index(uint64_t p, uint32_t n, uint32_t h, uint32_t s, uint32_t at) { return kv::record_index(p, n, h, s, at); }
-void visible(int32_t i, int32_t q, int32_t k, int c, uint32_t w, int32_t* r) {
+void visible(int32_t i, int32_t q, int32_t k, int c, int32_t w, int32_t* r) {
     const kv::Range x = kv::visible(i, q, k, c != 0, w); r[0] = x.lo; r[1] = x.hi;
 }
-void tile_range(uint32_t t, uint32_t ratio, int32_t q, int32_t k, int c, uint32_t w, int32_t* r) {
-    const kv::Range x = kv::tile_range(t, ratio, q, k, c != 0, w); r[0] = x.lo; r[1] = x.hi;
+void request_range(int32_t q, int32_t k, int c, int32_t w, int32_t* r) {
+    const kv::Range x = kv::request_range(q, k, c != 0, w); r[0] = x.lo; r[1] = x.hi;
 }
 void request(int32_t s, int32_t e, int32_t k, uint32_t n, uint32_t mq, uint32_t mk, int32_t* r) {
     const kv::Request x = kv::request(s, e, k, n, mq, mk); r[0] = x.first; r[1] = x.q_len; r[2] = x.kv_len;
@@ -34,9 +34,14 @@ void request(int32_t s, int32_t e, int32_t k, uint32_t n, uint32_t mq, uint32_t 
 void page_plan(int64_t c, int64_t a, uint32_t s, uint32_t w, int32_t* r) {
     const kv::PagePlan x = kv::page_plan(c, a, s, w); r[0] = x.before; r[1] = x.need;
 }
-void split(uint64_t units, uint32_t max_kv, uint32_t cus, uint32_t* r) {
-    const kv::Split x = kv::split(units, max_kv, cus); r[0] = x.chunk; r[1] = x.chunks;
+void share(uint32_t batch, uint32_t heads, uint32_t max_kv, uint32_t slots, uint32_t* r) {
+    const kv::Share x = kv::share(batch, heads, max_kv, slots); r[0] = x.whole; r[1] = x.grid;
 }
+uint32_t share_of(uint32_t total, uint32_t grid, uint32_t keys) {
+    return kv::share_of(total, grid, grid > 1 ? (uint32_t)((1ull << 32) / grid) : 0xffffffffu, keys);
+}
+uint32_t row_limit(uint32_t b, uint32_t q, uint32_t r) { return kv::row_limit(b, q, r); }
+uint32_t unit_keys() { return kv::kUnitKeys; }
 }
 """
 
@@ -52,7 +57,6 @@ def rules():
         r.record_index.restype = C.c_uint64
         r.record_index.argtypes = [C.c_uint64] + [C.c_uint32] * 4
         r.page_plan.argtypes = [C.c_int64, C.c_int64, C.c_uint32, C.c_uint32, C.c_void_p]
-        r.split.argtypes = [C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p]
         return r
 
 
@@ -99,12 +103,12 @@ def test_records_fill_the_cache():
     assert L.record_index(2 ** 27 - 1, 1024, 1023, 16, 15) == 2 ** 37 - 1  # past 32 bits
 
 
-def test_visible_and_tile_ranges_against_one_key_at_a_time():
+def test_visible_ranges_against_one_key_at_a_time():
     r = random.Random(5)
     L = rules()
     for _ in range(400):
         q, k = r.randint(1, 40), r.choice([0, 1, r.randint(0, 60)])
-        causal, window, ratio = r.random() < 0.7, r.choice([0, 0, 1, 7, 100]), r.choice([1, 3, 8, 20])
+        causal, window = r.random() < 0.7, r.choice([0, 0, 1, 7, 100, 2 ** 31 - 1])
 
         def keys(i):
             pos = k - q + i
@@ -113,13 +117,14 @@ def test_visible_and_tile_ranges_against_one_key_at_a_time():
         for i in range(q):
             lo, hi = _out(L.visible, 2, i, q, k, int(causal), window)
             assert list(range(lo, hi)) == keys(i), (i, q, k, causal, window)
-        for tile in range((q * ratio + 15) // 16):
-            rows = range(16 * tile, min(16 * tile + 16, q * ratio))
-            union = sorted(set().union(*[keys(x // ratio) for x in rows]))
-            lo, hi = _out(L.tile_range, 2, tile, ratio, q, k, int(causal), window)
-            assert all(lo <= t < hi for t in union)
-            if union:
-                assert hi == union[-1] + 1
+        union = sorted(set().union(*[keys(i) for i in range(q)]))
+        lo, hi = _out(L.request_range, 2, q, k, int(causal), window)
+        assert all(lo <= t < hi for t in union)
+        if union:
+            assert hi == union[-1] + 1
+    big = 2 ** 31 - 1
+    assert _out(L.visible, 2, 0, 1, big, 1, 0) == (0, big) and _out(L.visible, 2, 0, 1, big, 1, 5) == (big - 5, big)
+    assert _out(L.visible, 2, 0, 2 ** 24, 3, 1, 2) == (0, 0)
 
 
 def test_request_lengths_stay_inside_what_was_checked():
@@ -139,12 +144,28 @@ def test_page_plan_counts_new_pages():
     assert _out(rules().page_plan, 2, 2 ** 31 - 1, 2 ** 24, 4, 3) == (3, 0)
 
 
-def test_split_covers_every_key():
-    for units in (1, 2, 8, 40, 500, 1023, 1024, 10 ** 6):
-        for kv in (0, 1, 127, 128, 256, 257, 4096, 5000, 131072, 2 ** 31 - 1):
-            chunk, chunks = _out(rules().split, 2, units, kv, 256, kind=C.c_uint32)
-            assert chunk % 128 == 0 and chunk >= 128 and chunks >= 1
-            assert chunk * chunks >= kv and (chunks - 1) * chunk < max(kv, 1)
+def test_shares_cover_every_step():
+    for batch, heads, kv in ((1, 1, 513), (1, 8, 4096), (64, 8, 32768), (1000, 4, 700), (3, 1, 131072), (2, 8, 5000)):
+        whole, grid = _out(rules().share, 2, batch, heads, kv, 512, kind=C.c_uint32)
+        assert not whole and 1 <= grid <= 512
+        for keys in (32, 64):
+            most = batch * heads * (-(-(kv + keys - 1) // keys) + rules().unit_keys() // keys)
+            for total in (0, 1, 7, 8, 9, 100, most // 3, most, 2 ** 31 - 1):
+                per, least = rules().share_of(total, grid, keys), 256 // keys
+                assert per % 4 == 0 and per >= least and per * grid >= total
+                assert per == max(least, -(-(-(-total // grid)) // 4) * 4)
+                if grid < 512 and total <= most:  # fewer workgroups than slots: each has its least share
+                    assert per == least
+    for kv in (0, 1, 512):
+        assert _out(rules().share, 2, 5, 2, kv, 512, kind=C.c_uint32)[0] == 1
+
+
+def test_row_limits():
+    """Which requests the decode kernel takes: by the rows that a kv head's query heads and the new tokens make."""
+    for batch, query, ratio, want in ((1, 1, 4, 4), (1, 2, 4, 8), (9, 3, 4, 16), (1, 4, 4, 16), (1, 5, 4, 0), (2, 5, 4, 4),
+                                      (2, 100, 7, 8), (2, 100, 16, 16), (2, 100, 17, 0), (5, 1, 20, 0), (1, 16, 1, 16),
+                                      (1, 17, 1, 0), (3, 17, 1, 4)):
+        assert rules().row_limit(batch, query, ratio) == want, (batch, query, ratio)
 
 
 def _geometry(**kw):
