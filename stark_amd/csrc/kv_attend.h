@@ -27,17 +27,19 @@ struct AttendArgs {
     int32_t window;
     // decode rows (kv_attend_rows)
     uint32_t row_limit;      // requests with more rows to a kv head are kv_attend_tiles's; 0: all are
-    uint32_t ratio_inverse;  // ceil(65536 / ratio): x / ratio for x < 16
+    uint32_t row_block;      // 4, 8 or 16
+    uint32_t ratio_inverse;  // ceil(65536 / ratio): x / ratio for x < 64 and ratios up to 64
     uint32_t whole;          // a unit to a workgroup, no partial results
     uint32_t grid, inverse;  // else the workgroups that share the steps, and 2^32 / grid
     float* po;               // [2 grid][16 rows][dim] unnormalised partial outputs
     float2* pml;             // [2 grid][16 rows] (reference exponent, sum)
-    int4* begun;             // [grid] unit that begins in a workgroup and goes on in later ones: request (-1: none), head, how many
+    int4* begun;             // [grid] unit that begins in a workgroup and goes on in later ones: request (-1: none), head,
+                             // first row, how many
     // rows of prompts (kv_attend_tiles)
-    uint32_t tile_rows, tiles;  // rows of a tile; tiles that the longest request may have
-    uint32_t chunk, chunks;     // keys of a workgroup, a multiple of 64, and how many such chunks the longest request may have
-    float* tile_po;             // [token][head][chunk][dim] unnormalised partial outputs
-    float2* tile_pml;           // [token][head][chunk] (reference exponent, sum)
+    uint32_t tiles;             // that the longest request may have
+    uint32_t pieces;            // that a tile's keys may be cut into
+    float* tile_po;             // [token][head][piece][dim] unnormalised partial outputs
+    float2* tile_pml;           // [token][head][piece] (reference exponent, sum)
 };
 
 QMM_DEVICE float plane_scale(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[0]; }
@@ -53,14 +55,19 @@ QMM_DEVICE kv::Request request_of(const AttendArgs& a, uint32_t b) {
     return kv::request(a.query_start[b], a.query_start[b + 1], a.kv_lengths[b], a.tokens, a.max_query, a.max_kv);
 }
 
-// Eight values of a q row as f32.
-QMM_DEVICE void widen8(const u32x4& w, uint32_t is_bf16, float* x) {
+// N pieces of eight values of a q row as f32.
+template <int N>
+QMM_DEVICE void widen(const u32x4 (&w)[N], uint32_t is_bf16, float (&x)[N][8]) {
     if (is_bf16) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[j][e] = __uint_as_float(e & 1 ? w[j][e / 2] & 0xffff0000u : w[j][e / 2] << 16);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = (float)__builtin_bit_cast(f16x2, (uint32_t)w[e / 2])[e & 1];
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[j][e] = (float)__builtin_bit_cast(f16x2, (uint32_t)w[j][e / 2])[e & 1];
     }
 }
 

@@ -103,17 +103,19 @@ struct Running {
     }
 };
 
-// A unit of work: the rows of a request (row_limit at most) that share a kv head, over its keys.
+// A unit of work: one block of R rows of a request on a kv head, over the request's keys.
 struct Unit {
     kv::Request r;
     kv::Range span;  // keys that some row sees
     int32_t from;    // span.lo, aligned to a step
-    uint32_t rows, steps;
+    uint32_t rows;   // of the request on a kv head
+    uint32_t steps;
     uint32_t cost;   // steps, and what a unit costs to begin
+    uint32_t all;    // cost of the request's blocks on all kv heads
 };
 
 // steps: at least one where there are rows (they are written in any case); 0 (and no cost) without rows, or with too many.
-template <int KEYS>
+template <int KEYS, int R>
 QMM_DEVICE Unit unit_of(const AttendArgs& a, const kv::Request& r) {
     Unit u;
     u.r = r;
@@ -123,12 +125,13 @@ QMM_DEVICE Unit unit_of(const AttendArgs& a, const kv::Request& r) {
     u.steps = (uint32_t)max((u.span.hi - u.from + KEYS - 1) / KEYS, 1);
     if (u.rows == 0 || u.rows > a.row_limit) u.steps = 0;
     u.cost = u.steps ? u.steps + kv::kUnitKeys / KEYS : 0;
+    u.all = u.cost * ((u.rows + R - 1) / R) * a.cache.kv_heads;
     return u;
 }
 
 // Lengths of 64 requests, one to a lane of the wave, so that a wave finds its way through the batch without LDS,
 // barriers or a second read.
-template <int KEYS>
+template <int KEYS, int R>
 struct Requests {
     kv::Request mine;
     uint32_t b0;
@@ -138,12 +141,13 @@ struct Requests {
         mine = {0, 0, 0};
         if (b0 + lane < a.batch) mine = request_of(a, b0 + lane);
     }
-    QMM_DEVICE uint32_t cost(const AttendArgs& a) const { return unit_of<KEYS>(a, mine).cost * a.cache.kv_heads; }
+    QMM_DEVICE uint32_t cost(const AttendArgs& a) const { return unit_of<KEYS, R>(a, mine).all; }
     QMM_DEVICE Unit unit(const AttendArgs& a, uint32_t b, uint32_t lane) {
         if (b - b0 >= 64) load(a, b & ~63u, lane);
         const int l = (int)(b - b0);
-        return unit_of<KEYS>(a, kv::Request{__builtin_amdgcn_readlane(mine.first, l), __builtin_amdgcn_readlane(mine.q_len, l),
-                                            __builtin_amdgcn_readlane(mine.kv_len, l)});
+        return unit_of<KEYS, R>(a, kv::Request{__builtin_amdgcn_readlane(mine.first, l),
+                                               __builtin_amdgcn_readlane(mine.q_len, l),
+                                               __builtin_amdgcn_readlane(mine.kv_len, l)});
     }
 };
 
@@ -162,9 +166,9 @@ QMM_DEVICE uint32_t wave_scan(uint32_t v) {
     return v;
 }
 
-// Decode and short verify: requests of up to R = 16 / PACK rows (a kv head's query heads times the new tokens).
+// Decode and verify: requests of few rows (a kv head's query heads times the new tokens), in blocks of R = 16 / PACK.
 //
-// The work of a call is the steps (32 or 64 keys) of all (request, kv head) units, in that order; each workgroup takes
+// The work of a call is the steps (32 or 64 keys) of all (request, kv head, block) units, in that order; each workgroup takes
 // an equal run of them, so unlike lengths leave no CU idle and a workgroup pays its start once or twice, not once a
 // chunk. A unit inside one run is finished there; of the others each workgroup leaves partial results, which
 // kv_attend_join adds. Within a run the steps of a unit are dealt to four waves, each with its own running maximum and
@@ -204,12 +208,15 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
     // this workgroup's run of steps [at, end), and the request and step in it where the run begins; all steps of a
     // call are below 2^31
     uint32_t at = 0, end, per = 0, b = 0, offset;
-    Requests<KEYS> batch;
+    Requests<KEYS, R> batch;
     if (a.whole) {  // a unit to a workgroup
-        b = blockIdx.x / a.cache.kv_heads;
+        const uint32_t blocks = (a.row_limit + R - 1) / R * a.cache.kv_heads;
+        b = blockIdx.x / blocks;
         batch.load(a, b & ~63u, lane);
-        end = batch.unit(a, b, lane).cost;
-        offset = (blockIdx.x - b * a.cache.kv_heads) * end;
+        const Unit u = batch.unit(a, b, lane);
+        offset = (blockIdx.x - b * blocks) * u.cost;
+        if (offset >= u.all) return;
+        end = u.cost;
     } else {
         uint32_t total = 0, cost = 0, sum = 0;
         for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
@@ -246,9 +253,11 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
         Unit u;
         for (;; ++b, offset = 0) {  // at < total: a later request has steps
             u = batch.unit(a, b, lane);
-            if (offset < u.cost * a.cache.kv_heads) break;
+            if (offset < u.all) break;
         }
-        const uint32_t head = offset / u.cost, o0 = offset - head * u.cost, taken = min(u.cost - o0, end - at);
+        const uint32_t index = offset / u.cost, o0 = offset - index * u.cost, taken = min(u.cost - o0, end - at);
+        // a kv head's blocks of rows one after another: they meet in the caches
+        const uint32_t blocks = (u.rows + R - 1) / R, head = index / blocks, row0 = (index - head * blocks) * R;
         // a unit's first steps are its cost to begin: no work
         const uint32_t idle = u.cost - u.steps, s0 = max(o0, idle) - idle, s1 = max(o0 + taken, idle) - idle;
         const uint32_t unit_end = at + u.cost - o0;  // where the unit ends in the call's steps
@@ -256,9 +265,9 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
         at += taken;
         if (s0 == s1) continue;
 
-        const bool live = row < u.rows;
-        const uint32_t qi = live ? row * a.ratio_inverse >> 16 : 0;
-        const uint32_t qh = head * a.ratio + (live ? row - qi * a.ratio : 0), token = (uint32_t)u.r.first + qi;
+        const bool live = row0 + row < u.rows;
+        const uint32_t qi = live ? (row0 + row) * a.ratio_inverse >> 16 : 0;
+        const uint32_t qh = head * a.ratio + (live ? row0 + row - qi * a.ratio : 0), token = (uint32_t)u.r.first + qi;
         kv::Range see = kv::visible((int32_t)qi, u.r.q_len, u.r.kv_len, a.causal, a.window);
         if (!live) see = {0, 0x7fffffff};
         const int32_t from = u.from + KEYS * (int32_t)s0;
@@ -299,9 +308,9 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
         f32x4 less8[G];
         {
             float x[J][8], top = 0.0f;
+            widen(w, a.is_bf16, x);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                widen8(w[j], a.is_bf16, x[j]);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     x[j][e] *= a.sign;
@@ -598,7 +607,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
         // the rows' values, N neighbouring ones to a thread
         constexpr int N = DIM * R / 256 < 4 ? 4 : DIM * R / 256;
         const uint32_t rr = threadIdx.x / (DIM / N), d = threadIdx.x % (DIM / N) * N;
-        if (rr < R && rr < u.rows) {
+        if (rr < R && row0 + rr < u.rows) {
             float v[N], sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < N; e += 4) {
@@ -614,7 +623,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
                 sum += wave_sum_l[k / PACK][k % PACK * R + rr];
                 rref = fmaxf(rref, wave_ref[k / PACK][k % PACK * R + rr]);
             }
-            const uint32_t ti = rr * a.ratio_inverse >> 16, hh = head * a.ratio + rr - ti * a.ratio;
+            const uint32_t ti = (row0 + rr) * a.ratio_inverse >> 16, hh = head * a.ratio + row0 + rr - ti * a.ratio;
             const uint32_t tok = (uint32_t)u.r.first + ti;
             if (s0 == 0 && s1 == u.steps) {
                 const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
@@ -630,7 +639,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
                 for (int e = 0; e < N; e += 4) *(f32x4*)(a.po + slot * DIM + d + e) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
                 if (d == 0) a.pml[slot] = float2{rref, sum};
                 if (s0 == 0 && threadIdx.x == 0)  // goes on in the workgroups up to the one that holds its last step
-                    a.begun[blockIdx.x] = int4{(int)b, (int)head, (int)((unit_end - 1) / per - blockIdx.x), 0};
+                    a.begun[blockIdx.x] = int4{(int)b, (int)head, (int)row0, (int)((unit_end - 1) / per - blockIdx.x)};
             }
         }
         __syncthreads();  // the LDS buffers are free again
@@ -644,15 +653,17 @@ template <int DIM>
 __global__ __launch_bounds__(256) void kv_attend_join(AttendArgs a) {
     constexpr int V = DIM / 64;  // values of a lane
     typedef float vec __attribute__((ext_vector_type(V)));
-    const uint32_t w = blockIdx.x / 4, lane = threadIdx.x & 63, row = blockIdx.x % 4 * 4 + (threadIdx.x >> 6);
+    const uint32_t quarters = a.row_block / 4, w = blockIdx.x / quarters, lane = threadIdx.x & 63;
+    const uint32_t slot_row = blockIdx.x % quarters * 4 + (threadIdx.x >> 6);
     const int4 u = a.begun[w];
     if (u.x < 0) return;
     const kv::Request r = request_of(a, (uint32_t)u.x);
+    const uint32_t row = (uint32_t)u.z + slot_row;
     if (row >= (uint32_t)r.q_len * a.ratio) return;
     const uint32_t token = (uint32_t)r.first + row / a.ratio, qh = (uint32_t)u.y * a.ratio + row % a.ratio;
-    const uint32_t parts = (uint32_t)u.z + 1;
+    const uint32_t parts = (uint32_t)u.w + 1;
     // part 0 is the workgroup's last segment, part i the first of workgroup w + i
-    const auto slot = [&](uint32_t i) { return (size_t)(i ? 2 * (w + i) : 2 * w + 1) * 16 + row; };
+    const auto slot = [&](uint32_t i) { return (size_t)(i ? 2 * (w + i) : 2 * w + 1) * kRows + slot_row; };
     float m = kNone;
     for (uint32_t i = lane; i < parts; i += 64) m = fmaxf(m, a.pml[slot(i)].x);
 #pragma unroll
@@ -676,10 +687,12 @@ __global__ __launch_bounds__(256) void kv_attend_join(AttendArgs a) {
 
 template <int DIM, int G, int PACK>
 stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
-    hipLaunchKernelGGL((kv_attend_rows<DIM, G, PACK>), dim3(a.whole ? a.batch * a.cache.kv_heads : a.grid), dim3(256), 0, s, a);
+    const uint64_t units = (uint64_t)a.batch * a.cache.kv_heads * ((a.row_limit + a.row_block - 1) / a.row_block);
+    if (a.whole && units >= 1ull << 24) return STARK_QMM_UNSUPPORTED;
+    hipLaunchKernelGGL((kv_attend_rows<DIM, G, PACK>), dim3(a.whole ? (uint32_t)units : a.grid), dim3(256), 0, s, a);
     QMM_HIP_CHECK(hipGetLastError());
     if (!a.whole) {
-        hipLaunchKernelGGL((kv_attend_join<DIM>), dim3(4 * a.grid), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((kv_attend_join<DIM>), dim3(a.grid * (a.row_block / 4)), dim3(256), 0, s, a);
         QMM_HIP_CHECK(hipGetLastError());
     }
     return STARK_QMM_OK;
@@ -687,8 +700,8 @@ stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
 
 template <int DIM, int G>
 stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
-    if (a.row_limit <= 4) return launch<DIM, G, 4>(a, s);
-    return a.row_limit <= 8 ? launch<DIM, G, 2>(a, s) : launch<DIM, G, 1>(a, s);
+    if (a.row_block == 4) return launch<DIM, G, 4>(a, s);
+    return a.row_block == 8 ? launch<DIM, G, 2>(a, s) : launch<DIM, G, 1>(a, s);
 }
 
 }  // namespace

@@ -27,6 +27,11 @@ struct Tile {
 QMM_DEVICE f16x2 half2_of(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
 QMM_DEVICE uint32_t bits_of(f16x2 h) { return __builtin_bit_cast(uint32_t, h); }
 
+// Largest of three, one instruction; a NaN wins (its row is NaN in any case).
+QMM_DEVICE float max3(float a, float b, float c) {
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+
 // Two codes (bits 0-3 and 16-19 of w) as values: 1024 + c by its bits, less 1024 exactly, then one rounding of s c + b.
 QMM_DEVICE uint32_t two_values(uint32_t w, f16x2 s, f16x2 b) {
     const f16x2 c = half2_of(and_or(w, 0x000f000fu, 0x64006400u)) - (f16x2){(_Float16)1024.0f, (_Float16)1024.0f};
@@ -77,22 +82,23 @@ struct Codes {
     // live: bit e: the lane's token 4 (lane / 16) + e is a key of the request, in a page of the cache
     QMM_DEVICE void write_values(Tile<DIM, G>& t, uint32_t record, uint32_t lane, uint32_t live) {
         const uint32_t r = lane & 15, quad = lane >> 4;
+        u32x4 q[G];  // (copies: the loaded registers stay as they are, or the next load's would be copied, and waited for)
         uint32_t top = 0;
 #pragma unroll
         for (int gr = 0; gr < G; ++gr)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                vp[gr][e] = live >> e & 1 ? vp[gr][e] : 0u;
-                const uint32_t x = vp[gr][e] & 0x7c007c00u;
+                q[gr][e] = live >> e & 1 ? vp[gr][e] : 0u;
+                const uint32_t x = q[gr][e] & 0x7c007c00u;
                 top = max(top & 0x7c00u, x & 0x7c00u) | max(top & 0x7c000000u, x & 0x7c000000u);
             }
-        if ((top & 0x7c00u) == 0x7c00u || top >> 16 == 0x7c00u) {
+        if (__any((top & 0x7c00u) == 0x7c00u || top >> 16 == 0x7c00u)) {
 #pragma unroll
             for (int gr = 0; gr < G; ++gr)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    if ((vp[gr][e] & 0x7c00u) == 0x7c00u || (vp[gr][e] >> 16 & 0x7c00u) == 0x7c00u) {
-                        vp[gr][e] = 0;
+                    if ((q[gr][e] & 0x7c00u) == 0x7c00u || (q[gr][e] >> 16 & 0x7c00u) == 0x7c00u) {
+                        q[gr][e] = 0;
                         if (r == 0) atomicOr(&t.not_finite[gr], 1ull << (16 * record + 4 * quad + e));
                     }
         }
@@ -101,7 +107,7 @@ struct Codes {
 #pragma unroll
         for (int i = 0; i < DIM / 32; ++i) {  // byte i of the lane's value words: values 32 i + 2 r and the next
             constexpr int M = DIM / 32;
-            const u32x4 p = vp[i * G / M];
+            const u32x4 p = q[i * G / M];
             const f16x2 s01 = half2_of(permb(p[1], p[0], 0x05040100u)), b01 = half2_of(permb(p[1], p[0], 0x07060302u));
             const f16x2 s23 = half2_of(permb(p[3], p[2], 0x05040100u)), b23 = half2_of(permb(p[3], p[2], 0x07060302u));
             uint32_t w01, w23;
@@ -122,9 +128,9 @@ struct Codes {
     }
 };
 
-// Prompts: tiles of 32 W rows (a kv head's query heads times tokens, W waves of 32 rows) against tiles of 64 keys.
+// Prompts: tiles of 128 rows (a kv head's query heads times tokens, 32 to a wave) against tiles of 64 keys.
 //
-// The keys and values of a tile are made f16 values in LDS once for all W waves (2 packed operations a value); what that
+// The keys and values of a tile are made f16 values in LDS once for all four waves (2 packed operations a value); what that
 // rounds, 2^-12 of a value, is of the size of the probabilities' own rounding to f16. Scores come out transposed, from
 // v_mfma_f32_32x32x16_f16 with keys as rows and query rows as columns: a lane holds, of one row, 16 of each 32 keys, and
 // those are the second product's B operand as they stand: the order of the keys in the transposed values is chosen to
@@ -132,8 +138,8 @@ struct Codes {
 // Two tiles of LDS: the next tile is unpacked while this one is multiplied, and the one after that is in flight.
 // Bound by vector work beside the matrix cores: per 64 keys and 32 rows 64 products of 32x32x16 (1024 clocks) stand
 // against 32 exponentials (512 clocks), the maximum, conversion and sum (about 300), and the unpacking's share.
-template <int DIM, int G, int W>
-__global__ __launch_bounds__(64 * W, 1) void kv_attend_tiles(AttendArgs a) {
+template <int DIM, int G>
+__global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
     constexpr int J = DIM / 16;   // k blocks of a score product
     constexpr int O = DIM / 32;   // blocks of the output
     __shared__ Tile<DIM, G> tiles[2];
@@ -150,18 +156,18 @@ __global__ __launch_bounds__(64 * W, 1) void kv_attend_tiles(AttendArgs a) {
     const kv::Request r = request_of(a, b);
     const uint32_t rows = (uint32_t)r.q_len * a.ratio;
     if (rows <= a.row_limit) return;
-    const uint32_t mine = (rows + 32 * W - 1) / (32 * W);  // row tiles of this request
+    const uint32_t mine = (rows + kv::kTileRows - 1) / (kv::kTileRows);  // row tiles of this request
     if (turn >= mine) return;
     const uint32_t tile = turn < (mine + 1) / 2 ? mine - 1 - turn : turn - (mine + 1) / 2;
 
-    const uint32_t row0 = tile * 32 * W, row_end = min(row0 + 32 * W, rows);
+    const uint32_t row0 = tile * kv::kTileRows, row_end = min(row0 + kv::kTileRows, rows);
     const kv::Range top_row = kv::visible((int32_t)(row0 / a.ratio), r.q_len, r.kv_len, a.causal, a.window);
     const kv::Range last_row = kv::visible((int32_t)((row_end - 1) / a.ratio), r.q_len, r.kv_len, a.causal, a.window);
-    // this workgroup's keys: its chunk of those that the tile's rows see
-    const uint32_t cut0 = part * a.chunk;
-    const int32_t from = max(top_row.lo & ~(kKeys - 1), (int32_t)cut0);
-    const int32_t to = a.chunks > 1 ? (int32_t)min((uint32_t)last_row.hi, cut0 + a.chunk) : last_row.hi;
-    if (from >= to && a.chunks > 1) return;  // the join leaves it out as well
+    // this workgroup's keys: its piece of those that the tile's rows see
+    const int32_t begin = top_row.lo & ~(kKeys - 1);
+    const int32_t piece = a.pieces > 1 ? kv::piece_keys(last_row.hi - begin, a.pieces) : 0;
+    if (part && part * (uint64_t)piece >= (uint64_t)(last_row.hi - begin)) return;  // the join leaves it out as well
+    const int32_t from = begin + (int32_t)part * piece, to = a.pieces > 1 ? min(last_row.hi, from + piece) : last_row.hi;
     const int32_t steps = from < to ? (to - from + kKeys - 1) / kKeys : 0;
 
     const uint32_t first = row0 + 32 * wave;  // this wave's rows
@@ -179,9 +185,7 @@ __global__ __launch_bounds__(64 * W, 1) void kv_attend_tiles(AttendArgs a) {
     const int32_t inner_hi = __builtin_amdgcn_readfirstlane(min(wave_top.hi, to));
     const int32_t outer_hi = __builtin_amdgcn_readfirstlane(any_row ? min(wave_last.hi, to) : 0);
 
-    // unpacking: eight waves: one half keys, the other values, a record to a wave; four waves: both, a record to a wave
-    const uint32_t record = wave % 4;
-    const bool keys_mine = W == 4 || wave < 4, values_mine = W == 4 || wave >= 4;
+    const uint32_t record = wave;  // that this wave unpacks of each tile
     const int32_t* table = a.table + (size_t)b * a.stride;
     const uint32_t page_mask = (1u << a.cache.page_shift) - 1;
     const uint8_t* base = a.cache.data + (uint64_t)head * a.cache.head_bytes;
@@ -197,25 +201,21 @@ __global__ __launch_bounds__(64 * W, 1) void kv_attend_tiles(AttendArgs a) {
         const uint32_t t = (uint32_t)(from + kKeys * n) + 16 * record;
         in_cache = page < a.cache.page_count;
         const uint8_t* rec = base + (uint64_t)(in_cache ? page : 0) * a.cache.page_bytes + (t & page_mask) / 16 * a.cache.record;
-        if (keys_mine) codes.load_keys(rec, lane);
-        if (values_mine) {
-            codes.load_values(rec, lane);
-            const int32_t left = r.kv_len - (int32_t)(t + 4 * (lane >> 4));
-            live_keys = !in_cache || left <= 0 ? 0 : left >= 4 ? 15 : (1u << left) - 1;
-        }
+        codes.load_keys(rec, lane);
+        codes.load_values(rec, lane);
+        const int32_t left = r.kv_len - (int32_t)(t + 4 * (lane >> 4));
+        live_keys = !in_cache || left <= 0 ? 0 : left >= 4 ? 15 : (1u << left) - 1;
     };
     const auto unpack = [&](Tile<DIM, G>& t) {
-        if (keys_mine) {
-            codes.write_keys(t, record, lane);
-            if (lane == 0) t.absent[record] = !in_cache;
-        }
-        if (values_mine) codes.write_values(t, record, lane, live_keys);
+        codes.write_keys(t, record, lane);
+        codes.write_values(t, record, lane, live_keys);
+        if (lane == 0) t.absent[record] = !in_cache;
     };
     if (threadIdx.x < 2 * G) tiles[threadIdx.x / G].not_finite[threadIdx.x % G] = 0;
     uint32_t page = 0;  // of the tile to fetch next
     if (steps) {
         fetch(0, page_of(0));
-        page = page_of(1);
+        page = page_of(min(1, steps - 1));
     }
 
     // B operands of the score products: lane half hf holds values 8 (2 j + hf) .. + 7 of its row, in the pieces' order
@@ -233,25 +233,20 @@ __global__ __launch_bounds__(64 * W, 1) void kv_attend_tiles(AttendArgs a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) w[j][e] = p[16 * j + 2 * e] | (uint32_t)p[16 * j + 2 * e + 1] << 16;
         }
-        float top = 0.0f;
+        float x[J][8], top = 0.0f;
+        widen(w, a.is_bf16, x);
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            float x[8];
-            widen8(w[j], a.is_bf16, x);
+        for (int j = 0; j < J; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
-        }
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[j][e]));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         // 2^k puts the largest in [2^3, 2^4): scores of keys up to 2^15 stay far inside f32
         // (and rows of nothing but tiny values as they are, so that c1 stays a normal number)
         const int k = min(3 - (top > 0.0f && top < INFINITY ? ilogbf(top) : 0), 48);
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-            float x[8];
-            widen8(w[j], a.is_bf16, x);
+        for (int j = 0; j < J; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) qb[j][e] = (_Float16)(ldexp_f32(x[e / 2 + 4 * (e & 1)], k) * a.sign);
-        }
+            for (int e = 0; e < 8; ++e) qb[j][e] = (_Float16)(ldexp_f32(x[j][e / 2 + 4 * (e & 1)], k) * a.sign);
         c1 = ldexp_f32(a.scale, -k);  // positive: the sign is q's
     }
 
@@ -260,16 +255,20 @@ __global__ __launch_bounds__(64 * W, 1) void kv_attend_tiles(AttendArgs a) {
     for (int i = 0; i < O; ++i) o[i] = f32x16{};
     float m = kNone, l = 0.0f;
     __syncthreads();  // not_finite is clear
-    if (steps) unpack(tiles[0]);
-    if (steps > 1) {
-        fetch(1, page);
-        page = page_of(2);
+    if (steps) {
+        unpack(tiles[0]);
+        fetch(min(1, steps - 1), page);
+        page = page_of(min(2, steps - 1));
     }
     for (int32_t n = 0; n < steps; ++n) {
         __syncthreads();
         Tile<DIM, G>& t = tiles[n & 1];
         const int32_t t0 = from + kKeys * n;
         const u32x4 out = *(const u32x4*)t.absent;
+        uint64_t set = 0;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) set |= t.not_finite[gr];
+        const bool flags = __builtin_amdgcn_readfirstlane((int)(uint32_t)(set | set >> 32)) != 0;
         if (t0 < outer_hi && t0 + kKeys > outer_lo) {
             f32x16 s[2];
 #pragma unroll
@@ -306,7 +305,7 @@ __global__ __launch_bounds__(64 * W, 1) void kv_attend_tiles(AttendArgs a) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(s[h][i], s[h][i + 1]));
+                for (int i = 0; i < 16; i += 2) top = max3(top, s[h][i], s[h][i + 1]);
             top = top == -INFINITY ? top : top * scale;
             if (__any(top > m + 6.0f)) {
                 const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64))), f = __builtin_amdgcn_exp2f(m - mn);
@@ -337,43 +336,34 @@ __global__ __launch_bounds__(64 * W, 1) void kv_attend_tiles(AttendArgs a) {
                 }
             }
             // values that are not finite, of keys that the row sees
+            if (flags) {
 #pragma unroll
-            for (int gr = 0; gr < G; ++gr) {
-                const uint64_t bad = t.not_finite[gr];
-                if (bad) {
+                for (int gr = 0; gr < G; ++gr) {
+                    const uint64_t bad = t.not_finite[gr];
                     const int32_t lo = min(max(see.lo - t0, 0), 64), hi = min(max(see.hi - t0, 0), 64);
                     const uint64_t below_hi = hi >= 64 ? ~0ull : (1ull << hi) - 1, below_lo = lo >= 64 ? ~0ull : (1ull << lo) - 1;
-                    if (bad & below_hi & ~below_lo) {
+                    const float add = bad & below_hi & ~below_lo ? __builtin_nanf("") : 0.0f;
 #pragma unroll
-                        for (int i = gr * O / G; i < (gr + 1) * O / G; ++i) o[i] += __builtin_nanf("");
-                    }
+                    for (int i = gr * O / G; i < (gr + 1) * O / G; ++i) o[i] += add;
                 }
             }
         }
-        if (n + 1 < steps) {
-            Tile<DIM, G>& next = tiles[(n + 1) & 1];
-            unpack(next);
-            if (n + 2 < steps) {
-                fetch(n + 2, page);
-                page = page_of(n + 3);
-            }
-        }
+        // the tile after this (past the last: the last again), and the loads of the one after that
+        unpack(tiles[(n + 1) & 1]);
+        fetch(min(n + 2, steps - 1), page);
+        page = page_of(min(n + 3, steps - 1));
         // this tile's flags are clear again before the tile after the next sets them
-        if (n + 2 < steps) {
-            bool any = false;
-#pragma unroll
-            for (int gr = 0; gr < G; ++gr) any |= t.not_finite[gr] != 0;
-            if (any) {
-                __syncthreads();
-                if (threadIdx.x < G) t.not_finite[threadIdx.x] = 0;
-            }
+        if (flags) {
+            __syncthreads();
+            if (threadIdx.x < G) t.not_finite[threadIdx.x] = 0;
         }
     }
 
     l += __shfl_xor(l, 32, 64);
     if (!live) return;
     // value 4 q + e of block i: 32 i + 8 q + 4 hf + e
-    if (a.chunks == 1) {
+    // the pieces of a tile that fit one need no join
+    if (a.pieces == 1 || piece >= last_row.hi - begin) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         uint16_t* p = (uint16_t*)a.out.p + (token * a.out.token + qh * a.out.head + 4 * hf);
 #pragma unroll
@@ -386,7 +376,7 @@ __global__ __launch_bounds__(64 * W, 1) void kv_attend_tiles(AttendArgs a) {
         if (a.lse && hf == 0)
             a.lse[(size_t)token * a.heads + qh] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
     } else {
-        const size_t at = ((size_t)token * a.heads + qh) * a.chunks + part;
+        const size_t at = ((size_t)token * a.heads + qh) * a.pieces + part;
         float* dst = a.tile_po + at * DIM + 4 * hf;
 #pragma unroll
         for (int i = 0; i < O; ++i)
@@ -397,67 +387,65 @@ __global__ __launch_bounds__(64 * W, 1) void kv_attend_tiles(AttendArgs a) {
     }
 }
 
-// The chunks of one row, by one wave: out = sum_c o_c 2^(m_c - m) / sum_c l_c 2^(m_c - m), in the order of the chunks.
+// The pieces of a row: out = sum_c o_c 2^(m_c - m) / sum_c l_c 2^(m_c - m), in the order of the pieces. DIM / 4 lanes to a
+// row, four values each. Bound by the latency of its chain of reads (lengths, then statistics, then partial outputs).
 template <int DIM>
 __global__ __launch_bounds__(256) void kv_attend_tiles_join(AttendArgs a) {
-    constexpr int V = DIM / 64;
-    typedef float vec __attribute__((ext_vector_type(V)));
-    const uint32_t lane = threadIdx.x & 63;
-    uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const uint32_t qh = id % a.heads;
-    id /= a.heads;
-    const uint32_t qi = id % a.max_query, b = id / a.max_query;
-    if (b >= a.batch) return;
-    const kv::Request r = request_of(a, b);
-    const uint32_t rows = (uint32_t)r.q_len * a.ratio;
-    if ((int32_t)qi >= r.q_len || rows <= a.row_limit) return;
-    const uint32_t token = (uint32_t)r.first + qi, row0 = (qi * a.ratio + qh % a.ratio) / a.tile_rows * a.tile_rows;
-    // the chunks that hold a key of the row's tile: exactly those its workgroups wrote
+    constexpr uint32_t L = DIM / 4;
+    const uint32_t lane = threadIdx.x & 63, id = blockIdx.x * (256 / L) + threadIdx.x / L, d = threadIdx.x % L * 4;
+    const uint32_t token = min(id / a.heads, a.tokens - 1), qh = id % a.heads;
+    // the request of the token: the last that starts at or before it (the wave's rows may be of several tokens)
+    uint32_t before = 0;
+    const uint32_t low = (uint32_t)__builtin_amdgcn_readfirstlane((int)token);
+    for (uint32_t b0 = 0; b0 < a.batch; b0 += 64) {
+        const uint64_t here = __ballot(b0 + lane < a.batch && a.query_start[b0 + lane] <= (int32_t)low);
+        before += (uint32_t)__popcll((unsigned long long)here);
+        if (~here) break;
+    }
+    while (before < a.batch && a.query_start[before] <= (int32_t)token) ++before;
+    if (before == 0 || id / a.heads >= a.tokens) return;
+    const kv::Request r = request_of(a, before - 1);
+    const uint32_t rows = (uint32_t)r.q_len * a.ratio, qi = token - (uint32_t)r.first;
+    if ((int32_t)token < r.first || qi >= (uint32_t)r.q_len || rows <= a.row_limit) return;
+    const uint32_t row0 = (qi * a.ratio + qh % a.ratio) / kv::kTileRows * kv::kTileRows;
+    // the row's tile, its keys and its pieces, as kv_attend_tiles has them
     const kv::Range top_row = kv::visible((int32_t)(row0 / a.ratio), r.q_len, r.kv_len, a.causal, a.window);
-    const kv::Range last_row = kv::visible((int32_t)((min(row0 + a.tile_rows, rows) - 1) / a.ratio), r.q_len, r.kv_len, a.causal,
-                                           a.window);
-    const uint32_t c0 = (uint32_t)(top_row.lo & ~(kKeys - 1)) / a.chunk;
-    const uint32_t c1 = last_row.hi > (top_row.lo & ~(kKeys - 1)) ? ((uint32_t)last_row.hi + a.chunk - 1) / a.chunk : c0;
-    const size_t base = ((size_t)token * a.heads + qh) * a.chunks;
+    const kv::Range last_row = kv::visible((int32_t)((min(row0 + kv::kTileRows, rows) - 1) / a.ratio), r.q_len, r.kv_len,
+                                           a.causal, a.window);
+    const int32_t range = last_row.hi - (top_row.lo & ~(kKeys - 1)), piece = kv::piece_keys(range, a.pieces);
+    if (piece >= range) return;  // its tile wrote it
+    const uint32_t parts = (uint32_t)(range + piece - 1) / (uint32_t)piece;
+    const size_t base = ((size_t)token * a.heads + qh) * a.pieces;
     float m = kNone;
-    for (uint32_t c = c0 + lane; c < c1; c += 64) m = fmaxf(m, a.tile_pml[base + c].x);
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-    vec sum = 0.0f;
+    for (uint32_t c = 0; c < parts; ++c) m = fmaxf(m, a.tile_pml[base + c].x);
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     float l = 0.0f;
 #pragma unroll 4
-    for (uint32_t c = c0; c < c1; ++c) {
+    for (uint32_t c = 0; c < parts; ++c) {
         const float2 v = a.tile_pml[base + c];
         const float f = __builtin_amdgcn_exp2f(v.x - m);
         l = fmaf(v.y, f, l);
-        sum += *(const vec*)(a.tile_po + (base + c) * DIM + V * lane) * f;
+        sum += *(const f32x4*)(a.tile_po + (base + c) * DIM + d) * f;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* p = (uint16_t*)a.out.p + (token * a.out.token + qh * a.out.head + V * lane);
-#pragma unroll
-    for (int e = 0; e < V; ++e) p[e] = a.is_bf16 ? f32_to_bf16_bits(sum[e] * inv) : f32_to_f16_bits(sum[e] * inv);
-    if (a.lse && lane == 0) a.lse[(size_t)token * a.heads + qh] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+    const float y[4] = {sum[0], sum[1], sum[2], sum[3]};
+    uint16_t* p = (uint16_t*)a.out.p + (token * a.out.token + qh * a.out.head + d);
+    store_out<4>(p, a.out.vec, a.is_bf16, y, l == 0.0f ? 0.0f : 1.0f / l);
+    if (a.lse && d == 0) a.lse[(size_t)token * a.heads + qh] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-template <int DIM, int G, int W>
+template <int DIM, int G>
 stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
-    const uint64_t blocks = (uint64_t)a.cache.kv_heads * a.tiles * a.batch * a.chunks;
+    const uint64_t blocks = (uint64_t)a.cache.kv_heads * a.tiles * a.batch * a.pieces;
     if (blocks >= 1ull << 22) return STARK_QMM_UNSUPPORTED;
-    hipLaunchKernelGGL((kv_attend_tiles<DIM, G, W>), dim3((uint32_t)blocks), dim3(64 * W), 0, s, a);
+    hipLaunchKernelGGL((kv_attend_tiles<DIM, G>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
     QMM_HIP_CHECK(hipGetLastError());
-    if (a.chunks > 1) {
-        const uint64_t joins = ((uint64_t)a.heads * a.max_query * a.batch + 3) / 4;
+    if (a.pieces > 1) {
+        const uint64_t each = 1024 / DIM, joins = ((uint64_t)a.heads * a.tokens + each - 1) / each;
         if (joins >= 1ull << 24) return STARK_QMM_UNSUPPORTED;
         hipLaunchKernelGGL((kv_attend_tiles_join<DIM>), dim3((uint32_t)joins), dim3(256), 0, s, a);
         QMM_HIP_CHECK(hipGetLastError());
     }
     return STARK_QMM_OK;
-}
-
-template <int DIM, int G>
-stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
-    if (DIM != 256 && a.tile_rows == 256) return launch<DIM, G, DIM == 256 ? 4 : 8>(a, s);
-    return launch<DIM, G, 4>(a, s);
 }
 
 }  // namespace

@@ -1,4 +1,6 @@
 // Entry points of attention over the 4-bit paged key/value cache: checks, and which kernel takes which requests.
+#include <atomic>
+
 #include "kv_attend.h"
 
 namespace {
@@ -25,7 +27,7 @@ stark_qmm_status check(const stark_qmm_kv_attention_args* p, AttendArgs* a) {
     a->max_query = std::min(p->max_query, p->tokens);
     a->max_kv = std::min(p->max_kv, p->table_stride * p->cache.page_size);
     // steps of a call are counted in 31 bits
-    if ((uint64_t)a->batch * a->cache.kv_heads * (a->max_kv / 32 + 2ull) >= 1ull << 31) return STARK_QMM_UNSUPPORTED;
+    if ((uint64_t)a->batch * a->cache.kv_heads * 4 * (a->max_kv / 32 + 20ull) >= 1ull << 31) return STARK_QMM_UNSUPPORTED;
     a->is_bf16 = p->data_type == STARK_QMM_BF16;
     a->causal = p->causal != 0, a->window = (int32_t)std::min(p->window, 0x7fffffffu);
     const float scale = p->scale == 0.0f ? 1.0f : fabsf(p->scale);
@@ -35,25 +37,42 @@ stark_qmm_status check(const stark_qmm_kv_attention_args* p, AttendArgs* a) {
     return STARK_QMM_OK;
 }
 
+// Compute units of the current device, asked for once.
+stark_qmm_status compute_units(uint32_t* cus) {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    QMM_HIP_CHECK(hipGetDevice(&dev));
+    int n = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+    if (n == 0) {
+        QMM_HIP_CHECK(hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev));
+        if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
+    }
+    *cus = (uint32_t)n;
+    return STARK_QMM_OK;
+}
+
 // How the checked call's work is dealt, and the bytes that its partial results need.
 stark_qmm_status plan_work(AttendArgs* a, uint64_t* workspace) {
-    int dev = 0, cus = 0;
-    QMM_HIP_CHECK(hipGetDevice(&dev));
-    QMM_HIP_CHECK(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
-    a->row_limit = kv::row_limit(a->batch, a->max_query, a->ratio);
+    uint32_t cus = 0;
+    const stark_qmm_status st = compute_units(&cus);
+    if (st != STARK_QMM_OK) return st;
+    const kv::Rows rows = kv::row_limit(a->batch, a->max_query, a->ratio, a->max_kv);
+    const uint64_t most = (uint64_t)a->max_query * a->ratio;
+    a->row_limit = std::min<uint64_t>(rows.limit, most), a->row_block = rows.block;
     *workspace = 0;
     if (a->row_limit) {
         a->ratio_inverse = (65535 + a->ratio) / a->ratio;
-        const kv::Share w = kv::share(a->batch, a->cache.kv_heads, a->max_kv, (uint32_t)cus * (a->cache.dim == 256 ? 1 : 2));
+        const uint32_t blocks = (a->row_limit + a->row_block - 1) / a->row_block;
+        const kv::Share w = kv::share(a->batch, a->cache.kv_heads * blocks, a->max_kv,
+                                      cus * (a->cache.dim == 256 ? 1 : 2));
         a->whole = w.whole, a->grid = w.grid;
         a->inverse = w.grid > 1 ? (uint32_t)((1ull << 32) / w.grid) : 0xffffffffu;
         if (!w.whole) *workspace = (uint64_t)w.grid * (2 * kRows * (a->cache.dim * 4ull + 8) + 16);
     }
-    const uint64_t most = (uint64_t)a->max_query * a->ratio;
     if (most > a->row_limit) {
-        const kv::Tiling t = kv::tiling(a->batch, a->cache.kv_heads, most, a->max_kv, (uint32_t)cus, a->cache.dim != 256);
-        a->tile_rows = t.rows, a->tiles = t.tiles, a->chunk = t.chunk, a->chunks = t.chunks;
-        if (t.chunks > 1) *workspace += (uint64_t)a->tokens * a->heads * t.chunks * (a->cache.dim * 4ull + 8);
+        const kv::Tiling t = kv::tiling(a->batch, a->cache.kv_heads, (uint64_t)a->tokens * a->ratio, most, a->max_kv, cus);
+        a->tiles = t.tiles, a->pieces = t.pieces;
+        if (t.pieces > 1) *workspace += (uint64_t)a->tokens * a->heads * t.pieces * (a->cache.dim * 4ull + 8);
     }
     return STARK_QMM_OK;
 }
@@ -100,7 +119,7 @@ stark_qmm_status stark_qmm_kv_attention(const stark_qmm_kv_attention_args* p, vo
             p0 = (uint8_t*)(a.pml + 2ull * a.grid * kRows);
         }
         a.tile_po = (float*)p0;
-        a.tile_pml = (float2*)(a.tile_po + (uint64_t)a.tokens * a.heads * a.chunks * a.cache.dim);
+        a.tile_pml = (float2*)(a.tile_po + (uint64_t)a.tokens * a.heads * a.pieces * a.cache.dim);
     }
     const hipStream_t s = (hipStream_t)stream;
     if (a.row_limit) {

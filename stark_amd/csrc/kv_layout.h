@@ -98,13 +98,21 @@ KV_HD Range request_range(int32_t q_len, int32_t kv_len, bool causal, int32_t wi
     return {visible(0, q_len, kv_len, causal, window).lo, visible(q_len - 1, q_len, kv_len, causal, window).hi};
 }
 
-// Most rows (a kv head's query heads times new tokens) of a request that the decode kernel takes in a call: 4, 8 or 16, by
-// what the bounds say that any request has; in a call of longer requests, what one new token has (decode rows among
-// prompts), or 0 where there is one request. The others go to the tile kernel.
-KV_HD uint32_t row_limit(uint32_t batch, uint32_t max_query, uint32_t ratio) {
+// Requests that the decode kernel takes in a call: those of up to `limit` rows (a kv head's query heads times new tokens),
+// in blocks of `block` rows (4, 8 or 16). Where the bounds say that no request has more than 64 rows it takes all; in a
+// call of longer requests those of one block, which has what one new token has (decode rows among prompts), where there
+// may be enough of them to pay for two more launches (a prompt with 8 decode rows of 2000 keys 59 us with them, 61 us
+// without; 8 of 200 keys 28 against 19; 16 of 300 keys 30 against 33; 8 of 8000 keys 98 against 171), else none (0). The
+// others go to the tile kernel.
+struct Rows {
+    uint32_t limit, block;
+};
+KV_HD Rows row_limit(uint32_t batch, uint32_t max_query, uint32_t ratio, uint32_t max_kv) {
     const uint64_t most = (uint64_t)max_query * ratio;
-    const uint64_t rows = most <= 16 ? most : batch > 1 ? ratio : 17;
-    return rows <= 4 ? 4 : rows <= 8 ? 8 : rows <= 16 ? 16 : 0;
+    if (most <= 64) return {64, most <= 4 ? 4u : most <= 8 ? 8u : 16u};
+    if (ratio > 16 || (batch < 16 && (uint64_t)batch * max_kv < 49152) || batch == 1) return {0, 16};
+    const uint32_t block = ratio <= 4 ? 4 : ratio <= 8 ? 8 : 16;
+    return {block, block};
 }
 
 // Keys of a workgroup's least share of a decode call: one 64-key or two 32-key steps for each of its four waves.
@@ -134,25 +142,27 @@ KV_HD Share share(uint32_t batch, uint32_t kv_heads, uint32_t max_kv, uint32_t s
     return {0, most < slots ? (uint32_t)(most ? most : 1) : slots};
 }
 
-// Tiles of the tile kernel: 256 rows (eight waves) where a request may have as many and such tiles fill the GPU, else 128;
-// and chunks of the keys where the tiles do not fill it (two workgroups of four waves to a CU), of 512 keys at least.
+// Least keys of a piece of a row tile's keys.
+constexpr int32_t kPieceKeys = 256;
+
+// Keys of each of up to `pieces` pieces of a range: a multiple of 64, so that all pieces but the last are alike.
+KV_HD int32_t piece_keys(int32_t range, uint32_t pieces) {
+    const int64_t each = (((int64_t)range + pieces - 1) / pieces + 63) / 64 * 64;
+    return (int32_t)(each < kPieceKeys ? kPieceKeys : each > 0x7fffffc0 ? 0x7fffffc0 : each);
+}
+
+constexpr uint32_t kTileRows = 128;  // of the tile kernel
+
+// Row tiles of the tile kernel: how many a request has at most, and how many pieces the keys of a tile are cut into where
+// the tiles do not fill the GPU (two workgroups to a CU): into twice as many workgroups, for each request's last tile is
+// rarely full. `rows` is what the call's query rows come to on one kv head.
 struct Tiling {
-    uint32_t rows, tiles, chunk, chunks;
+    uint32_t tiles, pieces;
 };
-KV_HD Tiling tiling(uint32_t batch, uint32_t kv_heads, uint64_t most_rows, uint32_t max_kv, uint32_t cus, bool eight) {
-    const uint64_t units = (uint64_t)batch * kv_heads, wide = units * ((most_rows + 255) / 256);
-    Tiling t;
-    t.rows = eight && wide >= cus ? 256 : 128;
-    t.tiles = (uint32_t)((most_rows + t.rows - 1) / t.rows);
-    const uint64_t have = units * t.tiles, slots = 2ull * cus;
-    uint64_t parts = t.rows == 256 || have >= slots ? 1 : (slots + have - 1) / have;
-    const uint64_t longest = (max_kv + 511) / 512;
-    if (parts > longest) parts = longest ? longest : 1;
-    t.chunk = (uint32_t)((max_kv + parts - 1) / parts + 63) / 64 * 64;
-    if (t.chunk == 0) t.chunk = 64;
-    t.chunks = (uint32_t)(((uint64_t)max_kv + t.chunk - 1) / t.chunk);
-    if (t.chunks == 0) t.chunks = 1;
-    return t;
+KV_HD Tiling tiling(uint32_t batch, uint32_t kv_heads, uint64_t rows, uint64_t most_rows, uint32_t max_kv, uint32_t cus) {
+    const uint64_t have = kv_heads * (rows / kTileRows + batch), want = have >= 2ull * cus ? 1 : (4ull * cus + have - 1) / have;
+    const uint64_t longest = ((uint64_t)max_kv + kPieceKeys - 1) / kPieceKeys;
+    return {(uint32_t)((most_rows + kTileRows - 1) / kTileRows), (uint32_t)(want < longest ? want : longest ? longest : 1)};
 }
 
 }  // namespace kv

@@ -40,7 +40,11 @@ void share(uint32_t batch, uint32_t heads, uint32_t max_kv, uint32_t slots, uint
 uint32_t share_of(uint32_t total, uint32_t grid, uint32_t keys) {
     return kv::share_of(total, grid, grid > 1 ? (uint32_t)((1ull << 32) / grid) : 0xffffffffu, keys);
 }
-uint32_t row_limit(uint32_t b, uint32_t q, uint32_t r) { return kv::row_limit(b, q, r); }
+void row_limit(uint32_t b, uint32_t q, uint32_t r, uint32_t kv, uint32_t* o) { const kv::Rows x = kv::row_limit(b, q, r, kv); o[0] = x.limit; o[1] = x.block; }
+int32_t piece_keys(int32_t range, uint32_t pieces) { return kv::piece_keys(range, pieces); }
+void tiling(uint32_t batch, uint32_t heads, uint64_t rows, uint64_t most, uint32_t max_kv, uint32_t cus, uint32_t* o) {
+    const kv::Tiling t = kv::tiling(batch, heads, rows, most, max_kv, cus); o[0] = t.tiles; o[1] = t.pieces;
+}
 uint32_t unit_keys() { return kv::kUnitKeys; }
 }
 """
@@ -161,11 +165,29 @@ def test_shares_cover_every_step():
 
 
 def test_row_limits():
-    """Which requests the decode kernel takes: by the rows that a kv head's query heads and the new tokens make."""
-    for batch, query, ratio, want in ((1, 1, 4, 4), (1, 2, 4, 8), (9, 3, 4, 16), (1, 4, 4, 16), (1, 5, 4, 0), (2, 5, 4, 4),
-                                      (2, 100, 7, 8), (2, 100, 16, 16), (2, 100, 17, 0), (5, 1, 20, 0), (1, 16, 1, 16),
-                                      (1, 17, 1, 0), (3, 17, 1, 4)):
-        assert rules().row_limit(batch, query, ratio) == want, (batch, query, ratio)
+    """Which requests the decode kernel takes, and in what blocks: by the rows that a kv head's query heads and the new
+    tokens make."""
+    for batch, query, ratio, kv, want in (
+            (1, 1, 4, 9, (64, 4)), (1, 2, 4, 9, (64, 8)), (9, 3, 4, 9, (64, 16)), (1, 16, 4, 9, (64, 16)),
+            (1, 17, 4, 10 ** 6, (0, 16)), (2, 17, 4, 30000, (4, 4)), (2, 17, 4, 20000, (0, 16)), (16, 100, 7, 9, (8, 8)),
+            (15, 100, 7, 9, (0, 16)), (20, 100, 16, 9, (16, 16)), (20, 100, 17, 9, (0, 16)), (5, 1, 20, 9, (64, 16)),
+            (5, 1, 65, 10 ** 6, (0, 16)), (30, 65, 1, 9, (4, 4))):
+        assert _out(rules().row_limit, 2, batch, query, ratio, kv, kind=C.c_uint32) == want, (batch, query, ratio)
+
+
+def test_pieces_cover_a_tile_and_fill_the_gpu():
+    r = random.Random(9)
+    for _ in range(300):
+        keys, pieces = r.randint(1, 200000), r.randint(1, 64)
+        each = rules().piece_keys(keys, pieces)
+        assert each % 64 == 0 and each >= 256 and each * pieces >= keys
+    assert rules().piece_keys(2 ** 31 - 1, 2) * 2 >= 2 ** 31 - 1
+    t = rules().tiling
+    t.argtypes = [C.c_uint32, C.c_uint32, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p]
+    assert _out(t, 2, 1, 8, 2048 * 4, 2048 * 4, 6144, 256, kind=C.c_uint32) == (64, 1)
+    assert _out(t, 2, 1, 1, 300, 300, 100000, 256, kind=C.c_uint32)[1] == 342
+    assert _out(t, 2, 1, 1, 300, 300, 300, 256, kind=C.c_uint32)[1] == 2
+    assert _out(t, 2, 4, 2, 0, 100, 0, 256, kind=C.c_uint32)[1] == 1
 
 
 def _geometry(**kw):
