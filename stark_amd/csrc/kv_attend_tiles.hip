@@ -12,12 +12,15 @@ constexpr int kKeys = 64;  // keys of a tile: four records
 // LDS of one tile: keys [key][value of the head], values transposed [value of the head][key], both f16 in 16-byte pieces
 // whose place in a row is swizzled by the row, so that 16 lanes that read the same piece of 16 rows meet no bank twice.
 // not_finite: keys (bits) whose values' planes are not finite, for each group; they stand as zeros in v.
-template <int DIM, int G>
+// EXACT: keys are their codes less 8, and planes holds scales and middles (the value of code 8) of the keys, [group][scale
+// or middle][key].
+template <int DIM, int G, bool EXACT>
 struct Tile {
     u32x4 k[kKeys][DIM / 8];
     u32x4 v[DIM][kKeys / 8];
     unsigned long long not_finite[G];
     alignas(16) uint32_t absent[4];  // records whose page is not in the cache
+    alignas(16) float planes[EXACT ? G : 1][2][EXACT ? kKeys : 4];
     static QMM_DEVICE uint32_t key_piece(uint32_t key, uint32_t piece) {
         return piece ^ (DIM >= 128 ? key & 15 : key >> 1 & 7);
     }
@@ -36,6 +39,11 @@ QMM_DEVICE float max3(float a, float b, float c) {
 QMM_DEVICE uint32_t two_values(uint32_t w, f16x2 s, f16x2 b) {
     const f16x2 c = half2_of(and_or(w, 0x000f000fu, 0x64006400u)) - (f16x2){(_Float16)1024.0f, (_Float16)1024.0f};
     return bits_of(__builtin_elementwise_fma(c, s, b));
+}
+
+// Two codes less 8, exact.
+QMM_DEVICE uint32_t two_codes(uint32_t w) {
+    return bits_of(half2_of(and_or(w, 0x000f000fu, 0x64006400u)) - (f16x2){(_Float16)1032.0f, (_Float16)1032.0f});
 }
 
 // What one thread brings of a tile: of one record, a lane's key words and value words, and their planes.
@@ -69,18 +77,29 @@ struct Codes {
         for (int gr = 0; gr < G; ++gr) vp[gr] = *(const u32x4*)(rec + 16 * DIM + 64 * G + 64 * gr + 16 * (lane >> 4));
     }
     // record: 0 .. 3 in the tile
-    QMM_DEVICE void write_keys(Tile<DIM, G>& t, uint32_t record, uint32_t lane) const {
+    template <bool EXACT>
+    QMM_DEVICE void write_keys(Tile<DIM, G, EXACT>& t, uint32_t record, uint32_t lane) const {
         const uint32_t key = 16 * record + (lane & 15), g = lane >> 4;
 #pragma unroll
         for (int j = 0; j < N; ++j) {  // word 4 j + g: values 8 (4 j + g) .. + 7, of group j G / N
             const f16x2 plane = half2_of(kp[j * G / N]), s = {plane[0], plane[0]}, b = {plane[1], plane[1]};
             const uint32_t w = kc[j];
-            t.k[key][t.key_piece(key, 4 * j + g)] = u32x4{two_values(w, s, b), two_values(w >> 4, s, b),
-                                                          two_values(w >> 8, s, b), two_values(w >> 12, s, b)};
+            t.k[key][t.key_piece(key, 4 * j + g)] =
+                EXACT ? u32x4{two_codes(w), two_codes(w >> 4), two_codes(w >> 8), two_codes(w >> 12)}
+                      : u32x4{two_values(w, s, b), two_values(w >> 4, s, b), two_values(w >> 8, s, b), two_values(w >> 12, s, b)};
+        }
+        if (EXACT) {
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr)
+                if ((int)g == gr % 4) {
+                    t.planes[gr][0][key] = plane_scale(kp[gr]);
+                    t.planes[gr][1][key] = plane_middle(kp[gr]);
+                }
         }
     }
     // live: bit e: the lane's token 4 (lane / 16) + e is a key of the request, in a page of the cache
-    QMM_DEVICE void write_values(Tile<DIM, G>& t, uint32_t record, uint32_t lane, uint32_t live) {
+    template <bool EXACT>
+    QMM_DEVICE void write_values(Tile<DIM, G, EXACT>& t, uint32_t record, uint32_t lane, uint32_t live) {
         const uint32_t r = lane & 15, quad = lane >> 4;
         u32x4 q[G];  // (copies: the loaded registers stay as they are, or the next load's would be copied, and waited for)
         uint32_t top = 0;
@@ -138,11 +157,16 @@ struct Codes {
 // Two tiles of LDS: the next tile is unpacked while this one is multiplied, and the one after that is in flight.
 // Bound by vector work beside the matrix cores: per 64 keys and 32 rows 64 products of 32x32x16 (1024 clocks) stand
 // against 32 exponentials (512 clocks), the maximum, conversion and sum (about 300), and the unpacking's share.
-template <int DIM, int G>
+// EXACT (f16 outputs, or with lse): the score products take the codes themselves, exact in f16, one accumulator a scale
+// group, and a key's planes are applied to the scores in f32, as in kv_attend_rows; and the sum is of the probabilities
+// before they are rounded. Keys rounded to f16 move a score by up to 2^-11 of scale |q| |k|, which bf16 outputs do not
+// show, but an f32 lse and f16 outputs do.
+template <int DIM, int G, bool EXACT>
 __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
     constexpr int J = DIM / 16;   // k blocks of a score product
     constexpr int O = DIM / 32;   // blocks of the output
-    __shared__ Tile<DIM, G> tiles[2];
+    using T = Tile<DIM, G, EXACT>;
+    __shared__ T tiles[2];
     const uint32_t lane = threadIdx.x & 63, col = lane & 31, hf = lane >> 5;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // workgroup: kv head first (workgroups are dealt to the XCDs in turn: a head's row tiles meet in one L2), then the
@@ -206,9 +230,9 @@ __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
         const int32_t left = r.kv_len - (int32_t)(t + 4 * (lane >> 4));
         live_keys = !in_cache || left <= 0 ? 0 : left >= 4 ? 15 : (1u << left) - 1;
     };
-    const auto unpack = [&](Tile<DIM, G>& t) {
-        codes.write_keys(t, record, lane);
-        codes.write_values(t, record, lane, live_keys);
+    const auto unpack = [&](T& t) {
+        codes.template write_keys<EXACT>(t, record, lane);
+        codes.template write_values<EXACT>(t, record, lane, live_keys);
         if (lane == 0) t.absent[record] = !in_cache;
     };
     if (threadIdx.x < 2 * G) tiles[threadIdx.x / G].not_finite[threadIdx.x % G] = 0;
@@ -220,7 +244,7 @@ __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
 
     // B operands of the score products: lane half hf holds values 8 (2 j + hf) .. + 7 of its row, in the pieces' order
     f16x8 qb[J];
-    float c1;
+    float c1, qsum[G];
     {
         const uint16_t* p = (const uint16_t*)a.q.p + (token * a.q.token + qh * a.q.head + 8 * hf);
         u32x4 w[J];
@@ -248,6 +272,16 @@ __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) qb[j][e] = (_Float16)(ldexp_f32(x[j][e / 2 + 4 * (e & 1)], k) * a.sign);
         c1 = ldexp_f32(a.scale, -k);  // positive: the sign is q's
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = gr * J / G; j < (gr + 1) * J / G; ++j)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sum += x[j][e];
+            sum += __shfl_xor(sum, 32, 64);
+            qsum[gr] = sum * a.sign * a.scale;
+        }
     }
 
     f32x16 o[O];
@@ -262,7 +296,7 @@ __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
     }
     for (int32_t n = 0; n < steps; ++n) {
         __syncthreads();
-        Tile<DIM, G>& t = tiles[n & 1];
+        T& t = tiles[n & 1];
         const int32_t t0 = from + kKeys * n;
         const u32x4 out = *(const u32x4*)t.absent;
         uint64_t set = 0;
@@ -273,12 +307,36 @@ __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
             f32x16 s[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                s[h] = f32x16{};
+                constexpr int A = EXACT ? G : 1;  // accumulators
+                f32x16 acc[A];
                 const uint32_t key = 32 * h + col;
 #pragma unroll
                 for (int j = 0; j < J; ++j) {
                     const f16x8 k = __builtin_bit_cast(f16x8, t.k[key][t.key_piece(key, 2 * j + hf)]);
-                    s[h] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[j], s[h], 0, 0, 0);
+                    f32x16& c = acc[j * A / J];
+                    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[j], j % (J / A) ? c : f32x16{}, 0, 0, 0);
+                }
+                if (EXACT) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        f32x4 y, z;
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr) {
+                            const uint32_t at = 32 * h + 8 * q + 4 * hf;
+                            const f32x4 scale = *(const f32x4*)&t.planes[EXACT ? gr : 0][0][EXACT ? at : 0];
+                            const f32x4 mid = *(const f32x4*)&t.planes[EXACT ? gr : 0][1][EXACT ? at : 0];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float v = acc[EXACT ? gr : 0][4 * q + e];
+                                y[e] = gr ? fmaf(scale[e], v, y[e]) : scale[e] * v;
+                                z[e] = gr ? fmaf(mid[e], qsum[gr], z[e]) : mid[e] * qsum[gr];
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[h][4 * q + e] = fmaf(y[e], c1, z[e]);
+                    }
+                } else {
+                    s[h] = acc[0];
                 }
             }
             // value i of block h: key 32 h + 8 (i / 4) + 4 hf + i % 4
@@ -288,9 +346,9 @@ __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i)
                         s[h][i] = a.cap - 2.0f * a.cap *
-                                              __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(s[h][i] * c1));
+                                              __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(EXACT ? s[h][i] : s[h][i] * c1));
             }
-            const float scale = a.cap != 0.0f ? 1.0f : c1;
+            const float scale = EXACT || a.cap != 0.0f ? 1.0f : c1;
             if (t0 < inner_lo || t0 + kKeys > inner_hi || (out[0] | out[1] | out[2] | out[3])) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -314,16 +372,19 @@ __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
 #pragma unroll
                 for (int i = 0; i < O; ++i) o[i] *= f;
             }
-            // probabilities to f16 (2^-11 of each); the sum is of the same rounded values
+            // probabilities to f16 (2^-11 of each); the sum is of the same rounded values, which takes half the instructions
+            // and leaves the average of a row unbiased
             uint32_t p[2][8];
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const f16x2 v = {(_Float16)__builtin_amdgcn_exp2f(fmaf(s[h][2 * i], scale, -m)),
-                                     (_Float16)__builtin_amdgcn_exp2f(fmaf(s[h][2 * i + 1], scale, -m))};
+                    const float even = __builtin_amdgcn_exp2f(fmaf(s[h][2 * i], scale, -m));
+                    const float odd = __builtin_amdgcn_exp2f(fmaf(s[h][2 * i + 1], scale, -m));
+                    const f16x2 v = {(_Float16)even, (_Float16)odd};
                     p[h][i] = bits_of(v);
-                    l = __builtin_amdgcn_fdot2(v, (f16x2){(_Float16)1.0f, (_Float16)1.0f}, l, false);
+                    if (EXACT) l += even + odd;
+                    else l = __builtin_amdgcn_fdot2(v, (f16x2){(_Float16)1.0f, (_Float16)1.0f}, l, false);
                 }
 #pragma unroll
             for (int i = 0; i < O; ++i) {
@@ -437,7 +498,8 @@ template <int DIM, int G>
 stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
     const uint64_t blocks = (uint64_t)a.cache.kv_heads * a.tiles * a.batch * a.pieces;
     if (blocks >= 1ull << 22) return STARK_QMM_UNSUPPORTED;
-    hipLaunchKernelGGL((kv_attend_tiles<DIM, G>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
+    if (a.lse || !a.is_bf16) hipLaunchKernelGGL((kv_attend_tiles<DIM, G, true>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((kv_attend_tiles<DIM, G, false>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
     QMM_HIP_CHECK(hipGetLastError());
     if (a.pieces > 1) {
         const uint64_t each = 1024 / DIM, joins = ((uint64_t)a.heads * a.tokens + each - 1) / each;

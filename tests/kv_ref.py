@@ -82,10 +82,11 @@ def attention(q, k, v, scale, causal, window, cap, wide):
 
     The bound. A score is a sum of dim products of f32 sums, each rounded by 2^-24 of the magnitudes M = scale |q| (|k|
     + range of k's codes), at most dim + 16 times, plus the exponential's argument (2^-24 of the score and of the
-    reference) and result (2^-22): d relative error of each probability. With `wide` keys are f16 before the product
-    (2^-11 of |k|, on scale |q| |k|). Then out moves by at most 2 d max|v|. A probability times a value's scale, or the
-    probability and the value, are rounded to f16 (2^-11 each; 2^-10 where the conversion truncates) beside magnitudes
-    A = sum p (|v| + range); sums are f32 over the keys."""
+    reference) and result (2^-22): d relative error of each probability. Then out moves by at most 2 d max|v|. A
+    probability times a value's scale is rounded to f16 (2^-11) beside magnitudes A = sum p (|v| + range); sums are f32
+    over the keys. `wide` 1, as for prompts: the probability and the value are each rounded to f16 instead. `wide` 2, as
+    for prompts in bf16 without lse: the key too, before the product (2^-11 of |k|, on scale |q| |k|), and the sum is of
+    the rounded probabilities."""
     rows, n, dim = q.shape
     keys = k.shape[0]
     pos = keys - rows + np.arange(rows)[:, None]
@@ -104,8 +105,8 @@ def attention(q, k, v, scale, causal, window, cap, wide):
     for h in range(n):
         with np.errstate(all="ignore"):
             x = q[:, h] @ k.T * scale
-            mag = scale * (np.abs(q[:, h]) @ np.abs(k.T) + np.abs(q[:, h]).sum(-1, keepdims=True) * reach)
-            wide_mag = scale * (np.abs(q[:, h]) @ np.abs(k.T)) * 2.0 ** -11 if wide else 0.0
+            mag = abs(scale) * (np.abs(q[:, h]) @ np.abs(k.T) + np.abs(q[:, h]).sum(-1, keepdims=True) * reach)
+            wide_mag = abs(scale) * (np.abs(q[:, h]) @ np.abs(k.T)) * 2.0 ** -11 if wide == 2 else 0.0
             if cap:
                 x = cap * np.tanh(x / cap)
         x = np.where(seen, x, -np.inf)
@@ -129,6 +130,6 @@ def attention(q, k, v, scale, causal, window, cap, wide):
                                                           (keys / 4 + 64) * 2.0 ** -24)
             lse[:, h] = np.where(any_seen, m + np.log(total), -np.inf)
             dlse[:, h] = d + (keys / 4 + 64) * 2.0 ** -24 + 2.0 ** -22 * (np.abs(m) + 4) + \
-                (2.0 ** -11 if wide else 0.0)
+                (2.0 ** -11 if wide == 2 else 0.0)
         out[:, h] = o
     return out, lse, tol, dlse

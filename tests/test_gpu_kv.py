@@ -323,6 +323,8 @@ class Served:
         self.lse = torch.full((tokens, heads), 9.0, device="cuda")
 
     def operator(self, **kw):
+        if not kw.pop("with_lse", True):
+            self.lse = None
         kw.setdefault("max_query", self.max_query)
         kw.setdefault("max_kv", self.max_kv)
         return self.K.KvAttention(self.cache, self.q, self.out, self.table, self.query_start, self.kv_lengths,
@@ -330,16 +332,17 @@ class Served:
 
     def check(self, causal=True, window=0, soft_cap=0.0, scale=None, hidden=None):
         """hidden: request -> keys whose page is not in the cache."""
-        q, k, v, out, lse = _np(self.q), _np(self.k), _np(self.v), _np(self.out), _np(self.lse)
+        q, k, v, out = _np(self.q), _np(self.k), _np(self.v), _np(self.out)
+        lse = None if self.lse is None else _np(self.lse)
         each, at, kat = q.shape[1] // self.kvh, 0, 0
+        wide = 0 if self.max_query * each <= 64 else 2 if lse is None and self.dtype == "bf16" else 1
         scale = self.dim ** -0.5 if scale is None else scale
         for b, (n, kv) in enumerate(self.requests):
             for h in range(self.kvh):
                 rows = q[at:at + n, h * each:(h + 1) * each]
                 want, wl, tol, dl = R.attention(rows, k[kat:kat + kv, h], v[kat:kat + kv, h], scale, causal, window,
-                                                soft_cap, wide=n * each > 16)
+                                                soft_cap, wide)
                 got = out[at:at + n, h * each:(h + 1) * each]
-                gl = lse[at:at + n, h * each:(h + 1) * each]
                 label = f"request {b} ({n} rows, {kv} keys) head {h}"
                 assert np.array_equal(np.isnan(got), np.isnan(want)), f"{label}: NaN pattern"
                 ok = ~np.isnan(want)
@@ -348,12 +351,15 @@ class Served:
                 bound = tol[ok] * 1.001 + R.EPS[self.dtype] * (np.abs(want[ok]) + tol[ok]) + 2.0 ** -25
                 assert (err <= bound).all(), f"{label}: off by {err.max()} (bound there {bound[np.argmax(err - bound)]})"
                 dead = np.isneginf(wl)
+                assert (got[dead] == 0).all()
+                if lse is None:
+                    continue
+                gl = lse[at:at + n, h * each:(h + 1) * each]
                 assert np.array_equal(np.isneginf(gl), dead), f"{label}: empty rows"
                 fin = ~dead & np.isfinite(wl)
                 assert (np.abs(gl[fin] - wl[fin]) <= dl[fin] + 2.0 ** -23 * np.abs(wl[fin])).all(), f"{label}: lse"
-                assert (got[dead] == 0).all()
             at, kat = at + n, kat + kv
-        assert (out[at:] == 9.0).all() and (lse[at:] == 9.0).all(), "rows behind the last request"
+        assert (out[at:] == 9.0).all() and (lse is None or (lse[at:] == 9.0).all()), "rows behind the last request"
 
 
 ATTEND = [
@@ -387,6 +393,14 @@ ATTEND = [
     ([(64, 1700)], 6, 1, 256, 32, 32, "f16", {}),
     ([(90, 1300)], 5, 1, 64, 64, 64, "bf16", dict(window=700)),
     ([(48, 48)], 40, 2, 128, 128, 16, "bf16", {}),
+    ([(40, 60), (70, 70)], 4, 2, 64, 32, 16, "bf16", {}),
+    ([(200, 333)], 2, 2, 64, 64, 32, "bf16", dict(soft_cap=8.0)),
+    ([(80, 100)], 8, 4, 128, 32, 16, "bf16", dict(scale=-0.3)),
+    ([(50, 77), (1, 5)], 8, 4, 128, 64, 16, "bf16", dict(scale=0.0)),
+    ([(2, 77)], 8, 4, 128, 64, 16, "bf16", dict(scale=-0.2)),
+    ([(90, 200)], 2, 1, 256, 128, 16, "bf16", {}),
+    ([(3, 100)] * 70 + [(1, 30)] * 3, 4, 2, 64, 32, 16, "bf16", {}),   # more requests than lanes
+    ([(1, 600)] * 300, 2, 1, 64, 64, 16, "f16", {}),
 ]
 
 
@@ -394,6 +408,16 @@ ATTEND = [
 def test_attention(K, requests, heads, kvh, dim, group, page, dtype, options):
     s = Served(K, len(requests) + heads + dim, requests, heads, kvh, dim, group, page, dtype, pad_tokens=3)
     s.operator(**options).encode()
+    torch.cuda.synchronize()
+    s.check(**options)
+
+
+@pytest.mark.parametrize("requests,heads,kvh,dim,group,page,dtype,options", [
+    c for c in ATTEND if c[6] == "bf16"])
+def test_attention_without_lse(K, requests, heads, kvh, dim, group, page, dtype, options):
+    """bf16 outputs alone: prompts round the keys to f16."""
+    s = Served(K, len(requests) + heads + dim, requests, heads, kvh, dim, group, page, dtype, pad_tokens=3)
+    s.operator(with_lse=False, **options).encode()
     torch.cuda.synchronize()
     s.check(**options)
 
@@ -494,7 +518,7 @@ def test_page_ids_outside_the_cache_hide_their_keys(K, rows):
     q, k, v, out = _np(s.q), _np(s.k), _np(s.v), _np(s.out)
     for h in range(2):
         want, _, tol, _ = R.attention(q[:rows, 2 * h:2 * h + 2], k[:200][keep][:, h], v[:200][keep][:, h], 128 ** -0.5, False, 0,
-                                      0.0, wide=rows > 1)
+                                      0.0, 1 if rows > 1 else 0)
         got = out[:rows, 2 * h:2 * h + 2]
         assert (np.abs(got - want) <= tol + R.EPS["bf16"] * (np.abs(want) + tol)).all()
     s.table[0, :13] = -5
@@ -581,7 +605,7 @@ def _serve_loop(K, steps, capture, stream):
             lengths[b] += n
             for h in range(kvh):
                 want, _, tol, _ = R.attention(rq[:, 4 * h:4 * h + 4], rows_k[b][:, h], rows_v[b][:, h], dim ** -0.5, True, 0,
-                                              0.0, wide=True)
+                                              0.0, 2)
                 err = np.abs(got[at:at + n, 4 * h:4 * h + 4] - want)
                 assert (err <= tol + R.EPS["bf16"] * (np.abs(want) + tol)).all(), (b, n, lengths[b], err.max())
             at += n
@@ -646,7 +670,7 @@ def test_a_cache_past_32_bits(K):
     torch.cuda.synchronize()
     sk, sv = R.stored(k, 64), R.stored(v, 64)
     for h in range(8):
-        want, _, tol, _ = R.attention(q[:, h:h + 1], sk[:, h], sv[:, h], 128 ** -0.5, True, 0, 0.0, wide=False)
+        want, _, tol, _ = R.attention(q[:, h:h + 1], sk[:, h], sv[:, h], 128 ** -0.5, True, 0, 0.0, 0)
         err = np.abs(_np(out)[:, h:h + 1] - want)
         assert (err <= tol + R.EPS["bf16"] * (np.abs(want) + tol)).all(), (h, err.max())
 
