@@ -119,59 +119,53 @@ struct Rotary {
     const int32_t* positions;
     uint64_t position_stride;
     uint32_t rows, pairs, axes, interleaved;
-    uint16_t axis8[16];  // the axes of eight pairs, two bits each
+    uint32_t one_axis;    // the eight pairs of each octet turn by one axis, and rows of the table are 16-byte aligned
+    uint16_t axis8[16];   // the axes of eight pairs, two bits each
 };
 
 struct AppendArgs {
     KvCache cache;
     KvRows q, q_out, k, v;
     const int32_t* slots;
-    uint32_t dt, tokens, heads;
+    uint32_t tokens, heads;
+    uint32_t sets;  // threads of a lane place that share a token's heads: set i takes heads i, i + sets, ...
     Rotary rot;
 };
 
-// Eight values of a row.
-QMM_DEVICE void load8(const KvRows& r, uint32_t dt, uint32_t token, uint32_t head, uint32_t d, float* x) {
-    const size_t at = (size_t)(token * r.token + head * r.head + d);
-    if (r.vec) {
-        if (dt == STARK_QMM_F32) {
-            const float4 *p = (const float4*)((const float*)r.p + at), a = p[0], b = p[1];
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        } else {
-            const u32x4 w = *(const u32x4*)((const uint16_t*)r.p + at);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const uint32_t h = e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
-                x[e] = dt == STARK_QMM_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
-            }
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = load_as_f32(r.p, dt, at + e);
-    }
-}
+// Eight neighbouring values of a row as they are stored. Rows of any alignment: the compiler makes one unaligned 16-byte
+// access of the elements.
+template <uint32_t DT>
+struct Eight {
+    static constexpr int kWords = DT == STARK_QMM_F32 ? 8 : 4;
+    uint32_t w[kWords];
 
-QMM_DEVICE void store8(const KvRows& r, uint32_t dt, uint32_t token, uint32_t head, uint32_t d, const float* x) {
-    const size_t at = (size_t)(token * r.token + head * r.head + d);
-    if (r.vec) {
-        if (dt == STARK_QMM_F32) {
-            float4* p = (float4*)((float*)r.p + at);
-            p[0] = float4{x[0], x[1], x[2], x[3]}, p[1] = float4{x[4], x[5], x[6], x[7]};
-        } else {
-            u32x4 w;
+    QMM_DEVICE void load(const KvRows& r, uint32_t token, uint32_t head, uint32_t d) {
+        const size_t at = (size_t)(token * r.token + head * r.head + d);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float a = x[2 * e], b = x[2 * e + 1];
-                w[e] = dt == STARK_QMM_BF16 ? f32_to_bf16_bits(a) | (uint32_t)f32_to_bf16_bits(b) << 16
-                                            : f32_to_f16_bits(a) | (uint32_t)f32_to_f16_bits(b) << 16;
-            }
-            *(u32x4*)((uint16_t*)r.p + at) = w;
+        for (int i = 0; i < kWords; ++i) {
+            if (DT == STARK_QMM_F32) w[i] = ((const uint32_t*)r.p)[at + i];
+            else w[i] = ((const uint16_t*)r.p)[at + 2 * i] | (uint32_t)((const uint16_t*)r.p)[at + 2 * i + 1] << 16;
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) store_from_f32((void*)r.p, dt, at + e, x[e]);
     }
-}
+    QMM_DEVICE void store(const KvRows& r, uint32_t token, uint32_t head, uint32_t d) const {
+        const size_t at = (size_t)(token * r.token + head * r.head + d);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (DT == STARK_QMM_F32) ((uint32_t*)r.p)[at + i] = w[i % kWords];
+            else ((uint16_t*)r.p)[at + i] = (uint16_t)(w[i / 2] >> (16 * (i % 2)));
+        }
+    }
+    QMM_DEVICE float get(int e) const {
+        if (DT == STARK_QMM_F32) return __uint_as_float(w[e]);
+        const uint32_t h = e & 1 ? w[e / 2] >> 16 : w[e / 2] & 0xffffu;
+        return DT == STARK_QMM_BF16 ? bf16_bits_to_f32(h) : f16_bits_to_f32(h);
+    }
+    QMM_DEVICE void set(int e, float a, float b) {  // values e and e + 1, e even
+        if (DT == STARK_QMM_F32) w[e] = __float_as_uint(a), w[e + 1] = __float_as_uint(b);
+        else if (DT == STARK_QMM_BF16) w[e / 2] = __builtin_bit_cast(uint32_t, bf16x2_t{(__bf16)a, (__bf16)b});
+        else w[e / 2] = f32_to_f16_bits(a) | (uint32_t)f32_to_f16_bits(b) << 16;
+    }
+};
 
 // f64 to f16 through f32, two roundings, as the conversion of a 64-bit tensor does it. The barrier keeps the compiler
 // from making one rounding of them.
@@ -181,123 +175,220 @@ QMM_DEVICE uint32_t f64_to_f16_bits(double v) {
     return f32_to_f16_bits(f);
 }
 
-QMM_DEVICE double shfl_xor_f64(double v, int mask) { return __shfl_xor(v, mask, 64); }
+// v / 15 as a division rounds it: a product with the nearest 1 / 15, off by a step at most, and one correction.
+QMM_DEVICE double fifteenth(double v) {
+    const double q = v * (1.0 / 15.0);
+    return fma(fma(-15.0, q, v), 1.0 / 15.0, q);
+}
 
-// One (token, head) row to DIM / 8 lanes of a wave, eight neighbouring values a lane: query heads first, then key
-// heads, then value heads. Arithmetic in f64: a rotated value a c - b s of f32 factors has exact products and one
-// rounding there, and codes, scales and biases come out as from exact arithmetic (an f32 quotient beside a half way
-// point would take the wrong code, one step of the group's range / 15). Decode steps are bound by the launch.
-template <int DIM>
+// The value of another lane of the 16 that share a register row: the lane that CTRL names (quad permutation, or the mirror
+// image of 8 or 16 lanes).
+template <int CTRL>
+QMM_DEVICE double lane_f64(double v) {
+    const uint2 w = __builtin_bit_cast(uint2, v);
+    return __builtin_bit_cast(double, uint2{(uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.x, CTRL, 0xf, 0xf, true),
+                                            (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.y, CTRL, 0xf, 0xf, true)});
+}
+template <int CTRL>
+QMM_DEVICE void widen_range(double& lo, double& hi) {
+    const double l = lane_f64<CTRL>(lo), h = lane_f64<CTRL>(hi);
+    lo = fmin(lo, l), hi = fmax(hi, h);
+}
+
+// A row (a head of a token) to DIM / 8 lanes of a wave, eight neighbouring values a lane; a thread does every sets-th
+// query head of its token, then key heads, then value heads, with one read of the rotation.
+// Keys in f64: a rotated value a c - b s of f32 factors has exact products and one rounding there, and codes, scales and
+// biases come out as from exact arithmetic (an f32 sum or quotient beside a half way point would take the wrong code, one
+// step of the group's range / 15). Queries in f32: they are rounded once more in any case.
+// Bound by latency and vector work together: 2048 tokens of 32 + 2 * 8 heads of 128 (44 MB, 9 us as a copy) take 14.2 us,
+// 178 vector instructions a wave and row (7 us) after three dependent reads (positions, rotation, rows). One row a thread
+// took 23 us and all rows as 2^17 or 2^19 threads 16 and 16.5.
+template <int DIM, uint32_t DT>
 __global__ __launch_bounds__(256) void kv_append(AppendArgs a) {
     constexpr uint32_t L = DIM / 8;  // lanes of a row
     const uint32_t heads = a.heads + 2 * a.cache.kv_heads;
-    const uint64_t item = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const uint32_t item = blockIdx.x * (256 / L) + threadIdx.x / L;  // below 2^24 * 32
     const uint32_t l = threadIdx.x % L, d = 8 * l;
-    if (item >= (uint64_t)a.tokens * heads) return;  // whole rows: the lanes of a row leave together
-    const uint32_t token = (uint32_t)(item / heads), h = (uint32_t)(item % heads);
-    const bool is_q = h < a.heads, is_v = h >= a.heads + a.cache.kv_heads;
-    const uint32_t head = is_q ? h : is_v ? h - a.heads - a.cache.kv_heads : h - a.heads;
-    const KvRows& src = is_q ? a.q : is_v ? a.v : a.k;
-    float x[8];
-    load8(src, a.dt, token, head, d, x);
-    double y[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = (double)x[e];
+    if (item >= a.tokens * a.sets) return;  // whole rows: the lanes of a row leave together
+    const uint32_t token = item / a.sets, set = item - token * a.sets;
     const uint32_t pairs = a.rot.pairs;
-    if (!is_v && d < 2 * pairs) {
-        // the rotation partner's values: the same eight (interleaved), or those half the rotated width away
-        const bool high = !a.rot.interleaved && d >= pairs;
+    const bool turns = d < 2 * pairs;
+    // the rotation partner's values: the same eight (interleaved), or those half the rotated width away
+    const bool high = !a.rot.interleaved && d >= pairs;
+    float2 cs[8];
+    if (turns && set < a.heads + a.cache.kv_heads) {
         const uint32_t p0 = a.rot.interleaved ? d / 2 : high ? d - pairs : d;  // this lane's first pair
         const uint32_t np = a.rot.interleaved ? 4 : 8;
-        float o[8];
-        if (!a.rot.interleaved) load8(src, a.dt, token, head, high ? d - pairs : d + pairs, o);
-        uint32_t axes = a.rot.axis8[p0 / 8] >> (2 * (p0 % 8));
-        float2 cs[8];
+        const uint32_t axes = a.rot.axis8[p0 / 8] >> (2 * (p0 % 8));
+        const float2 nan = {__builtin_nanf(""), __builtin_nanf("")};
+        uint32_t pos[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            cs[e] = float2{0.0f, 0.0f};
-            if ((uint32_t)e < np) {
-                const uint32_t pos = (uint32_t)a.rot.positions[(axes & 3) * a.rot.position_stride + token];
-                cs[e] = pos < a.rot.rows ? a.rot.table[(size_t)pos * pairs + p0 + e]
-                                         : float2{__builtin_nanf(""), __builtin_nanf("")};
-            }
-            axes >>= 2;
-        }
-        if (a.rot.interleaved) {
+        for (int e = 0; e < 8; ++e)
+            pos[e] = (uint32_t)a.rot.positions[(axes >> (2 * ((uint32_t)e < np ? e : 0)) & 3) * a.rot.position_stride + token];
+        if (a.rot.one_axis) {
+            const float4* row = (const float4*)(a.rot.table + (size_t)(pos[0] < a.rot.rows ? pos[0] : 0) * pairs + p0);
+            float4 v[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const double u = y[2 * e], v = y[2 * e + 1], c = cs[e].x, s = cs[e].y;
-                y[2 * e] = fma(u, c, -(v * s));
-                y[2 * e + 1] = fma(v, c, u * s);
-            }
+            for (int e = 0; e < 4; ++e) v[e] = row[(uint32_t)e < np / 2 ? e : 0];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) cs[2 * e] = float2{v[e].x, v[e].y}, cs[2 * e + 1] = float2{v[e].z, v[e].w};
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const double c = cs[e].x, s = high ? cs[e].y : -cs[e].y;
-                y[e] = fma(y[e], c, (double)o[e] * s);
-            }
+            for (int e = 0; e < 8; ++e)
+                cs[e] = a.rot.table[(size_t)(pos[e] < a.rot.rows ? pos[e] : 0) * pairs + p0 + ((uint32_t)e < np ? e : 0)];
         }
-    }
-    if (is_q) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = (float)y[e];
-        store8(a.q_out, a.dt, token, head, d, x);
-        return;
-    }
-    // group minimum and maximum; a value that the format does not hold makes the minimum -inf
-    double lo = y[0], hi = y[0];
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        lo = fmin(lo, y[e]), hi = fmax(hi, y[e]);
-        bad |= !(fabs(y[e]) <= (double)kv::kLimit);
-    }
-    if (bad) lo = -__builtin_inf();
-    const uint32_t gl = L / a.cache.groups;  // lanes of a group: 4, 8 or 16
-    for (uint32_t o = 1; o < gl; o <<= 1) lo = fmin(lo, shfl_xor_f64(lo, o)), hi = fmax(hi, shfl_xor_f64(hi, o));
-    bad = !(lo >= -(double)kv::kLimit);
-    const uint32_t sb = bad ? 0x7e00u : f64_to_f16_bits((hi - lo) / 15.0);
-    const uint32_t bb = bad ? 0x7e00u : f64_to_f16_bits(lo);
-    const double s = (double)f16_bits_to_f32(sb), b = (double)f16_bits_to_f32(bb);
-    uint32_t w = 0;
-    if (s > 0.0) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w |= (uint32_t)fmin(fmax(rint((y[e] - b) / s), 0.0), 15.0) << (4 * e);
+        for (int e = 0; e < 8; ++e)
+            if (pos[e] >= a.rot.rows) cs[e] = nan;
     }
     const uint32_t slot = (uint32_t)a.slots[token];
     const uint32_t page = slot >> a.cache.page_shift, page_size = 1u << a.cache.page_shift;
     const bool stored = page < a.cache.page_count;
     const uint32_t in_page = slot & (page_size - 1), t = in_page % kv::kTile;
-    uint8_t* rec = a.cache.data + kv::record_index(stored ? page : 0, a.cache.kv_heads, head, page_size, in_page) *
-                                      (uint64_t)a.cache.record;
-    const uint32_t half_rec = kv::codes_bytes(DIM) + kv::planes_bytes(a.cache.groups);
-    if (is_v) rec += half_rec;
-    if (stored && l % gl == 0)
-        *(uint32_t*)(rec + kv::codes_bytes(DIM) + kv::plane_word(t, l / gl)) = sb | bb << 16;
-    if (!is_v) {
-        if (stored) *(uint32_t*)(rec + kv::key_word(DIM, t, l)) = w;
-        return;
-    }
-    // value bytes: byte i of lane r is byte r % 4 of code word 4 i + r / 4 (of its half of the head)
-    const int row = (int)(threadIdx.x & 63) - (int)l;
-    if (DIM == 64) {
+    uint8_t* const in_cache = a.cache.data + (uint64_t)(stored ? page : 0) * a.cache.page_bytes + in_page / kv::kTile * a.cache.record;
+    const uint32_t half_rec = kv::codes_bytes(DIM) + kv::planes_bytes(a.cache.groups), gl = L / a.cache.groups;
+
+    // A row as this lane holds it: its own values, and its rotation partner's where they are elsewhere. The next row is
+    // read before this one is worked on.
+    struct Row {
+        Eight<DT> x, o;
+    };
+    const bool elsewhere = turns && !a.rot.interleaved;
+    const uint32_t od = high ? d - pairs : d + pairs;
+    auto fetch = [&](const KvRows& src, uint32_t head, bool partner) {
+        Row r;
+        r.x.load(src, token, head, d);
+        if (partner) r.o.load(src, token, head, od);
+        return r;
+    };
+    const uint32_t kvh = a.cache.kv_heads;
+    // Scale and bias of the lane's group into a record half, and the lane's eight codes.
+    auto quantise = [&](const double* y, uint8_t* rec) {
+        // group minimum and maximum; a value that the format does not hold makes the minimum -inf
+        double lo = y[0], hi = y[0];
+        bool bad = false;
 #pragma unroll
-        for (uint32_t j = 0; j < 2; ++j) {
-            const uint32_t r = 2 * l + j;
+        for (int e = 0; e < 8; ++e) {
+            lo = fmin(lo, y[e]), hi = fmax(hi, y[e]);
+            bad |= !(fabs(y[e]) <= (double)kv::kLimit);
+        }
+        if (bad) lo = -__builtin_inf();
+        widen_range<0xb1>(lo, hi);  // lanes 1 0 3 2, then 2 3 0 1: groups of 4 lanes
+        widen_range<0x4e>(lo, hi);
+        if (gl > 4) widen_range<0x141>(lo, hi);  // mirror of 8 lanes
+        if (gl > 8) widen_range<0x140>(lo, hi);  // mirror of 16
+        bad = !(lo >= -(double)kv::kLimit);
+        const uint32_t sb = bad ? 0x7e00u : f64_to_f16_bits(fifteenth(hi - lo));
+        const uint32_t bb = bad ? 0x7e00u : f64_to_f16_bits(lo);
+        const double s = (double)f16_bits_to_f32(sb), b = (double)f16_bits_to_f32(bb);
+        if (stored && l % gl == 0) *(uint32_t*)(rec + kv::codes_bytes(DIM) + kv::plane_word(t, l / gl)) = sb | bb << 16;
+        uint32_t w = 0;
+        if (s > 0.0) {
+            // The code is the nearest step, ties to even, of exact arithmetic. In f32 the quotient is off by less than
+            // 2^-18 of its 0 .. 16; where that could matter (within 2^-16 of half way between two codes) f64 decides.
+            const float inverse = __builtin_amdgcn_rcpf((float)s);
+            float far = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float t = (float)(y[e] - b) * inverse, n = rintf(t);
+                far = fmaxf(far, fabsf(t - n));
+                w |= (uint32_t)fminf(fmaxf(n, 0.0f), 15.0f) << (4 * e);
+            }
+            if (far > 0.5f - 0x1p-16f) {
+                w = 0;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w |= (uint32_t)fmin(fmax(rint((y[e] - b) / s), 0.0), 15.0) << (4 * e);
+            }
+        }
+        return w;
+    };
+    uint32_t h = set;
+    Row r;
+    if (h < a.heads) r = fetch(a.q, h, elsewhere);
+    for (; h < a.heads; h += a.sets) {
+        const Row now = r;
+        if (h + a.sets < a.heads) r = fetch(a.q, h + a.sets, elsewhere);
+        Eight<DT> y = now.x;
+        if (turns) {
+            if (a.rot.interleaved) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float u = now.x.get(2 * e), v = now.x.get(2 * e + 1), c = cs[e].x, s = cs[e].y;
+                    y.set(2 * e, fmaf(u, c, -(v * s)), fmaf(v, c, u * s));
+                }
+            } else {
+                float t[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) t[e] = fmaf(now.x.get(e), cs[e].x, now.o.get(e) * (high ? cs[e].y : -cs[e].y));
+#pragma unroll
+                for (int e = 0; e < 8; e += 2) y.set(e, t[e], t[e + 1]);
+            }
+        }
+        y.store(a.q_out, token, h, d);
+    }
+    h -= a.heads;
+    if (h < kvh) r = fetch(a.k, h, elsewhere);
+    for (; h < kvh; h += a.sets) {
+        const Row now = r;
+        if (h + a.sets < kvh) r = fetch(a.k, h + a.sets, elsewhere);
+        // (converted row by row: kept in f64 over the loop they cost a wave of four a SIMD)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) asm("" : "+v"(cs[e].x), "+v"(cs[e].y));
+        double y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = (double)now.x.get(e);
+        if (turns) {
+            if (a.rot.interleaved) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const double u = y[2 * e], v = y[2 * e + 1], c = cs[e].x, s = cs[e].y;
+                    y[2 * e] = fma(u, c, -(v * s));
+                    y[2 * e + 1] = fma(v, c, u * s);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const double c = cs[e].x, s = high ? cs[e].y : -cs[e].y;
+                    y[e] = fma(y[e], c, (double)now.o.get(e) * s);
+                }
+            }
+        }
+        uint8_t* rec = in_cache + (uint64_t)h * a.cache.head_bytes;
+        const uint32_t w = quantise(y, rec);
+        if (stored) *(uint32_t*)(rec + kv::key_word(DIM, t, l)) = w;
+    }
+    h -= kvh;
+    if (h < kvh) r.x.load(a.v, token, h, d);
+    for (; h < kvh; h += a.sets) {
+        const Eight<DT> now = r.x;
+        if (h + a.sets < kvh) r.x.load(a.v, token, h + a.sets, d);
+        double y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = (double)now.get(e);
+        uint8_t* rec = in_cache + (uint64_t)h * a.cache.head_bytes + half_rec;
+        const uint32_t w = quantise(y, rec);
+        // value bytes: byte i of lane r is byte r % 4 of code word 4 i + r / 4 (of its half of the head). The exchange is
+        // of all lanes of the row, whatever it holds.
+        const int row = (int)(threadIdx.x & 63) - (int)l;
+        if (DIM == 64) {
+#pragma unroll
+            for (uint32_t j = 0; j < 2; ++j) {
+                const uint32_t r = 2 * l + j;
+                uint32_t out = 0;
+#pragma unroll
+                for (uint32_t i = 0; i < 2; ++i)
+                    out |= ((uint32_t)__shfl((int)w, row + (int)(4 * i + r / 4), 64) >> (8 * (r % 4)) & 0xffu) << (8 * i);
+                if (stored) *(uint16_t*)(rec + kv::value_byte(DIM, t, 0, r, 0)) = (uint16_t)out;
+            }
+        } else {
+            const uint32_t r = l % 16, half = l / 16;
             uint32_t out = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < 2; ++i)
-                out |= ((uint32_t)__shfl((int)w, row + (int)(4 * i + r / 4), 64) >> (8 * (r % 4)) & 0xffu) << (8 * i);
-            if (stored) *(uint16_t*)(rec + kv::value_byte(DIM, t, 0, r, 0)) = (uint16_t)out;
+            for (uint32_t i = 0; i < 4; ++i)
+                out |= ((uint32_t)__shfl((int)w, row + (int)(16 * half + 4 * i + r / 4), 64) >> (8 * (r % 4)) & 0xffu)
+                       << (8 * i);
+            if (stored) *(uint32_t*)(rec + kv::value_byte(DIM, t, half, r, 0)) = out;
         }
-    } else {
-        const uint32_t r = l % 16, half = l / 16;
-        uint32_t out = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i)
-            out |= ((uint32_t)__shfl((int)w, row + (int)(16 * half + 4 * i + r / 4), 64) >> (8 * (r % 4)) & 0xffu)
-                   << (8 * i);
-        if (stored) *(uint32_t*)(rec + kv::value_byte(DIM, t, half, r, 0)) = out;
     }
 }
 
@@ -307,44 +398,56 @@ struct ReadArgs {
     KvCache cache;
     KvRows k, v;
     const int32_t* slots;
-    uint32_t dt, tokens;
+    uint32_t tokens, sets;
 };
 
-// Eight neighbouring values to a lane, as in kv_append. s * code + b: the product of an f16 scale and a code is
-// exact in f32, so each value is rounded once (twice to 16 bits). Bound by HBM writes.
-template <int DIM>
+// Eight neighbouring values of a head's key and value to a lane, and every sets-th head of a token to a thread. s * code
+// + b: the product of an f16 scale and a code is exact in f32, so each value is rounded once (twice to 16 bits). Bound by
+// HBM writes.
+template <int DIM, uint32_t DT>
 __global__ __launch_bounds__(256) void kv_read(ReadArgs a) {
     constexpr uint32_t L = DIM / 8;
-    const uint32_t heads = 2 * a.cache.kv_heads;
-    const uint64_t item = (uint64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
-    const uint32_t l = threadIdx.x % L;
-    if (item >= (uint64_t)a.tokens * heads) return;
-    const uint32_t token = (uint32_t)(item / heads), h = (uint32_t)(item % heads);
-    const bool is_v = h >= a.cache.kv_heads;
-    const uint32_t head = is_v ? h - a.cache.kv_heads : h;
-    const KvRows& dst = is_v ? a.v : a.k;
+    const uint32_t item = blockIdx.x * (256 / L) + threadIdx.x / L, l = threadIdx.x % L;
+    if (item >= a.tokens * a.sets) return;
+    const uint32_t token = item / a.sets, set = item - token * a.sets;
     const uint32_t slot = (uint32_t)a.slots[token];
     const uint32_t page = slot >> a.cache.page_shift, page_size = 1u << a.cache.page_shift;
-    if (!dst.p || page >= a.cache.page_count) return;
+    if (page >= a.cache.page_count) return;
     const uint32_t in_page = slot & (page_size - 1), t = in_page % kv::kTile;
-    const uint8_t* rec = a.cache.data + kv::record_index(page, a.cache.kv_heads, head, page_size, in_page) *
-                                            (uint64_t)a.cache.record;
-    if (is_v) rec += kv::codes_bytes(DIM) + kv::planes_bytes(a.cache.groups);
-    const uint32_t plane = *(const uint32_t*)(rec + kv::codes_bytes(DIM) + kv::plane_word(t, l * a.cache.groups / L));
-    const float s = f16_bits_to_f32(plane & 0xffffu), b = f16_bits_to_f32(plane >> 16);
-    uint32_t w = 0;
-    if (!is_v) {
-        w = *(const uint32_t*)(rec + kv::key_word(DIM, t, l));
-    } else {
-        const uint32_t half = l / 16, i = l % 16 / 4;
+    const uint8_t* const in_cache = a.cache.data + (uint64_t)page * a.cache.page_bytes + in_page / kv::kTile * a.cache.record;
+    const uint32_t half_rec = kv::codes_bytes(DIM) + kv::planes_bytes(a.cache.groups);
+    const uint32_t plane_at = kv::codes_bytes(DIM) + kv::plane_word(t, l * a.cache.groups / L);
+    const uint32_t key_at = kv::key_word(DIM, t, l);
+    const uint32_t value_at = DIM == 64 ? kv::value_byte(DIM, t, 0, 2 * l, 0) : kv::value_byte(DIM, t, l / 16, l % 16, 0);
+    const int row = (int)(threadIdx.x & 63) - (int)l;
+    auto write = [&](const KvRows& dst, uint32_t head, uint32_t w, uint32_t plane) {
+        const float s = f16_bits_to_f32(plane & 0xffffu), b = f16_bits_to_f32(plane >> 16);
+        Eight<DT> out;
 #pragma unroll
-        for (uint32_t m = 0; m < 4; ++m)
-            w |= (uint32_t)rec[kv::value_byte(DIM, t, half, 4 * (l % 4) + m, i)] << (8 * m);
+        for (int e = 0; e < 8; e += 2)
+            out.set(e, fmaf(s, (float)(w >> (4 * e) & 15u), b), fmaf(s, (float)(w >> (4 * e + 4) & 15u), b));
+        if (dst.p) out.store(dst, token, head, 8 * l);
+    };
+    for (uint32_t head = set; head < a.cache.kv_heads; head += a.sets) {
+        const uint8_t* rec = in_cache + (uint64_t)head * a.cache.head_bytes;
+        const uint32_t k = *(const uint32_t*)(rec + key_at), kp = *(const uint32_t*)(rec + plane_at);
+        uint32_t u;
+        if (DIM == 64)  // rows of 8 bytes for four tokens
+            u = *(const uint16_t*)(rec + half_rec + value_at) | (uint32_t)*(const uint16_t*)(rec + half_rec + value_at + 8) << 16;
+        else
+            u = *(const uint32_t*)(rec + half_rec + value_at);
+        const uint32_t vp = *(const uint32_t*)(rec + half_rec + plane_at);
+        write(a.k, head, k, kp);
+        // the value's bytes are spread as kv_append puts them: code byte m of lane l is byte i of word 4 (l % 4) + m
+        uint32_t v = 0;
+#pragma unroll
+        for (uint32_t m = 0; m < 4; ++m) {
+            const uint32_t from = DIM == 64 ? 2 * (l % 4) + m / 2 : l / 16 * 16 + 4 * (l % 4) + m;
+            const uint32_t byte = DIM == 64 ? 2 * (m % 2) + l / 4 : l % 16 / 4;
+            v |= ((uint32_t)__shfl((int)u, row + (int)from, 64) >> (8 * byte) & 0xffu) << (8 * m);
+        }
+        write(a.v, head, v, vp);
     }
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = fmaf(s, (float)(w >> (4 * e) & 15u), b);
-    store8(dst, a.dt, token, head, 8 * l, x);
 }
 
 // Rows of DIM / 8 lanes, 256 lanes a workgroup; the grid stays below 2^24 workgroups.
@@ -356,6 +459,25 @@ stark_qmm_status launch_rows(uint32_t dim, uint64_t rows, F launch) {
     launch(dim3((uint32_t)blocks));
     QMM_HIP_CHECK(hipGetLastError());
     return STARK_QMM_OK;
+}
+
+template <uint32_t DT>
+void append_launch(dim3 grid, hipStream_t s, const AppendArgs& a) {
+    if (a.cache.dim == 64) hipLaunchKernelGGL((kv_append<64, DT>), grid, dim3(256), 0, s, a);
+    else if (a.cache.dim == 128) hipLaunchKernelGGL((kv_append<128, DT>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((kv_append<256, DT>), grid, dim3(256), 0, s, a);
+}
+
+template <uint32_t DT>
+void read_launch(dim3 grid, hipStream_t s, const ReadArgs& a) {
+    if (a.cache.dim == 64) hipLaunchKernelGGL((kv_read<64, DT>), grid, dim3(256), 0, s, a);
+    else if (a.cache.dim == 128) hipLaunchKernelGGL((kv_read<128, DT>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((kv_read<256, DT>), grid, dim3(256), 0, s, a);
+}
+
+uint32_t sets_of(uint32_t tokens, uint32_t heads, uint32_t dim) {
+    const uint32_t each = kv::rows_each((uint64_t)tokens * heads * (dim / 8));
+    return (heads + each - 1) / each;
 }
 
 bool dt_ok(uint32_t dt) { return dt == STARK_QMM_F32 || dt == STARK_QMM_F16 || dt == STARK_QMM_BF16; }
@@ -421,10 +543,11 @@ stark_qmm_status stark_qmm_kv_append(const stark_qmm_kv_append_args* p, void* st
             r.table_rows > 0x7fffffffu || (r.axes > 1 && (r.position_stride < p->tokens || r.position_stride >> 32)))
             return STARK_QMM_INVALID_ARGUMENT;
         a.rot = Rotary{(const float2*)r.table, r.positions, r.axes > 1 ? r.position_stride : 0, r.table_rows,
-                       r.rotary_dim / 2, r.axes, r.interleaved != 0, {}};
+                       r.rotary_dim / 2, r.axes, r.interleaved != 0, kv_aligned(r.table, 16), {}};
         for (uint32_t i = 0; i < a.rot.pairs; ++i) {
             if (r.axis_of_pair[i] >= r.axes) return STARK_QMM_INVALID_ARGUMENT;
             a.rot.axis8[i / 8] |= (uint16_t)(r.axis_of_pair[i] << (2 * (i % 8)));
+            if (r.axis_of_pair[i] != r.axis_of_pair[i / 8 * 8]) a.rot.one_axis = 0;
         }
     }
     a.q = kv_rows(p->q, p->q_token_stride, p->q_head_stride, dt);
@@ -432,12 +555,13 @@ stark_qmm_status stark_qmm_kv_append(const stark_qmm_kv_append_args* p, void* st
     a.k = kv_rows(p->k, p->k_token_stride, p->k_head_stride, dt);
     a.v = kv_rows(p->v, p->v_token_stride, p->v_head_stride, dt);
     a.slots = p->slots;
-    a.dt = dt, a.tokens = p->tokens, a.heads = heads;
+    a.tokens = p->tokens, a.heads = heads;
+    a.sets = sets_of(p->tokens, heads + 2 * a.cache.kv_heads, dim);
     const hipStream_t s = (hipStream_t)stream;
-    return launch_rows(dim, (uint64_t)p->tokens * (heads + 2 * a.cache.kv_heads), [&](dim3 grid) {
-        if (dim == 64) hipLaunchKernelGGL(kv_append<64>, grid, dim3(256), 0, s, a);
-        else if (dim == 128) hipLaunchKernelGGL(kv_append<128>, grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL(kv_append<256>, grid, dim3(256), 0, s, a);
+    return launch_rows(dim, (uint64_t)p->tokens * a.sets, [&](dim3 grid) {
+        if (dt == STARK_QMM_F32) append_launch<STARK_QMM_F32>(grid, s, a);
+        else if (dt == STARK_QMM_F16) append_launch<STARK_QMM_F16>(grid, s, a);
+        else append_launch<STARK_QMM_BF16>(grid, s, a);
     });
 }
 
@@ -458,12 +582,13 @@ stark_qmm_status stark_qmm_kv_read(const stark_qmm_kv_read_args* p, void* stream
     a.k = kv_rows(p->k, p->k_token_stride, p->k_head_stride, dt);
     a.v = kv_rows(p->v, p->v_token_stride, p->v_head_stride, dt);
     a.slots = p->slots;
-    a.dt = dt, a.tokens = p->tokens;
+    a.tokens = p->tokens;
     const hipStream_t s = (hipStream_t)stream;
-    return launch_rows(dim, (uint64_t)p->tokens * 2 * a.cache.kv_heads, [&](dim3 grid) {
-        if (dim == 64) hipLaunchKernelGGL(kv_read<64>, grid, dim3(256), 0, s, a);
-        else if (dim == 128) hipLaunchKernelGGL(kv_read<128>, grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL(kv_read<256>, grid, dim3(256), 0, s, a);
+    a.sets = (a.cache.kv_heads + 1) / 2;
+    return launch_rows(dim, (uint64_t)p->tokens * a.sets, [&](dim3 grid) {
+        if (dt == STARK_QMM_F32) read_launch<STARK_QMM_F32>(grid, s, a);
+        else if (dt == STARK_QMM_F16) read_launch<STARK_QMM_F16>(grid, s, a);
+        else read_launch<STARK_QMM_BF16>(grid, s, a);
     });
 }
 

@@ -81,6 +81,13 @@ KV_HD Request request(int32_t start, int32_t end, int32_t kv_len, uint32_t token
     return {a, q, k};
 }
 
+// Rows that a thread of the append does, one after another, with one read of their rotation: one while there are fewer
+// than 2^18 threads (4 waves a SIMD, which is what its registers leave room for), and up to eight.
+KV_HD uint32_t rows_each(uint64_t threads) {
+    const uint64_t each = threads / (1u << 18);
+    return each < 1 ? 1 : each > 8 ? 8 : (uint32_t)each;
+}
+
 // Plan of one request: pages it holds before and after the step, of at most `width`.
 struct PagePlan {
     int32_t before, need;

@@ -174,12 +174,21 @@ def test_append_and_read(K, dim, group, kvh, heads, tokens, page, dtype, axes, r
     for got, w, n in zip(outs, want, "kv"):
         _same(_np(got), _round(w, "f32"), n)
     if heads:
-        # the rotated value is rounded once (to f32 first where the type is shorter)
-        _same(_np(q_out), _round(wq, dtype), "q")
+        # products and sum in f32 (2^-24 of each), then the type's own rounding; without a rotation the values as they are
+        near = 2.0 ** -23 * 2 * np.abs(q).max(-1, keepdims=True)
+
+        def same_q(got, label):
+            if not axes:
+                return _same(got, q, label)
+            assert (np.abs(got - wq) <= near + R.EPS[dtype] * (np.abs(wq) + near) + 2.0 ** -25).all(), label
+            if rd < dim:
+                _same(got[..., rd:], q[..., rd:], label)
+
+        same_q(_np(q_out), "q")
         if how != "heads":
             K.KvAppend(cache, dk, dv, _ints(slots), dq, dq, rotary=rot).encode()  # in place
             torch.cuda.synchronize()
-            _same(_np(dq), _round(wq, dtype), "q in place")
+            same_q(_np(dq), "q in place")
     for name in DT:
         one = torch.zeros(tokens, kvh, dim, dtype=DT[name], device="cuda")
         K.KvRead(cache, _ints(slots), None, one).encode()
