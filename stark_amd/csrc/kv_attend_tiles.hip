@@ -5,6 +5,7 @@ namespace {
 
 using namespace qmm;
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr int kKeys = 64;  // keys of a tile: four records
@@ -102,16 +103,21 @@ struct Codes {
     QMM_DEVICE void write_values(Tile<DIM, G, EXACT>& t, uint32_t record, uint32_t lane, uint32_t live) {
         const uint32_t r = lane & 15, quad = lane >> 4;
         u32x4 q[G];  // (copies: the loaded registers stay as they are, or the next load's would be copied, and waited for)
-        uint32_t top = 0;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) q[gr] = vp[gr];
+        if (__any(live != 15)) {
+#pragma unroll
+            for (int gr = 0; gr < G; ++gr)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[gr][e] = live >> e & 1 ? q[gr][e] : 0u;
+        }
+        u16x2 top = {0, 0};  // largest magnitude bits
 #pragma unroll
         for (int gr = 0; gr < G; ++gr)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                q[gr][e] = live >> e & 1 ? vp[gr][e] : 0u;
-                const uint32_t x = q[gr][e] & 0x7c007c00u;
-                top = max(top & 0x7c00u, x & 0x7c00u) | max(top & 0x7c000000u, x & 0x7c000000u);
-            }
-        if (__any((top & 0x7c00u) == 0x7c00u || top >> 16 == 0x7c00u)) {
+            for (int e = 0; e < 4; ++e)
+                top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, (uint32_t)(q[gr][e] & 0x7fff7fffu)));
+        if (__any(top[0] >= 0x7c00u || top[1] >= 0x7c00u)) {
 #pragma unroll
             for (int gr = 0; gr < G; ++gr)
 #pragma unroll
@@ -147,22 +153,39 @@ struct Codes {
     }
 };
 
+// Schedule: N matrix products, each operand read from LDS four products ahead.
+template <int N>
+QMM_DEVICE void read_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    }
+}
+
 // Prompts: tiles of 128 rows (a kv head's query heads times tokens, 32 to a wave) against tiles of 64 keys.
 //
 // The keys and values of a tile are made f16 values in LDS once for all four waves (2 packed operations a value); what that
 // rounds, 2^-12 of a value, is of the size of the probabilities' own rounding to f16. Scores come out transposed, from
 // v_mfma_f32_32x32x16_f16 with keys as rows and query rows as columns: a lane holds, of one row, 16 of each 32 keys, and
 // those are the second product's B operand as they stand: the order of the keys in the transposed values is chosen to
-// match. One pass over the keys, running maximum and sum; a lane's maximum moves only when a score passes it by 2^6.
+// match. One pass over the keys, running reference of the exponents and sum; the reference moves only when a probability
+// nears the end of f16, which a tile's sum shows.
 // Two tiles of LDS: the next tile is unpacked while this one is multiplied, and the one after that is in flight.
-// Bound by vector work beside the matrix cores: per 64 keys and 32 rows 64 products of 32x32x16 (1024 clocks) stand
-// against 32 exponentials (512 clocks), the maximum, conversion and sum (about 300), and the unpacking's share.
+// Bound by vector work beside the matrix cores: per 64 keys and 32 rows 32 products of 32x32x16 (1024 clocks) stand beside
+// 32 exponentials (512 clocks) and some 285 other vector instructions (1140), of which the unpacking has 150. 2048 tokens of
+// 32 heads on 8 of 128 against 4096 + 2048 keys take 213 us (805 TFLOP/s; a large library product reaches 1306), and took
+// 160 when the unpacking was left out for a measurement, 189 without the products. Slower were 256 rows to a workgroup with
+// 8 waves (254, causal tiles of unlike length then stand alone on a CU) and with 64 rows to a wave (314, one wave a SIMD
+// does not hide its own latencies); a running maximum taken from every tile's scores took 221, and so did the compiler's
+// own order of LDS reads.
 // EXACT (f16 outputs, or with lse): the score products take the codes themselves, exact in f16, one accumulator a scale
 // group, and a key's planes are applied to the scores in f32, as in kv_attend_rows; and the sum is of the probabilities
 // before they are rounded. Keys rounded to f16 move a score by up to 2^-11 of scale |q| |k|, which bf16 outputs do not
 // show, but an f32 lse and f16 outputs do.
 template <int DIM, int G, bool EXACT>
-__global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
+__global__ __launch_bounds__(256, DIM + (EXACT ? 16 * G : 0) <= 160 ? 2 : 1) void kv_attend_tiles(AttendArgs a) {
     constexpr int J = DIM / 16;   // k blocks of a score product
     constexpr int O = DIM / 32;   // blocks of the output
     using T = Tile<DIM, G, EXACT>;
@@ -287,7 +310,7 @@ __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
     f32x16 o[O];
 #pragma unroll
     for (int i = 0; i < O; ++i) o[i] = f32x16{};
-    float m = kNone, l = 0.0f;
+    float m = kNone, l = 0.0f, le = 0.0f;  // (le: of the probabilities before rounding)
     __syncthreads();  // not_finite is clear
     if (steps) {
         unpack(tiles[0]);
@@ -305,17 +328,20 @@ __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
         const bool flags = __builtin_amdgcn_readfirstlane((int)(uint32_t)(set | set >> 32)) != 0;
         if (t0 < outer_hi && t0 + kKeys > outer_lo) {
             f32x16 s[2];
+            constexpr int A = EXACT ? G : 1;  // accumulators
+            f32x16 acc[2][A];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                constexpr int A = EXACT ? G : 1;  // accumulators
-                f32x16 acc[A];
-                const uint32_t key = 32 * h + col;
+            for (int j = 0; j < J; ++j)
 #pragma unroll
-                for (int j = 0; j < J; ++j) {
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t key = 32 * h + col;
                     const f16x8 k = __builtin_bit_cast(f16x8, t.k[key][t.key_piece(key, 2 * j + hf)]);
-                    f32x16& c = acc[j * A / J];
+                    f32x16& c = acc[h][j * A / J];
                     c = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[j], j % (J / A) ? c : f32x16{}, 0, 0, 0);
                 }
+            read_ahead<2 * J>();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
                 if (EXACT) {
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
@@ -327,7 +353,7 @@ __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
                             const f32x4 mid = *(const f32x4*)&t.planes[EXACT ? gr : 0][1][EXACT ? at : 0];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                const float v = acc[EXACT ? gr : 0][4 * q + e];
+                                const float v = acc[h][EXACT ? gr : 0][4 * q + e];
                                 y[e] = gr ? fmaf(scale[e], v, y[e]) : scale[e] * v;
                                 z[e] = gr ? fmaf(mid[e], qsum[gr], z[e]) : mid[e] * qsum[gr];
                             }
@@ -336,7 +362,7 @@ __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
                         for (int e = 0; e < 4; ++e) s[h][4 * q + e] = fmaf(y[e], c1, z[e]);
                     }
                 } else {
-                    s[h] = acc[0];
+                    s[h] = acc[h][0];
                 }
             }
             // value i of block h: key 32 h + 8 (i / 4) + 4 hf + i % 4
@@ -359,43 +385,53 @@ __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
                         s[h][i] = key >= see.lo && key < see.hi && key < to && !out[2 * h + i / 8] ? s[h][i] : -INFINITY;
                     }
             }
-            float top = -INFINITY;
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int i = 0; i < 16; i += 2) top = max3(top, s[h][i], s[h][i + 1]);
-            top = top == -INFINITY ? top : top * scale;
-            if (__any(top > m + 6.0f)) {
-                const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64))), f = __builtin_amdgcn_exp2f(m - mn);
-                m = mn;
-                l *= f;
-#pragma unroll
-                for (int i = 0; i < O; ++i) o[i] *= f;
-            }
             // probabilities to f16 (2^-11 of each); the sum is of the same rounded values, which takes half the instructions
             // and leaves the average of a row unbiased
             uint32_t p[2][8];
+            float sum, exact;
+            const auto probabilities = [&]() {
+                sum = exact = 0.0f;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float even = __builtin_amdgcn_exp2f(fmaf(s[h][2 * i], scale, -m));
-                    const float odd = __builtin_amdgcn_exp2f(fmaf(s[h][2 * i + 1], scale, -m));
-                    const f16x2 v = {(_Float16)even, (_Float16)odd};
-                    p[h][i] = bits_of(v);
-                    if (EXACT) l += even + odd;
-                    else l = __builtin_amdgcn_fdot2(v, (f16x2){(_Float16)1.0f, (_Float16)1.0f}, l, false);
-                }
+                    for (int i = 0; i < 8; ++i) {
+                        const float even = __builtin_amdgcn_exp2f(fmaf(s[h][2 * i], scale, -m));
+                        const float odd = __builtin_amdgcn_exp2f(fmaf(s[h][2 * i + 1], scale, -m));
+                        const f16x2 v = {(_Float16)even, (_Float16)odd};
+                        p[h][i] = bits_of(v);
+                        if (EXACT) exact += even + odd;
+                        sum = __builtin_amdgcn_fdot2(v, (f16x2){(_Float16)1.0f, (_Float16)1.0f}, sum, false);
+                    }
+            };
+            probabilities();
+            // the reference of the exponents moves only when a probability is near the end of f16 (at first, from kNone, all
+            // are infinite); whether one is shows in their sum
+            if (__any(sum > 0x1p13f)) {
+                float top = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < O; ++i) {
-                const uint32_t d = 32 * i + col;
+                for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
+                    for (int i = 0; i < 16; i += 2) top = max3(top, s[h][i], s[h][i + 1]);
+                top = top == -INFINITY ? top : top * scale;
+                const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64))), f = __builtin_amdgcn_exp2f(m - mn);
+                m = mn;
+                l *= f, le *= f;
+#pragma unroll
+                for (int i = 0; i < O; ++i) o[i] *= f;
+                probabilities();
+            }
+            l += sum, le += exact;
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+#pragma unroll
+                for (int i = 0; i < O; ++i) {
+                    const uint32_t d = 32 * i + col;
                     const f16x8 v = __builtin_bit_cast(f16x8, t.v[d][t.value_piece(d, 2 * h + hf)]);
                     const uint32_t* q = &p[h / 2][h % 2 * 4];
                     o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, operand(q[0], q[1], q[2], q[3]), o[i], 0, 0, 0);
                 }
             }
+            read_ahead<4 * O>();
             // values that are not finite, of keys that the row sees
             if (flags) {
 #pragma unroll
@@ -420,8 +456,9 @@ __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
         }
     }
 
-    l += __shfl_xor(l, 32, 64);
+    l += __shfl_xor(l, 32, 64), le += __shfl_xor(le, 32, 64);
     if (!live) return;
+    const float sum = EXACT ? le : l;
     // value 4 q + e of block i: 32 i + 8 q + 4 hf + e
     // the pieces of a tile that fit one need no join
     if (a.pieces == 1 || piece >= last_row.hi - begin) {
@@ -435,16 +472,18 @@ __global__ __launch_bounds__(256, 1) void kv_attend_tiles(AttendArgs a) {
                 store_out<4>(p + 32 * i + 8 * q, a.out.vec, a.is_bf16, v, inv);
             }
         if (a.lse && hf == 0)
-            a.lse[(size_t)token * a.heads + qh] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
+            a.lse[(size_t)token * a.heads + qh] = sum == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * kLn2;
     } else {
+        // (the join divides by the sum before rounding)
+        const float f = EXACT && l > 0.0f ? sum / l : 1.0f;
         const size_t at = ((size_t)token * a.heads + qh) * a.pieces + part;
         float* dst = a.tile_po + at * DIM + 4 * hf;
 #pragma unroll
         for (int i = 0; i < O; ++i)
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                *(f32x4*)(dst + 32 * i + 8 * q) = f32x4{o[i][4 * q], o[i][4 * q + 1], o[i][4 * q + 2], o[i][4 * q + 3]};
-        if (hf == 0) a.tile_pml[at] = float2{l == 0.0f ? kNone : m, l};
+                *(f32x4*)(dst + 32 * i + 8 * q) = f32x4{o[i][4 * q], o[i][4 * q + 1], o[i][4 * q + 2], o[i][4 * q + 3]} * f;
+        if (hf == 0) a.tile_pml[at] = float2{sum == 0.0f ? kNone : m, sum};
     }
 }
 

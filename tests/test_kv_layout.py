@@ -185,7 +185,7 @@ def test_pieces_cover_a_tile_and_fill_the_gpu():
     t = rules().tiling
     t.argtypes = [C.c_uint32, C.c_uint32, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p]
     assert _out(t, 2, 1, 8, 2048 * 4, 2048 * 4, 6144, 256, kind=C.c_uint32) == (64, 1)
-    assert _out(t, 2, 1, 1, 300, 300, 100000, 256, kind=C.c_uint32)[1] == 342
+    assert _out(t, 2, 1, 1, 300, 300, 100000, 256, kind=C.c_uint32)[1] == 171
     assert _out(t, 2, 1, 1, 300, 300, 300, 256, kind=C.c_uint32)[1] == 2
     assert _out(t, 2, 4, 2, 0, 100, 0, 256, kind=C.c_uint32)[1] == 1
 
