@@ -33,8 +33,8 @@ struct AttendArgs {
     uint32_t grid, inverse;  // else the workgroups that share the steps, and 2^32 / grid
     float* po;               // [2 grid][16 rows][dim] unnormalised partial outputs
     float2* pml;             // [2 grid][16 rows] (reference exponent, sum)
-    int4* begun;             // [grid] unit that begins in a workgroup and goes on in later ones: request (-1: none), head,
-                             // first row, how many
+    int4* begun;             // [grid] unit that begins in a workgroup and goes on in later ones: its request's first token
+                             // (-1: none), head, first row | rows of the request << 16, later ones
     // rows of prompts (kv_attend_tiles)
     uint32_t tiles;             // that the longest request may have
     uint32_t pieces;            // that a tile's keys may be cut into

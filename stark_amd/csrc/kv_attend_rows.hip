@@ -639,7 +639,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
                 for (int e = 0; e < N; e += 4) *(f32x4*)(a.po + slot * DIM + d + e) = f32x4{v[e], v[e + 1], v[e + 2], v[e + 3]};
                 if (d == 0) a.pml[slot] = float2{rref, sum};
                 if (s0 == 0 && threadIdx.x == 0)  // goes on in the workgroups up to the one that holds its last step
-                    a.begun[blockIdx.x] = int4{(int)b, (int)head, (int)row0, (int)((unit_end - 1) / per - blockIdx.x)};
+                    a.begun[blockIdx.x] = int4{u.r.first, (int)head, (int)(row0 | u.rows << 16), (int)((unit_end - 1) / per - blockIdx.x)};
             }
         }
         __syncthreads();  // the LDS buffers are free again
@@ -657,10 +657,9 @@ __global__ __launch_bounds__(256) void kv_attend_join(AttendArgs a) {
     const uint32_t slot_row = blockIdx.x % quarters * 4 + (threadIdx.x >> 6);
     const int4 u = a.begun[w];
     if (u.x < 0) return;
-    const kv::Request r = request_of(a, (uint32_t)u.x);
-    const uint32_t row = (uint32_t)u.z + slot_row;
-    if (row >= (uint32_t)r.q_len * a.ratio) return;
-    const uint32_t token = (uint32_t)r.first + row / a.ratio, qh = (uint32_t)u.y * a.ratio + row % a.ratio;
+    const uint32_t row = ((uint32_t)u.z & 0xffffu) + slot_row;
+    if (row >= (uint32_t)u.z >> 16) return;
+    const uint32_t i = row * a.ratio_inverse >> 16, token = (uint32_t)u.x + i, qh = (uint32_t)u.y * a.ratio + row - i * a.ratio;
     const uint32_t parts = (uint32_t)u.w + 1;
     // part 0 is the workgroup's last segment, part i the first of workgroup w + i
     const auto slot = [&](uint32_t i) { return (size_t)(i ? 2 * (w + i) : 2 * w + 1) * kRows + slot_row; };
