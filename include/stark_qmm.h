@@ -659,7 +659,7 @@ typedef struct stark_qmm_kv_attention_args {
     const int32_t* kv_lengths;   /* [batch] tokens in the cache, the new ones among them */
     uint32_t batch, tokens, heads, table_stride;
     uint32_t max_query;          /* bounds on the lengths of any request; what is longer is cut */
-    uint32_t max_kv;
+    uint32_t max_kv;             /* (this or table_stride * page_size is at most 2^31 - 2^16) */
     float scale;                 /* of the scores: 0, or 2^-64 <= |scale| <= 2^64 */
     float soft_cap;              /* 0, or 2^-20 .. 2^20: scores become soft_cap * tanh(score / soft_cap) */
     uint32_t causal;             /* query i of n sees keys up to kv_length - n + i */

@@ -26,6 +26,7 @@ stark_qmm_status check(const stark_qmm_kv_attention_args* p, AttendArgs* a) {
     a->stride = p->table_stride;
     a->max_query = std::min(p->max_query, p->tokens);
     a->max_kv = std::min(p->max_kv, p->table_stride * p->cache.page_size);
+    if (a->max_kv > 0x7fff0000u) return STARK_QMM_INVALID_ARGUMENT;  // positions past a tile's end are int32 as well
     // steps of a call are counted in 31 bits
     if ((uint64_t)a->batch * a->cache.kv_heads * 4 * (a->max_kv / 32 + 20ull) >= 1ull << 31) return STARK_QMM_UNSUPPORTED;
     a->is_bf16 = p->data_type == STARK_QMM_BF16;

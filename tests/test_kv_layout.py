@@ -339,7 +339,8 @@ def test_attention_refusals():
                 dict(max_kv=2 ** 31), dict(table_stride=0), dict(table_stride=2 ** 25), dict(scale=float("nan")),
                 dict(scale=float("inf")), dict(soft_cap=-1.0), dict(soft_cap=float("nan")), dict(soft_cap=float("inf")),
                 dict(q=None), dict(out=None), dict(block_table=None), dict(query_start=None), dict(kv_lengths=None),
-                dict(q=FAKE + 1), dict(lse=FAKE + 2), dict(q_head_stride=64), dict(out_token_stride=128)):
+                dict(q=FAKE + 1), dict(lse=FAKE + 2), dict(q_head_stride=64), dict(out_token_stride=128),
+                dict(max_kv=2 ** 31 - 1, table_stride=2 ** 25 - 1)):
         assert call(args(**bad), None) == Q.INVALID_ARGUMENT, bad
 
 
