@@ -27,7 +27,7 @@ struct AttendArgs {
     int32_t window;
     // decode rows (kv_attend_rows)
     uint32_t row_limit;      // requests with more rows to a kv head are kv_attend_tiles's; 0: all are
-    uint32_t row_block;      // 4, 8 or 16
+    uint32_t row_block;      // 8 or 16
     uint32_t ratio_inverse;  // ceil(65536 / ratio): x / ratio for x < 64 and ratios up to 64
     uint32_t whole;          // a unit to a workgroup, no partial results
     uint32_t grid, inverse;  // else the workgroups that share the steps, and 2^32 / grid

@@ -5,11 +5,11 @@ namespace {
 
 using namespace qmm;
 
-// Records of a step and how they are packed. PACK: records whose scores share one 16 x 16 block.
+// Records of a step and how they are packed. PACK (1 or 2): records whose scores share one 16 x 16 block.
 template <int PACK>
 struct Shape {
     static constexpr int R = 16 / PACK;            // rows of a request
-    static constexpr int T = PACK == 4 ? 4 : 2;    // records of a step
+    static constexpr int T = 2;                    // records of a step
     static constexpr int KEYS = 16 * T;            // keys of a step
     static constexpr int B = T / PACK;             // score blocks of a step
 };
@@ -124,7 +124,7 @@ QMM_DEVICE Unit unit_of(const AttendArgs& a, const kv::Request& r) {
     u.from = u.span.lo & ~(KEYS - 1);
     u.steps = (uint32_t)max((u.span.hi - u.from + KEYS - 1) / KEYS, 1);
     if (u.rows == 0 || u.rows > a.row_limit) u.steps = 0;
-    u.cost = u.steps ? u.steps + kv::kUnitKeys / KEYS : 0;
+    u.cost = u.steps ? u.steps + kv::unit_keys(R) / KEYS : 0;
     u.all = u.cost * ((u.rows + R - 1) / R) * a.cache.kv_heads;
     return u;
 }
@@ -168,7 +168,7 @@ QMM_DEVICE uint32_t wave_scan(uint32_t v) {
 
 // Decode and verify: requests of few rows (a kv head's query heads times the new tokens), in blocks of R = 16 / PACK.
 //
-// The work of a call is the steps (32 or 64 keys) of all (request, kv head, block) units, in that order; each workgroup takes
+// The work of a call is the steps (32 keys) of all (request, kv head, block) units, in that order; each workgroup takes
 // an equal run of them, so unlike lengths leave no CU idle and a workgroup pays its start once or twice, not once a
 // chunk. A unit inside one run is finished there; of the others each workgroup leaves partial results, which
 // kv_attend_join adds. Within a run the steps of a unit are dealt to four waves, each with its own running maximum and
@@ -595,11 +595,10 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
                     y[2 * e] = l == 0.0f ? 0.0f : fmaf(even, 0x1p24f, s) * f;
                     y[2 * e + 1] = l == 0.0f ? 0.0f : fmaf(odd, 0x1p24f, s) * f;
                 }
-                // the columns of a row: rotations of the 16-lane row by R, 2 R, ...
+                // the two columns of a row: the 16-lane row rotated by 8
+                if (PACK == 2) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (PACK >= 2) y[e] += dpp_f32<0x128>(y[e]);
-                    if (PACK >= 4) y[e] += dpp_f32<0x124>(y[e]);
+                    for (int e = 0; e < 8; ++e) y[e] += dpp_f32<0x128>(y[e]);
                 }
                 if (pack == 0) {
                     float* dst = &sh.join[wave][row * kRow + 32 * i + 8 * g];
@@ -704,7 +703,6 @@ stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
 
 template <int DIM, int G>
 stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
-    if (a.row_block == 4) return launch<DIM, G, 4>(a, s);
     return a.row_block == 8 ? launch<DIM, G, 2>(a, s) : launch<DIM, G, 1>(a, s);
 }
 

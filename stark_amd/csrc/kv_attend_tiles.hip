@@ -185,7 +185,7 @@ QMM_DEVICE void read_ahead() {
 // before they are rounded. Keys rounded to f16 move a score by up to 2^-11 of scale |q| |k|, which bf16 outputs do not
 // show, but an f32 lse and f16 outputs do.
 template <int DIM, int G, bool EXACT>
-__global__ __launch_bounds__(256, DIM + (EXACT ? 16 * G : 0) <= 160 ? 2 : 1) void kv_attend_tiles(AttendArgs a) {
+__global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(AttendArgs a) {
     constexpr int J = DIM / 16;   // k blocks of a score product
     constexpr int O = DIM / 32;   // blocks of the output
     using T = Tile<DIM, G, EXACT>;
@@ -328,41 +328,45 @@ __global__ __launch_bounds__(256, DIM + (EXACT ? 16 * G : 0) <= 160 ? 2 : 1) voi
         const bool flags = __builtin_amdgcn_readfirstlane((int)(uint32_t)(set | set >> 32)) != 0;
         if (t0 < outer_hi && t0 + kKeys > outer_lo) {
             f32x16 s[2];
-            constexpr int A = EXACT ? G : 1;  // accumulators
-            f32x16 acc[2][A];
+            constexpr int A = EXACT ? G : 1;  // accumulators of a block of 32 keys
+            constexpr int H = A > 1 ? 1 : 2;  // blocks at a time: two sums at least, so that no product waits for the last
 #pragma unroll
-            for (int j = 0; j < J; ++j)
+            for (int h0 = 0; h0 < 2; h0 += H) {
+                f32x16 acc[H][A];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t key = 32 * h + col;
-                    const f16x8 k = __builtin_bit_cast(f16x8, t.k[key][t.key_piece(key, 2 * j + hf)]);
-                    f32x16& c = acc[h][j * A / J];
-                    c = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[j], j % (J / A) ? c : f32x16{}, 0, 0, 0);
-                }
-            read_ahead<2 * J>();
+                for (int n = 0; n < J; ++n)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                if (EXACT) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        f32x4 y, z;
-#pragma unroll
-                        for (int gr = 0; gr < G; ++gr) {
-                            const uint32_t at = 32 * h + 8 * q + 4 * hf;
-                            const f32x4 scale = *(const f32x4*)&t.planes[EXACT ? gr : 0][0][EXACT ? at : 0];
-                            const f32x4 mid = *(const f32x4*)&t.planes[EXACT ? gr : 0][1][EXACT ? at : 0];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float v = acc[h][EXACT ? gr : 0][4 * q + e];
-                                y[e] = gr ? fmaf(scale[e], v, y[e]) : scale[e] * v;
-                                z[e] = gr ? fmaf(mid[e], qsum[gr], z[e]) : mid[e] * qsum[gr];
-                            }
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) s[h][4 * q + e] = fmaf(y[e], c1, z[e]);
+                    for (int h = 0; h < H; ++h) {
+                        const int gr = n % A, j = gr * (J / A) + n / A;
+                        const uint32_t key = 32 * (h0 + h) + col;
+                        const f16x8 k = __builtin_bit_cast(f16x8, t.k[key][t.key_piece(key, 2 * j + hf)]);
+                        acc[h][gr] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[j], n < A ? f32x16{} : acc[h][gr], 0, 0, 0);
                     }
-                } else {
-                    s[h] = acc[h][0];
+                read_ahead<J * H>();
+#pragma unroll
+                for (int h = h0; h < h0 + H; ++h) {
+                    if (EXACT) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            f32x4 y, z;
+#pragma unroll
+                            for (int gr = 0; gr < G; ++gr) {
+                                const uint32_t at = 32 * h + 8 * q + 4 * hf;
+                                const f32x4 scale = *(const f32x4*)&t.planes[EXACT ? gr : 0][0][EXACT ? at : 0];
+                                const f32x4 mid = *(const f32x4*)&t.planes[EXACT ? gr : 0][1][EXACT ? at : 0];
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const float v = acc[h - h0][EXACT ? gr : 0][4 * q + e];
+                                    y[e] = gr ? fmaf(scale[e], v, y[e]) : scale[e] * v;
+                                    z[e] = gr ? fmaf(mid[e], qsum[gr], z[e]) : mid[e] * qsum[gr];
+                                }
+                            }
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[h][4 * q + e] = fmaf(y[e], c1, z[e]);
+                        }
+                    } else {
+                        s[h] = acc[h - h0][0];
+                    }
                 }
             }
             // value i of block h: key 32 h + 8 (i / 4) + 4 hf + i % 4

@@ -28,7 +28,7 @@ stark_qmm_status check(const stark_qmm_kv_attention_args* p, AttendArgs* a) {
     a->max_kv = std::min(p->max_kv, p->table_stride * p->cache.page_size);
     if (a->max_kv > 0x7fff0000u) return STARK_QMM_INVALID_ARGUMENT;  // positions past a tile's end are int32 as well
     // steps of a call are counted in 31 bits
-    if ((uint64_t)a->batch * a->cache.kv_heads * 4 * (a->max_kv / 32 + 20ull) >= 1ull << 31) return STARK_QMM_UNSUPPORTED;
+    if ((uint64_t)a->batch * a->cache.kv_heads * 4 * (a->max_kv / 32 + 40ull) >= 1ull << 31) return STARK_QMM_UNSUPPORTED;
     a->is_bf16 = p->data_type == STARK_QMM_BF16;
     a->causal = p->causal != 0, a->window = (int32_t)std::min(p->window, 0x7fffffffu);
     const float scale = p->scale == 0.0f ? 1.0f : fabsf(p->scale);
@@ -64,7 +64,7 @@ stark_qmm_status plan_work(AttendArgs* a, uint64_t* workspace) {
     if (a->row_limit) {
         a->ratio_inverse = (65535 + a->ratio) / a->ratio;
         const uint32_t blocks = (a->row_limit + a->row_block - 1) / a->row_block;
-        const kv::Share w = kv::share(a->batch, a->cache.kv_heads * blocks, a->max_kv,
+        const kv::Share w = kv::share(a->batch, a->cache.kv_heads * blocks, a->row_block, a->max_kv,
                                       cus * (a->cache.dim == 256 ? 1 : 2));
         a->whole = w.whole, a->grid = w.grid;
         a->inverse = w.grid > 1 ? (uint32_t)((1ull << 32) / w.grid) : 0xffffffffu;

@@ -106,27 +106,30 @@ KV_HD Range request_range(int32_t q_len, int32_t kv_len, bool causal, int32_t wi
 }
 
 // Requests that the decode kernel takes in a call: those of up to `limit` rows (a kv head's query heads times new tokens),
-// in blocks of `block` rows (4, 8 or 16). Where the bounds say that no request has more than 64 rows it takes all; in a
-// call of longer requests those of one block, which has what one new token has (decode rows among prompts), where there
-// may be enough of them to pay for two more launches (a prompt with 8 decode rows of 2000 keys 59 us with them, 61 us
-// without; 8 of 200 keys 28 against 19; 16 of 300 keys 30 against 33; 8 of 8000 keys 98 against 171), else none (0). The
-// others go to the tile kernel.
+// in blocks of `block` rows (8 or 16). Where the bounds say that no request has more than 64 rows it takes all (16 requests
+// of 16 to 40 rows and 900 to 9000 keys 27 us with it, 50 in tiles, 64 of them 64 and 135; where many requests have 64 rows
+// and one length tiles are up to 1.4 times faster, 64 of 2000 keys 127 and 90); in a call of longer requests those of one
+// block, which has what one new token has (decode rows among prompts), where there may be enough of them to pay for two more
+// launches (a prompt with 8 decode rows of 2000 keys 59 us with them, 61 us without; 8 of 200 keys 28 against 19; 16 of 300
+// keys 30 against 33; 8 of 8000 keys 98 against 171), else none (0). The others go to the tile kernel.
 struct Rows {
     uint32_t limit, block;
 };
 KV_HD Rows row_limit(uint32_t batch, uint32_t max_query, uint32_t ratio, uint32_t max_kv) {
     const uint64_t most = (uint64_t)max_query * ratio;
-    if (most <= 64) return {64, most <= 4 ? 4u : most <= 8 ? 8u : 16u};
+    if (most <= 64) return {64, most <= 8 ? 8u : 16u};
     if (ratio > 16 || (batch < 16 && (uint64_t)batch * max_kv < 49152) || batch == 1) return {0, 16};
-    const uint32_t block = ratio <= 4 ? 4 : ratio <= 8 ? 8 : 16;
+    const uint32_t block = ratio <= 8 ? 8 : 16;
     return {block, block};
 }
 
-// Keys of a workgroup's least share of a decode call: one 64-key or two 32-key steps for each of its four waves.
+// Keys of a workgroup's least share of a decode call: two steps for each of its four waves.
 constexpr uint32_t kLeastKeys = 256;
 
-// What beginning a unit costs a workgroup, in keys: its steps are counted as so many more.
-constexpr uint32_t kUnitKeys = 512;
+// What beginning a unit costs a workgroup, in keys: its steps are counted as so many more. Blocks of 8 rows, us with 512,
+// 1024 and 2048: 16 requests of 900 to 9000 keys 26.0, 22.4 and 23.9; 64 of 500 to 32768 134, 132 and 137; 256 of 100 to 2000
+// 75, 70 and 72. Blocks of 16, whose keys take longer: 26.6, 28.0 and 30.2.
+KV_HD uint32_t unit_keys(uint32_t block) { return block == 8 ? 1024 : 512; }
 
 // Steps of each of `grid` workgroups that share `total` (below 2^31): a multiple of four, one for each wave.
 // inverse: 2^32 / grid, rounded down (2^32 - 1 for 1).
@@ -139,13 +142,15 @@ KV_HD uint32_t share_of(uint32_t total, uint32_t grid, uint32_t inverse, uint32_
 }
 
 // How a decode call's work is dealt: whole units (a request's rows on one kv head) to a workgroup where no unit has more
-// keys than twice the least share; else `grid` workgroups share all steps (no more workgroups than shares).
+// than 1024 keys, or 2048 with 128 units; else `grid` workgroups share all steps (no more workgroups than shares). Us, whole
+// and shared, 8 kv heads: 8 requests of 1000 keys 12.6 and 15.2, 64 of 100 to 1000 16.2 and 23.8, 16 of 100 to 2000 14.8 and
+// 16.1, 64 of them 20.6 and 24.5; one of 2000 keys 19.2 and 12.0, 64 of 100 to 4000 34.7 and 30.9.
 struct Share {
     uint32_t whole, grid;
 };
-KV_HD Share share(uint32_t batch, uint32_t kv_heads, uint32_t max_kv, uint32_t slots) {
-    if (max_kv <= 2 * kLeastKeys) return {1, 0};
-    const uint64_t keys = (uint64_t)batch * kv_heads * (max_kv + 128ull + kUnitKeys), most = (keys + kLeastKeys - 1) / kLeastKeys;
+KV_HD Share share(uint32_t batch, uint32_t kv_heads, uint32_t block, uint32_t max_kv, uint32_t slots) {
+    if (max_kv <= 1024 || (max_kv <= 2048 && (uint64_t)batch * kv_heads >= 128)) return {1, 0};
+    const uint64_t keys = (uint64_t)batch * kv_heads * (max_kv + 128ull + unit_keys(block)), most = (keys + kLeastKeys - 1) / kLeastKeys;
     return {0, most < slots ? (uint32_t)(most ? most : 1) : slots};
 }
 

@@ -34,8 +34,8 @@ void request(int32_t s, int32_t e, int32_t k, uint32_t n, uint32_t mq, uint32_t 
 void page_plan(int64_t c, int64_t a, uint32_t s, uint32_t w, int32_t* r) {
     const kv::PagePlan x = kv::page_plan(c, a, s, w); r[0] = x.before; r[1] = x.need;
 }
-void share(uint32_t batch, uint32_t heads, uint32_t max_kv, uint32_t slots, uint32_t* r) {
-    const kv::Share x = kv::share(batch, heads, max_kv, slots); r[0] = x.whole; r[1] = x.grid;
+void share(uint32_t batch, uint32_t heads, uint32_t block, uint32_t max_kv, uint32_t slots, uint32_t* r) {
+    const kv::Share x = kv::share(batch, heads, block, max_kv, slots); r[0] = x.whole; r[1] = x.grid;
 }
 uint32_t share_of(uint32_t total, uint32_t grid, uint32_t keys) {
     return kv::share_of(total, grid, grid > 1 ? (uint32_t)((1ull << 32) / grid) : 0xffffffffu, keys);
@@ -45,7 +45,7 @@ int32_t piece_keys(int32_t range, uint32_t pieces) { return kv::piece_keys(range
 void tiling(uint32_t batch, uint32_t heads, uint64_t rows, uint64_t most, uint32_t max_kv, uint32_t cus, uint32_t* o) {
     const kv::Tiling t = kv::tiling(batch, heads, rows, most, max_kv, cus); o[0] = t.tiles; o[1] = t.pieces;
 }
-uint32_t unit_keys() { return kv::kUnitKeys; }
+uint32_t unit_keys(uint32_t block) { return kv::unit_keys(block); }
 }
 """
 
@@ -149,29 +149,31 @@ def test_page_plan_counts_new_pages():
 
 
 def test_shares_cover_every_step():
-    for batch, heads, kv in ((1, 1, 513), (1, 8, 4096), (64, 8, 32768), (1000, 4, 700), (3, 1, 131072), (2, 8, 5000)):
-        whole, grid = _out(rules().share, 2, batch, heads, kv, 512, kind=C.c_uint32)
-        assert not whole and 1 <= grid <= 512
-        for keys in (32, 64):
-            most = batch * heads * (-(-(kv + keys - 1) // keys) + rules().unit_keys() // keys)
-            for total in (0, 1, 7, 8, 9, 100, most // 3, most, 2 ** 31 - 1):
-                per, least = rules().share_of(total, grid, keys), 256 // keys
-                assert per % 4 == 0 and per >= least and per * grid >= total
-                assert per == max(least, -(-(-(-total // grid)) // 4) * 4)
-                if grid < 512 and total <= most:  # fewer workgroups than slots: each has its least share
-                    assert per == least
-    for kv in (0, 1, 512):
-        assert _out(rules().share, 2, 5, 2, kv, 512, kind=C.c_uint32)[0] == 1
+    for batch, heads, kv in ((1, 1, 1025), (1, 8, 4096), (64, 8, 32768), (1000, 4, 2100), (3, 1, 131072), (2, 8, 5000)):
+        for block in (8, 16):
+            whole, grid = _out(rules().share, 2, batch, heads, block, kv, 512, kind=C.c_uint32)
+            assert not whole and 1 <= grid <= 512
+            for keys in (32, 64):
+                most = batch * heads * (-(-(kv + keys - 1) // keys) + rules().unit_keys(block) // keys)
+                for total in (0, 1, 7, 8, 9, 100, most // 3, most, 2 ** 31 - 1):
+                    per, least = rules().share_of(total, grid, keys), 256 // keys
+                    assert per % 4 == 0 and per >= least and per * grid >= total
+                    assert per == max(least, -(-(-(-total // grid)) // 4) * 4)
+                    if grid < 512 and total <= most:  # fewer workgroups than slots: each has its least share
+                        assert per == least
+    for batch, heads, kv, want in ((5, 2, 0, 1), (5, 2, 1, 1), (5, 2, 1024, 1), (5, 2, 1025, 0), (64, 2, 2048, 1),
+                                   (63, 2, 2048, 0), (500, 8, 2049, 0)):
+        assert _out(rules().share, 2, batch, heads, 8, kv, 512, kind=C.c_uint32)[0] == want
 
 
 def test_row_limits():
     """Which requests the decode kernel takes, and in what blocks: by the rows that a kv head's query heads and the new
     tokens make."""
     for batch, query, ratio, kv, want in (
-            (1, 1, 4, 9, (64, 4)), (1, 2, 4, 9, (64, 8)), (9, 3, 4, 9, (64, 16)), (1, 16, 4, 9, (64, 16)),
-            (1, 17, 4, 10 ** 6, (0, 16)), (2, 17, 4, 30000, (4, 4)), (2, 17, 4, 20000, (0, 16)), (16, 100, 7, 9, (8, 8)),
+            (1, 1, 4, 9, (64, 8)), (1, 2, 4, 9, (64, 8)), (9, 3, 4, 9, (64, 16)), (1, 16, 4, 9, (64, 16)),
+            (1, 17, 4, 10 ** 6, (0, 16)), (2, 17, 4, 30000, (8, 8)), (2, 17, 4, 20000, (0, 16)), (16, 100, 7, 9, (8, 8)),
             (15, 100, 7, 9, (0, 16)), (20, 100, 16, 9, (16, 16)), (20, 100, 17, 9, (0, 16)), (5, 1, 20, 9, (64, 16)),
-            (5, 1, 65, 10 ** 6, (0, 16)), (30, 65, 1, 9, (4, 4))):
+            (5, 1, 65, 10 ** 6, (0, 16)), (30, 65, 1, 9, (8, 8))):
         assert _out(rules().row_limit, 2, batch, query, ratio, kv, kind=C.c_uint32) == want, (batch, query, ratio)
 
 
