@@ -180,10 +180,11 @@ QMM_DEVICE void read_ahead() {
 // 8 waves (254, causal tiles of unlike length then stand alone on a CU) and with 64 rows to a wave (314, one wave a SIMD
 // does not hide its own latencies); a running maximum taken from every tile's scores took 221, and so did the compiler's
 // own order of LDS reads.
-// EXACT (f16 outputs, or with lse): the score products take the codes themselves, exact in f16, one accumulator a scale
-// group, and a key's planes are applied to the scores in f32, as in kv_attend_rows; and the sum is of the probabilities
-// before they are rounded. Keys rounded to f16 move a score by up to 2^-11 of scale |q| |k|, which bf16 outputs do not
-// show, but an f32 lse and f16 outputs do.
+// EXACT (f16 outputs, or with lse): the score products take the codes themselves, exact in f16, one sum a scale group, and
+// a key's planes are applied to the scores in f32, as in kv_attend_rows; and lse is of the sum of the probabilities before
+// they are rounded. Keys rounded to f16 move a score by up to 2^-11 of scale |q| |k|, which bf16 outputs do not show, but
+// an f32 lse and f16 outputs do. The planes cost 2 G + 1 operations a score: the same chunk takes 235, 270 and 412 us with
+// 1, 2 and 4 groups (206, 215 and 222 without).
 template <int DIM, int G, bool EXACT>
 __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(AttendArgs a) {
     constexpr int J = DIM / 16;   // k blocks of a score product
@@ -328,44 +329,49 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
         const bool flags = __builtin_amdgcn_readfirstlane((int)(uint32_t)(set | set >> 32)) != 0;
         if (t0 < outer_hi && t0 + kKeys > outer_lo) {
             f32x16 s[2];
-            constexpr int A = EXACT ? G : 1;  // accumulators of a block of 32 keys
-            constexpr int H = A > 1 ? 1 : 2;  // blocks at a time: two sums at least, so that no product waits for the last
+            // two sums at a time, so that no product waits for the last: of both blocks of 32 keys, or of two scale groups
+            constexpr int P = EXACT && G > 1 ? 2 : 1, H = 3 - P;
 #pragma unroll
             for (int h0 = 0; h0 < 2; h0 += H) {
-                f32x16 acc[H][A];
+                f32x16 z;  // of the keys' middles
 #pragma unroll
-                for (int n = 0; n < J; ++n)
+                for (int g0 = 0; g0 < (EXACT ? G : 1); g0 += P) {
+                    constexpr int N = EXACT ? J / G * P : J;  // products of P groups
+                    f32x16 acc[H][P];
+#pragma unroll
+                    for (int n = 0; n < N; ++n)
+#pragma unroll
+                        for (int h = 0; h < H; ++h) {
+                            const int gr = n % P, j = (g0 + gr) * (N / P) + n / P;
+                            const uint32_t key = 32 * (h0 + h) + col;
+                            const f16x8 k = __builtin_bit_cast(f16x8, t.k[key][t.key_piece(key, 2 * j + hf)]);
+                            acc[h][gr] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[j], n < P ? f32x16{} : acc[h][gr], 0, 0, 0);
+                        }
+                    read_ahead<N * H>();
 #pragma unroll
                     for (int h = 0; h < H; ++h) {
-                        const int gr = n % A, j = gr * (J / A) + n / A;
-                        const uint32_t key = 32 * (h0 + h) + col;
-                        const f16x8 k = __builtin_bit_cast(f16x8, t.k[key][t.key_piece(key, 2 * j + hf)]);
-                        acc[h][gr] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[j], n < A ? f32x16{} : acc[h][gr], 0, 0, 0);
-                    }
-                read_ahead<J * H>();
+                        if (!EXACT) {
+                            s[h0 + h] = acc[h][0];
+                            continue;
+                        }
 #pragma unroll
-                for (int h = h0; h < h0 + H; ++h) {
-                    if (EXACT) {
+                        for (int q = 0; q < 4; ++q)
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            f32x4 y, z;
-#pragma unroll
-                            for (int gr = 0; gr < G; ++gr) {
-                                const uint32_t at = 32 * h + 8 * q + 4 * hf;
-                                const f32x4 scale = *(const f32x4*)&t.planes[EXACT ? gr : 0][0][EXACT ? at : 0];
-                                const f32x4 mid = *(const f32x4*)&t.planes[EXACT ? gr : 0][1][EXACT ? at : 0];
+                            for (int gr = 0; gr < P; ++gr) {
+                                const uint32_t at = 32 * (h0 + h) + 8 * q + 4 * hf;
+                                const f32x4 scale = *(const f32x4*)&t.planes[EXACT ? g0 + gr : 0][0][EXACT ? at : 0];
+                                const f32x4 mid = *(const f32x4*)&t.planes[EXACT ? g0 + gr : 0][1][EXACT ? at : 0];
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
-                                    const float v = acc[h - h0][EXACT ? gr : 0][4 * q + e];
-                                    y[e] = gr ? fmaf(scale[e], v, y[e]) : scale[e] * v;
-                                    z[e] = gr ? fmaf(mid[e], qsum[gr], z[e]) : mid[e] * qsum[gr];
+                                    const int i = 4 * q + e;
+                                    const float v = acc[h][gr][i];
+                                    s[h0 + h][i] = g0 + gr ? fmaf(scale[e], v, s[h0 + h][i]) : scale[e] * v;
+                                    z[i] = g0 + gr ? fmaf(mid[e], qsum[g0 + gr], z[i]) : mid[e] * qsum[0];
                                 }
                             }
+                        if (g0 + P == G)
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) s[h][4 * q + e] = fmaf(y[e], c1, z[e]);
-                        }
-                    } else {
-                        s[h] = acc[h - h0][0];
+                            for (int i = 0; i < 16; ++i) s[h0 + h][i] = fmaf(s[h0 + h][i], c1, z[i]);
                     }
                 }
             }

