@@ -192,8 +192,8 @@ QMM_DEVICE uint32_t wave_scan(uint32_t v) {
 //
 // Bound by HBM where there are many long requests: 64 of 500 to 32768 keys, 32 heads on 8 of 128 (781 MB), take 128.5 us,
 // 6.08 TB/s (a pure read of the same size 6.2). Bound by its own latency where there are few: one of 4096 keys (4.7 MB) takes
-// 9.4 us and 3.9 to join, of which 3.3 are the chain of lengths, page ids, codes and queries, 1.9 a step and 1.8 the joining
-// of the waves (a wave alone on its SIMD issues an instruction in 6 to 8 clocks). Blocks of 4 rows (four records to a score
+// 9.4 us and 3.9 to join; of a workgroup's 8.5 us with 64 keys 3.3 are the chain of lengths, page ids, codes and queries, 3.2
+// a step and its wait, 2.0 the joining of the waves (a wave alone on its SIMD issues an instruction in 6 to 8 clocks). Blocks of 4 rows (four records to a score
 // block) took 134 us there, blocks of 16 for 4 rows 67 us against 60 (64 requests of 4096 keys); more workgroups, loads three
 // and four steps ahead and more waves a SIMD were no faster.
 template <int DIM, int G, int PACK>
