@@ -255,6 +255,31 @@ def test_groups_at_the_edges(K, dim, group):
     _same(_np(v), want, "v")
 
 
+@pytest.mark.parametrize("dim,dtype,inter,axes,shift", [(64, "bf16", False, 3, 0), (128, "f16", True, 1, 2), (64, "f32", False, 1, 0)])
+def test_an_append_of_many_rows_is_its_parts(K, dim, dtype, inter, axes, shift):
+    """Several rows to a thread (a large call) and one (small ones) leave the same cache and the same queries."""
+    rng = np.random.default_rng(dim + axes)
+    tokens, heads, kvh, page, group = 6001, 41, 5, 64, 32
+    q, k, v = (_round(rng.normal(0, 1, (tokens, n, dim)), dtype) for n in (heads, kvh, kvh))
+    q, k, v = (_dev(x, DT[dtype]) for x in (q, k, v))
+    flat = torch.zeros(500 * dim + shift, device="cuda")  # shift: rows of the table that are not 16-byte aligned
+    table = flat[shift:].view(500, dim // 2, 2)
+    table.copy_(_dev(_table(500, dim // 2), torch.float32))
+    positions = _ints(rng.integers(0, 500, (axes, tokens)))
+    pick = np.sort(rng.integers(0, axes, dim // 2))
+    slots = _ints(rng.permutation(100 * page)[:tokens])
+    caches, outs = [], []
+    for step in (tokens, 37):
+        cache, out = K.KvCache(100, page, kvh, dim, group), q.clone()
+        for a in range(0, tokens, step):
+            part = slice(a, a + step)
+            K.KvAppend(cache, k[part], v[part], slots[part], out[part], out[part],
+                       K.Rotary(table, positions[:, part], pick, inter)).encode()
+        caches.append(cache.data), outs.append(out)
+    torch.cuda.synchronize()
+    assert torch.equal(*caches) and torch.equal(outs[0].view(torch.uint8), outs[1].view(torch.uint8))
+
+
 def test_slots_outside_the_cache_write_and_read_nothing(K):
     rng = np.random.default_rng(1)
     cache = K.KvCache(3, 16, 2, 64, 32)
@@ -410,6 +435,12 @@ ATTEND = [
     ([(90, 200)], 2, 1, 256, 128, 16, "bf16", {}),
     ([(3, 100)] * 70 + [(1, 30)] * 3, 4, 2, 64, 32, 16, "bf16", {}),   # more requests than lanes
     ([(1, 600)] * 300, 2, 1, 64, 64, 16, "f16", {}),
+    # lengths whose steps workgroups share, in blocks of 8 and of 16 rows
+    ([(1, 30)] * 70 + [(1, 2100), (2, 40)], 4, 2, 64, 32, 16, "bf16", {}),
+    ([(1, 1100), (0, 3), (1, 2500), (1, 90)], 8, 2, 128, 64, 64, "bf16", {}),
+    ([(5, 1400), (3, 1100), (1, 0)], 32, 4, 128, 32, 16, "f16", {}),
+    ([(1, 1700), (2, 1200)], 4, 1, 256, 32, 32, "bf16", dict(soft_cap=20.0)),
+    ([(1, 1900), (1, 1300)], 20, 1, 64, 64, 16, "bf16", dict(window=1200)),
 ]
 
 
@@ -481,6 +512,20 @@ def test_nan_keys_reach_only_rows_that_see_them(K, rows):
     torch.cuda.synchronize()
     s.check(window=20)
     assert not np.isnan(_np(s.out)).any()
+
+
+@pytest.mark.parametrize("with_lse", [True, False])
+@pytest.mark.parametrize("rows,group", [(2, 64), (70, 64), (70, 32), (70, 128)])
+def test_scores_that_rise_along_the_keys(K, rows, group, with_lse):
+    """Scores that grow (or fall, by the sign of a row's sum) by some 60 binary orders: the running reference of the
+    exponents has to move several times."""
+    def ramp(k, v):
+        k += np.linspace(0, 40, len(k))[:, None, None]
+
+    s = Served(K, 29, [(rows, 900)], 4, 2, 128, group, 64, "bf16", edit=ramp)
+    s.operator(with_lse=with_lse).encode()
+    torch.cuda.synchronize()
+    s.check()
 
 
 @pytest.mark.parametrize("rows", [1, 40])
