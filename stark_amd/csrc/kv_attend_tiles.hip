@@ -204,7 +204,7 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
     const kv::Request r = request_of(a, b);
     const uint32_t rows = (uint32_t)r.q_len * a.ratio;
     if (rows <= a.row_limit) return;
-    const uint32_t mine = (rows + kv::kTileRows - 1) / (kv::kTileRows);  // row tiles of this request
+    const uint32_t mine = (rows + kv::kTileRows - 1) / kv::kTileRows;  // row tiles of this request
     if (turn >= mine) return;
     const uint32_t tile = turn < (mine + 1) / 2 ? mine - 1 - turn : turn - (mine + 1) / 2;
 
@@ -546,7 +546,7 @@ __global__ __launch_bounds__(256) void kv_attend_tiles_join(AttendArgs a) {
 template <int DIM, int G>
 stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
     const uint64_t blocks = (uint64_t)a.cache.kv_heads * a.tiles * a.batch * a.pieces;
-    if (blocks >= 1ull << 22) return STARK_QMM_UNSUPPORTED;
+    if (blocks >= 1ull << 24) return STARK_QMM_UNSUPPORTED;
     if (a.lse || !a.is_bf16) hipLaunchKernelGGL((kv_attend_tiles<DIM, G, true>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
     else hipLaunchKernelGGL((kv_attend_tiles<DIM, G, false>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
     QMM_HIP_CHECK(hipGetLastError());

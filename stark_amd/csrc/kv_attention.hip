@@ -102,6 +102,7 @@ stark_qmm_status stark_qmm_kv_attention(const stark_qmm_kv_attention_args* p, vo
     if (!kv_rows_ok(p->q, p->q_token_stride, p->q_head_stride, a.tokens, a.heads, a.cache.dim, p->data_type) ||
         !kv_rows_ok(p->out, p->out_token_stride, p->out_head_stride, a.tokens, a.heads, a.cache.dim, p->data_type))
         return STARK_QMM_INVALID_ARGUMENT;
+    if (p->q == p->out) return STARK_QMM_INVALID_ARGUMENT;  // workgroups read rows that others would have written
     uint64_t need = 0;
     st = plan_work(&a, &need);
     if (st != STARK_QMM_OK) return st;

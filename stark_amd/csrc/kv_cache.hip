@@ -538,6 +538,9 @@ stark_qmm_status stark_qmm_kv_append(const stark_qmm_kv_append_args* p, void* st
     if (p->q && (!kv_rows_ok(p->q, p->q_token_stride, p->q_head_stride, p->tokens, heads, dim, dt) ||
                  !kv_rows_ok(p->q_out, p->q_out_token_stride, p->q_out_head_stride, p->tokens, heads, dim, dt)))
         return STARK_QMM_INVALID_ARGUMENT;
+    if (p->q && p->q == p->q_out && ((p->tokens > 1 && p->q_token_stride != p->q_out_token_stride) ||
+                                     (heads > 1 && p->q_head_stride != p->q_out_head_stride)))
+        return STARK_QMM_INVALID_ARGUMENT;  // a row would be written where another is still to be read
     const stark_qmm_rotary& r = p->rotary;
     if (r.rotary_dim) {
         if (r.rotary_dim % 16 || r.rotary_dim > dim || r.axes < 1 || r.axes > 4) return STARK_QMM_INVALID_ARGUMENT;

@@ -287,7 +287,8 @@ def test_append_refusals():
                 dict(tokens=2 ** 24 + 1), dict(rot, rotary__rotary_dim=24), dict(rot, rotary__rotary_dim=144),
                 dict(rot, rotary__axes=0), dict(rot, rotary__axes=5), dict(rot, rotary__table=None),
                 dict(rot, rotary__table=FAKE + 4), dict(rot, rotary__positions=None), dict(rot, rotary__table_rows=2 ** 31),
-                dict(rot, rotary__axes=2, rotary__position_stride=3)):
+                dict(rot, rotary__axes=2, rotary__position_stride=3), dict(q_out=FAKE, q_out_token_stride=17 * 128),
+                dict(q_out=FAKE, q_out_head_stride=256, q_out_token_stride=32 * 128)):
         assert call(C.byref(_append(**bad)), None) == Q.INVALID_ARGUMENT, bad
     s = _append(**rot)
     s.rotary.axis_of_pair[63] = 1
@@ -322,7 +323,8 @@ def test_attention_refusals():
     def args(**kw):
         s = K._AttentionArgs()
         s.struct_size, s.cache, s.data_type = C.sizeof(s), _cache(), Q.BF16
-        s.q = s.out = s.block_table = s.query_start = s.kv_lengths = FAKE
+        s.q = s.block_table = s.query_start = s.kv_lengths = FAKE
+        s.out = FAKE + 2 ** 16
         s.batch, s.tokens, s.heads, s.table_stride, s.max_query, s.max_kv = 2, 4, 16, 8, 2, 512
         s.q_token_stride = s.out_token_stride = 16 * 128
         s.q_head_stride = s.out_head_stride = 128
@@ -340,7 +342,7 @@ def test_attention_refusals():
     for bad in (dict(heads=0), dict(heads=12), dict(heads=65536 + 8), dict(batch=2 ** 20 + 1), dict(tokens=2 ** 24 + 1),
                 dict(max_kv=2 ** 31), dict(table_stride=0), dict(table_stride=2 ** 25), dict(scale=float("nan")),
                 dict(scale=float("inf")), dict(soft_cap=-1.0), dict(soft_cap=float("nan")), dict(soft_cap=float("inf")),
-                dict(q=None), dict(out=None), dict(block_table=None), dict(query_start=None), dict(kv_lengths=None),
+                dict(q=None), dict(out=None), dict(out=FAKE), dict(block_table=None), dict(query_start=None), dict(kv_lengths=None),
                 dict(q=FAKE + 1), dict(lse=FAKE + 2), dict(q_head_stride=64), dict(out_token_stride=128),
                 dict(max_kv=2 ** 31 - 1, table_stride=2 ** 25 - 1)):
         assert call(args(**bad), None) == Q.INVALID_ARGUMENT, bad
