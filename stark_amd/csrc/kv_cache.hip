@@ -9,7 +9,6 @@ using namespace qmm;
 // ---------------------------------------------------------------- plan
 
 constexpr uint32_t kPlanThreads = 256;
-constexpr uint32_t kPlanTokens = 1024;  // tokens of a workgroup
 
 struct PlanArgs {
     const int32_t *cached, *added, *free_pages, *free_count;
@@ -32,17 +31,20 @@ QMM_DEVICE int64_t plan_scan(int64_t v, int64_t* part) {
     return v;
 }
 
-// One launch, no workspace: every workgroup scans the lengths of all requests itself (256 at a time) and then
-// handles 1024 of the new tokens. Each new page holds exactly one new token at its start, and that token's thread
-// writes the block table's entry. Bound by latency (two dependent reads and two scans per 256 requests), not by bytes: 3.3 us
-// for 8 requests, 7.8 for 512.
+// One launch, no workspace: every workgroup scans the lengths of all requests itself (256 N at a time, N neighbours to a
+// thread) and then handles 256 of the new tokens. Each new page holds exactly one new token at its start, and that token's
+// thread writes the block table's entry. Bound by latency (two dependent reads and two scans a pass, then a table entry's
+// read), not by bytes: 3.3 us for 8 requests of one token, 4.7 for 512 with 24 chunks, 11.4 for 4096. With one request a
+// thread 5.5 and 25 (but 4.2 against 4.5 for 256), with 1024 tokens a workgroup 7.0 and 14.7.
+template <int N>
 __global__ __launch_bounds__(kPlanThreads) void kv_plan(PlanArgs a) {
+    constexpr uint32_t kPass = kPlanThreads * N;  // requests
     __shared__ int64_t part[4];
-    __shared__ int32_t start[kPlanThreads + 1], had[kPlanThreads], before[kPlanThreads];
-    __shared__ int32_t first_page[kPlanThreads];
+    __shared__ int32_t start[kPass + 1], had[kPass], before[kPass];
+    __shared__ int32_t first_page[kPass];
     __shared__ int64_t total[2];
     __shared__ uint32_t all_flags;
-    const uint32_t t = threadIdx.x, n0 = blockIdx.x * kPlanTokens;
+    const uint32_t t = threadIdx.x, token = blockIdx.x * kPlanThreads + t;
     const int32_t capacity = (int32_t)a.capacity;
     const int32_t free_count = min(max(*a.free_count, 0), (int32_t)a.free_capacity);
     const int32_t page_mask = (1 << a.page_shift) - 1;
@@ -50,37 +52,55 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan(PlanArgs a) {
     uint32_t flags = 0;
     const bool first = blockIdx.x == 0;
     if (first && t == 0) a.query_start[0] = 0;
-    for (uint32_t r0 = 0; r0 < a.batch; r0 += kPlanThreads) {
-        const uint32_t r = r0 + t;
-        const bool live = r < a.batch;
-        int32_t c = live ? a.cached[r] : 0, n = live ? a.added[r] : 0;
-        if (c < 0 || n < 0) flags |= STARK_QMM_KV_BAD_LENGTH;
-        c = max(c, 0), n = max(n, 0);
-        const int64_t end = tokens + plan_scan(n, part);
-        if (end > capacity) flags |= STARK_QMM_KV_TOO_MANY_TOKENS;
-        const int32_t s = (int32_t)min(end - n, (int64_t)capacity), e = (int32_t)min(end, (int64_t)capacity);
-        const kv::PagePlan p = kv::page_plan(c, e - s, a.page_shift, a.stride);
-        const int64_t held = (int64_t)a.stride << a.page_shift;
-        if (c + (int64_t)(e - s) > held) flags |= STARK_QMM_KV_TABLE_FULL;
-        const int64_t last = pages + plan_scan(p.need, part);
-        if (last > free_count && p.need) flags |= STARK_QMM_KV_OUT_OF_PAGES;
-        start[t] = s, had[t] = c, before[t] = p.before;
-        first_page[t] = (int32_t)min(last - p.need, (int64_t)0x7fffffff);
-        if (t == kPlanThreads - 1) start[kPlanThreads] = e;
-        if (first && live) {
-            a.query_start[r + 1] = e;
-            a.kv_lengths[r] = (int32_t)min((int64_t)c + (e - s), (int64_t)0x7fffffff);
-        }
-        if (t == kPlanThreads - 1) total[0] = end, total[1] = last;
-        __syncthreads();
-        const int32_t lo = start[0], hi = start[kPlanThreads];
-        for (uint32_t n = n0 + t; n < min(n0 + kPlanTokens, a.capacity); n += kPlanThreads) {
-            if ((int32_t)n < lo || (int32_t)n >= hi) continue;
-            uint32_t b = 0;  // last request that starts at or before n (empty ones behind it start later or hold nothing)
+    for (uint32_t r0 = 0; r0 < a.batch; r0 += kPass) {
+        const uint32_t r = r0 + t * N;
+        int32_t c[N], n[N];
+        int64_t added = 0, need = 0;  // of the thread's requests
 #pragma unroll
-            for (uint32_t step = kPlanThreads / 2; step; step >>= 1)
-                if (start[b + step] <= (int32_t)n) b += step;
-            const int64_t pos = (int64_t)had[b] + ((int32_t)n - start[b]);
+        for (int i = 0; i < N; ++i) {
+            const bool live = r + i < a.batch;
+            c[i] = live ? a.cached[r + i] : 0, n[i] = live ? a.added[r + i] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if (c[i] < 0 || n[i] < 0) flags |= STARK_QMM_KV_BAD_LENGTH;
+            c[i] = max(c[i], 0), n[i] = max(n[i], 0);
+            added += n[i];
+        }
+        int64_t end = tokens + plan_scan(added, part) - added;
+        int32_t s[N], e[N], need_i[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            s[i] = (int32_t)min(end, (int64_t)capacity);
+            end += n[i];
+            if (end > capacity && n[i]) flags |= STARK_QMM_KV_TOO_MANY_TOKENS;
+            e[i] = (int32_t)min(end, (int64_t)capacity);
+            const kv::PagePlan p = kv::page_plan(c[i], e[i] - s[i], a.page_shift, a.stride);
+            const int64_t held = (int64_t)a.stride << a.page_shift;
+            if (c[i] + (int64_t)(e[i] - s[i]) > held) flags |= STARK_QMM_KV_TABLE_FULL;
+            need_i[i] = p.need, need += p.need;
+            start[t * N + i] = s[i], had[t * N + i] = c[i], before[t * N + i] = p.before;
+        }
+        int64_t last = pages + plan_scan(need, part) - need;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            first_page[t * N + i] = (int32_t)min(last, (int64_t)0x7fffffff);
+            last += need_i[i];
+            if (last > free_count && need_i[i]) flags |= STARK_QMM_KV_OUT_OF_PAGES;
+            if (first && r + i < a.batch) {
+                a.query_start[r + i + 1] = e[i];
+                a.kv_lengths[r + i] = (int32_t)min((int64_t)c[i] + (e[i] - s[i]), (int64_t)0x7fffffff);
+            }
+        }
+        if (t == kPlanThreads - 1) start[kPass] = e[N - 1], total[0] = end, total[1] = last;
+        __syncthreads();
+        const int32_t lo = start[0], hi = start[kPass];
+        if (token < a.capacity && (int32_t)token >= lo && (int32_t)token < hi) {
+            uint32_t b = 0;  // last request that starts at or before it (empty ones behind it start later or hold nothing)
+#pragma unroll
+            for (uint32_t step = kPass / 2; step; step >>= 1)
+                if (start[b + step] <= (int32_t)token) b += step;
+            const int64_t pos = (int64_t)had[b] + ((int32_t)token - start[b]);
             const int64_t page = pos >> a.page_shift;
             int32_t id = -1;
             if (page < (int64_t)a.stride) {
@@ -94,14 +114,13 @@ __global__ __launch_bounds__(kPlanThreads) void kv_plan(PlanArgs a) {
                 }
             }
             const int64_t slot = id < 0 ? -1 : ((int64_t)id << a.page_shift) + (pos & page_mask);
-            a.slots[n] = slot > 0x7fffffff ? -1 : (int32_t)slot;
-            a.positions[n] = (int32_t)min(pos, (int64_t)0x7fffffff);
+            a.slots[token] = slot > 0x7fffffff ? -1 : (int32_t)slot;
+            a.positions[token] = (int32_t)min(pos, (int64_t)0x7fffffff);
         }
         tokens = total[0], pages = total[1];
         __syncthreads();
     }
-    for (uint32_t n = n0 + t; n < min(n0 + kPlanTokens, a.capacity); n += kPlanThreads)
-        if ((int64_t)n >= tokens) a.slots[n] = -1, a.positions[n] = 0;
+    if (token < a.capacity && (int64_t)token >= tokens) a.slots[token] = -1, a.positions[token] = 0;
     if (!first) return;
     if (t == 0) all_flags = 0;
     __syncthreads();
@@ -513,8 +532,9 @@ stark_qmm_status stark_qmm_kv_plan(const stark_qmm_kv_plan_args* p, void* stream
     PlanArgs a{p->cached, p->added, p->free_pages, p->free_count, p->block_table, p->query_start, p->kv_lengths, p->slots,
                p->positions, p->free_left, p->status, p->batch, p->token_capacity, p->free_capacity, p->table_stride, 4};
     while ((1u << a.page_shift) < p->page_size) ++a.page_shift;
-    const uint32_t blocks = std::max(1u, (p->token_capacity + kPlanTokens - 1) / kPlanTokens);
-    hipLaunchKernelGGL(kv_plan, dim3(blocks), dim3(kPlanThreads), 0, (hipStream_t)stream, a);
+    const uint32_t blocks = std::max(1u, (p->token_capacity + kPlanThreads - 1) / kPlanThreads);
+    if (p->batch <= kPlanThreads) hipLaunchKernelGGL(kv_plan<1>, dim3(blocks), dim3(kPlanThreads), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL(kv_plan<4>, dim3(blocks), dim3(kPlanThreads), 0, (hipStream_t)stream, a);
     QMM_HIP_CHECK(hipGetLastError());
     return STARK_QMM_OK;
 }
