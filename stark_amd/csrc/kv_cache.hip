@@ -1,5 +1,7 @@
 // 4-bit paged key/value cache: the plan of a step, the append of new rows (after the rotary embedding) and the
 // read of rows back. Attention over the cache: kv_attention.hip; layout: kv_layout.h.
+#include <type_traits>
+
 #include "kv_common.h"
 
 namespace {
@@ -204,15 +206,26 @@ QMM_DEVICE double fifteenth(double v) {
 // The value of another lane of the 16 that share a register row: the lane that CTRL names (quad permutation, or the mirror
 // image of 8 or 16 lanes).
 template <int CTRL>
-QMM_DEVICE double lane_f64(double v) {
-    const uint2 w = __builtin_bit_cast(uint2, v);
-    return __builtin_bit_cast(double, uint2{(uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.x, CTRL, 0xf, 0xf, true),
-                                            (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w.y, CTRL, 0xf, 0xf, true)});
+QMM_DEVICE uint32_t of_lane(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
 }
 template <int CTRL>
-QMM_DEVICE void widen_range(double& lo, double& hi) {
-    const double l = lane_f64<CTRL>(lo), h = lane_f64<CTRL>(hi);
-    lo = fmin(lo, l), hi = fmax(hi, h);
+QMM_DEVICE float of_lane(float v) {
+    return __uint_as_float(of_lane<CTRL>(__float_as_uint(v)));
+}
+template <int CTRL>
+QMM_DEVICE double of_lane(double v) {
+    const uint2 w = __builtin_bit_cast(uint2, v);
+    return __builtin_bit_cast(double, uint2{of_lane<CTRL>(w.x), of_lane<CTRL>(w.y)});
+}
+QMM_DEVICE float least(float a, float b) { return fminf(a, b); }
+QMM_DEVICE double least(double a, double b) { return fmin(a, b); }
+QMM_DEVICE float most(float a, float b) { return fmaxf(a, b); }
+QMM_DEVICE double most(double a, double b) { return fmax(a, b); }
+template <int CTRL, typename T>
+QMM_DEVICE void widen_range(T& lo, T& hi) {
+    const T l = of_lane<CTRL>(lo), h = of_lane<CTRL>(hi);
+    lo = least(lo, l), hi = most(hi, h);
 }
 
 // A row (a head of a token) to DIM / 8 lanes of a wave, eight neighbouring values a lane; a thread does every sets-th
@@ -220,8 +233,8 @@ QMM_DEVICE void widen_range(double& lo, double& hi) {
 // Keys in f64: a rotated value a c - b s of f32 factors has exact products and one rounding there, and codes, scales and
 // biases come out as from exact arithmetic (an f32 sum or quotient beside a half way point would take the wrong code, one
 // step of the group's range / 15). Queries in f32: they are rounded once more in any case.
-// Bound by latency and vector work together: 2048 tokens of 32 + 2 * 8 heads of 128 (44 MB, 9 us as a copy) take 14.2 us,
-// 178 vector instructions a wave and row (7 us) after three dependent reads (positions, rotation, rows). One row a thread
+// Bound by latency and vector work together: 2048 tokens of 32 + 2 * 8 heads of 128 (44 MB, 9 us as a copy) take 14.5 us,
+// about 170 vector instructions a wave and row (7 us) after two dependent reads (positions, rotation). One row a thread
 // took 23 us and all rows as 2^17 or 2^19 threads 16 and 16.5.
 template <int DIM, uint32_t DT>
 __global__ __launch_bounds__(256) void kv_append(AppendArgs a) {
@@ -235,41 +248,8 @@ __global__ __launch_bounds__(256) void kv_append(AppendArgs a) {
     const bool turns = d < 2 * pairs;
     // the rotation partner's values: the same eight (interleaved), or those half the rotated width away
     const bool high = !a.rot.interleaved && d >= pairs;
-    float2 cs[8];
-    if (turns && set < a.heads + a.cache.kv_heads) {
-        const uint32_t p0 = a.rot.interleaved ? d / 2 : high ? d - pairs : d;  // this lane's first pair
-        const uint32_t np = a.rot.interleaved ? 4 : 8;
-        const uint32_t axes = a.rot.axis8[p0 / 8] >> (2 * (p0 % 8));
-        const float2 nan = {__builtin_nanf(""), __builtin_nanf("")};
-        uint32_t pos[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            pos[e] = (uint32_t)a.rot.positions[(axes >> (2 * ((uint32_t)e < np ? e : 0)) & 3) * a.rot.position_stride + token];
-        if (a.rot.one_axis) {
-            const float4* row = (const float4*)(a.rot.table + (size_t)(pos[0] < a.rot.rows ? pos[0] : 0) * pairs + p0);
-            float4 v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = row[(uint32_t)e < np / 2 ? e : 0];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) cs[2 * e] = float2{v[e].x, v[e].y}, cs[2 * e + 1] = float2{v[e].z, v[e].w};
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                cs[e] = a.rot.table[(size_t)(pos[e] < a.rot.rows ? pos[e] : 0) * pairs + p0 + ((uint32_t)e < np ? e : 0)];
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (pos[e] >= a.rot.rows) cs[e] = nan;
-    }
-    const uint32_t slot = (uint32_t)a.slots[token];
-    const uint32_t page = slot >> a.cache.page_shift, page_size = 1u << a.cache.page_shift;
-    const bool stored = page < a.cache.page_count;
-    const uint32_t in_page = slot & (page_size - 1), t = in_page % kv::kTile;
-    uint8_t* const in_cache = a.cache.data + (uint64_t)(stored ? page : 0) * a.cache.page_bytes + in_page / kv::kTile * a.cache.record;
-    const uint32_t half_rec = kv::codes_bytes(DIM) + kv::planes_bytes(a.cache.groups), gl = L / a.cache.groups;
-
     // A row as this lane holds it: its own values, and its rotation partner's where they are elsewhere. The next row is
-    // read before this one is worked on.
+    // read before this one is worked on, and the first before the rotation.
     struct Row {
         Eight<DT> x, o;
     };
@@ -281,50 +261,89 @@ __global__ __launch_bounds__(256) void kv_append(AppendArgs a) {
         if (partner) r.o.load(src, token, head, od);
         return r;
     };
-    const uint32_t kvh = a.cache.kv_heads;
+    const uint32_t kvh = a.cache.kv_heads, slot = (uint32_t)a.slots[token];
+    Row r;
+    if (set < a.heads) r = fetch(a.q, set, elsewhere);
+    else if (set < a.heads + kvh) r = fetch(a.k, set - a.heads, elsewhere);
+    else r.x.load(a.v, token, set - a.heads - kvh, d);
+    float2 cs[8];
+    if (turns && set < a.heads + a.cache.kv_heads) {
+        const uint32_t p0 = a.rot.interleaved ? d / 2 : high ? d - pairs : d;  // this lane's first pair
+        const uint32_t np = a.rot.interleaved ? 4 : 8;
+        const uint32_t axes = a.rot.axes > 1 ? a.rot.axis8[p0 / 8] >> (2 * (p0 % 8)) : 0;
+        const auto position = [&](uint32_t axis) { return (uint32_t)a.rot.positions[axis * a.rot.position_stride + token]; };
+        const float2 nan = {__builtin_nanf(""), __builtin_nanf("")};
+        if (a.rot.one_axis) {
+            const uint32_t pos = position(axes & 3);
+            const float4* row = (const float4*)(a.rot.table + (size_t)(pos < a.rot.rows ? pos : 0) * pairs + p0);
+            float4 v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = row[(uint32_t)e < np / 2 ? e : 0];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) cs[2 * e] = float2{v[e].x, v[e].y}, cs[2 * e + 1] = float2{v[e].z, v[e].w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (pos >= a.rot.rows) cs[e] = nan;
+        } else {
+            uint32_t pos[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pos[e] = position(axes >> (2 * ((uint32_t)e < np ? e : 0)) & 3);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                cs[e] = a.rot.table[(size_t)(pos[e] < a.rot.rows ? pos[e] : 0) * pairs + p0 + ((uint32_t)e < np ? e : 0)];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                if (pos[e] >= a.rot.rows) cs[e] = nan;
+        }
+    }
+    const uint32_t page = slot >> a.cache.page_shift, page_size = 1u << a.cache.page_shift;
+    const bool stored = page < a.cache.page_count;
+    const uint32_t in_page = slot & (page_size - 1), t = in_page % kv::kTile;
+    uint8_t* const in_cache = a.cache.data + (uint64_t)(stored ? page : 0) * a.cache.page_bytes + in_page / kv::kTile * a.cache.record;
+    const uint32_t half_rec = kv::codes_bytes(DIM) + kv::planes_bytes(a.cache.groups), gl = L / a.cache.groups;
+
     // Scale and bias of the lane's group into a record half, and the lane's eight codes.
-    auto quantise = [&](const double* y, uint8_t* rec) {
+    auto quantise = [&](const auto* y, uint8_t* rec) {
+        using T = std::remove_cv_t<std::remove_reference_t<decltype(*y)>>;
         // group minimum and maximum; a value that the format does not hold makes the minimum -inf
-        double lo = y[0], hi = y[0];
+        T lo = y[0], hi = y[0];
         bool bad = false;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            lo = fmin(lo, y[e]), hi = fmax(hi, y[e]);
-            bad |= !(fabs(y[e]) <= (double)kv::kLimit);
+            lo = least(lo, y[e]), hi = most(hi, y[e]);
+            bad |= !(fabs(y[e]) <= (T)kv::kLimit);
         }
-        if (bad) lo = -__builtin_inf();
+        if (bad) lo = -(T)__builtin_inf();
         widen_range<0xb1>(lo, hi);  // lanes 1 0 3 2, then 2 3 0 1: groups of 4 lanes
         widen_range<0x4e>(lo, hi);
         if (gl > 4) widen_range<0x141>(lo, hi);  // mirror of 8 lanes
         if (gl > 8) widen_range<0x140>(lo, hi);  // mirror of 16
-        bad = !(lo >= -(double)kv::kLimit);
-        const uint32_t sb = bad ? 0x7e00u : f64_to_f16_bits(fifteenth(hi - lo));
-        const uint32_t bb = bad ? 0x7e00u : f64_to_f16_bits(lo);
-        const double s = (double)f16_bits_to_f32(sb), b = (double)f16_bits_to_f32(bb);
+        bad = !(lo >= -(T)kv::kLimit);
+        const uint32_t sb = bad ? 0x7e00u : f64_to_f16_bits(fifteenth((double)hi - (double)lo));
+        const uint32_t bb = bad ? 0x7e00u : f64_to_f16_bits((double)lo);
+        const float s = f16_bits_to_f32(sb), b = f16_bits_to_f32(bb);
         if (stored && l % gl == 0) *(uint32_t*)(rec + kv::codes_bytes(DIM) + kv::plane_word(t, l / gl)) = sb | bb << 16;
         uint32_t w = 0;
-        if (s > 0.0) {
+        if (s > 0.0f) {
             // The code is the nearest step, ties to even, of exact arithmetic. In f32 the quotient is off by less than
             // 2^-18 of its 0 .. 16; where that could matter (within 2^-16 of half way between two codes) f64 decides.
-            const float inverse = __builtin_amdgcn_rcpf((float)s);
+            const float inverse = __builtin_amdgcn_rcpf(s);
             float far = 0.0f;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float t = (float)(y[e] - b) * inverse, n = rintf(t);
+                const float t = (float)(y[e] - (T)b) * inverse, n = rintf(t);
                 far = fmaxf(far, fabsf(t - n));
                 w |= (uint32_t)fminf(fmaxf(n, 0.0f), 15.0f) << (4 * e);
             }
             if (far > 0.5f - 0x1p-16f) {
                 w = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) w |= (uint32_t)fmin(fmax(rint((y[e] - b) / s), 0.0), 15.0) << (4 * e);
+                for (int e = 0; e < 8; ++e) w |= (uint32_t)fmin(fmax(rint(((double)y[e] - (double)b) / (double)s), 0.0), 15.0) << (4 * e);
             }
         }
         return w;
     };
     uint32_t h = set;
-    Row r;
-    if (h < a.heads) r = fetch(a.q, h, elsewhere);
     for (; h < a.heads; h += a.sets) {
         const Row now = r;
         if (h + a.sets < a.heads) r = fetch(a.q, h + a.sets, elsewhere);
@@ -347,7 +366,7 @@ __global__ __launch_bounds__(256) void kv_append(AppendArgs a) {
         y.store(a.q_out, token, h, d);
     }
     h -= a.heads;
-    if (h < kvh) r = fetch(a.k, h, elsewhere);
+    if (set < a.heads && h < kvh) r = fetch(a.k, h, elsewhere);
     for (; h < kvh; h += a.sets) {
         const Row now = r;
         if (h + a.sets < kvh) r = fetch(a.k, h + a.sets, elsewhere);
@@ -378,13 +397,13 @@ __global__ __launch_bounds__(256) void kv_append(AppendArgs a) {
         if (stored) *(uint32_t*)(rec + kv::key_word(DIM, t, l)) = w;
     }
     h -= kvh;
-    if (h < kvh) r.x.load(a.v, token, h, d);
+    if (set < a.heads + kvh && h < kvh) r.x.load(a.v, token, h, d);
     for (; h < kvh; h += a.sets) {
         const Eight<DT> now = r.x;
         if (h + a.sets < kvh) r.x.load(a.v, token, h + a.sets, d);
-        double y[8];
+        float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = (double)now.get(e);
+        for (int e = 0; e < 8; ++e) y[e] = now.get(e);
         uint8_t* rec = in_cache + (uint64_t)h * a.cache.head_bytes + half_rec;
         const uint32_t w = quantise(y, rec);
         // value bytes: byte i of lane r is byte r % 4 of code word 4 i + r / 4 (of its half of the head). The exchange is
