@@ -16,7 +16,10 @@ struct Shape {
 
 // The keys of a step of one kv head as a wave's loads leave them: code words, and of the planes each word in one lane
 // only (lane 32 i + 16 v + t of pair h: record 2 h + i, keys' planes (v = 0) or values', token t).
-template <int DIM, int G, int T>
+// STREAM: loads that leave the caches to others, for blocks of 8 rows: no other workgroup reads the same codes (us with and
+// without, 64 requests of 4000 keys and 4 rows 58 and 66). A head's blocks of 16 rows may be several and share them (64 of 16
+// to 40 rows and 900 to 9000 keys 62 and 57, 16 of 32 rows 40.2 and 37.5, 16 of 12 rows 27.1 and 25.6; 64 of 12 rows 67 and 70).
+template <int DIM, int G, int T, bool STREAM>
 struct Step {
     uint32_t kc[T][DIM / 32], vc[T][DIM / 32], plane[T / 2][G];
     uint32_t absent;  // bit i: record i's page is not in the cache
@@ -34,13 +37,13 @@ struct Step {
             const uint8_t* kq = base + rec[i] + (DIM == 64 ? c * 32 + g * 8 : c * 64 + g * 16);
             const uint8_t* vq = base + rec[i] + 8 * DIM + 64 * G + lane * (DIM == 64 ? 8 : 16);
             if (DIM == 64) {
-                *(u32x2*)&kc[i][0] = __builtin_nontemporal_load((const u32x2*)kq);
-                *(u32x2*)&vc[i][0] = __builtin_nontemporal_load((const u32x2*)vq);
+                *(u32x2*)&kc[i][0] = STREAM ? __builtin_nontemporal_load((const u32x2*)kq) : *(const u32x2*)kq;
+                *(u32x2*)&vc[i][0] = STREAM ? __builtin_nontemporal_load((const u32x2*)vq) : *(const u32x2*)vq;
             } else {
 #pragma unroll
                 for (int h = 0; h < DIM / 128; ++h) {
-                    *(u32x4*)&kc[i][4 * h] = load_stream(kq + 1024 * h);
-                    *(u32x4*)&vc[i][4 * h] = load_stream(vq + 1024 * h);
+                    *(u32x4*)&kc[i][4 * h] = STREAM ? load_stream(kq + 1024 * h) : *(const u32x4*)(kq + 1024 * h);
+                    *(u32x4*)&vc[i][4 * h] = STREAM ? load_stream(vq + 1024 * h) : *(const u32x4*)(vq + 1024 * h);
                 }
             }
         }
@@ -199,6 +202,7 @@ QMM_DEVICE uint32_t wave_scan(uint32_t v) {
 template <int DIM, int G, int PACK>
 __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(AttendArgs a) {
     using S = Shape<PACK>;
+    using Codes = Step<DIM, G, S::T, PACK == 2>;
     constexpr int R = S::R, T = S::T, KEYS = S::KEYS, B = S::B;
     constexpr int J = DIM / 32;       // k blocks of a score product, and 32-value blocks of the output
     constexpr int JG = J / G;         // of one scale group
@@ -299,12 +303,12 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
         const uint32_t steps = s0 + wave < s1 ? (s1 - s0 - wave + 3) / 4 : 0, mine = (uint32_t)from + KEYS * wave;
         PageIds<T> pages{a.table + (size_t)b * a.stride, mine, 4 * KEYS, a.cache.page_shift, a.stride - 1, 0, 0};
         const uint8_t* base = a.cache.data + (uint64_t)head * a.cache.head_bytes;
-        const auto load = [&](Step<DIM, G, T>& st, uint32_t n) {
+        const auto load = [&](Codes& st, uint32_t n) {
             uint32_t page[T];
             pages.get(n, lane, page);
             st.load(a.cache, base, page, mine + 4 * KEYS * n, lane);
         };
-        Step<DIM, G, T> st[2];
+        Codes st[2];
         if (steps) {
             pages.fill(0, lane);
             load(st[0], 0);
@@ -386,7 +390,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
             smax = max(smax, (uint32_t)__shfl_xor((int)smax, 32, 64));
             return smax ? 8 - ilogbf(f16_bits_to_f32(smax)) : 0;
         };
-        const auto step = [&](Step<DIM, G, T>& st, uint32_t n) {
+        const auto step = [&](Codes& st, uint32_t n) {
             const int32_t t0 = (int32_t)(mine + 4 * KEYS * n);
 #pragma unroll
             for (int h = 0; h < T / 2; ++h)
