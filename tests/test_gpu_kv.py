@@ -74,7 +74,8 @@ def _run_plan(K, cached, added, free, count, table, page, capacity):
 
 
 @pytest.mark.parametrize("batch,page,chunk,idle", [(1, 16, 1, 0.0), (8, 64, 1, 0.3), (5, 16, 40, 0.0), (255, 32, 9, 0.2),
-                                                   (256, 16, 3, 0.5), (257, 128, 200, 0.1), (700, 16, 5, 0.9), (3, 1024, 3000, 0)])
+                                                   (256, 16, 3, 0.5), (257, 128, 200, 0.1), (700, 16, 5, 0.9), (3, 1024, 3000, 0), (1024, 16, 2, 0.5),
+                                                   (1025, 32, 3, 0.2), (2300, 16, 1, 0.6)])
 def test_plan(K, batch, page, chunk, idle):
     cached, added, table, free = _plan_case(np.random.default_rng(batch), batch, page, 4, chunk, idle)
     _run_plan(K, cached, added, free, len(free), table, page, int(added.sum()) + 5)
