@@ -604,7 +604,7 @@ typedef struct stark_qmm_rotary {
     const float* table;          /* [table_rows, rotary_dim / 2] pairs (cos, sin), 8-byte aligned */
     const int32_t* positions;    /* [axes] rows of position_stride */
     uint64_t position_stride;
-    uint32_t table_rows;
+    uint32_t table_rows;         /* at least 1 */
     uint32_t rotary_dim;         /* multiple of 16, <= head_dim; 0: no rotation */
     uint32_t axes;               /* 1 .. 4 */
     uint32_t interleaved;

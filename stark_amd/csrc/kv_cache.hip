@@ -584,7 +584,7 @@ stark_qmm_status stark_qmm_kv_append(const stark_qmm_kv_append_args* p, void* st
     if (r.rotary_dim) {
         if (r.rotary_dim % 16 || r.rotary_dim > dim || r.axes < 1 || r.axes > 4) return STARK_QMM_INVALID_ARGUMENT;
         if (!r.table || !kv_aligned(r.table, 8) || !r.positions || !kv_aligned(r.positions, 4) ||
-            r.table_rows > 0x7fffffffu || (r.axes > 1 && (r.position_stride < p->tokens || r.position_stride >> 32)))
+            r.table_rows == 0 || r.table_rows > 0x7fffffffu || (r.axes > 1 && (r.position_stride < p->tokens || r.position_stride >> 32)))
             return STARK_QMM_INVALID_ARGUMENT;
         a.rot = Rotary{(const float2*)r.table, r.positions, r.axes > 1 ? r.position_stride : 0, r.table_rows,
                        r.rotary_dim / 2, r.axes, r.interleaved != 0, kv_aligned(r.table, 16), {}};

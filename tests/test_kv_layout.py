@@ -361,3 +361,10 @@ def test_the_plain_plan_gives_each_token_one_slot():
     used = p["slots"][:sum(added)]
     assert len(set(used)) == sum(added) and (used >= 0).all() and (p["slots"][sum(added):] == -1).all()
     assert p["status"][0] == 0 and list(np.diff(p["query_start"])) == added
+
+
+def test_a_rotation_table_without_rows_is_refused():
+    """A position outside the table gives NaN, but its thread still reads row 0: there has to be one."""
+    from stark_amd import qmm as Q
+    rot = dict(rotary__rotary_dim=128, rotary__axes=1, rotary__table=FAKE, rotary__positions=FAKE, rotary__table_rows=0)
+    assert Q.lib().stark_qmm_kv_append(C.byref(_append(**rot)), None) == Q.INVALID_ARGUMENT
