@@ -54,13 +54,14 @@ stark_qmm_status compute_units(uint32_t* cus) {
 
 // How the checked call's work is dealt, and the bytes that its partial results need.
 stark_qmm_status plan_work(AttendArgs* a, uint64_t* workspace) {
+    *workspace = 0;
+    if (a->batch == 0 || a->max_query == 0) return STARK_QMM_OK;  // (tiling divides by the requests)
     uint32_t cus = 0;
     const stark_qmm_status st = compute_units(&cus);
     if (st != STARK_QMM_OK) return st;
     const kv::Rows rows = kv::row_limit(a->batch, a->max_query, a->ratio, a->max_kv);
     const uint64_t most = (uint64_t)a->max_query * a->ratio;
     a->row_limit = std::min<uint64_t>(rows.limit, most), a->row_block = rows.block;
-    *workspace = 0;
     if (a->row_limit) {
         a->ratio_inverse = (65535 + a->ratio) / a->ratio;
         const uint32_t blocks = (a->row_limit + a->row_block - 1) / a->row_block;

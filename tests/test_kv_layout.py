@@ -368,3 +368,14 @@ def test_a_rotation_table_without_rows_is_refused():
     from stark_amd import qmm as Q
     rot = dict(rotary__rotary_dim=128, rotary__axes=1, rotary__table=FAKE, rotary__positions=FAKE, rotary__table_rows=0)
     assert Q.lib().stark_qmm_kv_append(C.byref(_append(**rot)), None) == Q.INVALID_ARGUMENT
+
+
+def test_the_workspace_of_a_call_without_rows():
+    """No requests, no rows or a bound of none: nothing is launched, so nothing is needed."""
+    from stark_amd import kv as K, qmm as Q
+    for batch, tokens, most in ((0, 100, 100), (0, 5, 1), (3, 0, 7), (3, 100, 0)):
+        s = K._AttentionArgs()
+        s.struct_size, s.cache, s.data_type = C.sizeof(s), _geometry(), Q.BF16
+        s.batch, s.tokens, s.heads, s.table_stride, s.max_query, s.max_kv = batch, tokens, 8, 64, most, 4096
+        n = C.c_uint64(77)
+        assert Q.lib().stark_qmm_kv_attention_workspace_size(C.byref(s), C.byref(n)) == Q.OK and n.value == 0
