@@ -1,6 +1,8 @@
 // Shared by the attention kernels over the 4-bit paged key/value cache.
 #pragma once
 
+#include <float.h>
+
 #include "kv_common.h"
 
 namespace qmm {

@@ -330,30 +330,34 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
             }
             top = fmaxf(top, __shfl_xor(top, 16, 64));
             top = fmaxf(top, __shfl_xor(top, 32, 64));
-            // 2^k puts the largest in [2^13, 2^14)
+            // 2^k puts the largest in [2^13, 2^14). Sums are of the scaled values, and the keys' scales bring the codes' 2^-24
+            // back: no factor passes f32 where the scores do not. (The least of f32's largest: 0 stays 0 under any scale.)
             const int k = live ? 13 - (top > 0.0f && top < INFINITY ? ilogbf(top) : 0) : 0;
+            c1 = fminf(ldexp_f32(a.scale, -k), FLT_MAX);
 #pragma unroll
             for (int gr = 0; gr < G; ++gr) {
                 float s = 0.0f;
 #pragma unroll
                 for (int j = gr * JG; j < (gr + 1) * JG; ++j)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) s += x[j][e];
+                    for (int e = 0; e < 8; ++e) {
+                        x[j][e] = ldexp_f32(x[j][e], k);
+                        s += x[j][e];
+                    }
                 s += __shfl_xor(s, 16, 64);
                 s += __shfl_xor(s, 32, 64);
                 s = live ? s : 0.0f;
-                qsum[gr] = s * a.scale;
-                const float v = -ldexp_f32(s, k - 21);  // -8 sum q, in the accumulator's scale
+                qsum[gr] = s * c1;
+                const float v = s * -0x1p-21f;  // -8 sum q, in the accumulator's scale
                 less8[gr] = f32x4{v, v, v, v};
             }
-            c1 = ldexp_f32(a.scale, 24 - k);
             // every wave has the same rows: wave w writes the blocks w, w + 4, ...
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 // code pairs of a word: nibbles (0, 4), (1, 5) sixteenfold, (2, 6), (3, 7) sixteenfold
                 f16x8 h;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) h[e] = (_Float16)ldexp_f32(x[j][e / 2 + 4 * (e & 1)], (e / 2) & 1 ? k - 4 : k);
+                for (int e = 0; e < 8; ++e) h[e] = (_Float16)(x[j][e / 2 + 4 * (e & 1)] * ((e / 2) & 1 ? 0.0625f : 1.0f));
                 const u32x4 bits = __builtin_bit_cast(u32x4, h);
                 if (j % 4 == (int)wave) sh.q[j][lane] = live ? bits : u32x4{0, 0, 0, 0};
             }
@@ -390,6 +394,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
             smax = max(smax, (uint32_t)__shfl_xor((int)smax, 32, 64));
             return smax ? 8 - ilogbf(f16_bits_to_f32(smax)) : 0;
         };
+        const float plane_factor = lane & 16 ? 1.0f : 0x1p24f;  // on the scales of the lane's plane words: keys' codes are c 2^-24
         const auto step = [&](Codes& st, uint32_t n) {
             const int32_t t0 = (int32_t)(mine + 4 * KEYS * n);
 #pragma unroll
@@ -397,7 +402,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
                     float* p = &planes.v[2 * h + (lane >> 5)][(lane >> 4) & 1][gr][0][c];
-                    p[0] = plane_scale(st.plane[h][gr]);
+                    p[0] = plane_scale(st.plane[h][gr]) * plane_factor;
                     p[16] = plane_middle(st.plane[h][gr]);
                 }
             // the reads are of other lanes' words: a wave's LDS operations run in order, and this keeps the compiler's too

@@ -1,0 +1,80 @@
+"""The 4-bit cache's operators at the ends of what they accept: magnitudes of queries, scores, values and soft caps, rows
+behind a window that nothing wrote, and calls that both attention kernels share."""
+import numpy as np
+import pytest
+import torch
+
+from tests import kv_ref as R
+from tests.test_gpu_kv import Served, _np
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def K(qmm):
+    from stark_amd import kv
+    return kv
+
+
+def _run(s, **kw):
+    op = s.operator(**kw)
+    op.encode()
+    torch.cuda.synchronize()
+    return op
+
+
+def _requests(s):
+    """Of each request and key head: its rows' slice of the call, the query heads, q, k, v (64 bits)."""
+    q, k, v = _np(s.q), _np(s.k), _np(s.v)
+    each, at, kat = q.shape[1] // s.kvh, 0, 0
+    for n, kv in s.requests:
+        for h in range(s.kvh):
+            heads = slice(h * each, (h + 1) * each)
+            yield slice(at, at + n), heads, q[at:at + n, heads], k[kat:kat + kv, h], v[kat:kat + kv, h]
+        at, kat = at + n, kat + kv
+
+
+def _one_key_wins(s, scale, wide):
+    """Scores so far apart that the softmax is 1 at one key and 0 at all others. The winner's probability times its
+    value's scale is one rounding to f16 (2^-11 of that part, beside at most twice the largest value), with `wide` the
+    value another, then the output's own. The score: f32 products and sums of dim terms (kv_ref), f32 lse."""
+    out = _np(s.out)
+    lse = None if s.lse is None else _np(s.lse)
+    for rows, heads, q, k, v in _requests(s):
+        n, each, dim = q.shape
+        reach = 2 * np.abs(k).max()
+        for h in range(each):
+            x = q[:, h] @ k.T * scale
+            mag = abs(scale) * (np.abs(q[:, h]) @ np.abs(k.T) + np.abs(q[:, h]).sum(-1, keepdims=True) * reach)
+            x = np.where(np.arange(len(k)) <= len(k) - n + np.arange(n)[:, None], x, -np.inf)
+            win = x.argmax(-1)
+            top = x.max(-1)
+            error = (mag * ((dim + 16) * 2.0 ** -24 + (2.0 ** -11 if wide == 2 else 0.0))).max(-1)
+            second = np.where(np.arange(len(k)) == win[:, None], -np.inf, x).max(-1)
+            assert (top - second > 2 * error + 100).all(), "the inputs leave more than one key"
+            want = v[win]
+            # (|s c| <= |v| + |b|, and |b| at most the row's largest value)
+            tol = (2.0 ** -11 + (2.0 ** -11 if wide else 0.0) + 2.0 ** -20) * (np.abs(want) + np.abs(want).max(-1, keepdims=True))
+            got = out[rows, heads][:, h]
+            assert np.isfinite(got).all(), f"head {h}: not finite in rows {np.argwhere(~np.isfinite(got).all(-1)).ravel()}"
+            assert (np.abs(got - want) <= tol + R.EPS[s.dtype] * (np.abs(want) + tol) + 2.0 ** -25).all(), f"head {h}"
+            if lse is not None:
+                gl = lse[rows, heads][:, h]
+                assert (np.abs(gl - top) <= error + 2.0 ** -21 * np.abs(top)).all(), f"lse of head {h}"
+
+
+@pytest.mark.parametrize("with_lse", [True, False])
+@pytest.mark.parametrize("rows", [2])
+@pytest.mark.parametrize("power,one_sign", [(100, False), (118, False), (121, False), (122, True)])
+def test_queries_near_the_end_of_bf16(K, rows, power, one_sign, with_lse):
+    """Finite scores of queries of 2^power, where the power of two that brings them to f16 meets the scale. One sign: the
+    sum of a row's values passes f32, its scores do not."""
+    def edit(k, v):
+        k[:] = np.where(np.arange(128) % 2, 1.0, -1.0) * (1.0 if one_sign else np.sign(k)) * 0.25
+        k[7] += 1.0
+
+    s = Served(K, 41, [(rows, 300)], 4, 2, 128, 64, 16, "bf16", edit=edit)
+    x = torch.ones_like(s.q) if one_sign else torch.where(s.q > 0, 1.0, 1.25)
+    s.q.copy_((x + torch.arange(rows, device="cuda").view(-1, 1, 1) / 128).to(torch.bfloat16) * 2.0 ** power)
+    _run(s, with_lse=with_lse)
+    _one_key_wins(s, 128 ** -0.5, 0 if rows == 2 else 1 if with_lse else 2)
