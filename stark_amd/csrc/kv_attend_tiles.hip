@@ -384,7 +384,7 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
                         s[h][i] = a.cap - 2.0f * a.cap *
                                               __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(EXACT ? s[h][i] : s[h][i] * c1));
             }
-            const float scale = EXACT || a.cap != 0.0f ? 1.0f : c1;
+            float scale = EXACT || a.cap != 0.0f ? 1.0f : c1;
             if (t0 < inner_lo || t0 + kKeys > inner_hi || (out[0] | out[1] | out[2] | out[3])) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -417,12 +417,18 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
             // the reference of the exponents moves only when a probability is near the end of f16 (at first, from kNone, all
             // are infinite); whether one is shows in their sum
             if (__any(sum > 0x1p13f)) {
+                // With scores past 2^24 s * scale - m in one rounding is not 0 where m is s * scale rounded: infinite
+                // probabilities of 2^64 and more also come here, and go once both are rounded alike.
                 float top = -INFINITY;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < 16; i += 2) top = max3(top, s[h][i], s[h][i + 1]);
-                top = top == -INFINITY ? top : top * scale;
+                    for (int i = 0; i < 16; i += 2) {
+                        s[h][i] *= scale, s[h][i + 1] *= scale;
+                        asm("" : "+v"(s[h][i]), "+v"(s[h][i + 1]));  // (the compiler would make one rounding of it again)
+                        top = max3(top, s[h][i], s[h][i + 1]);
+                    }
+                scale = 1.0f;
                 const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64))), f = __builtin_amdgcn_exp2f(m - mn);
                 m = mn;
                 l *= f, le *= f;

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests import kv_ref as R
-from tests.test_gpu_kv import Served, _np
+from tests.test_gpu_kv import DT, Served, _dev, _np
 
 pytestmark = pytest.mark.gpu
 
@@ -76,5 +76,28 @@ def test_queries_near_the_end_of_bf16(K, rows, power, one_sign, with_lse):
     s = Served(K, 41, [(rows, 300)], 4, 2, 128, 64, 16, "bf16", edit=edit)
     x = torch.ones_like(s.q) if one_sign else torch.where(s.q > 0, 1.0, 1.25)
     s.q.copy_((x + torch.arange(rows, device="cuda").view(-1, 1, 1) / 128).to(torch.bfloat16) * 2.0 ** power)
+    _run(s, with_lse=with_lse)
+    _one_key_wins(s, 128 ** -0.5, 0 if rows == 2 else 1 if with_lse else 2)
+
+
+@pytest.mark.parametrize("with_lse", [True, False])
+@pytest.mark.parametrize("rows,dtype", [(40, "bf16"), (40, "f16")])
+@pytest.mark.parametrize("size", [200.0, 3413.0, 5000.0, 20000.0])
+def test_scores_past_the_whole_numbers_of_f32(K, rows, dtype, size, with_lse):
+    """Scores of 2^20 to 2^33, whose neighbours in f32 are up to 512 apart: one key wins by far, and what a sum of two
+    roundings leaves must not count as a probability of 2^64."""
+    if dtype == "f16" and not with_lse:
+        return
+    sign = np.where(np.random.default_rng(3).random(128) < 0.5, -1.0, 1.0)
+
+    def edit(k, v):
+        k[:] = 0.1 * size * np.sign(k)
+        k[61] = size * sign
+        v *= 8.0  # scales of 1 to 2: the product with a probability of 1 stands well inside f16
+
+    s = Served(K, 43, [(rows, 300)], 4, 2, 128, 64, 16, dtype, edit=edit)
+    x = _dev(sign, torch.float32) * (1 + torch.arange(rows, device="cuda").view(-1, 1, 1) / 64)
+    x = x * (1 + torch.arange(4, device="cuda").view(1, -1, 1) / 8)
+    s.q.copy_((x * size).to(DT[dtype]))
     _run(s, with_lse=with_lse)
     _one_key_wins(s, 128 ** -0.5, 0 if rows == 2 else 1 if with_lse else 2)
