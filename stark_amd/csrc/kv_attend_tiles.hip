@@ -288,24 +288,24 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[j][e]));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
-        // 2^k puts the largest in [2^3, 2^4): scores of keys up to 2^15 stay far inside f32
-        // (and rows of nothing but tiny values as they are, so that c1 stays a normal number)
-        const int k = min(3 - (top > 0.0f && top < INFINITY ? ilogbf(top) : 0), 48);
+        // 2^k puts the largest in [2^3, 2^4): scores of keys up to 2^15 stay far inside f32 (and rows of nothing but tiny
+        // values, under a scale that leaves their scores tiny as well, as they are, so that c1 stays a normal number).
+        // Sums are of the scaled values, so that they pass f32 only where the scores do.
+        const int k = min(3 - (top > 0.0f && top < INFINITY ? ilogbf(top) : 0), 100 + ilogbf(a.scale));
+        c1 = fminf(ldexp_f32(a.scale, -k), FLT_MAX);  // positive: the sign is q's
+        float sum[G];
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) sum[gr] = 0.0f;
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) qb[j][e] = (_Float16)(ldexp_f32(x[j][e / 2 + 4 * (e & 1)], k) * a.sign);
-        c1 = ldexp_f32(a.scale, -k);  // positive: the sign is q's
+            for (int e = 0; e < 8; ++e) {
+                const float v = ldexp_f32(x[j][e / 2 + 4 * (e & 1)], k) * a.sign;
+                qb[j][e] = (_Float16)v;
+                sum[j * G / J] += v;
+            }
 #pragma unroll
-        for (int gr = 0; gr < G; ++gr) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int j = gr * J / G; j < (gr + 1) * J / G; ++j)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sum += x[j][e];
-            sum += __shfl_xor(sum, 32, 64);
-            qsum[gr] = sum * a.sign * a.scale;
-        }
+        for (int gr = 0; gr < G; ++gr) qsum[gr] = (sum[gr] + __shfl_xor(sum[gr], 32, 64)) * c1;
     }
 
     f32x16 o[O];

@@ -64,7 +64,7 @@ def _one_key_wins(s, scale, wide):
 
 
 @pytest.mark.parametrize("with_lse", [True, False])
-@pytest.mark.parametrize("rows", [2])
+@pytest.mark.parametrize("rows", [2, 40])
 @pytest.mark.parametrize("power,one_sign", [(100, False), (118, False), (121, False), (122, True)])
 def test_queries_near_the_end_of_bf16(K, rows, power, one_sign, with_lse):
     """Finite scores of queries of 2^power, where the power of two that brings them to f16 meets the scale. One sign: the
@@ -78,6 +78,15 @@ def test_queries_near_the_end_of_bf16(K, rows, power, one_sign, with_lse):
     s.q.copy_((x + torch.arange(rows, device="cuda").view(-1, 1, 1) / 128).to(torch.bfloat16) * 2.0 ** power)
     _run(s, with_lse=with_lse)
     _one_key_wins(s, 128 ** -0.5, 0 if rows == 2 else 1 if with_lse else 2)
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_tiny_queries_with_a_large_scale(K, rows):
+    """Queries of 2^-76 under a scale of 2^64 and more: scores of ordinary size."""
+    s = Served(K, 42, [(rows, 200)], 4, 2, 128, 64, 16, "bf16")
+    s.q.mul_(2.0 ** -66)
+    _run(s, scale=2.0 ** 63)
+    s.check(scale=2.0 ** 63)
 
 
 @pytest.mark.parametrize("with_lse", [True, False])
