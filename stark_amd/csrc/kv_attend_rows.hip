@@ -460,8 +460,9 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
             }
             float top = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3]));
             if (B == 2) top = fmaxf(top, fmaxf(fmaxf(x[B - 1][0], x[B - 1][1]), fmaxf(x[B - 1][2], x[B - 1][3])));
-            // the reference moves only when a score passes it by 2^6: rescaling is then rare
-            if (__any(top > run.m + 6.0f)) {
+            // the reference moves only when a score passes it by 2^6: rescaling is then rare (the difference is exact; a
+            // reference of 2^26 plus 6 would be 8 more)
+            if (__any(top - run.m > 6.0f)) {
                 top = fmaxf(top, __shfl_xor(top, 16, 64));
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
                 const float mn = fmaxf(run.m, top), f = __builtin_amdgcn_exp2f(run.m - mn);
