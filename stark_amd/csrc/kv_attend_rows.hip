@@ -91,14 +91,12 @@ struct PageIds {
 template <int DIM, int G>
 struct Running {
     static constexpr int J = DIM / 32;
-    f32x4 o[2 * J];          // [32-value block, parity]: codes times p s, values 32 i + 2 (4 g + e) + parity
+    f32x4 o[2 * J];          // [32-value block, parity]: codes times p s 2^exponent, values 32 i + 2 (4 g + e) + parity
     f32x4 rounded[G];        // 8 sum p s, of the same roundings
-    float beta[G], l, m, mf; // sum p (b + 8 s) and sum p over the lane's keys; reference; reference - exponent
-    int fexp;
+    float beta[G], l, m;     // sum p (b + 8 s) and sum p over the lane's keys; reference of the exponents
 
-    QMM_DEVICE void start(int exponent) {
-        fexp = exponent;
-        m = kNone, mf = kNone - (float)exponent, l = 0.0f;
+    QMM_DEVICE void start() {
+        m = kNone, l = 0.0f;
 #pragma unroll
         for (int j = 0; j < 2 * J; ++j) o[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -374,7 +372,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
         const int32_t inner_hi = min(kv::visible(0, u.r.q_len, u.r.kv_len, a.causal, a.window).hi, to);
 
         Running<DIM, G> run;
-        run.start(0);
+        run.start();
         PlaneBuffer<G, T>& planes = plane_buffers[wave];
         // largest value scale (f16 bits) of plane words of a record's keys before `to`; t: this lane's key
         const auto scale_max = [&](const uint32_t (&plane)[G], int32_t t, bool ok, uint32_t smax) {
@@ -394,7 +392,10 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
             smax = max(smax, (uint32_t)__shfl_xor((int)smax, 32, 64));
             return smax ? 8 - ilogbf(f16_bits_to_f32(smax)) : 0;
         };
-        const float plane_factor = lane & 16 ? 1.0f : 0x1p24f;  // on the scales of the lane's plane words: keys' codes are c 2^-24
+        // On the scales of the lane's plane words: 2^24 for keys, whose codes are c 2^-24, and the values' power of two. (Not
+        // on the probabilities: the reference less an exponent would be rounded where scores pass 2^24.)
+        int value_exponent = 0;
+        float plane_factor = 0x1p24f;
         const auto step = [&](Codes& st, uint32_t n) {
             const int32_t t0 = (int32_t)(mine + 4 * KEYS * n);
 #pragma unroll
@@ -467,7 +468,6 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
                 top = fmaxf(top, __shfl_xor(top, 32, 64));
                 const float mn = fmaxf(run.m, top), f = __builtin_amdgcn_exp2f(run.m - mn);
                 run.m = mn;
-                run.mf = mn - (float)run.fexp;
                 run.l *= f;
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) run.beta[gr] *= f, run.rounded[gr] *= f;
@@ -481,7 +481,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
                 float p[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    p[e] = __builtin_amdgcn_exp2f(x[u][e] - run.mf);
+                    p[e] = __builtin_amdgcn_exp2f(x[u][e] - run.m);
                     run.l += p[e];
                 }
 #pragma unroll
@@ -544,7 +544,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
             }
         };
 
-        // Power of two on the probabilities: p s below 2^15 while p < 2^6, taken from the scales of the wave's first
+        // Power of two on the values' scales: p s below 2^15 while p < 2^6, taken from the scales of the wave's first
         // records. Should a later scale be far larger, the products overflow to infinity, which shows in the sums at the
         // end: then the wave starts again with the largest scale of all its keys.
         for (int attempt = 0; attempt < 2 && steps; ++attempt) {
@@ -566,7 +566,9 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
             } else {
                 smax = scale_max(st[0].plane[0], t_lane, !(st[0].absent >> (lane >> 5) & 1), 0);
             }
-            run.start(exponent(smax));
+            run.start();
+            value_exponent = exponent(smax);
+            if (lane & 16) plane_factor = ldexp_f32(1.0f, value_exponent);
             // The next step's loads go out before a step is computed (past the last step: of the last again). Two copies
             // of the body, so that each register of a step stays where it was loaded: a copy would wait for the loads.
             for (uint32_t n = 0; n < steps; n += 2) {
@@ -584,18 +586,19 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
         }
 
         // the four lane groups hold different keys of one column
-        float l = run.l, mf = run.mf;
+        float l = run.l, m = run.m;
         l += __shfl_xor(l, 16, 64);
         l += __shfl_xor(l, 32, 64);
-        if (l == 0.0f) mf = kNone;
-        if (g == 0) wave_ref[wave][c] = mf;
+        if (l == 0.0f) m = kNone;
+        if (g == 0) wave_ref[wave][c] = m;
         __syncthreads();
         // a row's reference: over the waves and its columns
         float ref = kNone;
 #pragma unroll
         for (int k = 0; k < 4 * PACK; ++k) ref = fmaxf(ref, wave_ref[k / PACK][k % PACK * R + row]);
-        const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(mf - ref);
+        const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - ref);
         if (g == 0) wave_sum_l[wave][c] = l == 0.0f ? 0.0f : l * f;
+        const float unscale = ldexp_f32(0x1p24f, -value_exponent);
         // lane: values 32 i + 8 g + 0 .. 7 of its column
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
@@ -609,8 +612,8 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
                 for (int e = 0; e < 4; ++e) {
                     const float even = run.o[2 * i][e] - run.rounded[gr][e];
                     const float odd = fmaf(run.o[2 * i + 1][e], 0.0625f, -run.rounded[gr][e]);
-                    y[2 * e] = l == 0.0f ? 0.0f : fmaf(even, 0x1p24f, s) * f;
-                    y[2 * e + 1] = l == 0.0f ? 0.0f : fmaf(odd, 0x1p24f, s) * f;
+                    y[2 * e] = l == 0.0f ? 0.0f : fmaf(even, unscale, s) * f;
+                    y[2 * e + 1] = l == 0.0f ? 0.0f : fmaf(odd, unscale, s) * f;
                 }
                 // the two columns of a row: the 16-lane row rotated by 8
                 if (PACK == 2) {
