@@ -13,7 +13,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr float kNone = -1e30f;  // running maximum before any key
+constexpr float kNone = -FLT_MAX;  // running maximum before any key: no score is below it
 constexpr uint32_t kRows = 16;   // query rows of a matrix-core column block
 
 struct AttendArgs {

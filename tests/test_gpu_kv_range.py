@@ -110,3 +110,17 @@ def test_scores_past_the_whole_numbers_of_f32(K, rows, dtype, size, with_lse):
     s.q.copy_((x * size).to(DT[dtype]))
     _run(s, with_lse=with_lse)
     _one_key_wins(s, 128 ** -0.5, 0 if rows == 2 else 1 if with_lse else 2)
+
+
+@pytest.mark.parametrize("with_lse", [True, False])
+@pytest.mark.parametrize("rows", [2, 40])
+def test_rows_of_nothing_but_very_low_scores(K, rows, with_lse):
+    """Scores of -1e31 and below are scores: the row is not an empty one."""
+    def edit(k, v):
+        k[:] = -1.0
+        k[5] = -0.25
+
+    s = Served(K, 44, [(rows, 90)], 4, 2, 128, 64, 16, "bf16", edit=edit)
+    s.q.copy_(torch.ones_like(s.q) * (1 + torch.arange(rows, device="cuda").view(-1, 1, 1) / 64) * 2.0 ** 108)
+    _run(s, with_lse=with_lse)
+    _one_key_wins(s, 128 ** -0.5, 0 if rows == 2 else 1 if with_lse else 2)
