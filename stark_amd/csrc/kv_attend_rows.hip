@@ -441,12 +441,12 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[u][e] = fmaf(y[e], c1, z[e]);
             }
-            if (a.cap != 0.0f) {  // cap tanh(s / cap) = cap (1 - 2 / (1 + e^(2 s / cap)))
+            if (a.cap != 0.0f) {
 #pragma unroll
                 for (int u = 0; u < B; ++u)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        x[u][e] = a.cap - 2.0f * a.cap * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x[u][e]));
+                        x[u][e] = a.cap <= kPlainCap ? soft_capped(x[u][e], a.cap) : soft_capped_exact(x[u][e], a.cap);
             }
             const bool masked = t0 < inner_lo || t0 + KEYS > inner_hi || st.absent;
             if (masked) {

@@ -376,13 +376,15 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
                 }
             }
             // value i of block h: key 32 h + 8 (i / 4) + 4 hf + i % 4
-            if (a.cap != 0.0f) {
+            const auto cap_scores = [&](auto capped) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        s[h][i] = a.cap - 2.0f * a.cap *
-                                              __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(EXACT ? s[h][i] : s[h][i] * c1));
+                    for (int i = 0; i < 16; ++i) s[h][i] = capped(EXACT ? s[h][i] : s[h][i] * c1, a.cap);
+            };
+            if (a.cap != 0.0f) {
+                if (a.cap <= kPlainCap) cap_scores(soft_capped);
+                else cap_scores(soft_capped_exact);
             }
             float scale = EXACT || a.cap != 0.0f ? 1.0f : c1;
             if (t0 < inner_lo || t0 + kKeys > inner_hi || (out[0] | out[1] | out[2] | out[3])) {

@@ -124,3 +124,23 @@ def test_rows_of_nothing_but_very_low_scores(K, rows, with_lse):
     s.q.copy_(torch.ones_like(s.q) * (1 + torch.arange(rows, device="cuda").view(-1, 1, 1) / 64) * 2.0 ** 108)
     _run(s, with_lse=with_lse)
     _one_key_wins(s, 128 ** -0.5, 0 if rows == 2 else 1 if with_lse else 2)
+
+
+@pytest.mark.parametrize("with_lse", [True, False])
+@pytest.mark.parametrize("rows", [2, 40])
+@pytest.mark.parametrize("cap", [0.5, 30.0, 1e3, 1e5, 2.0 ** 20])
+def test_soft_caps(K, rows, cap, with_lse):
+    """A large cap leaves small scores as they are. The bound is kv_ref's with the cap's own error, 2^-20 of it there, put
+    at 2^-20 of the largest score: cap tanh(s / cap) is never larger than s, and no term of it is."""
+    s = Served(K, 45, [(rows, 300)], 4, 2, 128, 64, 16, "bf16")
+    _run(s, soft_cap=cap, with_lse=with_lse)
+    out, wide = _np(s.out), 0 if rows == 2 else 1 if with_lse else 2
+    for rs, heads, q, k, v in _requests(s):
+        want, wl, tol, dl = R.attention(q, k, v, 128 ** -0.5, True, 0, cap, wide)
+        top = np.abs(np.einsum("nhd,td->nht", q, k) * 128 ** -0.5).max(-1)
+        less = 2.0 ** -20 * cap - 2.0 ** -20 * np.minimum(top, cap)  # [n, heads]
+        tol = tol - 2 * less[..., None] * np.abs(v).max(0)
+        err = np.abs(out[rs, heads] - want)
+        assert (err <= tol * 1.001 + R.EPS["bf16"] * (np.abs(want) + tol)).all(), (err / tol).max()
+        if with_lse:
+            assert (np.abs(_np(s.lse)[rs, heads] - wl) <= dl - less + 2.0 ** -23 * np.abs(wl)).all()
