@@ -386,11 +386,10 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
             return smax;
         };
         const int32_t t_lane = (int32_t)mine + 16 * (int32_t)(lane >> 5) + (int32_t)c;  // of step 0's first plane words
-        const auto exponent = [&](uint32_t smax) {
+        const auto wave_max = [&](uint32_t smax) {
             smax = group_max<16>(smax);
             smax = max(smax, (uint32_t)__shfl_xor((int)smax, 16, 64));
-            smax = max(smax, (uint32_t)__shfl_xor((int)smax, 32, 64));
-            return smax ? 8 - ilogbf(f16_bits_to_f32(smax)) : 0;
+            return max(smax, (uint32_t)__shfl_xor((int)smax, 32, 64));
         };
         // On the scales of the lane's plane words: 2^24 for keys, whose codes are c 2^-24, and the values' power of two. (Not
         // on the probabilities: the reference less an exponent would be rounded where scores pass 2^24.)
@@ -546,7 +545,8 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
 
         // Power of two on the values' scales: p s below 2^15 while p < 2^6, taken from the scales of the wave's first
         // records. Should a later scale be far larger, the products overflow to infinity, which shows in the sums at the
-        // end: then the wave starts again with the largest scale of all its keys.
+        // end: then the wave starts again with the largest scale of all its keys. Scales of 0 in the first records (zeros)
+        // say nothing of the others: the wave looks at all at once.
         for (int attempt = 0; attempt < 2 && steps; ++attempt) {
             uint32_t smax = 0;
             if (attempt) {
@@ -566,8 +566,10 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
             } else {
                 smax = scale_max(st[0].plane[0], t_lane, !(st[0].absent >> (lane >> 5) & 1), 0);
             }
+            smax = wave_max(smax);
+            if (smax == 0 && attempt == 0) continue;
             run.start();
-            value_exponent = exponent(smax);
+            value_exponent = smax ? 8 - ilogbf(f16_bits_to_f32(smax)) : 0;
             if (lane & 16) plane_factor = ldexp_f32(1.0f, value_exponent);
             // The next step's loads go out before a step is computed (past the last step: of the last again). Two copies
             // of the body, so that each register of a step stays where it was loaded: a copy would wait for the loads.

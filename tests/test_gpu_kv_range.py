@@ -144,3 +144,30 @@ def test_soft_caps(K, rows, cap, with_lse):
         assert (err <= tol * 1.001 + R.EPS["bf16"] * (np.abs(want) + tol)).all(), (err / tol).max()
         if with_lse:
             assert (np.abs(_np(s.lse)[rs, heads] - wl) <= dl - less + 2.0 ** -23 * np.abs(wl)).all()
+
+
+def _small_values(s, wide):
+    """As Served.check for outputs in bf16, without its 2^-25 of f16 outputs."""
+    out = _np(s.out)
+    for rows, heads, q, k, v in _requests(s):
+        k, v = k[-s.window:], v[-s.window:]  # (0: all; a window is for one row)
+        want, _, tol, _ = R.attention(q, k, v, 128 ** -0.5, True, 0, 0.0, wide)
+        got = out[rows, heads]
+        err = np.abs(got - want)
+        assert (err <= tol * 1.001 + R.EPS["bf16"] * (np.abs(want) + tol)).all(), (err / np.abs(want)).max()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("first,later", [(0.0, 1e-5), (0.0, 1e-4), (0.0, 1.0), (0.0, 3000.0), (1e-5, 1e-5)])
+@pytest.mark.parametrize("keys", [129, 140, 900])
+def test_zeros_before_small_values(K, rows, first, later, keys):
+    """Value groups of zeros have a scale of 0, which says nothing of the scales behind them."""
+    def edit(k, v):
+        k *= 0.1  # near-equal weights
+        v[:128] *= first
+        v[128:] *= later
+
+    s = Served(K, 46, [(rows, keys)], 8, 2, 128, 64, 16, "bf16", edit=edit)
+    s.window = 0
+    _run(s)
+    _small_values(s, 0 if rows == 1 else 1)
