@@ -374,9 +374,9 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
         Running<DIM, G> run;
         run.start();
         PlaneBuffer<G, T>& planes = plane_buffers[wave];
-        // largest value scale (f16 bits) of plane words of a record's keys before `to`; t: this lane's key
+        // largest value scale (f16 bits) of plane words of a record's keys that some row sees; t: this lane's key
         const auto scale_max = [&](const uint32_t (&plane)[G], int32_t t, bool ok, uint32_t smax) {
-            if ((lane & 16) && t < to && ok) {
+            if ((lane & 16) && t >= u.span.lo && t < to && ok) {
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
                     const uint32_t h = plane[gr] & 0xffffu;

@@ -171,3 +171,16 @@ def test_zeros_before_small_values(K, rows, first, later, keys):
     s.window = 0
     _run(s)
     _small_values(s, 0 if rows == 1 else 1)
+
+
+def test_values_before_the_window_do_not_set_the_scale(K):
+    """Large values of keys that a window leaves behind, in the step where it begins."""
+    def edit(k, v):
+        k *= 0.1
+        v[:] *= 1e-5
+        v[512:543] = np.sign(v[512:543]) * 30000.0
+
+    s = Served(K, 47, [(1, 546)], 8, 2, 128, 64, 16, "bf16", edit=edit)
+    s.window = 546 - 543
+    _run(s, window=s.window)
+    _small_values(s, 0)
