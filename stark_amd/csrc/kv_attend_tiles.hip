@@ -416,9 +416,10 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
                     }
             };
             probabilities();
-            // the reference of the exponents moves only when a probability is near the end of f16 (at first, from kNone, all
-            // are infinite); whether one is shows in their sum
-            if (__any(sum > 0x1p13f)) {
+            // The reference of the exponents moves only when a probability is near the end of f16 (at first, from kNone, all
+            // are infinite); whether one is shows in their sum. It moves to 2^-8 of the largest: probabilities keep all their
+            // bits down to 2^-22 of it (15 in natural logarithms), and some down to 2^-33.
+            if (__any(sum > 0x1p15f)) {
                 // With scores past 2^24 s * scale - m in one rounding is not 0 where m is s * scale rounded: infinite
                 // probabilities of 2^64 and more also come here, and go once both are rounded alike.
                 float top = -INFINITY;
@@ -431,7 +432,9 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
                         top = max3(top, s[h][i], s[h][i + 1]);
                     }
                 scale = 1.0f;
-                const float mn = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64))), f = __builtin_amdgcn_exp2f(m - mn);
+                top = fmaxf(top, __shfl_xor(top, 32, 64));
+                const float low = top - 8.0f;  // (past 2^27 this may be 16 less)
+                const float mn = fmaxf(m, top - low > 8.0f ? top : low), f = __builtin_amdgcn_exp2f(m - mn);
                 m = mn;
                 l *= f, le *= f;
 #pragma unroll

@@ -184,3 +184,39 @@ def test_values_before_the_window_do_not_set_the_scale(K):
     s.window = 546 - 543
     _run(s, window=s.window)
     _small_values(s, 0)
+
+
+@pytest.mark.parametrize("with_lse", [True, False])
+@pytest.mark.parametrize("rows", [2, 40])
+def test_a_first_key_above_all_others(K, rows, with_lse):
+    """An attention sink: a key 15 above the rest (in natural logarithms) whose value is zero, so that the output is what
+    the other keys' small probabilities make. An error d of the scores moves it by 2 d sum w |v - out|; a probability is
+    held to 2^-12 of itself (2^-11 in kv_ref's bound), or below f16's normal range to 2^-33 of the largest."""
+    def edit(k, v):
+        k[:, :, 1:] *= 0.2
+        k[:, :, 0] = 0.0
+        k[0], v[0] = 0.0, 0.0
+        k[0, :, 0] = 16.0
+
+    s = Served(K, 48, [(rows, 100)], 4, 2, 128, 64, 16, "bf16", edit=edit)
+    s.q[:, :, 0] = 10.625
+    _run(s, with_lse=with_lse)
+    out, wide = _np(s.out), 0 if rows == 2 else 1 if with_lse else 2
+    for rs, heads, q, k, v in _requests(s):
+        n = q.shape[0]
+        seen = np.arange(len(k)) <= len(k) - n + np.arange(n)[:, None]
+        for h in range(q.shape[1]):
+            x = np.where(seen, q[:, h] @ k.T * 128 ** -0.5, -np.inf)
+            mag = 128 ** -0.5 * (np.abs(q[:, h]) @ np.abs(k.T) + np.abs(q[:, h]).sum(-1, keepdims=True) * 2 *
+                                 np.abs(k).max(-1))
+            w = np.exp(x - x.max(-1, keepdims=True))
+            total = w.sum(-1, keepdims=True)
+            w /= total
+            want = w @ v
+            d = np.where(seen, 144 * 2.0 ** -24 * mag + (2.0 ** -11 * mag if wide == 2 else 0.0) + 2.0 ** -22 * 40, 0.0)
+            a = w @ (np.abs(v) + np.abs(v).max(-1, keepdims=True))
+            tol = np.einsum("nt,ntd->nd", 2 * w * d, np.abs(v - want[:, None])) + a * (2.0 ** -11 + (2.0 ** -10 if wide else 0)
+                                                                                       + 2.0 ** -18)
+            tol += 2.0 ** -33 * (np.abs(v).sum(0) + np.abs(v).max(-1).sum())
+            err = np.abs(out[rs, heads][:, h] - want)
+            assert (err <= tol + R.EPS["bf16"] * (np.abs(want) + tol)).all(), (err / tol).max()
