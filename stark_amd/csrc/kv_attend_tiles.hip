@@ -98,7 +98,7 @@ struct Codes {
                 }
         }
     }
-    // live: bit e: the lane's token 4 (lane / 16) + e is a key of the request, in a page of the cache
+    // live: bit e: the lane's token 4 (lane / 16) + e is a key that some row may see, in a page of the cache
     template <bool EXACT>
     QMM_DEVICE void write_values(Tile<DIM, G, EXACT>& t, uint32_t record, uint32_t lane, uint32_t live) {
         const uint32_t r = lane & 15, quad = lane >> 4;
@@ -314,6 +314,9 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
     float m = kNone, l = 0.0f, le = 0.0f;  // (le: of the probabilities before rounding)
     __syncthreads();  // not_finite is clear
     if (steps) {
+        // the first tile may begin before the window of its first row: what stands there may be anything by now
+        const int32_t hidden = top_row.lo - (from + 16 * (int32_t)record + 4 * (int32_t)(lane >> 4));
+        if (hidden > 0) live_keys = hidden >= 4 ? 0 : live_keys >> hidden << hidden;
         unpack(tiles[0]);
         fetch(min(1, steps - 1), page);
         page = page_of(min(2, steps - 1));

@@ -220,3 +220,21 @@ def test_a_first_key_above_all_others(K, rows, with_lse):
             tol += 2.0 ** -33 * (np.abs(v).sum(0) + np.abs(v).max(-1).sum())
             err = np.abs(out[rs, heads][:, h] - want)
             assert (err <= tol + R.EPS["bf16"] * (np.abs(want) + tol)).all(), (err / tol).max()
+
+
+@pytest.mark.parametrize("with_lse", [True, False])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_unwritten_rows_before_the_window(K, rows, with_lse):
+    """Pages that lie wholly before every row's window may have been given away: what they hold, finite planes whose
+    values pass f16 here, reaches nothing."""
+    n = 500
+    s = Served(K, 49, [(rows, n)], 4, 2, 128, 64, 16, "bf16")
+    window = n - rows + 1 - 432  # the first row's window begins in the fourth page of a tile of 64 keys
+    assert s.table.shape[1] == 32 and window > 0
+    used = set(_np(s.table).ravel().tolist())
+    spare = next(p for p in range(s.cache.page_count) if p not in used)
+    page = s.cache.data.view(s.cache.page_count, -1)
+    page[spare] = 0x7B
+    s.table[0, :432 // 16] = spare
+    _run(s, window=window, with_lse=with_lse)
+    s.check(window=window)
