@@ -232,7 +232,7 @@ QMM_DEVICE void widen_range(T& lo, T& hi) {
 // query head of its token, then key heads, then value heads, with one read of the rotation.
 // Keys in f64: a rotated value a c - b s of f32 factors has exact products and one rounding there, and codes, scales and
 // biases come out as from exact arithmetic (an f32 sum or quotient beside a half way point would take the wrong code, one
-// step of the group's range / 15). Queries in f32: they are rounded once more in any case.
+// step of the group's range / 15). Queries of 16 bits in f32, of f32 in f64 as well.
 // Bound by latency and vector work together: 2048 tokens of 32 + 2 * 8 heads of 128 (44 MB, 9 us as a copy) take 14.5 us,
 // about 170 vector instructions a wave and row (7 us) after two dependent reads (positions, rotation). One row a thread
 // took 23 us and all rows as 2^17 or 2^19 threads 16 and 16.5.
@@ -349,19 +349,22 @@ __global__ __launch_bounds__(256) void kv_append(AppendArgs a) {
         if (h + a.sets < a.heads) r = fetch(a.q, h + a.sets, elsewhere);
         Eight<DT> y = now.x;
         if (turns) {
+            // 16-bit rows in f32 (they are rounded once more in any case), f32 rows in f64: one rounding, also where the two
+            // products nearly cancel
+            using T = std::conditional_t<DT == STARK_QMM_F32, double, float>;
+            T t[8];
             if (a.rot.interleaved) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float u = now.x.get(2 * e), v = now.x.get(2 * e + 1), c = cs[e].x, s = cs[e].y;
-                    y.set(2 * e, fmaf(u, c, -(v * s)), fmaf(v, c, u * s));
+                    const T u = now.x.get(2 * e), v = now.x.get(2 * e + 1), c = cs[e].x, s = cs[e].y;
+                    t[2 * e] = fma(u, c, -(v * s)), t[2 * e + 1] = fma(v, c, u * s);
                 }
             } else {
-                float t[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) t[e] = fmaf(now.x.get(e), cs[e].x, now.o.get(e) * (high ? cs[e].y : -cs[e].y));
-#pragma unroll
-                for (int e = 0; e < 8; e += 2) y.set(e, t[e], t[e + 1]);
+                for (int e = 0; e < 8; ++e) t[e] = fma((T)now.x.get(e), (T)cs[e].x, (T)now.o.get(e) * (T)(high ? cs[e].y : -cs[e].y));
             }
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) y.set(e, (float)t[e], (float)t[e + 1]);
         }
         y.store(a.q_out, token, h, d);
     }

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests import kv_ref as R
-from tests.test_gpu_kv import DT, Served, _dev, _np
+from tests.test_gpu_kv import DT, Served, _dev, _ints, _np, _round, _same, _strided, _table
 
 pytestmark = pytest.mark.gpu
 
@@ -238,3 +238,27 @@ def test_unwritten_rows_before_the_window(K, rows, with_lse):
     s.table[0, :432 // 16] = spare
     _run(s, window=window, with_lse=with_lse)
     s.check(window=window)
+
+
+def test_f32_queries_that_nearly_cancel(K):
+    """A rotated f32 value is rounded once: what is left of a difference of nearly equal products is as exact as any."""
+    rng = np.random.default_rng(50)
+    t, heads, dim = 64, 4, 128
+    table, positions = _table(300, 64), rng.integers(1, 300, (1, t))
+    q = rng.normal(0, 1, (t, heads, dim))
+    c, s = (table[positions[0], :, i].astype(np.float64)[:, None] for i in (0, 1))
+    q[:, ::2, :64] = q[:, ::2, 64:] * s / np.where(np.abs(c) > 1e-3, c, 1.0)     # first halves go to about 0
+    q[:, 1::2, 64:] = -q[:, 1::2, :64] * s / np.where(np.abs(c) > 1e-3, c, 1.0)  # second halves do
+    q = _round(q, "f32")
+    for inter in (False, True):
+        rows = q if not inter else q.reshape(t, heads, 2, 64).swapaxes(2, 3).reshape(t, heads, dim)
+        cache, out = K.KvCache(4, 16, 1, dim, 64), torch.zeros(t, heads, dim, device="cuda")
+        k = torch.zeros(t, 1, dim, device="cuda")
+        K.KvAppend(cache, k, k, _ints(np.arange(t)), _dev(rows, torch.float32), out,
+                   K.Rotary(_dev(table), _ints(positions[0]), interleaved=inter)).encode()
+        torch.cuda.synchronize()
+        want = R.rotate(rows, table, positions, [0] * 64, inter)
+        assert (np.abs(want) < 1e-6).mean() > 0.2
+        # one rounding of the exact products' sum to 64 bits, and one to f32
+        size = np.abs(rows).max()
+        assert (np.abs(_np(out) - want) <= 2.0 ** -24 * np.abs(want) + 2.0 ** -51 * size + 2.0 ** -149).all()
