@@ -38,7 +38,8 @@ struct AttendArgs {
     int4* begun;             // [grid] unit that begins in a workgroup and goes on in later ones: its request's first token
                              // (-1: none), head, first row | rows of the request << 16, later ones
     // rows of prompts (kv_attend_tiles)
-    uint32_t tiles;             // that the longest request may have
+    uint32_t tiles;             // workgroups of a request, where that is no more than turns; else 0
+    uint32_t turns;             // workgroups of a kv head (and piece)
     uint32_t pieces;            // that a tile's keys may be cut into
     float* tile_po;             // [token][head][piece][dim] unnormalised partial outputs
     float2* tile_pml;           // [token][head][piece] (reference exponent, sum)

@@ -73,7 +73,9 @@ stark_qmm_status plan_work(AttendArgs* a, uint64_t* workspace) {
     }
     if (most > a->row_limit) {
         const kv::Tiling t = kv::tiling(a->batch, a->cache.kv_heads, (uint64_t)a->tokens * a->ratio, most, a->max_kv, cus);
-        a->tiles = t.tiles, a->pieces = t.pieces;
+        const uint64_t even = (uint64_t)t.tiles * a->batch, need = kv::row_tiles((uint64_t)a->tokens * a->ratio, a->batch);
+        a->tiles = even <= need ? t.tiles : 0, a->turns = (uint32_t)std::min({even, need, (uint64_t)0xffffffffu});
+        a->pieces = t.pieces;
         if (t.pieces > 1) *workspace += (uint64_t)a->tokens * a->heads * t.pieces * (a->cache.dim * 4ull + 8);
     }
     return STARK_QMM_OK;

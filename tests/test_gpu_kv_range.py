@@ -262,3 +262,42 @@ def test_f32_queries_that_nearly_cancel(K):
         # one rounding of the exact products' sum to 64 bits, and one to f32
         size = np.abs(rows).max()
         assert (np.abs(_np(out) - want) <= 2.0 ** -24 * np.abs(want) + 2.0 ** -51 * size + 2.0 ** -149).all()
+
+
+@pytest.mark.parametrize("requests,heads,kvh,dim,group,page,dtype,options", [
+    ([(1, 40)] * 150 + [(300, 500)] + [(1, 70)] * 100, 8, 2, 64, 32, 16, "bf16", {}),
+    ([(600, 700)] + [(0, 3)] * 70 + [(1, 33)] * 130, 4, 2, 128, 64, 16, "f16", {}),
+    ([(1, 20)] * 64 + [(2, 9)] + [(129, 140)] * 2, 16, 8, 64, 64, 16, "bf16", dict(window=30)),
+])
+def test_few_long_requests_among_many_short_ones(K, requests, heads, kvh, dim, group, page, dtype, options):
+    """Workgroups by the rows that the call has: each request's are found by its place, in batches of more than 64."""
+    s = Served(K, 51, requests, heads, kvh, dim, group, page, dtype, pad_tokens=3)
+    _run(s, **options)
+    s.check(**options)
+
+
+def test_thousands_of_requests_with_a_long_bound(K):
+    """4096 requests, any of which could be 16384 rows long: one row tile each and head would be 2^24 workgroups."""
+    rng = np.random.default_rng(52)
+    batch, long, heads, kvh, dim = 4096, 300, 32, 8, 64
+    cache = K.KvCache(20, 16, kvh, dim, 32)
+    k, v = (_dev(rng.normal(0, 1, (320, kvh, dim)), torch.float32) for _ in range(2))
+    K.KvAppend(cache, k, v, _ints(np.arange(320))).encode()
+    K.KvRead(cache, _ints(np.arange(320)), k, v).encode()
+    rows = batch - 1 + long
+    q = torch.zeros(16384, heads, dim, dtype=torch.bfloat16, device="cuda")
+    q[:rows] = _dev(rng.normal(0, 1, (rows, heads, dim)), torch.bfloat16)
+    out = torch.full_like(q, 9.0)
+    table = np.zeros((batch, 20))
+    table[-1] = np.arange(20)
+    start = np.append(np.arange(batch), rows)
+    op = K.KvAttention(cache, q, out, _ints(table), _ints(start), _ints([7] * (batch - 1) + [long]), max_query=16384, max_kv=320)
+    op.encode()
+    torch.cuda.synchronize()
+    assert (out[rows:] == 9.0).all()
+    hq, hk, hv, ho = _np(q[:rows]), _np(k), _np(v), _np(out[:rows])
+    for h in range(kvh):
+        mine = slice(4 * h, 4 * h + 4)
+        for part, n, causal in ((slice(0, batch - 1), 7, False), (slice(batch - 1, rows), long, True)):
+            want, _, tol, _ = R.attention(hq[part, mine], hk[:n, h], hv[:n, h], dim ** -0.5, causal, 0, 0.0, 2)
+            assert (np.abs(ho[part, mine] - want) <= tol + R.EPS["bf16"] * (np.abs(want) + tol)).all()
