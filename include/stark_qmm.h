@@ -674,7 +674,12 @@ STARK_QMM_API stark_qmm_status stark_qmm_kv_attention_workspace_size(const stark
 
 /* Attention of new query rows over the cache: decode, verify and prompt rows in
  * one call, heads / kv_heads query heads to a key head. An empty row gives
- * zeros; rows that no request has stay as they were. */
+ * zeros; rows that no request has stay as they were. UNSUPPORTED, from the size
+ * query as well and before anything is launched, where the call is more than its
+ * launches count: u = batch * kv_heads (times 4 where a request may have more
+ * than 16 and up to 64 rows, max_query * heads / kv_heads) of 2^24 with up to 2048
+ * keys, or u * (max_kv / 32 + 40) of 2^31; where it may have more than 64 rows,
+ * tokens * heads / 128 + batch * kv_heads of 2^24 - 2^17. */
 STARK_QMM_API stark_qmm_status stark_qmm_kv_attention(const stark_qmm_kv_attention_args* args, void* stream);
 
 /* ------------------------------------------------------------------ */

@@ -713,7 +713,6 @@ __global__ __launch_bounds__(256) void kv_attend_join(AttendArgs a) {
 template <int DIM, int G, int PACK>
 stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
     const uint64_t units = (uint64_t)a.batch * a.cache.kv_heads * ((a.row_limit + a.row_block - 1) / a.row_block);
-    if (a.whole && units >= 1ull << 24) return STARK_QMM_UNSUPPORTED;
     hipLaunchKernelGGL((kv_attend_rows<DIM, G, PACK>), dim3(a.whole ? (uint32_t)units : a.grid), dim3(256), 0, s, a);
     QMM_HIP_CHECK(hipGetLastError());
     if (!a.whole) {

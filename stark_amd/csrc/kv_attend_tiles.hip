@@ -587,15 +587,13 @@ __global__ __launch_bounds__(256) void kv_attend_tiles_join(AttendArgs a) {
 
 template <int DIM, int G>
 stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
-    const uint64_t blocks = (uint64_t)a.cache.kv_heads * a.turns * a.pieces;
-    if (blocks >= 1ull << 24) return STARK_QMM_UNSUPPORTED;
-    if (a.lse || !a.is_bf16) hipLaunchKernelGGL((kv_attend_tiles<DIM, G, true>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((kv_attend_tiles<DIM, G, false>), dim3((uint32_t)blocks), dim3(256), 0, s, a);
+    const uint32_t blocks = a.cache.kv_heads * a.turns * a.pieces;  // below 2^24 (kv::fits)
+    if (a.lse || !a.is_bf16) hipLaunchKernelGGL((kv_attend_tiles<DIM, G, true>), dim3(blocks), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((kv_attend_tiles<DIM, G, false>), dim3(blocks), dim3(256), 0, s, a);
     QMM_HIP_CHECK(hipGetLastError());
-    if (a.pieces > 1) {
-        const uint64_t each = 1024 / DIM, joins = ((uint64_t)a.heads * a.tokens + each - 1) / each;
-        if (joins >= 1ull << 24) return STARK_QMM_UNSUPPORTED;
-        hipLaunchKernelGGL((kv_attend_tiles_join<DIM>), dim3((uint32_t)joins), dim3(256), 0, s, a);
+    if (a.pieces > 1) {  // then the row tiles are fewer than workgroups fit the GPU
+        const uint32_t each = 1024 / DIM, joins = (a.heads * a.tokens + each - 1) / each;
+        hipLaunchKernelGGL((kv_attend_tiles_join<DIM>), dim3(joins), dim3(256), 0, s, a);
         QMM_HIP_CHECK(hipGetLastError());
     }
     return STARK_QMM_OK;

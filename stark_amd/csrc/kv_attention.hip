@@ -27,8 +27,6 @@ stark_qmm_status check(const stark_qmm_kv_attention_args* p, AttendArgs* a) {
     a->max_query = std::min(p->max_query, p->tokens);
     a->max_kv = std::min(p->max_kv, p->table_stride * p->cache.page_size);
     if (a->max_kv > 0x7fff0000u) return STARK_QMM_INVALID_ARGUMENT;  // positions past a tile's end are int32 as well
-    // steps of a call are counted in 31 bits
-    if ((uint64_t)a->batch * a->cache.kv_heads * 4 * (a->max_kv / 32 + 40ull) >= 1ull << 31) return STARK_QMM_UNSUPPORTED;
     a->is_bf16 = p->data_type == STARK_QMM_BF16;
     a->causal = p->causal != 0, a->window = (int32_t)std::min(p->window, 0x7fffffffu);
     const float scale = p->scale == 0.0f ? 1.0f : fabsf(p->scale);
@@ -56,15 +54,17 @@ stark_qmm_status compute_units(uint32_t* cus) {
 stark_qmm_status plan_work(AttendArgs* a, uint64_t* workspace) {
     *workspace = 0;
     if (a->batch == 0 || a->max_query == 0) return STARK_QMM_OK;  // (tiling divides by the requests)
+    const kv::Rows rows = kv::row_limit(a->batch, a->max_query, a->ratio, a->max_kv);
+    const uint64_t most = (uint64_t)a->max_query * a->ratio, all = (uint64_t)a->tokens * a->ratio;
+    a->row_limit = std::min<uint64_t>(rows.limit, most), a->row_block = rows.block;
+    const uint32_t blocks = (a->row_limit + a->row_block - 1) / a->row_block;
+    // all refusals are here: none after a launch
+    if (!kv::fits(a->batch, a->cache.kv_heads, blocks, a->max_kv, most > a->row_limit ? all : 0)) return STARK_QMM_UNSUPPORTED;
     uint32_t cus = 0;
     const stark_qmm_status st = compute_units(&cus);
     if (st != STARK_QMM_OK) return st;
-    const kv::Rows rows = kv::row_limit(a->batch, a->max_query, a->ratio, a->max_kv);
-    const uint64_t most = (uint64_t)a->max_query * a->ratio;
-    a->row_limit = std::min<uint64_t>(rows.limit, most), a->row_block = rows.block;
     if (a->row_limit) {
         a->ratio_inverse = (65535 + a->ratio) / a->ratio;
-        const uint32_t blocks = (a->row_limit + a->row_block - 1) / a->row_block;
         const kv::Share w = kv::share(a->batch, a->cache.kv_heads * blocks, a->row_block, a->max_kv,
                                       cus * (a->cache.dim == 256 ? 1 : 2));
         a->whole = w.whole, a->grid = w.grid;
@@ -72,9 +72,9 @@ stark_qmm_status plan_work(AttendArgs* a, uint64_t* workspace) {
         if (!w.whole) *workspace = (uint64_t)w.grid * (2 * kRows * (a->cache.dim * 4ull + 8) + 16);
     }
     if (most > a->row_limit) {
-        const kv::Tiling t = kv::tiling(a->batch, a->cache.kv_heads, (uint64_t)a->tokens * a->ratio, most, a->max_kv, cus);
-        const uint64_t even = (uint64_t)t.tiles * a->batch, need = kv::row_tiles((uint64_t)a->tokens * a->ratio, a->batch);
-        a->tiles = even <= need ? t.tiles : 0, a->turns = (uint32_t)std::min({even, need, (uint64_t)0xffffffffu});
+        const kv::Tiling t = kv::tiling(a->batch, a->cache.kv_heads, all, most, a->max_kv, cus);
+        const uint64_t even = (uint64_t)t.tiles * a->batch, need = kv::row_tiles(all, a->batch);
+        a->tiles = even <= need ? t.tiles : 0, a->turns = (uint32_t)std::min(even, need);
         a->pieces = t.pieces;
         if (t.pieces > 1) *workspace += (uint64_t)a->tokens * a->heads * t.pieces * (a->cache.dim * 4ull + 8);
     }

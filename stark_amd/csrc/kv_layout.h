@@ -181,4 +181,14 @@ KV_HD Tiling tiling(uint32_t batch, uint32_t kv_heads, uint64_t rows, uint64_t m
     return {(uint32_t)((most_rows + kTileRows - 1) / kTileRows), (uint32_t)(want < longest ? want : longest ? longest : 1)};
 }
 
+// Whether the launches of a call stay inside what is counted: workgroups in 24 bits and shared steps in 31. blocks: of rows in
+// the decode kernel (0: it takes none); rows: of the call on a kv head, where some are the tile kernel's, else 0. (Pieces add
+// less than two workgroups a CU.)
+KV_HD bool fits(uint32_t batch, uint32_t kv_heads, uint32_t blocks, uint32_t max_kv, uint64_t rows) {
+    const uint64_t units = (uint64_t)batch * kv_heads * blocks;
+    const bool whole = share(batch, kv_heads * blocks, 16, max_kv, 1).whole;
+    if (blocks && (whole ? units >= 1ull << 24 : units * (max_kv / 32 + 40ull) >= 1ull << 31)) return false;
+    return !rows || kv_heads * row_tiles(rows, batch) < (1ull << 24) - (1u << 17);
+}
+
 }  // namespace kv
