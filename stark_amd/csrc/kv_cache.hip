@@ -619,9 +619,9 @@ stark_qmm_status stark_qmm_kv_read(const stark_qmm_kv_read_args* p, void* stream
     const stark_qmm_status st = kv_view(p->cache, &a.cache);
     if (st != STARK_QMM_OK) return st;
     if (!dt_ok(p->data_type)) return STARK_QMM_UNSUPPORTED_DATA_TYPE;
-    if (p->tokens > (1u << 24) || (!p->k && !p->v)) return STARK_QMM_INVALID_ARGUMENT;
+    if (p->tokens > (1u << 24)) return STARK_QMM_INVALID_ARGUMENT;
     if (p->tokens == 0) return STARK_QMM_OK;
-    if (!p->slots || !kv_aligned(p->slots, 4)) return STARK_QMM_INVALID_ARGUMENT;
+    if ((!p->k && !p->v) || !p->slots || !kv_aligned(p->slots, 4)) return STARK_QMM_INVALID_ARGUMENT;
     const uint32_t dim = a.cache.dim, dt = p->data_type;
     if ((p->k && !kv_rows_ok(p->k, p->k_token_stride, p->k_head_stride, p->tokens, a.cache.kv_heads, dim, dt)) ||
         (p->v && !kv_rows_ok(p->v, p->v_token_stride, p->v_head_stride, p->tokens, a.cache.kv_heads, dim, dt)))

@@ -379,3 +379,11 @@ def test_the_workspace_of_a_call_without_rows():
         s.batch, s.tokens, s.heads, s.table_stride, s.max_query, s.max_kv = batch, tokens, 8, 64, most, 4096
         n = C.c_uint64(77)
         assert Q.lib().stark_qmm_kv_attention_workspace_size(C.byref(s), C.byref(n)) == Q.OK and n.value == 0
+
+
+def test_a_read_of_no_tokens():
+    """Tensors of no rows have no address."""
+    from stark_amd import kv as K, qmm as Q
+    s = K._ReadArgs()
+    s.struct_size, s.cache, s.data_type = C.sizeof(s), _cache(), Q.F32
+    assert Q.lib().stark_qmm_kv_read(C.byref(s), None) == Q.OK
