@@ -628,8 +628,9 @@ typedef struct stark_qmm_kv_append_args {
 } stark_qmm_kv_append_args;
 
 /* Rotates the query and key rows of new tokens and writes their keys (rotated,
- * not rounded in between) and values to the cache. Slots must be distinct: of
- * two rows for one slot each group keeps one or the other. */
+ * not rounded in between) and values to the cache. Slots must be distinct: a
+ * slot with two rows ends with each group's scale and bias of one of them, and
+ * codes of either. */
 STARK_QMM_API stark_qmm_status stark_qmm_kv_append(const stark_qmm_kv_append_args* args, void* stream);
 
 typedef struct stark_qmm_kv_read_args {

@@ -301,3 +301,123 @@ def test_thousands_of_requests_with_a_long_bound(K):
         for part, n, causal in ((slice(0, batch - 1), 7, False), (slice(batch - 1, rows), long, True)):
             want, _, tol, _ = R.attention(hq[part, mine], hk[:n, h], hv[:n, h], dim ** -0.5, causal, 0, 0.0, 2)
             assert (np.abs(ho[part, mine] - want) <= tol + R.EPS["bf16"] * (np.abs(want) + tol)).all()
+
+
+SHARED = [
+    # decode rows in blocks of 8 or 16 whose steps workgroups share, and prompts in pieces: one workspace for both
+    ([(1, 2500)] * 15 + [(100, 3000)], 8, 2, 128, 64, 64, "bf16", {}),
+    ([(1, 2100), (2, 2300), (3, 40)] * 6 + [(150, 2200), (0, 7)], 12, 2, 64, 32, 16, "f16", dict(window=1500)),
+    ([(70, 2600)] + [(1, 2200)] * 16 + [(90, 100)], 32, 2, 128, 128, 32, "bf16", {}),
+    ([(1, 2100)] * 16 + [(40, 2100)], 14, 1, 256, 64, 64, "bf16", dict(soft_cap=20.0)),
+    ([(1, 16000), (60, 9000), (1, 20000), (1, 3)], 4, 2, 64, 64, 64, "bf16", {}),
+    # each unit a workgroup of its own, beside prompts
+    ([(1, 900)] * 17 + [(30, 900)], 10, 1, 256, 32, 32, "f16", {}),
+    ([(1, 64), (5, 64), (1, 0), (33, 200)] * 8, 6, 3, 64, 32, 16, "bf16", dict(causal=False)),
+    # blocks of 16 rows of wide heads
+    ([(1, 300), (2, 1500), (4, 90)], 16, 1, 256, 128, 64, "bf16", {}),
+    ([(3, 700)], 16, 2, 256, 32, 16, "f16", dict(window=300)),
+    ([(5, 1300), (5, 2000), (2, 10)], 12, 1, 256, 64, 32, "bf16", dict(soft_cap=12.0)),
+]
+
+
+@pytest.mark.parametrize("with_lse", [True, False])
+@pytest.mark.parametrize("requests,heads,kvh,dim,group,page,dtype,options", SHARED)
+def test_decode_rows_and_prompts_in_one_call(K, requests, heads, kvh, dim, group, page, dtype, options, with_lse):
+    s = Served(K, 53, requests, heads, kvh, dim, group, page, dtype, pad_tokens=2)
+    _run(s, with_lse=with_lse, **options)
+    s.check(**options)
+
+
+def test_decode_rows_and_prompts_in_one_captured_call(K):
+    """The combined call captured, replayed over other lengths within its bounds, and against the eager call each time."""
+    s = Served(K, 54, [(1, 2500)] * 17 + [(90, 2600)], 8, 2, 128, 64, 64, "bf16", pad_tokens=2)
+    op = s.operator()
+    op.encode()
+    torch.cuda.synchronize()
+    s.check()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph, stream=stream):
+        op.encode()
+    lengths, start = s.kv_lengths.clone(), s.query_start.clone()
+    for i, cut in enumerate((0, 700, 2000, 2400, 0)):
+        s.kv_lengths.copy_(lengths - cut)
+        s.query_start.copy_(start)
+        if i % 2:
+            s.query_start[-1] = 17 + 40  # a shorter prompt
+        s.out.fill_(9.0), s.lse.fill_(9.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = s.out.clone(), s.lse.clone()
+        s.out.fill_(9.0), s.lse.fill_(9.0)
+        op.encode()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0].view(torch.int16), s.out.view(torch.int16)) and torch.equal(got[1], s.lse)
+    s.check()
+
+
+@pytest.mark.parametrize("heads,kvh,cut", [(4, 2, 2), (60, 2, 5)])
+def test_lengths_past_the_bounds_give_the_rows_that_are_left(K, heads, kvh, cut):
+    """query_start below 0 and past the rows, a negative length and one past the bound: what kv::request leaves of each
+    request is computed, and every other row stays as it was."""
+    s = Served(K, 55, [(2, 60), (9, 50)], heads, kvh, 64, 32, 16, "bf16", pad_tokens=2)
+    q, k, v = _np(s.q), _np(s.k), _np(s.v)
+    for start, lengths, rows, keys in (([0, 2, 2 ** 31 - 1], [60, 2 ** 31 - 1], [(0, 2), (2, cut)], [60, 60]),
+                                       ([-4, -2, 5], [-1, 50], [(0, 0), (0, cut)], [0, 50])):
+        s.query_start.copy_(_ints(start))
+        s.kv_lengths.copy_(_ints(lengths))
+        s.out.fill_(9.0), s.lse.fill_(9.0)
+        _run(s, max_query=cut)
+        out, lse = _np(s.out), _np(s.lse)
+        left = np.ones(q.shape[0], bool)
+        for b, ((at, n), kv) in enumerate(zip(rows, keys)):
+            left[at:at + n] = False
+            if kv > s.requests[b][1]:
+                continue  # keys that nothing wrote: what these rows are is not said
+            kk, vv = (x[:kv] if b == 0 else x[60:60 + kv] for x in (k, v))
+            for h in range(kvh if n else 0):
+                each = heads // kvh
+                mine = slice(h * each, (h + 1) * each)
+                want, wl, tol, dl = R.attention(q[at:at + n, mine], kk[:, h], vv[:, h], 64 ** -0.5, True, 0, 0.0,
+                                                1 if cut * each > 64 else 0)
+                assert (np.abs(out[at:at + n, mine] - want) <= tol + R.EPS["bf16"] * (np.abs(want) + tol)).all()
+                assert (np.abs(lse[at:at + n, mine] - wl) <= dl + 2.0 ** -23 * np.abs(wl)).all()
+        assert (out[left] == 9.0).all() and (lse[left] == 9.0).all()
+
+
+@pytest.mark.parametrize("requests,heads,kvh", [([(1, 70), (2, 300), (1, 9)], 8, 2), ([(1, 70)] * 70 + [(100, 300)], 8, 2),
+                                                ([(60, 300), (130, 200)], 4, 2), ([(1, 2100)] * 30 + [(90, 2200)], 8, 2)])
+def test_rows_ahead_of_the_first_request(K, requests, heads, kvh):
+    """query_start may begin behind row 0: the rows before it are no request's."""
+    s = Served(K, 56, requests, heads, kvh, 128, 64, 16, "bf16", pad_tokens=300)
+    s.query_start += 290
+    s.q = torch.roll(s.q, 290, 0)
+    _run(s)
+    s.q, s.out, s.lse = (torch.roll(t, -290, 0) for t in (s.q, s.out, s.lse))
+    s.check()
+
+
+def test_two_rows_for_one_slot(K):
+    """What the slot holds is of the two: each group has one row's scale and bias, and codes of either. No other slot
+    changes."""
+    rng = np.random.default_rng(57)
+    t, kvh, dim, group = 64, 2, 128, 32
+    x = _round(rng.normal(0, 1, (2 * t, kvh, dim)) + rng.normal(0, 3, (2 * t, 1, 1)), "bf16")
+    cache = K.KvCache(t // 16 + 1, 16, kvh, dim, group)
+    cache.data.fill_(0xA5)
+    slots = _ints(np.concatenate([np.arange(t), rng.permutation(t)]))
+    dev = _dev(x, torch.bfloat16)
+    K.KvAppend(cache, dev, dev, slots).encode()
+    out = [torch.zeros(t, kvh, dim, device="cuda") for _ in range(2)]
+    K.KvRead(cache, _ints(np.arange(t)), *out).encode()
+    torch.cuda.synchronize()
+    assert (cache.data.view(t // 16 + 1, -1)[-1] == 0xA5).all()
+    order = _np(slots)
+    sums = [p.astype(np.float64)[..., None] for p in R.planes(x, group)]
+    for got in out:
+        g = _np(got).reshape(t, kvh, dim // group, group)
+        fits = np.zeros(g.shape[:-1], bool)
+        for rows in (np.arange(t), t + np.argsort(order[t:])):
+            scale, bias = (p[rows] for p in sums)
+            code = (g - bias) / scale
+            fits |= ((np.abs(code - np.rint(code)) < 1e-3) & (code > -0.5) & (code < 15.5)).all(-1)
+        assert fits.all()
