@@ -269,7 +269,8 @@ class KvAttention(_Operator):
         s.soft_cap, s.causal, s.window = soft_cap, int(causal), window
         need = C.c_uint64()
         s.struct_size = C.sizeof(s)
-        Q._check(Q.lib().stark_qmm_kv_attention_workspace_size(C.byref(s), C.byref(need)), "KvAttention")
+        with torch.cuda.device(q.device):  # its size depends on the device's compute units
+            Q._check(Q.lib().stark_qmm_kv_attention_workspace_size(C.byref(s), C.byref(need)), "KvAttention")
         self.workspace_bytes = need.value
         if workspace is None and need.value:
             workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)

@@ -421,3 +421,18 @@ def test_two_rows_for_one_slot(K):
             code = (g - bias) / scale
             fits |= ((np.abs(code - np.rint(code)) < 1e-3) & (code > -0.5) & (code < 15.5)).all(-1)
         assert fits.all()
+
+
+def test_the_workspace_is_that_of_the_tensors_device(K, monkeypatch):
+    """Its size depends on the device's compute units: the query is made with that device current."""
+    s = Served(K, 58, [(1, 5000)], 8, 2, 128, 64, 16, "bf16")
+    seen, inner = [], torch.cuda.device
+
+    class Spy(inner):
+        def __enter__(self):
+            seen.append(self.idx)
+            return super().__enter__()
+
+    monkeypatch.setattr(torch.cuda, "device", Spy)
+    op = s.operator()
+    assert op.workspace_bytes and s.q.device.index in seen
