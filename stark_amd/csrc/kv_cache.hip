@@ -551,6 +551,14 @@ stark_qmm_status stark_qmm_kv_plan(const stark_qmm_kv_plan_args* p, void* stream
                          p->slots, p->positions, p->free_left, p->status};
     for (const void* x : all)
         if (!kv_aligned(x, 4)) return STARK_QMM_INVALID_ARGUMENT;
+    // what is written overlaps nothing else: workgroups read while others write
+    const uint64_t words[] = {p->batch, p->batch, p->free_capacity, 1, (uint64_t)p->batch * p->table_stride, p->batch + 1ull,
+                              p->batch, p->token_capacity, p->token_capacity, 1, 1};
+    for (int i = 4; i < 11; ++i)
+        for (int j = 0; j < 11; ++j) {
+            const uintptr_t x = (uintptr_t)all[i], y = (uintptr_t)all[j];
+            if (i != j && words[i] && words[j] && x < y + 4 * words[j] && y < x + 4 * words[i]) return STARK_QMM_INVALID_ARGUMENT;
+        }
     PlanArgs a{p->cached, p->added, p->free_pages, p->free_count, p->block_table, p->query_start, p->kv_lengths, p->slots,
                p->positions, p->free_left, p->status, p->batch, p->token_capacity, p->free_capacity, p->table_stride, 4};
     while ((1u << a.page_shift) < p->page_size) ++a.page_shift;

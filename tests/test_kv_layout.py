@@ -387,3 +387,20 @@ def test_a_read_of_no_tokens():
     s = K._ReadArgs()
     s.struct_size, s.cache, s.data_type = C.sizeof(s), _cache(), Q.F32
     assert Q.lib().stark_qmm_kv_read(C.byref(s), None) == Q.OK
+
+
+def test_a_plan_whose_outputs_overlap_is_refused():
+    """Workgroups read the lengths and the free list while others write."""
+    from stark_amd import qmm as Q
+    call = Q.lib().stark_qmm_kv_plan
+    names = ("cached", "added", "free_pages", "free_count", "block_table", "query_start", "kv_lengths", "slots", "positions",
+             "free_left", "status")
+    sizes = dict(cached=2, added=2, free_pages=4, free_count=1, block_table=8, query_start=3, kv_lengths=2, slots=8, positions=8,
+                 free_left=1, status=1)
+    apart = {n: FAKE + 4096 * i for i, n in enumerate(names)}
+    outputs = names[4:]
+    for o in outputs:
+        for n in names:
+            if n != o:
+                for at in (apart[n], apart[n] + 4 * (sizes[n] - 1), apart[n] - 4 * (sizes[o] - 1)):
+                    assert call(C.byref(_plan(**dict(apart, **{o: at}))), None) == Q.INVALID_ARGUMENT, (o, n)
