@@ -197,7 +197,25 @@ QMM_DEVICE uint32_t wave_scan(uint32_t v) {
 // a step and its wait, 2.0 the joining of the waves (a wave alone on its SIMD issues an instruction in 6 to 8 clocks). Blocks of 4 rows (four records to a score
 // block) took 134 us there, blocks of 16 for 4 rows 67 us against 60 (64 requests of 4096 keys); more workgroups, loads three
 // and four steps ahead and more waves a SIMD were no faster.
-template <int DIM, int G, int PACK>
+// MODE. The matrix cores multiply subnormal codes exactly, but align the products of a sum by the exponent fields of their
+// factors, so that some 2^-17 of the largest is cut off: scores are off by 2e-6 to 1e-5 (root mean square, scores of 2).
+// kPlain (bf16 without lse): that, and one rounding of p s to f16, stand beside outputs that are rounded to 2^-9: 1.01 times
+// as far from exact arithmetic as a rounding alone.
+// kLse (f16, or with lse): codes of keys are made f16 numbers, c - 8, which takes one packed operation for two of them; scores
+// are then as f32 sums give them (1e-7). 64 sequences 137 us, 129 without.
+enum { kPlain, kLse };
+
+// Two codes less 8 (bits 0-3 and 16-19 of w, or 4 bits higher and sixteenfold): 1024 + c by its bits, less 1032, exact.
+QMM_DEVICE uint32_t less_8(uint32_t w) {
+    const f16x2 c = __builtin_bit_cast(f16x2, and_or(w, 0x000f000fu, 0x64006400u));
+    return __builtin_bit_cast(uint32_t, c - (f16x2){(_Float16)1032.0f, (_Float16)1032.0f});
+}
+QMM_DEVICE uint32_t less_8_sixteenfold(uint32_t w) {
+    const f16x2 c = __builtin_bit_cast(f16x2, and_or(w, 0x00f000f0u, 0x64006400u));
+    return __builtin_bit_cast(uint32_t, c - (f16x2){(_Float16)1152.0f, (_Float16)1152.0f});
+}
+
+template <int DIM, int G, int PACK, int MODE>
 __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(AttendArgs a) {
     using S = Shape<PACK>;
     using Codes = Step<DIM, G, S::T, PACK == 2>;
@@ -346,7 +364,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
                 s += __shfl_xor(s, 32, 64);
                 s = live ? s : 0.0f;
                 qsum[gr] = s * c1;
-                const float v = s * -0x1p-21f;  // -8 sum q, in the accumulator's scale
+                const float v = MODE == kPlain ? s * -0x1p-21f : 0.0f;  // -8 sum q, in the accumulator's scale
                 less8[gr] = f32x4{v, v, v, v};
             }
             // every wave has the same rows: wave w writes the blocks w, w + 4, ...
@@ -391,10 +409,10 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
             smax = max(smax, (uint32_t)__shfl_xor((int)smax, 16, 64));
             return max(smax, (uint32_t)__shfl_xor((int)smax, 32, 64));
         };
-        // On the scales of the lane's plane words: 2^24 for keys, whose codes are c 2^-24, and the values' power of two. (Not
-        // on the probabilities: the reference less an exponent would be rounded where scores pass 2^24.)
+        // On the scales of the lane's plane words: what the keys' codes are short of (c 2^-24 where they are subnormals), and the
+        // values' power of two. (Not on the probabilities: the reference less an exponent would be rounded where scores pass 2^24.)
         int value_exponent = 0;
-        float plane_factor = 0x1p24f;
+        float plane_factor = MODE == kPlain ? 0x1p24f : 1.0f;
         const auto step = [&](Codes& st, uint32_t n) {
             const int32_t t0 = (int32_t)(mine + 4 * KEYS * n);
 #pragma unroll
@@ -421,7 +439,9 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
                     const int i = n / J, j = n % J;
                     if (n + 2 < PACK * J) q[(n + 2) % 3] = q_operand((n + 2) / J, (n + 2) % J);
                     const uint32_t w = st.kc[PACK * u + i][j], v = w >> 8;
-                    const f16x8 k = operand(w & 0x000f000fu, w & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u);
+                    const f16x8 k = MODE == kPlain
+                                        ? operand(w & 0x000f000fu, w & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u)
+                                        : operand(less_8(w), less_8_sixteenfold(w), less_8(v), less_8_sixteenfold(v));
                     acc[j / JG] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
                         k, q[n % 3], i == 0 && j % JG == 0 ? less8[j / JG] : acc[j / JG], 0, 0, 0);
                     __builtin_amdgcn_sched_barrier(0);
@@ -710,10 +730,10 @@ __global__ __launch_bounds__(256) void kv_attend_join(AttendArgs a) {
     if (a.lse && lane == 0) a.lse[(size_t)token * a.heads + qh] = l == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-template <int DIM, int G, int PACK>
+template <int DIM, int G, int PACK, int MODE>
 stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
     const uint64_t units = (uint64_t)a.batch * a.cache.kv_heads * ((a.row_limit + a.row_block - 1) / a.row_block);
-    hipLaunchKernelGGL((kv_attend_rows<DIM, G, PACK>), dim3(a.whole ? (uint32_t)units : a.grid), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((kv_attend_rows<DIM, G, PACK, MODE>), dim3(a.whole ? (uint32_t)units : a.grid), dim3(256), 0, s, a);
     QMM_HIP_CHECK(hipGetLastError());
     if (!a.whole) {
         hipLaunchKernelGGL((kv_attend_join<DIM>), dim3(a.grid * (a.row_block / 4)), dim3(256), 0, s, a);
@@ -724,7 +744,8 @@ stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
 
 template <int DIM, int G>
 stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
-    return a.row_block == 8 ? launch<DIM, G, 2>(a, s) : launch<DIM, G, 1>(a, s);
+    if (a.lse || !a.is_bf16) return a.row_block == 8 ? launch<DIM, G, 2, kLse>(a, s) : launch<DIM, G, 1, kLse>(a, s);
+    return a.row_block == 8 ? launch<DIM, G, 2, kPlain>(a, s) : launch<DIM, G, 1, kPlain>(a, s);
 }
 
 }  // namespace

@@ -436,3 +436,22 @@ def test_the_workspace_is_that_of_the_tensors_device(K, monkeypatch):
     monkeypatch.setattr(torch.cuda, "device", Spy)
     op = s.operator()
     assert op.workspace_bytes and s.q.device.index in seen
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,dim,group", [(1, 128, 32), (2, 64, 64), (3, 256, 128), (20, 128, 32), (40, 64, 64)])
+def test_lse_is_as_exact_as_f32_sums(K, rows, dim, group, dtype):
+    """With one key the lse is the score. A dozen f32 roundings (sums of each scale group, planes) of terms of some two times
+    a score's size, beside the seven or so of a plain sum in f32: within 8 times that sum's error, as root mean square."""
+    batch = 64
+    s = Served(K, 61, [(rows, 1)] * batch, 16, 2, dim, group, 16, dtype)
+    _run(s, causal=False)
+    lse, ours, plain = _np(s.lse), 0.0, 0.0
+    q32, k32 = s.q.float(), s.k
+    for i, (at, mine, q, k, v) in enumerate(_requests(s)):
+        b, h = divmod(i, 2)
+        want = np.einsum("nhd,d->nh", q, k[0]) * dim ** -0.5
+        f32 = _np((q32[at, mine] * k32[b, h]).sum(-1) * dim ** -0.5)
+        ours += ((lse[at, mine] - want) ** 2).sum()
+        plain += ((f32 - want) ** 2).sum()
+    assert ours <= 64 * plain, (ours / plain) ** 0.5
