@@ -201,9 +201,11 @@ QMM_DEVICE uint32_t wave_scan(uint32_t v) {
 // factors, so that some 2^-17 of the largest is cut off: scores are off by 2e-6 to 1e-5 (root mean square, scores of 2).
 // kPlain (bf16 without lse): that, and one rounding of p s to f16, stand beside outputs that are rounded to 2^-9: 1.01 times
 // as far from exact arithmetic as a rounding alone.
-// kLse (f16, or with lse): codes of keys are made f16 numbers, c - 8, which takes one packed operation for two of them; scores
+// kLse (bf16 with lse): codes of keys are made f16 numbers, c - 8, which takes one packed operation for two of them; scores
 // are then as f32 sums give them (1e-7). 64 sequences 137 us, 129 without.
-enum { kPlain, kLse };
+// kFine (f16): values' codes as well, and p s as two f16, the second what the first leaves (2^-22 of it): an output is off by
+// its own rounding, where one f16 made it 1.3 to 1.4 times as much. 64 sequences 155 us.
+enum { kPlain, kLse, kFine };
 
 // Two codes less 8 (bits 0-3 and 16-19 of w, or 4 bits higher and sixteenfold): 1024 + c by its bits, less 1032, exact.
 QMM_DEVICE uint32_t less_8(uint32_t w) {
@@ -493,8 +495,8 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
 #pragma unroll
                 for (int j = 0; j < 2 * J; ++j) run.o[j] *= f;
             }
-            // p s to f16, half a unit of 2^-11: the codes it multiplies are exact
-            u32x2 ps[B][G];
+            // p s to f16, half a unit of 2^-11 (kFine: and the rest): the codes it multiplies are exact
+            u32x2 ps[B][G], rest[B][G];
 #pragma unroll
             for (int u = 0; u < B; ++u) {
                 float p[4];
@@ -518,25 +520,32 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
                     }
 #pragma unroll
                     for (int e = 0; e < 4; ++e) run.beta[gr] = fmaf(p[e], mid[e], run.beta[gr]);
-                    ps[u][gr][0] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)(p[0] * s[0]), (_Float16)(p[1] * s[1])});
-                    ps[u][gr][1] = __builtin_bit_cast(uint32_t, f16x2{(_Float16)(p[2] * s[2]), (_Float16)(p[3] * s[3])});
+#pragma unroll
+                    for (int e = 0; e < 4; e += 2) {
+                        const float v = p[e] * s[e], w = p[e + 1] * s[e + 1];
+                        const f16x2 h = {(_Float16)v, (_Float16)w};
+                        ps[u][gr][e / 2] = __builtin_bit_cast(uint32_t, h);
+                        if (MODE == kFine)
+                            rest[u][gr][e / 2] =
+                                __builtin_bit_cast(uint32_t, f16x2{(_Float16)(v - (float)h[0]), (_Float16)(w - (float)h[1])});
+                    }
                 }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // before the next step's planes are written
             const f16x8 eights = operand(0x00080008u, 0x00080008u, 0x00080008u, 0x00080008u);  // 8 2^-24
 #pragma unroll
             for (int h = 0; h < T / 2; ++h) {  // records 2 h and 2 h + 1
-                f16x8 pb[G];
+                f16x8 pb[G], pr[G];
+                const auto p_operand = [&](const u32x2 (&w)[B][G], int gr) {
+                    if (PACK == 1) return operand(w[0][gr][0], w[0][gr][1], w[B - 1][gr][0], w[B - 1][gr][1]);
+                    const bool lo = (int)pack == 2 * h, hi = (int)pack == 2 * h + 1;
+                    return operand(lo ? w[0][gr][0] : 0, lo ? w[0][gr][1] : 0, hi ? w[0][gr][0] : 0, hi ? w[0][gr][1] : 0);
+                };
 #pragma unroll
                 for (int gr = 0; gr < G; ++gr) {
-                    if (PACK == 1) {
-                        pb[gr] = operand(ps[0][gr][0], ps[0][gr][1], ps[B - 1][gr][0], ps[B - 1][gr][1]);
-                    } else {
-                        const bool lo = (int)pack == 2 * h, hi = (int)pack == 2 * h + 1;
-                        pb[gr] = operand(lo ? ps[0][gr][0] : 0, lo ? ps[0][gr][1] : 0, hi ? ps[0][gr][0] : 0,
-                                         hi ? ps[0][gr][1] : 0);
-                    }
-                    run.rounded[gr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eights, pb[gr], run.rounded[gr], 0, 0, 0);
+                    pb[gr] = p_operand(ps, gr);
+                    if (MODE == kFine) pr[gr] = p_operand(rest, gr);
+                    else run.rounded[gr] = __builtin_amdgcn_mfma_f32_16x16x32_f16(eights, pb[gr], run.rounded[gr], 0, 0, 0);
                 }
 #pragma unroll
                 for (int i = 0; i < J; ++i) {  // 32-value blocks; byte i of a lane's value words
@@ -555,10 +564,21 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
                             w[2 * u + 1] = permb(v[3], v[2], sel);
                         }
                     }
-                    const f16x8 lo = operand(w[0] & 0x000f000fu, w[1] & 0x000f000fu, w[2] & 0x000f000fu, w[3] & 0x000f000fu);
-                    const f16x8 hi = operand(w[0] & 0x00f000f0u, w[1] & 0x00f000f0u, w[2] & 0x00f000f0u, w[3] & 0x00f000f0u);
+                    f16x8 lo, hi;
+                    if (MODE == kFine) {
+                        lo = operand(less_8(w[0]), less_8(w[1]), less_8(w[2]), less_8(w[3]));
+                        hi = operand(less_8_sixteenfold(w[0]), less_8_sixteenfold(w[1]), less_8_sixteenfold(w[2]),
+                                     less_8_sixteenfold(w[3]));
+                    } else {
+                        lo = operand(w[0] & 0x000f000fu, w[1] & 0x000f000fu, w[2] & 0x000f000fu, w[3] & 0x000f000fu);
+                        hi = operand(w[0] & 0x00f000f0u, w[1] & 0x00f000f0u, w[2] & 0x00f000f0u, w[3] & 0x00f000f0u);
+                    }
                     run.o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, pb[i / JG], run.o[2 * i], 0, 0, 0);
                     run.o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, pb[i / JG], run.o[2 * i + 1], 0, 0, 0);
+                    if (MODE == kFine) {
+                        run.o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo, pr[i / JG], run.o[2 * i], 0, 0, 0);
+                        run.o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi, pr[i / JG], run.o[2 * i + 1], 0, 0, 0);
+                    }
                 }
             }
         };
@@ -620,7 +640,7 @@ __global__ __launch_bounds__(256, DIM == 256 ? 1 : 2) void kv_attend_rows(Attend
         for (int k = 0; k < 4 * PACK; ++k) ref = fmaxf(ref, wave_ref[k / PACK][k % PACK * R + row]);
         const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - ref);
         if (g == 0) wave_sum_l[wave][c] = l == 0.0f ? 0.0f : l * f;
-        const float unscale = ldexp_f32(0x1p24f, -value_exponent);
+        const float unscale = ldexp_f32(MODE == kFine ? 1.0f : 0x1p24f, -value_exponent);
         // lane: values 32 i + 8 g + 0 .. 7 of its column
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) {
@@ -744,7 +764,8 @@ stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
 
 template <int DIM, int G>
 stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
-    if (a.lse || !a.is_bf16) return a.row_block == 8 ? launch<DIM, G, 2, kLse>(a, s) : launch<DIM, G, 1, kLse>(a, s);
+    if (!a.is_bf16) return a.row_block == 8 ? launch<DIM, G, 2, kFine>(a, s) : launch<DIM, G, 1, kFine>(a, s);
+    if (a.lse) return a.row_block == 8 ? launch<DIM, G, 2, kLse>(a, s) : launch<DIM, G, 1, kLse>(a, s);
     return a.row_block == 8 ? launch<DIM, G, 2, kPlain>(a, s) : launch<DIM, G, 1, kPlain>(a, s);
 }
 

@@ -438,6 +438,29 @@ def test_the_workspace_is_that_of_the_tensors_device(K, monkeypatch):
     assert op.workspace_bytes and s.q.device.index in seen
 
 
+@pytest.mark.parametrize("requests,heads,kvh,dim,group,options", [
+    ([(1, 3000), (3, 5000), (1, 40)], 8, 1, 128, 32, {}),
+    ([(1, 20000)], 8, 2, 64, 64, {}),
+    ([(5, 700), (2, 1500)], 8, 1, 256, 64, dict(soft_cap=30.0)),
+])
+def test_f16_outputs_are_off_by_their_own_rounding(K, requests, heads, kvh, dim, group, options):
+    """Over all rows of a call, as root mean square: the error of a correctly rounded output, and 5 % for all else. That is
+    products of probabilities and values to 2^-22 of each and sums in f32, two orders below f16's 2^-12; a probability or a
+    value held in one f16 alone would make it 30 % and more."""
+    def edit(k, v):
+        k *= 0.5
+        v -= v.mean(0)  # outputs as small as the keys' average leaves them: its parts' errors show
+
+    s = Served(K, 60, requests, heads, kvh, dim, group, 16, "f16", edit=edit)
+    _run(s, **options)
+    out, got, best = _np(s.out), 0.0, 0.0
+    for rows, mine, q, k, v in _requests(s):
+        want = R.attention(q, k, v, dim ** -0.5, True, options.get("window", 0), options.get("soft_cap", 0.0), 0)[0]
+        got += ((out[rows, mine] - want) ** 2).sum()
+        best += ((want.astype(np.float16).astype(np.float64) - want) ** 2).sum()
+    assert got <= 1.05 ** 2 * best, (got / best) ** 0.5
+
+
 @pytest.mark.parametrize("dtype", ["f16", "bf16"])
 @pytest.mark.parametrize("rows,dim,group", [(1, 128, 32), (2, 64, 64), (3, 256, 128), (20, 128, 32), (40, 64, 64)])
 def test_lse_is_as_exact_as_f32_sums(K, rows, dim, group, dtype):
