@@ -13,15 +13,20 @@ constexpr int kKeys = 64;  // keys of a tile: four records
 // LDS of one tile: keys [key][value of the head], values transposed [value of the head][key], both f16 in 16-byte pieces
 // whose place in a row is swizzled by the row, so that 16 lanes that read the same piece of 16 rows meet no bank twice.
 // not_finite: keys (bits) whose values' planes are not finite, for each group; they stand as zeros in v.
-// EXACT: keys are their codes less 8, and planes holds scales and middles (the value of code 8) of the keys, [group][scale
-// or middle][key].
-template <int DIM, int G, bool EXACT>
+// kLse and kFine: keys are their codes less 8, and planes holds scales and middles (the value of code 8) of the keys, [group]
+// [scale or middle][key].
+// kFine: values are code times the leading bits of their scale, exact, and rest holds what the two leave of a value: (scale /
+// leading - 1) | bias << 16, f16.
+enum { kPlain, kLse, kFine };
+template <int DIM, int G, int MODE>
 struct Tile {
+    static constexpr bool EXACT = MODE != kPlain, FINE = MODE == kFine;
     u32x4 k[kKeys][DIM / 8];
     u32x4 v[DIM][kKeys / 8];
     unsigned long long not_finite[G];
     alignas(16) uint32_t absent[4];  // records whose page is not in the cache
     alignas(16) float planes[EXACT ? G : 1][2][EXACT ? kKeys : 4];
+    alignas(16) uint32_t rest[FINE ? G : 1][FINE ? kKeys : 4];
     static QMM_DEVICE uint32_t key_piece(uint32_t key, uint32_t piece) {
         return piece ^ (DIM >= 128 ? key & 15 : key >> 1 & 7);
     }
@@ -42,6 +47,13 @@ QMM_DEVICE uint32_t two_values(uint32_t w, f16x2 s, f16x2 b) {
     return bits_of(__builtin_elementwise_fma(c, s, b));
 }
 
+// Of two f16 scales the seven leading bits (less where that would leave a subnormal with nothing): a product with a code has
+// eleven and is exact.
+QMM_DEVICE uint32_t leading(uint32_t w) {
+    const u16x2 h = __builtin_bit_cast(u16x2, w), low = {127, 127}, cut = __builtin_bit_cast(u16x2, w & 0xfff0fff0u);
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(cut, __builtin_elementwise_min(h, low)));
+}
+
 // Two codes less 8, exact.
 QMM_DEVICE uint32_t two_codes(uint32_t w) {
     return bits_of(half2_of(and_or(w, 0x000f000fu, 0x64006400u)) - (f16x2){(_Float16)1032.0f, (_Float16)1032.0f});
@@ -53,6 +65,7 @@ struct Codes {
     static constexpr int N = DIM / 32;  // words of a lane
     uint32_t kc[N], vc[N], kp[G];
     u32x4 vp[G];
+    uint32_t own[(G + 3) / 4];  // kFine: value planes of the lane's key lane % 16, groups lane / 16 and lane / 16 + 4
 
     QMM_DEVICE void load_keys(const uint8_t* rec, uint32_t lane) {
         const uint32_t c = lane & 15, g = lane >> 4;
@@ -66,6 +79,7 @@ struct Codes {
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) kp[gr] = *(const uint32_t*)(rec + 8 * DIM + 64 * gr + 4 * c);
     }
+    template <int MODE>
     QMM_DEVICE void load_values(const uint8_t* rec, uint32_t lane) {
         const uint8_t* p = rec + 8 * DIM + 64 * G + lane * (DIM == 64 ? 8 : 16);
         if (DIM == 64) {
@@ -76,10 +90,15 @@ struct Codes {
         }
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) vp[gr] = *(const u32x4*)(rec + 16 * DIM + 64 * G + 64 * gr + 16 * (lane >> 4));
+        if (MODE == kFine)
+#pragma unroll
+            for (int j = 0; j < (G + 3) / 4; ++j)
+                own[j] = *(const uint32_t*)(rec + 16 * DIM + 64 * G + 64 * ((lane >> 4) % G + 4 * j) + 4 * (lane & 15));
     }
     // record: 0 .. 3 in the tile
-    template <bool EXACT>
-    QMM_DEVICE void write_keys(Tile<DIM, G, EXACT>& t, uint32_t record, uint32_t lane) const {
+    template <int MODE>
+    QMM_DEVICE void write_keys(Tile<DIM, G, MODE>& t, uint32_t record, uint32_t lane) const {
+        constexpr bool EXACT = MODE != kPlain;
         const uint32_t key = 16 * record + (lane & 15), g = lane >> 4;
 #pragma unroll
         for (int j = 0; j < N; ++j) {  // word 4 j + g: values 8 (4 j + g) .. + 7, of group j G / N
@@ -99,8 +118,8 @@ struct Codes {
         }
     }
     // live: bit e: the lane's token 4 (lane / 16) + e is a key that some row may see, in a page of the cache
-    template <bool EXACT>
-    QMM_DEVICE void write_values(Tile<DIM, G, EXACT>& t, uint32_t record, uint32_t lane, uint32_t live) {
+    template <int MODE>
+    QMM_DEVICE void write_values(Tile<DIM, G, MODE>& t, uint32_t record, uint32_t lane, uint32_t live) {
         const uint32_t r = lane & 15, quad = lane >> 4;
         u32x4 q[G];  // (copies: the loaded registers stay as they are, or the next load's would be copied, and waited for)
 #pragma unroll
@@ -127,14 +146,29 @@ struct Codes {
                         if (r == 0) atomicOr(&t.not_finite[gr], 1ull << (16 * record + 4 * quad + e));
                     }
         }
+        if (MODE == kFine) {
+#pragma unroll
+            for (int j = 0; j < (G + 3) / 4; ++j) {
+                const uint32_t w = own[j];
+                const float all = plane_scale(w), lead = plane_scale(leading(w));
+                const bool finite = (w & 0x7c00u) != 0x7c00u && (w >> 16 & 0x7c00u) != 0x7c00u;
+                const float part = lead != 0.0f ? (all - lead) * __builtin_amdgcn_rcpf(lead) : 0.0f;
+                const uint32_t v = (uint32_t)f32_to_f16_bits(part) | (w & 0xffff0000u);
+                if (quad < (uint32_t)G) t.rest[MODE == kFine ? quad + 4 * j : 0][MODE == kFine ? 16 * record + r : 0] = finite ? v : 0u;
+            }
+        }
         // quads 0 and 2 of a record share a piece, and 1 and 3: the order of the probabilities in their operand
         const uint32_t piece = 2 * record + (quad & 1), half = quad >> 1;
 #pragma unroll
         for (int i = 0; i < DIM / 32; ++i) {  // byte i of the lane's value words: values 32 i + 2 r and the next
             constexpr int M = DIM / 32;
             const u32x4 p = q[i * G / M];
-            const f16x2 s01 = half2_of(permb(p[1], p[0], 0x05040100u)), b01 = half2_of(permb(p[1], p[0], 0x07060302u));
-            const f16x2 s23 = half2_of(permb(p[3], p[2], 0x05040100u)), b23 = half2_of(permb(p[3], p[2], 0x07060302u));
+            f16x2 s01 = half2_of(permb(p[1], p[0], 0x05040100u)), b01 = half2_of(permb(p[1], p[0], 0x07060302u));
+            f16x2 s23 = half2_of(permb(p[3], p[2], 0x05040100u)), b23 = half2_of(permb(p[3], p[2], 0x07060302u));
+            if (MODE == kFine) {
+                s01 = half2_of(leading(bits_of(s01))), s23 = half2_of(leading(bits_of(s23)));
+                b01 = b23 = f16x2{(_Float16)0.0f, (_Float16)0.0f};
+            }
             uint32_t w01, w23;
             if (DIM == 64) {
                 const uint32_t sel = 0x0c000c00u | (uint32_t)(2 + i) << 16 | (uint32_t)i;
@@ -198,21 +232,26 @@ QMM_DEVICE void read_ahead() {
 // Two tiles of LDS: the next tile is unpacked while this one is multiplied, and the one after that is in flight.
 // Bound by vector work beside the matrix cores: per 64 keys and 32 rows 32 products of 32x32x16 (1024 clocks) stand beside
 // 32 exponentials (512 clocks) and some 285 other vector instructions (1140), of which the unpacking has 150. 2048 tokens of
-// 32 heads on 8 of 128 against 4096 + 2048 keys take 213 us (805 TFLOP/s; a large library product reaches 1306), and took
-// 160 when the unpacking was left out for a measurement, 189 without the products. Slower were 256 rows to a workgroup with
-// 8 waves (254, causal tiles of unlike length then stand alone on a CU) and with 64 rows to a wave (314, one wave a SIMD
-// does not hide its own latencies); a running maximum taken from every tile's scores took 221, and so did the compiler's
-// own order of LDS reads.
-// EXACT (f16 outputs, or with lse): the score products take the codes themselves, exact in f16, one sum a scale group, and
-// a key's planes are applied to the scores in f32, as in kv_attend_rows; and lse is of the sum of the probabilities before
-// they are rounded. Keys rounded to f16 move a score by up to 2^-11 of scale |q| |k|, which bf16 outputs do not show, but
-// an f32 lse and f16 outputs do. The planes cost 2 G + 1 operations a score: the same chunk takes 235, 270 and 412 us with
-// 1, 2 and 4 groups (206, 215 and 222 without).
-template <int DIM, int G, bool EXACT>
+// 32 heads on 8 of 128 against 4096 + 2048 keys take 207 to 224 us by the card, 256 on one (830 to 770 TFLOP/s; a large library
+// product reaches 1130 to 1306). On a card where they took 213 they took 160 when the unpacking was left out for a measurement,
+// 189 without the products. Slower were 256 rows to a workgroup with 8 waves (254, causal tiles of unlike length then stand
+// alone on a CU) and with 64 rows to a wave (314, one wave a SIMD does not hide its own latencies); a running maximum taken from
+// every tile's scores took 221, and so did the compiler's own order of LDS reads.
+// kLse (bf16 with lse): the score products take the codes themselves, exact in f16, one sum a scale group, and a key's planes
+// are applied to the scores in f32, as in kv_attend_rows; and lse is of the sum of the probabilities before they are rounded.
+// Keys rounded to f16 move a score by up to 2^-11 of scale |q| |k|, which bf16 outputs do not show, but an f32 lse does.
+// kFine (f16): that, and neither a probability nor a value is rounded to one f16, which left outputs 1.5 times as far from exact
+// arithmetic as their own rounding. A value is s c + b = s' c (1 + r) + b with the seven leading bits s' of its scale, so that s' c
+// is exact, and sum p v = sum p' s' c + sum (p - p' + p r) s' c + sum p b: p' the probability's f16, the second factor one f16 for
+// each scale group (r below 2^-6: it is held to 2^-17 of p), the third sum f32. The keys' planes cost 2 G + 1 operations a score,
+// and the values' 2.5 G + 2 and a second product: the same chunk takes 213, 217 and 224 us with 1, 2 and 4 groups in bf16, 240,
+// 272 and 403 with lse, 333, 377 and 509 in f16.
+template <int DIM, int G, int MODE>
 __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(AttendArgs a) {
+    constexpr bool EXACT = MODE != kPlain, FINE = MODE == kFine;
     constexpr int J = DIM / 16;   // k blocks of a score product
     constexpr int O = DIM / 32;   // blocks of the output
-    using T = Tile<DIM, G, EXACT>;
+    using T = Tile<DIM, G, MODE>;
     __shared__ T tiles[2];
     const uint32_t lane = threadIdx.x & 63, col = lane & 31, hf = lane >> 5;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -278,13 +317,13 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
         in_cache = page < a.cache.page_count;
         const uint8_t* rec = base + (uint64_t)(in_cache ? page : 0) * a.cache.page_bytes + (t & page_mask) / 16 * a.cache.record;
         codes.load_keys(rec, lane);
-        codes.load_values(rec, lane);
+        codes.template load_values<MODE>(rec, lane);
         const int32_t left = r.kv_len - (int32_t)(t + 4 * (lane >> 4));
         live_keys = !in_cache || left <= 0 ? 0 : left >= 4 ? 15 : (1u << left) - 1;
     };
     const auto unpack = [&](T& t) {
-        codes.template write_keys<EXACT>(t, record, lane);
-        codes.template write_values<EXACT>(t, record, lane, live_keys);
+        codes.template write_keys<MODE>(t, record, lane);
+        codes.template write_values<MODE>(t, record, lane, live_keys);
         if (lane == 0) t.absent[record] = !in_cache;
     };
     if (threadIdx.x < 2 * G) tiles[threadIdx.x / G].not_finite[threadIdx.x % G] = 0;
@@ -340,6 +379,9 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
 #pragma unroll
     for (int i = 0; i < O; ++i) o[i] = f32x16{};
     float m = kNone, l = 0.0f, le = 0.0f;  // (le: of the probabilities before rounding)
+    float beta[FINE ? G : 1];              // kFine: sum p b of the lane's keys
+#pragma unroll
+    for (int gr = 0; gr < (FINE ? G : 1); ++gr) beta[gr] = 0.0f;
     __syncthreads();  // not_finite is clear
     if (steps) {
         // the first tile may begin before the window of its first row: what stands there may be anything by now
@@ -358,7 +400,118 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
 #pragma unroll
         for (int gr = 0; gr < G; ++gr) set |= t.not_finite[gr];
         const bool flags = __builtin_amdgcn_readfirstlane((int)(uint32_t)(set | set >> 32)) != 0;
-        if (t0 < outer_hi && t0 + kKeys > outer_lo) {
+        if (FINE && t0 < outer_hi && t0 + kKeys > outer_lo) {
+            // 32 keys after 32, to leave registers for the operands that each scale group has of its own
+#pragma unroll (DIM == 64 ? 2 : 1)
+            for (int h = 0; h < 2; ++h) {
+                // two sums at a time, of two groups or of the halves of one
+                constexpr int PARTS = G > 1 ? G : 2, N = J / PARTS;
+                f32x16 s, z;
+#pragma unroll
+                for (int g0 = 0; g0 < PARTS; g0 += 2) {
+                    f32x16 acc[2];
+#pragma unroll
+                    for (int n = 0; n < 2 * N; ++n) {
+                        const int part = n % 2, j = (g0 + part) * N + n / 2;
+                        const uint32_t key = 32 * h + col;
+                        const f16x8 k = __builtin_bit_cast(f16x8, t.k[key][t.key_piece(key, 2 * j + hf)]);
+                        acc[part] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qb[j], n < 2 ? f32x16{} : acc[part], 0, 0, 0);
+                    }
+                    if (G == 1) acc[0] += acc[1];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int part = 0; part < (G > 1 ? 2 : 1); ++part) {
+                            const int gr = G > 1 ? g0 + part : 0;
+                            const uint32_t at = 32 * h + 8 * q + 4 * hf;
+                            const f32x4 scale = *(const f32x4*)&t.planes[EXACT ? gr : 0][0][EXACT ? at : 0];
+                            const f32x4 mid = *(const f32x4*)&t.planes[EXACT ? gr : 0][1][EXACT ? at : 0];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int i = 4 * q + e;
+                                s[i] = gr ? fmaf(scale[e], acc[part][i], s[i]) : scale[e] * acc[part][i];
+                                z[i] = gr ? fmaf(mid[e], qsum[gr], z[i]) : mid[e] * qsum[0];
+                            }
+                        }
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) s[i] = fmaf(s[i], c1, z[i]);
+                if (a.cap != 0.0f) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        s[i] = a.cap <= kPlainCap ? soft_capped(s[i], a.cap) : soft_capped_exact(s[i], a.cap);
+                }
+                const int32_t k0 = t0 + 32 * h;
+                const uint32_t out0 = h ? out[2] : out[0], out1 = h ? out[3] : out[1];
+                if (k0 < inner_lo || k0 + 32 > inner_hi || (out0 | out1)) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int32_t key = k0 + 8 * (i / 4) + 4 * (int32_t)hf + i % 4;
+                        s[i] = key >= see.lo && key < see.hi && key < to && !(i / 8 ? out1 : out0) ? s[i] : -INFINITY;
+                    }
+                }
+                float top = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) top = max3(top, s[i], s[i + 1]);
+                // the reference moves where a probability would pass 2^15, to 2^-8 of the largest (as below)
+                if (__any(top - m > 15.0f)) {
+                    top = fmaxf(top, __shfl_xor(top, 32, 64));
+                    const float low = top - 8.0f;
+                    const float mn = fmaxf(m, top - low > 8.0f ? top : low), f = __builtin_amdgcn_exp2f(m - mn);
+                    m = mn;
+                    le *= f;
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) beta[gr] *= f;
+#pragma unroll
+                    for (int i = 0; i < O; ++i) o[i] *= f;
+                }
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {  // 16 keys
+                    float p[8], left[8];  // a probability, and what its f16 leaves of it
+                    uint32_t first[4];
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const float x = __builtin_amdgcn_exp2f(s[8 * k + e] - m), y = __builtin_amdgcn_exp2f(s[8 * k + e + 1] - m);
+                        const f16x2 v = {(_Float16)x, (_Float16)y};
+                        le += x, le += y;
+                        p[e] = x, p[e + 1] = y;
+                        left[e] = x - (float)v[0], left[e + 1] = y - (float)v[1];
+                        first[e / 2] = bits_of(v);
+                    }
+                    const f16x8 pf = operand(first[0], first[1], first[2], first[3]);
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) {
+                        uint32_t second[4];
+#pragma unroll
+                        for (int q = 0; q < 2; ++q) {  // four keys
+                            const u32x4 w = *(const u32x4*)&t.rest[FINE ? gr : 0][FINE ? 32 * h + 16 * k + 8 * q + 4 * hf : 0];
+#pragma unroll
+                            for (int e = 0; e < 4; e += 2) {
+                                const f16x2 u = half2_of(w[e]), v = half2_of(w[e + 1]);
+                                const float x = p[4 * q + e], y = p[4 * q + e + 1];
+                                second[2 * q + e / 2] = bits_of(f16x2{(_Float16)fmaf(x, (float)u[0], left[4 * q + e]),
+                                                                      (_Float16)fmaf(y, (float)v[0], left[4 * q + e + 1])});
+                                beta[gr] = fmaf(x, (float)u[1], beta[gr]);
+                                beta[gr] = fmaf(y, (float)v[1], beta[gr]);
+                            }
+                        }
+                        const f16x8 ps = operand(second[0], second[1], second[2], second[3]);
+                        f16x8 v[O / G];
+#pragma unroll
+                        for (int i = 0; i < O / G; ++i) {
+                            const uint32_t d = 32 * (gr * O / G + i) + col;
+                            v[i] = __builtin_bit_cast(f16x8, t.v[d][t.value_piece(d, 2 * (2 * h + k) + hf)]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < O / G; ++i)
+                            o[gr * O / G + i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i], pf, o[gr * O / G + i], 0, 0, 0);
+#pragma unroll
+                        for (int i = 0; i < O / G; ++i)
+                            o[gr * O / G + i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[i], ps, o[gr * O / G + i], 0, 0, 0);
+                    }
+                }
+            }
+        } else if (!FINE && t0 < outer_hi && t0 + kKeys > outer_lo) {
             f32x16 s[2];
             // two sums at a time, so that no product waits for the last: of both blocks of 32 keys, or of two scale groups
             constexpr int P = EXACT && G > 1 ? 2 : 1, H = 3 - P;
@@ -484,17 +637,17 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
                 }
             }
             read_ahead<4 * O>();
-            // values that are not finite, of keys that the row sees
-            if (flags) {
+        }
+        // values that are not finite, of keys that the row sees
+        if (flags && t0 < outer_hi && t0 + kKeys > outer_lo) {
 #pragma unroll
-                for (int gr = 0; gr < G; ++gr) {
-                    const uint64_t bad = t.not_finite[gr];
-                    const int32_t lo = min(max(see.lo - t0, 0), 64), hi = min(max(see.hi - t0, 0), 64);
-                    const uint64_t below_hi = hi >= 64 ? ~0ull : (1ull << hi) - 1, below_lo = lo >= 64 ? ~0ull : (1ull << lo) - 1;
-                    const float add = bad & below_hi & ~below_lo ? __builtin_nanf("") : 0.0f;
+            for (int gr = 0; gr < G; ++gr) {
+                const uint64_t bad = t.not_finite[gr];
+                const int32_t lo = min(max(see.lo - t0, 0), 64), hi = min(max(see.hi - t0, 0), 64);
+                const uint64_t below_hi = hi >= 64 ? ~0ull : (1ull << hi) - 1, below_lo = lo >= 64 ? ~0ull : (1ull << lo) - 1;
+                const float add = bad & below_hi & ~below_lo ? __builtin_nanf("") : 0.0f;
 #pragma unroll
-                    for (int i = gr * O / G; i < (gr + 1) * O / G; ++i) o[i] += add;
-                }
+                for (int i = gr * O / G; i < (gr + 1) * O / G; ++i) o[i] += add;
             }
         }
         // the tile after this (past the last: the last again), and the loads of the one after that
@@ -509,6 +662,15 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
     }
 
     l += __shfl_xor(l, 32, 64), le += __shfl_xor(le, 32, 64);
+    if (FINE) {
+        l = le;
+#pragma unroll
+        for (int gr = 0; gr < G; ++gr) {
+            const float bias = beta[FINE ? gr : 0] + __shfl_xor(beta[FINE ? gr : 0], 32, 64);
+#pragma unroll
+            for (int i = gr * O / G; i < (gr + 1) * O / G; ++i) o[i] += bias;
+        }
+    }
     if (!live) return;
     const float sum = EXACT ? le : l;
     // value 4 q + e of block i: 32 i + 8 q + 4 hf + e
@@ -527,7 +689,7 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
             a.lse[(size_t)token * a.heads + qh] = sum == 0.0f ? -INFINITY : (m + __builtin_amdgcn_logf(sum)) * kLn2;
     } else {
         // (the join divides by the sum before rounding)
-        const float f = EXACT && l > 0.0f ? sum / l : 1.0f;
+        const float f = MODE == kLse && l > 0.0f ? sum / l : 1.0f;
         const size_t at = ((size_t)token * a.heads + qh) * a.pieces + part;
         float* dst = a.tile_po + at * DIM + 4 * hf;
 #pragma unroll
@@ -588,8 +750,9 @@ __global__ __launch_bounds__(256) void kv_attend_tiles_join(AttendArgs a) {
 template <int DIM, int G>
 stark_qmm_status launch(const AttendArgs& a, hipStream_t s) {
     const uint32_t blocks = a.cache.kv_heads * a.turns * a.pieces;  // below 2^24 (kv::fits)
-    if (a.lse || !a.is_bf16) hipLaunchKernelGGL((kv_attend_tiles<DIM, G, true>), dim3(blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((kv_attend_tiles<DIM, G, false>), dim3(blocks), dim3(256), 0, s, a);
+    if (!a.is_bf16) hipLaunchKernelGGL((kv_attend_tiles<DIM, G, kFine>), dim3(blocks), dim3(256), 0, s, a);
+    else if (a.lse) hipLaunchKernelGGL((kv_attend_tiles<DIM, G, kLse>), dim3(blocks), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((kv_attend_tiles<DIM, G, kPlain>), dim3(blocks), dim3(256), 0, s, a);
     QMM_HIP_CHECK(hipGetLastError());
     if (a.pieces > 1) {  // then the row tiles are fewer than workgroups fit the GPU
         const uint32_t each = 1024 / DIM, joins = (a.heads * a.tokens + each - 1) / each;

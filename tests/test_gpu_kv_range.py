@@ -186,9 +186,9 @@ def test_values_before_the_window_do_not_set_the_scale(K):
     _small_values(s, 0)
 
 
-@pytest.mark.parametrize("with_lse", [True, False])
+@pytest.mark.parametrize("dtype,with_lse", [("bf16", True), ("bf16", False), ("f16", True)])
 @pytest.mark.parametrize("rows", [2, 40])
-def test_a_first_key_above_all_others(K, rows, with_lse):
+def test_a_first_key_above_all_others(K, rows, dtype, with_lse):
     """An attention sink: a key 15 above the rest (in natural logarithms) whose value is zero, so that the output is what
     the other keys' small probabilities make. An error d of the scores moves it by 2 d sum w |v - out|; a probability is
     held to 2^-12 of itself (2^-11 in kv_ref's bound), or below f16's normal range to 2^-33 of the largest."""
@@ -198,7 +198,7 @@ def test_a_first_key_above_all_others(K, rows, with_lse):
         k[0], v[0] = 0.0, 0.0
         k[0, :, 0] = 16.0
 
-    s = Served(K, 48, [(rows, 100)], 4, 2, 128, 64, 16, "bf16", edit=edit)
+    s = Served(K, 48, [(rows, 100)], 4, 2, 128, 64, 16, dtype, edit=edit)
     s.q[:, :, 0] = 10.625
     _run(s, with_lse=with_lse)
     out, wide = _np(s.out), 0 if rows == 2 else 1 if with_lse else 2
@@ -219,16 +219,17 @@ def test_a_first_key_above_all_others(K, rows, with_lse):
                                                                                        + 2.0 ** -18)
             tol += 2.0 ** -33 * (np.abs(v).sum(0) + np.abs(v).max(-1).sum())
             err = np.abs(out[rs, heads][:, h] - want)
-            assert (err <= tol + R.EPS["bf16"] * (np.abs(want) + tol)).all(), (err / tol).max()
+            own = 2.0 ** -25 if dtype == "f16" else 0.0  # of outputs below f16's normal range
+            assert (err <= tol + R.EPS[dtype] * (np.abs(want) + tol) + own).all(), (err / tol).max()
 
 
-@pytest.mark.parametrize("with_lse", [True, False])
+@pytest.mark.parametrize("dtype,with_lse", [("bf16", True), ("bf16", False), ("f16", True)])
 @pytest.mark.parametrize("rows", [1, 40])
-def test_unwritten_rows_before_the_window(K, rows, with_lse):
+def test_unwritten_rows_before_the_window(K, rows, dtype, with_lse):
     """Pages that lie wholly before every row's window may have been given away: what they hold, finite planes whose
     values pass f16 here, reaches nothing."""
     n = 500
-    s = Served(K, 49, [(rows, n)], 4, 2, 128, 64, 16, "bf16")
+    s = Served(K, 49, [(rows, n)], 4, 2, 128, 64, 16, dtype)
     window = n - rows + 1 - 432  # the first row's window begins in the fourth page of a tile of 64 keys
     assert s.table.shape[1] == 32 and window > 0
     used = set(_np(s.table).ravel().tolist())
@@ -442,6 +443,10 @@ def test_the_workspace_is_that_of_the_tensors_device(K, monkeypatch):
     ([(1, 3000), (3, 5000), (1, 40)], 8, 1, 128, 32, {}),
     ([(1, 20000)], 8, 2, 64, 64, {}),
     ([(5, 700), (2, 1500)], 8, 1, 256, 64, dict(soft_cap=30.0)),
+    ([(70, 2500), (30, 900)], 8, 2, 128, 64, {}),
+    ([(200, 1200)], 4, 2, 64, 32, dict(window=700)),
+    ([(90, 6000)], 4, 1, 256, 128, {}),
+    ([(1, 900)] * 17 + [(60, 3000)], 8, 2, 128, 128, {}),
 ])
 def test_f16_outputs_are_off_by_their_own_rounding(K, requests, heads, kvh, dim, group, options):
     """Over all rows of a call, as root mean square: the error of a correctly rounded output, and 5 % for all else. That is
@@ -478,3 +483,36 @@ def test_lse_is_as_exact_as_f32_sums(K, rows, dim, group, dtype):
         ours += ((lse[at, mine] - want) ** 2).sum()
         plain += ((f32 - want) ** 2).sum()
     assert ours <= 64 * plain, (ours / plain) ** 0.5
+
+
+@pytest.mark.parametrize("rows,dim,group", [(6, 128, 32), (70, 128, 64), (70, 64, 64), (70, 256, 32)])
+def test_values_that_are_no_numbers_in_f16_calls(K, rows, dim, group):
+    """They reach the rows that see them, in their scale group and no other value."""
+    kv, bad = rows + 140, dim - 3
+
+    def edit(k, v):
+        v[kv - 3, :, bad] = np.inf
+
+    s = Served(K, 62, [(rows, kv)], 4, 2, dim, group, 16, "f16", edit=edit)
+    _run(s)
+    s.check()
+    nan = np.isnan(_np(s.out))
+    at = bad // group * group
+    assert nan[rows - 3:, :, at:at + group].all() and nan.sum() == 3 * 4 * group
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+@pytest.mark.parametrize("size", [2.0 ** -24, 2.0 ** -20, 2.0 ** -17, 2.0 ** -14, 3000.0])
+def test_value_scales_at_both_ends_in_f16_calls(K, rows, size):
+    """Scales that are f16 subnormals, and the largest: the stored values are exact multiples, and so are the operands that
+    the kernels make of them. Outputs below f16's normal range are off by half its least step."""
+    def edit(k, v):
+        v[:] = np.clip(v, -2.5, 2.5) / 2.5 * 8 * size
+
+    s = Served(K, 63, [(rows, 200)], 4, 2, 128, 64, 16, "f16", edit=edit)
+    _run(s)
+    s.check()
+    out = _np(s.out)
+    for rs, mine, q, k, v in _requests(s):
+        want, _, tol, _ = R.attention(q, k, v, 128 ** -0.5, True, 0, 0.0, 0)
+        assert (np.abs(out[rs, mine] - want) <= tol + R.EPS["f16"] * (np.abs(want) + tol) + 2.0 ** -25).all()
