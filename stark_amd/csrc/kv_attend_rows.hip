@@ -16,9 +16,10 @@ struct Shape {
 
 // The keys of a step of one kv head as a wave's loads leave them: code words, and of the planes each word in one lane
 // only (lane 32 i + 16 v + t of pair h: record 2 h + i, keys' planes (v = 0) or values', token t).
-// STREAM: loads that leave the caches to others, for blocks of 8 rows: no other workgroup reads the same codes (us with and
-// without, 64 requests of 4000 keys and 4 rows 58 and 66). A head's blocks of 16 rows may be several and share them (64 of 16
-// to 40 rows and 900 to 9000 keys 62 and 57, 16 of 32 rows 40.2 and 37.5, 16 of 12 rows 27.1 and 25.6; 64 of 12 rows 67 and 70).
+// STREAM: loads that leave the caches to others, for blocks of 8 rows, of which a head has one: no other workgroup reads the same
+// codes (us with and without, 64 requests of 4000 keys and 4 rows 58 and 66). A head's blocks of 16 rows may be several and share
+// them (64 of 16 to 40 rows and 900 to 9000 keys 62 and 57, 16 of 32 rows 40.2 and 37.5). Where they turn out to be one, as the
+// call's bound does not say, both sides win by turns (16 requests of 12 rows 27.1 and 25.6, 64 of them 67 and 70).
 template <int DIM, int G, int T, bool STREAM>
 struct Step {
     uint32_t kc[T][DIM / 32], vc[T][DIM / 32], plane[T / 2][G];
@@ -177,11 +178,11 @@ QMM_DEVICE uint32_t wave_scan(uint32_t v) {
 //
 // Keys and values stay codes. With C the codes less 8,
 //   q . k = sum over groups (s_g C_g . q + (b_g + 8 s_g) sum q),   out = sum over tokens (p s_g) C + sum p (b_g + 8 s_g),
-// so a key's planes are a few fma per score and group, a value's scale goes into the probability (f16, p s_g scaled by a
-// power of two that keeps it in f16's normal range), and a code becomes an f16 operand by a mask: the bits of c in the
-// low (or 4 bits higher) end of an f16 are the subnormal c 2^-24 (c 2^-20), exact. The 8 is taken off by the score
-// accumulator's start value, and for the outputs by 8 sum (p s_g), summed as it was rounded: f32 sums and f16 roundings
-// then stand beside codes of either sign instead of 0 .. 15 (2.7 times less rounding error).
+// so a key's planes are a few fma per score and group, a value's scale goes into the probability (f16, the scales times a
+// power of two that keeps p s_g in f16's normal range where p s_g is 2^-22 of the wave's largest s_g or more), and a code becomes
+// an f16 operand by a mask: the bits of c in the low (or 4 bits higher) end of an f16 are the subnormal c 2^-24 (c 2^-20). The 8
+// is taken off by the score accumulator's start value, and for the outputs by 8 sum (p s_g), summed as it was rounded: f32 sums
+// and f16 roundings then stand beside codes of either sign instead of 0 .. 15 (2.7 times less rounding error).
 //
 // Scores come out transposed (A rows = 16 keys, B columns = query rows): a lane holds four keys of one column in each
 // block, which is the B operand of the second product as it stands, with no lane exchange. With few rows most of a
@@ -194,17 +195,19 @@ QMM_DEVICE uint32_t wave_scan(uint32_t v) {
 // Bound by HBM where there are many long requests: 64 of 500 to 32768 keys, 32 heads on 8 of 128 (781 MB), take 128.5 us,
 // 6.08 TB/s (a pure read of the same size 6.2). Bound by its own latency where there are few: one of 4096 keys (4.7 MB) takes
 // 9.4 us and 3.9 to join; of a workgroup's 8.5 us with 64 keys 3.3 are the chain of lengths, page ids, codes and queries, 3.2
-// a step and its wait, 2.0 the joining of the waves (a wave alone on its SIMD issues an instruction in 6 to 8 clocks). Blocks of 4 rows (four records to a score
-// block) took 134 us there, blocks of 16 for 4 rows 67 us against 60 (64 requests of 4096 keys); more workgroups, loads three
-// and four steps ahead and more waves a SIMD were no faster.
-// MODE. The matrix cores multiply subnormal codes exactly, but align the products of a sum by the exponent fields of their
-// factors, so that some 2^-17 of the largest is cut off: scores are off by 2e-6 to 1e-5 (root mean square, scores of 2).
+// a step and its wait, 2.0 the joining of the waves (a wave alone on its SIMD issues an instruction in 6 to 8 clocks). Blocks
+// of 4 rows (four records to a score block) took 134 us there, blocks of 16 for 4 rows 67 us against 60 (64 requests of 4096
+// keys); more workgroups, loads three and four steps ahead and more waves a SIMD were no faster.
+//
+// MODE: what the call's outputs show. Sums of products of subnormal codes lose what is below some 2^-17 of the largest product
+// (measured; as if products were aligned by their factors' exponent fields): scores are off by 2e-6 to 1e-5 (root mean square,
+// scores of 2), 20 to 75 times what f32 sums leave.
 // kPlain (bf16 without lse): that, and one rounding of p s to f16, stand beside outputs that are rounded to 2^-9: 1.01 times
 // as far from exact arithmetic as a rounding alone.
 // kLse (bf16 with lse): codes of keys are made f16 numbers, c - 8, which takes one packed operation for two of them; scores
-// are then as f32 sums give them (1e-7). 64 sequences 137 us, 129 without.
+// are then as f32 sums give them (1e-7). 64 sequences 137 us, 129 without; 16 of 16 to 40 rows 26.6, 25.
 // kFine (f16): values' codes as well, and p s as two f16, the second what the first leaves (2^-22 of it): an output is off by
-// its own rounding, where one f16 made it 1.3 to 1.4 times as much. 64 sequences 155 us.
+// its own rounding, where one f16 made it 1.3 to 1.4 times as much. 64 sequences 155 us, 16 of 16 to 40 rows 29.9.
 enum { kPlain, kLse, kFine };
 
 // Two codes less 8 (bits 0-3 and 16-19 of w, or 4 bits higher and sixteenfold): 1024 + c by its bits, less 1032, exact.

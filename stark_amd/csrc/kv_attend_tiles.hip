@@ -243,7 +243,7 @@ QMM_DEVICE void read_ahead() {
 // kFine (f16): that, and neither a probability nor a value is rounded to one f16, which left outputs 1.5 times as far from exact
 // arithmetic as their own rounding. A value is s c + b = s' c (1 + r) + b with the seven leading bits s' of its scale, so that s' c
 // is exact, and sum p v = sum p' s' c + sum (p - p' + p r) s' c + sum p b: p' the probability's f16, the second factor one f16 for
-// each scale group (r below 2^-6: it is held to 2^-17 of p), the third sum f32. The keys' planes cost 2 G + 1 operations a score,
+// each scale group (r below 2^-6, so it is held to 2^-17 of p; 2^-3 and 2^-14 where a scale is subnormal), the third sum f32. The keys' planes cost 2 G + 1 operations a score,
 // and the values' 2.5 G + 2 and a second product: the same chunk takes 213, 217 and 224 us with 1, 2 and 4 groups in bf16, 240,
 // 272 and 403 with lse, 333, 377 and 509 in f16.
 template <int DIM, int G, int MODE>

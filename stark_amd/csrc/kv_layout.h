@@ -81,8 +81,8 @@ KV_HD Request request(int32_t start, int32_t end, int32_t kv_len, uint32_t token
     return {a, q, k};
 }
 
-// Rows that a thread of the append does, one after another, with one read of their rotation: one while there are fewer
-// than 2^18 threads (4 waves a SIMD, which is what its registers leave room for), and up to eight.
+// Rows that a thread of the append does, one after another, with one read of their rotation: as many as leave 2^18 threads or
+// more (4 waves a SIMD, which is what its registers leave room for), so one below 2^19 rows' threads, and up to eight.
 KV_HD uint32_t rows_each(uint64_t threads) {
     const uint64_t each = threads / (1u << 18);
     return each < 1 ? 1 : each > 8 ? 8 : (uint32_t)each;
@@ -110,8 +110,10 @@ KV_HD Range request_range(int32_t q_len, int32_t kv_len, bool causal, int32_t wi
 // of 16 to 40 rows and 900 to 9000 keys 27 us with it, 50 in tiles, 64 of them 64 and 135; where many requests have 64 rows
 // and one length tiles are up to 1.4 times faster, 64 of 2000 keys 127 and 90); in a call of longer requests those of one
 // block, which has what one new token has (decode rows among prompts), where there may be enough of them to pay for two more
-// launches (a prompt with 8 decode rows of 2000 keys 59 us with them, 61 us without; 8 of 200 keys 28 against 19; 16 of 300
-// keys 30 against 33; 8 of 8000 keys 98 against 171), else none (0). The others go to the tile kernel.
+// launches, else none (0). The others go to the tile kernel. Us with them and without: beside a prompt of 300, 2 decode rows of
+// 2000 keys 58 and 46, 8 58 and 50, 16 65 and 57, 64 106 and 125; beside one of 100, 8 of 200 keys 27 and 19, 16 of 300 29 and 21,
+// 64 of 300 32 and 35, 16 of 8000 119 and 121. (So 16 requests are few: tiles won ground there when their workgroups came to be
+// counted by rows.)
 struct Rows {
     uint32_t limit, block;
 };
@@ -127,8 +129,9 @@ KV_HD Rows row_limit(uint32_t batch, uint32_t max_query, uint32_t ratio, uint32_
 constexpr uint32_t kLeastKeys = 256;
 
 // What beginning a unit costs a workgroup, in keys: its steps are counted as so many more. Blocks of 8 rows, us with 512,
-// 1024 and 2048: 16 requests of 900 to 9000 keys 26.0, 22.4 and 23.9; 64 of 500 to 32768 134, 132 and 137; 256 of 100 to 2000
-// 75, 70 and 72. Blocks of 16, whose keys take longer: 26.6, 28.0 and 30.2.
+// 1024 and 2048: 16 requests of 900 to 9000 keys 24.9, 23.2 and 24.8; 64 of 500 to 32768 132, 128.4 and 136; 256 of 100 to 2100
+// 68, 67.5 and 75. Blocks of 16, whose keys take longer: 16 requests of 900 to 9000 keys and 16 to 40 rows 26.6 with 512, 28.7
+// with 1024.
 KV_HD uint32_t unit_keys(uint32_t block) { return block == 8 ? 1024 : 512; }
 
 // Steps of each of `grid` workgroups that share `total` (below 2^31): a multiple of four, one for each wave.
