@@ -593,7 +593,7 @@ typedef struct stark_qmm_kv_plan_args {
 /* Plan of a serving step from request lengths, on the device: new pages for the
  * new tokens (request by request, in order), the slot and position of each of
  * them, and the lengths that stark_qmm_kv_attention reads. One launch; outputs
- * must not overlap inputs or each other. */
+ * that overlap inputs or each other are INVALID_ARGUMENT. */
 STARK_QMM_API stark_qmm_status stark_qmm_kv_plan(const stark_qmm_kv_plan_args* args, void* stream);
 
 /* Rotary embedding of query and key rows: pair i is values (i, i + rotary_dim / 2),

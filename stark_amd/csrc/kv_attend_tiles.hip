@@ -154,7 +154,8 @@ struct Codes {
                 const bool finite = (w & 0x7c00u) != 0x7c00u && (w >> 16 & 0x7c00u) != 0x7c00u;
                 const float part = lead != 0.0f ? (all - lead) * __builtin_amdgcn_rcpf(lead) : 0.0f;
                 const uint32_t v = (uint32_t)f32_to_f16_bits(part) | (w & 0xffff0000u);
-                if (quad < (uint32_t)G) t.rest[MODE == kFine ? quad + 4 * j : 0][MODE == kFine ? 16 * record + r : 0] = finite ? v : 0u;
+                if (quad < (uint32_t)G)
+                    t.rest[MODE == kFine ? quad + 4 * j : 0][MODE == kFine ? 16 * record + r : 0] = finite ? v : 0u;
             }
         }
         // quads 0 and 2 of a record share a piece, and 1 and 3: the order of the probabilities in their operand
@@ -240,12 +241,12 @@ QMM_DEVICE void read_ahead() {
 // kLse (bf16 with lse): the score products take the codes themselves, exact in f16, one sum a scale group, and a key's planes
 // are applied to the scores in f32, as in kv_attend_rows; and lse is of the sum of the probabilities before they are rounded.
 // Keys rounded to f16 move a score by up to 2^-11 of scale |q| |k|, which bf16 outputs do not show, but an f32 lse does.
-// kFine (f16): that, and neither a probability nor a value is rounded to one f16, which left outputs 1.5 times as far from exact
-// arithmetic as their own rounding. A value is s c + b = s' c (1 + r) + b with the seven leading bits s' of its scale, so that s' c
-// is exact, and sum p v = sum p' s' c + sum (p - p' + p r) s' c + sum p b: p' the probability's f16, the second factor one f16 for
-// each scale group (r below 2^-6, so it is held to 2^-17 of p; 2^-3 and 2^-14 where a scale is subnormal), the third sum f32. The keys' planes cost 2 G + 1 operations a score,
-// and the values' 2.5 G + 2 and a second product: the same chunk takes 213, 217 and 224 us with 1, 2 and 4 groups in bf16, 240,
-// 272 and 403 with lse, 333, 377 and 509 in f16.
+// kFine (f16): that, and neither a probability nor a value is rounded to one f16, which left outputs 1.5 times as far from
+// exact arithmetic as their own rounding. With s' the seven leading bits of a value's scale, so that s' c is exact, a value is
+// s c + b = s' c (1 + r) + b, and sum p v = sum p' s' c + sum (p - p' + p r) s' c + sum p b: p' is the probability's f16, the
+// second factor one f16 for each scale group (r is below 2^-6, so it is held to 2^-17 of p; 2^-3 and 2^-14 where a scale is
+// subnormal), the third sum f32. The keys' planes cost 2 G + 1 operations a score, the values' 2.5 G + 2 and a second product:
+// the same chunk takes 213, 217 and 224 us with 1, 2 and 4 groups in bf16, 240, 272 and 403 with lse, 333, 377 and 509 in f16.
 template <int DIM, int G, int MODE>
 __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(AttendArgs a) {
     constexpr bool EXACT = MODE != kPlain, FINE = MODE == kFine;
