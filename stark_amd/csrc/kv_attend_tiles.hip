@@ -15,8 +15,8 @@ constexpr int kKeys = 64;  // keys of a tile: four records
 // not_finite: keys (bits) whose values' planes are not finite, for each group; they stand as zeros in v.
 // kLse and kFine: keys are their codes less 8, and planes holds scales and middles (the value of code 8) of the keys, [group]
 // [scale or middle][key].
-// kFine: values are code times the leading bits of their scale, exact, and rest holds what the two leave of a value: (scale /
-// leading - 1) | bias << 16, f16.
+// kFine: values are code times the leading bits of their scale, exact, and rest holds what the two leave of a value, f16, by four
+// keys: scale / leading - 1 of each, then their biases.
 enum { kPlain, kLse, kFine };
 template <int DIM, int G, int MODE>
 struct Tile {
@@ -26,7 +26,7 @@ struct Tile {
     unsigned long long not_finite[G];
     alignas(16) uint32_t absent[4];  // records whose page is not in the cache
     alignas(16) float planes[EXACT ? G : 1][2][EXACT ? kKeys : 4];
-    alignas(16) uint32_t rest[FINE ? G : 1][FINE ? kKeys : 4];
+    alignas(16) uint16_t rest[FINE ? G : 1][FINE ? kKeys / 4 : 1][2][4];
     static QMM_DEVICE uint32_t key_piece(uint32_t key, uint32_t piece) {
         return piece ^ (DIM >= 128 ? key & 15 : key >> 1 & 7);
     }
@@ -153,9 +153,10 @@ struct Codes {
                 const float all = plane_scale(w), lead = plane_scale(leading(w));
                 const bool finite = (w & 0x7c00u) != 0x7c00u && (w >> 16 & 0x7c00u) != 0x7c00u;
                 const float part = lead != 0.0f ? (all - lead) * __builtin_amdgcn_rcpf(lead) : 0.0f;
-                const uint32_t v = (uint32_t)f32_to_f16_bits(part) | (w & 0xffff0000u);
-                if (quad < (uint32_t)G)
-                    t.rest[MODE == kFine ? quad + 4 * j : 0][MODE == kFine ? 16 * record + r : 0] = finite ? v : 0u;
+                if (quad < (uint32_t)G) {
+                    auto& to = t.rest[MODE == kFine ? quad + 4 * j : 0][MODE == kFine ? 4 * record + r / 4 : 0];
+                    to[0][r % 4] = finite ? (uint16_t)f32_to_f16_bits(part) : 0, to[1][r % 4] = finite ? (uint16_t)(w >> 16) : 0;
+                }
             }
         }
         // quads 0 and 2 of a record share a piece, and 1 and 3: the order of the probabilities in their operand
@@ -245,8 +246,8 @@ QMM_DEVICE void read_ahead() {
 // exact arithmetic as their own rounding. With s' the seven leading bits of a value's scale, so that s' c is exact, a value is
 // s c + b = s' c (1 + r) + b, and sum p v = sum p' s' c + sum (p - p' + p r) s' c + sum p b: p' is the probability's f16, the
 // second factor one f16 for each scale group (r is below 2^-6, so it is held to 2^-17 of p; 2^-3 and 2^-14 where a scale is
-// subnormal), the third sum f32. The keys' planes cost 2 G + 1 operations a score, the values' 2.5 G + 2 and a second product:
-// the same chunk takes 213, 217 and 224 us with 1, 2 and 4 groups in bf16, 240, 272 and 403 with lse, 333, 377 and 509 in f16.
+// subnormal), the third sum f32. The keys' planes cost 2 G + 1 operations a score, the values' 1.5 G + 3 and a second product:
+// the same chunk takes 213, 217 and 224 us with 1, 2 and 4 groups in bf16, 240, 272 and 403 with lse, 336, 369 and 478 in f16.
 template <int DIM, int G, int MODE>
 __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(AttendArgs a) {
     constexpr bool EXACT = MODE != kPlain, FINE = MODE == kFine;
@@ -468,32 +469,30 @@ __global__ __launch_bounds__(256, DIM <= 128 ? 2 : 1) void kv_attend_tiles(Atten
                 }
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {  // 16 keys
-                    float p[8], left[8];  // a probability, and what its f16 leaves of it
-                    uint32_t first[4];
+                    float p[8];
+                    f16x2 first[4], left[4];  // a probability's f16, and what that leaves of it
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) {
                         const float x = __builtin_amdgcn_exp2f(s[8 * k + e] - m), y = __builtin_amdgcn_exp2f(s[8 * k + e + 1] - m);
                         const f16x2 v = {(_Float16)x, (_Float16)y};
                         le += x, le += y;
                         p[e] = x, p[e + 1] = y;
-                        left[e] = x - (float)v[0], left[e + 1] = y - (float)v[1];
-                        first[e / 2] = bits_of(v);
+                        first[e / 2] = v;
+                        left[e / 2] = f16x2{(_Float16)(x - (float)v[0]), (_Float16)(y - (float)v[1])};
                     }
-                    const f16x8 pf = operand(first[0], first[1], first[2], first[3]);
+                    const f16x8 pf = operand(bits_of(first[0]), bits_of(first[1]), bits_of(first[2]), bits_of(first[3]));
 #pragma unroll
                     for (int gr = 0; gr < G; ++gr) {
                         uint32_t second[4];
 #pragma unroll
                         for (int q = 0; q < 2; ++q) {  // four keys
-                            const u32x4 w = *(const u32x4*)&t.rest[FINE ? gr : 0][FINE ? 32 * h + 16 * k + 8 * q + 4 * hf : 0];
+                            const u32x4 w = *(const u32x4*)&t.rest[FINE ? gr : 0][FINE ? 8 * h + 4 * k + 2 * q + hf : 0];
 #pragma unroll
-                            for (int e = 0; e < 4; e += 2) {
-                                const f16x2 u = half2_of(w[e]), v = half2_of(w[e + 1]);
-                                const float x = p[4 * q + e], y = p[4 * q + e + 1];
-                                second[2 * q + e / 2] = bits_of(f16x2{(_Float16)fmaf(x, (float)u[0], left[4 * q + e]),
-                                                                      (_Float16)fmaf(y, (float)v[0], left[4 * q + e + 1])});
-                                beta[gr] = fmaf(x, (float)u[1], beta[gr]);
-                                beta[gr] = fmaf(y, (float)v[1], beta[gr]);
+                            for (int e = 0; e < 2; ++e) {
+                                const f16x2 b = half2_of(w[2 + e]);
+                                second[2 * q + e] = bits_of(__builtin_elementwise_fma(first[2 * q + e], half2_of(w[e]), left[2 * q + e]));
+                                beta[gr] = fmaf(p[4 * q + 2 * e], (float)b[0], beta[gr]);
+                                beta[gr] = fmaf(p[4 * q + 2 * e + 1], (float)b[1], beta[gr]);
                             }
                         }
                         const f16x8 ps = operand(second[0], second[1], second[2], second[3]);
