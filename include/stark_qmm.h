@@ -684,6 +684,127 @@ STARK_QMM_API stark_qmm_status stark_qmm_kv_attention_workspace_size(const stark
 STARK_QMM_API stark_qmm_status stark_qmm_kv_attention(const stark_qmm_kv_attention_args* args, void* stream);
 
 /* ------------------------------------------------------------------ */
+/* Products of 8-bit floating-point codes with block scales            */
+/* ------------------------------------------------------------------ */
+
+/* No counterpart in the reference, whose 8-bit weights are integers. For
+ * checkpoints in e4m3 (the finite form: one sign, four exponent and three
+ * mantissa bits, largest value 448, 0x7f and 0xff not a number) whose weights
+ * have an f32 scale for each 128 x 128 block and whose activations get one for
+ * each row and 128 values. Codes are bytes; the last block of an axis may be
+ * short. Rows of codes start on 16-byte boundaries, and the bytes between a
+ * row's last code and the next boundary are the caller's: they may be read,
+ * what they hold does not matter, and they are not written.
+ *
+ * A dense layer is quantize, matmul; routed experts are stark_qmm_moe_route,
+ * expert_plan, quantize, grouped matmul (a_rows = the plan's tokens), quantize
+ * with the gate, grouped matmul, expert_combine. */
+#define STARK_QMM_FP8_BLOCK 128u
+
+typedef struct stark_qmm_fp8_quantize_args {
+    uint32_t struct_size;
+    uint32_t data_type;          /* of x: F32, F16 or BF16 */
+    const void* x;               /* [rows, columns]; gated: [rows, 2 * columns], a row's values, then its gates */
+    uint64_t x_row_stride;       /* elements */
+    uint8_t* codes;              /* [rows, columns] e4m3, 16-byte aligned */
+    uint64_t code_row_stride;    /* bytes, a multiple of 16 */
+    float* scales;               /* [rows, ceil(columns / 128)] */
+    uint64_t scale_row_stride, scale_block_stride; /* elements */
+    uint32_t rows, columns;
+    uint32_t gated;              /* x = value * gate / (1 + exp(-gate)), in f32 */
+    const int32_t* row_count;    /* device: rows from here on stay as they were (at most `rows`), or NULL */
+} stark_qmm_fp8_quantize_args;
+
+/* Rows to e4m3. A block's scale is max|x| / 448 rounded to f32, 2^-126 at
+ * least; a code is the e4m3 value nearest to x / scale (ties to even, at most
+ * 448 in magnitude), as exact arithmetic has it. A block that holds an infinity
+ * or a NaN gets the scale NaN and codes 0. x, codes and scales may not overlap. */
+STARK_QMM_API stark_qmm_status stark_qmm_fp8_quantize(const stark_qmm_fp8_quantize_args* args, void* stream);
+
+typedef struct stark_qmm_fp8_matmul_args {
+    uint32_t struct_size;
+    uint32_t d_type;             /* of d and bias: F32, F16 or BF16 */
+    const uint8_t* a;            /* [m, k] e4m3, 16-byte aligned */
+    uint64_t a_row_stride;       /* bytes, a multiple of 16, at most 2^24 */
+    const float* a_scales;       /* [m, ceil(k / 128)] */
+    uint64_t a_scale_row_stride, a_scale_block_stride; /* elements, at most 2^22 and 2^32 */
+    const uint8_t* b;            /* [n, k] e4m3, 16-byte aligned */
+    uint64_t b_row_stride;       /* as a's */
+    const float* b_scales;       /* [ceil(n / 128), ceil(k / 128)] */
+    uint64_t b_scale_row_stride, b_scale_block_stride; /* elements */
+    void* d;                     /* [m, n] */
+    uint64_t d_row_stride;       /* elements */
+    stark_qmm_d_ops d_ops;       /* bias in d_type; rht_factors: STARK_QMM_UNSUPPORTED_D_OP */
+    uint32_t m, n, k;            /* at most 2^24, 2^24 and 2^20; k at least 1 */
+    void* workspace;             /* device, 16-byte aligned, >= the size query's bytes */
+    uint64_t workspace_size;     /* its contents do not survive the call; calls that may overlap need their own */
+} stark_qmm_fp8_matmul_args;
+
+/* d[m, n] = ab_scale * sum over blocks of (a_scale * b_scale) * (sum of a * b in
+ * the block), then the other d_ops in the order of stark_qmm_encode. The two
+ * scales are multiplied first, in f32; sums are f32. d may not overlap an input. */
+STARK_QMM_API stark_qmm_status stark_qmm_fp8_matmul(const stark_qmm_fp8_matmul_args* args, void* stream);
+/* 0 where the call needs none (workspace may then be NULL). */
+STARK_QMM_API stark_qmm_status stark_qmm_fp8_matmul_workspace_size(const stark_qmm_fp8_matmul_args* args, uint64_t* bytes);
+
+typedef struct stark_qmm_fp8_grouped_args {
+    uint32_t struct_size;
+    stark_qmm_fp8_matmul_args product; /* m: rows of d; b, b_scales and bias: of expert 0 */
+    uint32_t experts;            /* 1 .. 1024 */
+    const int32_t* group_start;  /* device [experts + 1]: expert e has rows group_start[e] .. group_start[e + 1] - 1 of d */
+    uint64_t b_expert_stride;    /* bytes, a multiple of 16 */
+    uint64_t b_scale_expert_stride; /* elements */
+    uint64_t bias_expert_stride; /* elements */
+    const int32_t* a_rows;       /* device [m]: row i of d is computed from row a_rows[i] of a; NULL: from row i */
+    uint32_t a_row_count;        /* rows of a and a_scales, with a_rows */
+} stark_qmm_fp8_grouped_args;
+
+/* The product of each expert's rows with its own matrix, all in one call; group
+ * sizes are read on the device. Rows that no group has stay as they were. Starts
+ * are taken as no less than the one before and no more than m. A row of a outside
+ * a_row_count gives NaN. a and a_scales span less than 4 GiB each with a_rows
+ * (else STARK_QMM_UNSUPPORTED). */
+STARK_QMM_API stark_qmm_status stark_qmm_fp8_grouped_matmul(const stark_qmm_fp8_grouped_args* args, void* stream);
+STARK_QMM_API stark_qmm_status stark_qmm_fp8_grouped_matmul_workspace_size(const stark_qmm_fp8_grouped_args* args,
+                                                                           uint64_t* bytes);
+
+typedef struct stark_qmm_expert_plan_args {
+    uint32_t struct_size;
+    const uint32_t* ids;         /* [tokens, active] expert of each route (stark_qmm_moe_route's ids) */
+    int32_t* group_start;        /* [experts + 1] first position of each expert's routes, then their number */
+    int32_t* tokens_out;         /* [tokens * active] token of the route at each position; -1 behind the last */
+    int32_t* slots;              /* [tokens, active] position of each route; -1: not one of these experts */
+    uint32_t tokens, active;     /* tokens * active at most 2^24 */
+    uint32_t experts;            /* 1 .. 1024 */
+    uint32_t first;              /* the experts are ids first .. first + experts - 1 */
+    void* workspace;             /* device, 16-byte aligned, >= the size query's bytes */
+    uint64_t workspace_size;     /* its contents do not survive the call; calls that may overlap need their own */
+} stark_qmm_expert_plan_args;
+
+/* Routes in expert order, those of one expert in the order of their tokens.
+ * Outputs that overlap ids or each other are INVALID_ARGUMENT. */
+STARK_QMM_API stark_qmm_status stark_qmm_expert_plan(const stark_qmm_expert_plan_args* args, void* stream);
+/* 0 where the call needs none (workspace may then be NULL). */
+STARK_QMM_API stark_qmm_status stark_qmm_expert_plan_workspace_size(const stark_qmm_expert_plan_args* args, uint64_t* bytes);
+
+typedef struct stark_qmm_expert_combine_args {
+    uint32_t struct_size;
+    uint32_t data_type;          /* of x and out: F32, F16 or BF16 */
+    const void* x;               /* [rows, width] */
+    const int32_t* slots;        /* [tokens, active] row of x; outside 0 .. rows - 1: not counted */
+    const float* weights;        /* [tokens, active] */
+    void* out;                   /* [tokens, width] */
+    uint64_t x_row_stride, out_row_stride; /* elements */
+    uint32_t tokens, active, rows, width;  /* active 1 .. 1024 */
+    uint32_t accumulate;         /* out += instead of out = */
+} stark_qmm_expert_combine_args;
+
+/* out[t] = (accumulate: out[t]) + sum over j of weights[t, j] * x[slots[t, j]], in
+ * that order, in f32, rounded once. The weight of a route that is not counted is
+ * not read into the sum. out may not overlap an input. */
+STARK_QMM_API stark_qmm_status stark_qmm_expert_combine(const stark_qmm_expert_combine_args* args, void* stream);
+
+/* ------------------------------------------------------------------ */
 /* Weight files: Stark's converted artifact (model.safetensors) and      */
 /* GGUF v3 checkpoints                                                    */
 /* ------------------------------------------------------------------ */

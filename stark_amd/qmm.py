@@ -238,6 +238,14 @@ SIGNATURES = {
     "stark_qmm_kv_read": (C.c_uint32, [C.c_void_p, C.c_void_p]),
     "stark_qmm_kv_attention_workspace_size": (C.c_uint32, [C.c_void_p, C.POINTER(C.c_uint64)]),
     "stark_qmm_kv_attention": (C.c_uint32, [C.c_void_p, C.c_void_p]),
+    "stark_qmm_fp8_quantize": (C.c_uint32, [C.c_void_p, C.c_void_p]),
+    "stark_qmm_fp8_matmul": (C.c_uint32, [C.c_void_p, C.c_void_p]),
+    "stark_qmm_fp8_matmul_workspace_size": (C.c_uint32, [C.c_void_p, C.POINTER(C.c_uint64)]),
+    "stark_qmm_fp8_grouped_matmul": (C.c_uint32, [C.c_void_p, C.c_void_p]),
+    "stark_qmm_fp8_grouped_matmul_workspace_size": (C.c_uint32, [C.c_void_p, C.POINTER(C.c_uint64)]),
+    "stark_qmm_expert_plan": (C.c_uint32, [C.c_void_p, C.c_void_p]),
+    "stark_qmm_expert_plan_workspace_size": (C.c_uint32, [C.c_void_p, C.POINTER(C.c_uint64)]),
+    "stark_qmm_expert_combine": (C.c_uint32, [C.c_void_p, C.c_void_p]),
 }
 
 _lib = None
