@@ -32,6 +32,7 @@ FILE_FLAGS = {
     # copied them from and to the accumulation registers: 64 of about 370 instructions)
     "kv_attend_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "kv_attend_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "fp8_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "fp8_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 

@@ -121,46 +121,65 @@ struct Fp8Tile {
     uint32_t expert, first, rows;
 };
 
-// Row tiles of TILE rows of all groups, and the index-th of them; the same in every lane of the wave.
-template <uint32_t TILE>
-QMM_DEVICE uint32_t fp8_row_tiles(const Fp8Product& p) {
-    if (!p.group_start) return (p.m + TILE - 1) / TILE;
-    const uint32_t lane = threadIdx.x & 63;
-    uint32_t total = 0;
-    for (uint32_t e = lane; e < p.experts; e += 64)
-        total += (fp8::group(p.group_start[e], p.group_start[e + 1], p.m).count + TILE - 1) / TILE;
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) total += __shfl_xor(total, off, 64);
-    return __builtin_amdgcn_readfirstlane(total);
-}
-template <uint32_t TILE>
-QMM_DEVICE Fp8Tile fp8_row_tile(const Fp8Product& p, uint32_t index) {
-    if (!p.group_start) return {0, index * TILE, min(p.m - index * TILE, TILE)};
-    const uint32_t lane = threadIdx.x & 63;
-    uint32_t before = 0;
-    for (uint32_t e0 = 0; e0 < p.experts; e0 += 64) {
-        const uint32_t e = e0 + lane;
-        const fp8::Range g = e < p.experts ? fp8::group(p.group_start[e], p.group_start[e + 1], p.m) : fp8::Range{0, 0};
-        const uint32_t tiles = (g.count + TILE - 1) / TILE;
-        uint32_t sum = tiles;  // inclusive scan
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t u = __shfl_up(sum, d, 64);
-            if (lane >= (uint32_t)d) sum += u;
-        }
-        const uint32_t start = before + sum - tiles;
-        const uint64_t mine = __ballot(index >= start && index < start + tiles);
-        if (mine) {
-            const int at = __ffsll((unsigned long long)mine) - 1;
-            const uint32_t i = index - __shfl(start, at, 64), first = __shfl(g.first, at, 64), count = __shfl(g.count, at, 64);
-            return {(uint32_t)__builtin_amdgcn_readfirstlane(e0 + at), (uint32_t)__builtin_amdgcn_readfirstlane(first + i * TILE),
-                    (uint32_t)__builtin_amdgcn_readfirstlane(min(count - i * TILE, TILE))};
-        }
-        before += __builtin_amdgcn_readfirstlane(__shfl(sum, 63, 64));
-    }
-    return {0, 0, 0};
+// Sum over the lanes up to and with this one.
+QMM_DEVICE uint32_t fp8_scan(uint32_t v) {
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
+    return v;
 }
 
+// The groups of a call as one wave sees them: lane l has up to sixteen consecutive ones, all loaded at once.
+template <uint32_t TILE>
+struct Fp8Groups {
+    static constexpr uint32_t kEach = 16;  // 64 lanes, 1024 groups
+    int32_t start[kEach + 1];
+    uint32_t each, total, before, mine;  // groups a lane; row tiles of all, of the lanes before this one, of this one
+
+    QMM_DEVICE static uint32_t tiles(fp8::Range g) { return (g.count + TILE - 1) / TILE; }
+
+    QMM_DEVICE explicit Fp8Groups(const Fp8Product& p) {
+        if (!p.group_start) {
+            total = (p.m + TILE - 1) / TILE;
+            return;
+        }
+        const uint32_t lane = threadIdx.x & 63;
+        each = (p.experts + 63) / 64;
+#pragma unroll
+        for (uint32_t i = 0; i <= kEach; ++i)
+            if (i <= each) start[i] = p.group_start[min(lane * each + i, p.experts)];
+        mine = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i)
+            if (i < each) mine += tiles(fp8::group(start[i], start[i + 1], p.m));
+        const uint32_t sum = fp8_scan(mine);
+        before = sum - mine;
+        total = (uint32_t)__builtin_amdgcn_readlane((int)sum, 63);
+    }
+
+    // The index-th row tile; the same in every lane.
+    QMM_DEVICE Fp8Tile tile(const Fp8Product& p, uint32_t index) const {
+        if (!p.group_start) return {0, index * TILE, index < total ? min(p.m - index * TILE, TILE) : 0};
+        const uint64_t found = __ballot(index - before < mine);
+        if (!found) return {0, 0, 0};
+        const int at = __ffsll((unsigned long long)found) - 1;
+        uint32_t i = index - (uint32_t)__builtin_amdgcn_readlane((int)before, at);
+        Fp8Tile t{0, 0, 0};
+#pragma unroll
+        for (uint32_t e = 0; e < kEach; ++e) {
+            if (e >= each || t.rows) continue;
+            const fp8::Range g = fp8::group(__builtin_amdgcn_readlane(start[e], at), __builtin_amdgcn_readlane(start[e + 1], at), p.m);
+            if (i < tiles(g)) t = Fp8Tile{at * each + e, g.first + i * TILE, min(g.count - i * TILE, TILE)};
+            else i -= tiles(g);
+        }
+        return t;
+    }
+};
+
+stark_qmm_status launch_fp8_rows(const Fp8Product& p, hipStream_t stream);
 stark_qmm_status launch_fp8_tiles(const Fp8Product& p, hipStream_t stream);
 
 }  // namespace qmm

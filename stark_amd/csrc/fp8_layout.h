@@ -37,6 +37,22 @@ FP8_BOTH uint32_t tile_of(uint32_t i, uint32_t tiles) {
     return local < per ? (i & 7) * per + local : tiles;
 }
 
+// Strips of 16 columns and waves of a workgroup of the few-rows kernel. Some eight waves a CU are enough loads in flight; more
+// only shorten their runs, and a run of less than four blocks is mostly its own start (N 12288, K 4096, one row: 4 waves 10.6 us,
+// 8 waves 14.4, 16 waves 20.9; N 4096, K 12288, five rows: 8 waves 12.9, 16 waves 15.8). With strips for every CU several
+// times over, two strips share a row's codes and a start (128 experts of N 1536, K 2048, one or two rows each: 2 strips and 4
+// waves 43.3 us, 1 and 2 44.4, 1 and 4 57.5).
+struct RowShare {
+    uint32_t strips, waves;
+};
+FP8_BOTH RowShare row_share(uint64_t row_tiles, uint32_t n, uint32_t k) {
+    const uint64_t units = row_tiles * ((n + 15) / 16);
+    if (units >= 4096) return {2, 4};
+    uint32_t waves = 2;
+    while (waves < 16 && units * waves < 2048 && waves < blocks(k)) waves *= 2;
+    return {1, waves};
+}
+
 // item / blocks by the inverse floor(2^32 / blocks) (0xffffffff for 1): the estimate is at most one short.
 struct Split {
     uint32_t row, block;

@@ -173,11 +173,12 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN>& l
 template <int BM, int BN, int WM, int WN, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN) void fp8_tiles(Fp8Product p) {
     __shared__ TileLds<BM, BN> lds;
-    const uint32_t columns = (p.n + BN - 1) / BN, tiles = fp8_row_tiles<BM>(p) * columns;
+    const Fp8Groups<BM> groups(p);
+    const uint32_t columns = (p.n + BN - 1) / BN, tiles = groups.total * columns;
     for (uint32_t i = blockIdx.x; i < (tiles + 7) / 8 * 8; i += gridDim.x) {
         const uint32_t t = fp8::tile_of(i, tiles);
         if (t >= tiles) continue;
-        const Fp8Tile rows = fp8_row_tile<BM>(p, t / columns);
+        const Fp8Tile rows = groups.tile(p, t / columns);
         if (rows.rows) fp8_tile<BM, BN, WM, WN, EXACT>(p, lds, rows, (t % columns) * BN);
     }
 }

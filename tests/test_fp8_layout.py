@@ -21,6 +21,7 @@ extern "C" {
 void group(int32_t a, int32_t b, uint32_t n, uint32_t* r) { const fp8::Range x = fp8::group(a, b, n); r[0] = x.first; r[1] = x.count; }
 uint32_t row_tiles(uint32_t rows, uint32_t groups, uint32_t tile) { return fp8::row_tiles(rows, groups, tile); }
 uint32_t tile_of(uint32_t i, uint32_t tiles) { return fp8::tile_of(i, tiles); }
+void row_share(uint64_t t, uint32_t n, uint32_t k, uint32_t* r) { const fp8::RowShare x = fp8::row_share(t, n, k); r[0] = x.strips; r[1] = x.waves; }
 void split(uint32_t i, uint32_t b, uint32_t* r) { const fp8::Split x = fp8::split(i, b, fp8::inverse(b)); r[0] = x.row; r[1] = x.block; }
 }
 """
@@ -70,6 +71,14 @@ def test_items_split_into_rows_and_blocks():
     for blocks in (1, 2, 3, 6, 7, 31, 32, 96, 8191, 8192):
         for item in [0, 1, blocks - 1, blocks, 2 ** 32 - 1, 2 ** 32 - blocks] + [r.randrange(2 ** 32) for _ in range(200)]:
             assert _pair(L.split, item, blocks) == divmod(item, blocks)
+
+
+def test_row_shares_fill_the_gpu_and_no_more():
+    L = rules()
+    L.row_share.argtypes = [C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p]
+    assert _pair(L.row_share, 1, 12288, 4096) == (1, 4) and _pair(L.row_share, 1, 4096, 12288) == (1, 8)
+    assert _pair(L.row_share, 128, 1536, 2048) == (2, 4) and _pair(L.row_share, 1, 16, 65536) == (1, 16)
+    assert _pair(L.row_share, 1, 16, 100) == (1, 2) and _pair(L.row_share, 2 ** 20, 2 ** 24, 128) == (2, 4)
 
 
 def test_plain_codes_are_the_nearest():
