@@ -761,7 +761,8 @@ typedef struct stark_qmm_fp8_grouped_args {
 
 /* The product of each expert's rows with its own matrix, all in one call; group
  * sizes are read on the device. Rows that no group has stay as they were. Starts
- * are taken as no less than the one before and no more than m. A row of a outside
+ * are cut to 0 .. m, and a group that ends before it starts has no rows; groups
+ * must not share rows (what those then hold is not defined). A row of a outside
  * a_row_count gives NaN. a and a_scales span less than 4 GiB each with a_rows
  * (else STARK_QMM_UNSUPPORTED). */
 STARK_QMM_API stark_qmm_status stark_qmm_fp8_grouped_matmul(const stark_qmm_fp8_grouped_args* args, void* stream);

@@ -23,7 +23,8 @@ struct Fp8Product {
     uint32_t m, n, k, experts, a_row_count;
     uint32_t d_dt, flags;
     float ab_scale, soft_cap;
-    uint32_t vec;  // four outputs of a row may be stored at once
+    uint32_t vec;    // four outputs of a row may be stored at once
+    uint32_t plain;  // eight 16-bit ones, that are the scaled sums
 };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -85,6 +86,13 @@ QMM_DEVICE float fp8_finish(const Fp8Product& p, float sum, size_t d_at, const v
     if (bias) v += load_as_f32(bias, p.d_dt, n);
     if (p.flags & FLAG_SOFT_CAP) v = p.soft_cap * tanhf(v / p.soft_cap);
     return v;
+}
+
+// Two outputs in 16 bits.
+typedef __bf16 fp8_bf16x2 __attribute__((ext_vector_type(2)));
+QMM_DEVICE uint32_t fp8_pack2(uint32_t dt, float a, float b) {
+    if (dt == STARK_QMM_BF16) return __builtin_bit_cast(uint32_t, fp8_bf16x2{(__bf16)a, (__bf16)b});
+    return f32_to_f16_bits(a) | (uint32_t)f32_to_f16_bits(b) << 16;
 }
 
 // Four consecutive outputs of a row from column n on.

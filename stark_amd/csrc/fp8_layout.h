@@ -37,6 +37,24 @@ FP8_BOTH uint32_t tile_of(uint32_t i, uint32_t tiles) {
     return local < per ? (i & 7) * per + local : tiles;
 }
 
+// Place of a tile among row tiles and column tiles: bands of eight row tiles, in a band a column of tiles after the other, so
+// that the tiles that run at once on an XCD (32) share eight row tiles' and four column tiles' operands.
+struct Place {
+    uint32_t row, column;  // row: not below `rows` where there is no such tile
+};
+FP8_BOTH Place place(uint32_t i, uint32_t rows, uint32_t columns) {
+    constexpr uint32_t kBand = 8;
+    if (i >= rows * columns) return {rows, 0};
+    const uint32_t band = i / (kBand * columns), in = i - band * kBand * columns, left = rows - band * kBand;
+    const uint32_t high = left < kBand ? left : kBand;
+    return {band * kBand + in % high, in / high};
+}
+
+// Whether tiles of 256 x 256 pay, against 128 x 128: they read half the operands, and need rows and tiles enough.
+FP8_BOTH bool wide_tiles(uint32_t rows, uint32_t groups, uint32_t n) {
+    return rows / groups >= 256 && (uint64_t)row_tiles(rows, groups, 256) * ((n + 255) / 256) >= 192;
+}
+
 // Strips of 16 columns and waves of a workgroup of the few-rows kernel. Some eight waves a CU are enough loads in flight; more
 // only shorten their runs, and a run of less than four blocks is mostly its own start (N 12288, K 4096, one row: 4 waves 10.6 us,
 // 8 waves 14.4, 16 waves 20.9; N 4096, K 12288, five rows: 8 waves 12.9, 16 waves 15.8). With strips for every CU several

@@ -71,7 +71,8 @@ stark_qmm_status run(const stark_qmm_fp8_matmul_args& q, const Groups& g, const 
     p.a = q.a, p.b = q.b, p.as = q.a_scales, p.bs = q.b_scales, p.d = q.d, p.bias = q.d_ops.bias;
     p.group_start = start, p.a_rows = rows;
     p.vec = fp8_aligned(q.d, 4 * e) && p.d_stride % 4 == 0;
-    if (p.m <= 16ull * p.experts) return launch_fp8_rows(p, stream);
+    p.plain = e == 2 && !p.flags && !p.bias && fp8_aligned(q.d, 16) && p.d_stride % 8 == 0;
+    if (p.m <= 16ull * p.experts || p.k < fp8::kBlock) return launch_fp8_rows(p, stream);
     return launch_fp8_tiles(p, stream);
 }
 

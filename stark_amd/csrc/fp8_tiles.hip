@@ -13,27 +13,37 @@ typedef __attribute__((address_space(3))) void lds_void;
 
 constexpr uint32_t kStep = fp8::kBlock;  // codes (and bytes) of a row in a step
 
-// LDS rows of 128 bytes, 16-byte piece c of row r at piece c ^ (r & 7): eight consecutive lanes of an operand read (rows
-// r .. r + 7, one piece) and of a staging store cover the banks once.
-template <int BM, int BN>
+// What a 32-bit offset reaches from p on: the offsets here stay inside the operands by themselves.
+QMM_DEVICE __amdgpu_buffer_rsrc_t everything(const void* p) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, 0xffffffff, 0x00020000); }
+
+constexpr uint32_t kChunk = 8;  // steps whose scales of the rows are staged together
+
+// LDS rows of 128 bytes, 16-byte piece c of row r at piece c ^ (r / 2 % 8). Sixteen lanes of an operand read cover the 64 banks
+// once, be they lanes with one piece of sixteen rows or, as a 16-byte read takes them, four lanes each of rows r and r + 12 with
+// piece c and of r + 4 and r + 8 with piece c + 1.
+template <int BM, int BN, int W>
 struct TileLds {
     u32x4 a[2][BM * 8];
     u32x4 b[2][BN * 8];
+    float sa[2][BM * kChunk];  // [8 rows][step][row] of a chunk
+    float sb[2][64];           // [128 columns][step]
 };
 
 // Output tile of BM rows and BN columns by WM x WN waves.
 template <int BM, int BN, int WM, int WN, bool EXACT>
-__device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN>& lds, const Fp8Tile t, uint32_t n0) {
+__device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM * WN>& lds, const Fp8Tile t, uint32_t n0) {
     constexpr int W = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, LA = BM / 8 / W, LB = BN / 8 / W;
     static_assert(BM % (16 * WM) == 0 && BN % (16 * WN) == 0 && BM % (8 * W) == 0 && BN % (8 * W) == 0, "whole pieces a wave");
     static_assert(BN <= 128 || BN / WN <= 128, "one weight scale a wave and step");
+    static_assert(W % 2 == 0, "a wave's staged rows have one swizzle");
     const uint32_t tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t wm = wave / WN, wn = wave % WN, col = lane & 15, kq = lane >> 4;
     const uint32_t steps = p.k / kStep, tail = p.k % kStep;
+    const uint32_t before = tail ? 1 : 0, total = steps + before;  // a short last block is the first step
 
     // staging: a wave's i-th load takes rows 8 (i W + wave) .. + 7; rows past the tile's last are read from it
-    const uint32_t srow = lane >> 3, piece = (lane & 7) ^ srow;
+    const uint32_t srow = lane >> 3, piece = (lane & 7) ^ ((4 * wave + (srow >> 1)) & 7);
     const uint8_t* abase = p.a_rows ? p.a : p.a + (uint64_t)t.first * p.a_stride;
     const uint8_t* bbase = p.b + t.expert * p.b_expert + (uint64_t)n0 * p.b_stride;
     const uint32_t nlast = min((uint32_t)BN, p.n - n0) - 1;
@@ -47,29 +57,15 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN>& l
 #pragma unroll
     for (int i = 0; i < LB; ++i) bo[i] = min(8 * (i * W + wave) + srow, nlast) * (uint32_t)p.b_stride + 16 * piece;
 
-    // scales: of the lane's row in each of its row blocks, and of the wave's columns
-    const float* asbase = p.a_rows ? p.as : p.as + (uint64_t)t.first * p.as_row;
-    const float* bsbase = p.bs + t.expert * p.bs_expert + (uint64_t)((n0 + wn * (BN / WN)) / kStep < fp8::blocks(p.n)
-                                                                       ? (n0 + wn * (BN / WN)) / kStep : 0) * p.bs_row;
-    uint32_t so[MT];
-#pragma unroll
-    for (int i = 0; i < MT; ++i) so[i] = a_row(wm * (BM / WM) + 16 * i + col) * (uint32_t)p.as_row;
-    float sa[MT], sb;
-    const auto load_scales = [&](uint32_t s) {
-#pragma unroll
-        for (int i = 0; i < MT; ++i) sa[i] = asbase[s * p.as_block + so[i]];
-        sb = bsbase[s * p.bs_block];
-    };
-
-    const auto load = [&](uint32_t s, int buf) {
-        const uint8_t* ab = abase + s * kStep;
-        const uint8_t* bb = bbase + s * kStep;
+    const __amdgpu_buffer_rsrc_t ra = everything(abase), rb = everything(bbase);
+    const auto load = [&](uint32_t s, int buf) {  // a step that is not the short one
+        const uint32_t k0 = __builtin_amdgcn_readfirstlane((s - before) * kStep);
 #pragma unroll
         for (int i = 0; i < LA; ++i)
-            __builtin_amdgcn_global_load_lds(ab + ao[i], (lds_void*)&lds.a[buf][64 * (i * W + wave)], 16, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)&lds.a[buf][64 * (i * W + wave)], 16, ao[i], k0, 0, 0);
 #pragma unroll
         for (int i = 0; i < LB; ++i)
-            __builtin_amdgcn_global_load_lds(bb + bo[i], (lds_void*)&lds.b[buf][64 * (i * W + wave)], 16, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void*)&lds.b[buf][64 * (i * W + wave)], 16, bo[i], k0, 0, 0);
     };
     // The last, short block: pieces past the row's end are not read, codes past it in its last piece are cleared.
     const auto load_tail = [&](int buf) {
@@ -89,60 +85,112 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN>& l
 #pragma unroll
         for (int i = 0; i < LB; ++i) lds.b[buf][64 * (i * W + wave) + lane] = cut(bbase + steps * kStep + bo[i]);
     };
-
+    // Scales of a chunk of steps: a load takes eight rows' (one line each where a row's scales are contiguous).
+    const float* asbase = p.a_rows ? p.as : p.as + (uint64_t)t.first * p.as_row;
+    const float* bsbase = p.bs + t.expert * p.bs_expert;
+    uint32_t so[LA];
+#pragma unroll
+    for (int i = 0; i < LA; ++i) so[i] = a_row(8 * (i * W + wave) + (lane & 7)) * (uint32_t)p.as_row;
+    const auto load_scales = [&](uint32_t chunk) {
+        const auto block = [&](uint32_t in) {
+            const uint32_t s = min(chunk * kChunk + in, total - 1);
+            return s < before ? steps : s - before;
+        };
+        const uint32_t s = block(lane >> 3);
+#pragma unroll
+        for (int i = 0; i < LA; ++i)
+            __builtin_amdgcn_global_load_lds(asbase + s * p.as_block + so[i], (lds_void*)&lds.sa[chunk & 1][64 * (i * W + wave)], 4, 0, 0);
+        if (wave == 0) {
+            const uint32_t nb = min(n0 / kStep + (lane >> 3), fp8::blocks(p.n) - 1), sl = block(lane & 7);
+            __builtin_amdgcn_global_load_lds(bsbase + nb * p.bs_row + sl * p.bs_block, (lds_void*)&lds.sb[chunk & 1][0], 4, 0, 0);
+        }
+    };
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
-    const auto operand = [&](const u32x4* rows, uint32_t r) {
-        const u32x4 x = rows[8 * r + ((2 * kq) ^ (r & 7))], y = rows[8 * r + ((2 * kq + 1) ^ (r & 7))];
+    const uint32_t p0 = 8 * col + (kq ^ (col >> 1)), p1 = p0 ^ 4;  // pieces kq and kq + 4
+    const auto operand = [&](const u32x4* rows) {  // 16 rows from `rows` on
+        const u32x4 x = rows[p0], y = rows[p1];
         return Fp8Operand<EXACT>(i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]});
     };
-    const auto compute = [&](int buf, const float (&ca)[MT], float cb) {
-        // (the operands of fewer columns at once where they are wide)
-        constexpr int NC = EXACT ? 2 : NT;
+    const auto compute = [&](int buf, uint32_t s) {
+        const uint32_t in = s % kChunk, cb = s / kChunk & 1;
+        const float sb = lds.sb[cb][8 * (wn * (BN / WN) / kStep) + in];
+        Fp8Operand<EXACT> x[MT];
+        float c[MT];
 #pragma unroll
-        for (int j0 = 0; j0 < NT; j0 += NC) {
-            Fp8Operand<EXACT> w[NC];
+        for (int i = 0; i < MT; ++i) {
+            x[i] = operand(lds.a[buf] + 8 * (wm * (BM / WM) + 16 * i));
+            c[i] = lds.sa[cb][8 * (wm * (BM / WM) + 16 * i) + 64 * (col >> 3) + 8 * in + (col & 7)] * sb;
+        }
+        // A matrix instruction's result takes some twelve issue slots: each sum is scaled two instructions later, and the
+        // columns' codes are read two column blocks ahead. The order is held as it is written.
+        constexpr int D = 2, Q = MT * NT;
+        f32x4 v[D + 1];
+        Fp8Operand<EXACT> w[2];
+        const auto columns = [&](int j) { return operand(lds.b[buf] + 8 * (wn * (BN / WN) + 16 * j)); };
+        w[0] = columns(0);
+        if (NT > 1) w[1] = columns(1);
+        if (!EXACT) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < NC; ++j) w[j] = operand(lds.b[buf], wn * (BN / WN) + 16 * (j0 + j) + col);
+        for (int q = 0; q < Q + D; ++q) {
+            if (q < Q) v[q % (D + 1)] = fp8_block(w[q / MT % 2], x[q % MT]);
+            if (!EXACT) __builtin_amdgcn_sched_barrier(0);
+            if (q >= D) {
+                const int i = (q - D) % MT, j = (q - D) / MT;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const auto x = operand(lds.a[buf], wm * (BM / WM) + 16 * i + col);
-                const float s = ca[i] * cb;
-#pragma unroll
-                for (int j = 0; j < NC; ++j) {
-                    const f32x4 v = fp8_block(w[j], x);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc[i][j0 + j][e] = fmaf(s, v[e], acc[i][j0 + j][e]);
-                }
+                for (int e = 0; e < 4; ++e) acc[i][j][e] = fmaf(c[i], v[(q - D) % (D + 1)][e], acc[i][j][e]);
             }
+            if (q < Q && q % MT == MT - 1 && q / MT + 2 < NT) w[q / MT % 2] = columns(q / MT + 2);
+            if (!EXACT) __builtin_amdgcn_sched_barrier(0);
         }
     };
 
-    __syncthreads();  // a tile before this one may still be read
-    int buf = 0;
-    if (steps) load(0, 0);
+    // A step's loads are issued a step ahead and waited for at its start: where a wave passes the barrier, all waves' pieces
+    // are in LDS and none still reads the other buffer.
+    if (tail) load_tail(0);
+    else load(0, 0);
     load_scales(0);
-    for (uint32_t s = 0; s < steps; ++s) {
-        __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0): this wave's pieces are in LDS
+#pragma unroll 1
+    for (uint32_t s = 0; s < total; ++s) {
+        const int buf = s & 1;
+        __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0)
         __syncthreads();
-        float ca[MT], cb = sb;
-#pragma unroll
-        for (int i = 0; i < MT; ++i) ca[i] = sa[i];
-        if (s + 1 < steps) load(s + 1, buf ^ 1);
-        if (s + 1 < steps || tail) load_scales(s + 1);
-        compute(buf, ca, cb);
-        buf ^= 1;
-    }
-    if (tail) {
-        load_tail(buf);
-        __syncthreads();
-        compute(buf, sa, sb);
+        if (s + 1 < total) {
+            load(s + 1, buf ^ 1);
+            if (s % kChunk == kChunk - 1) load_scales(s / kChunk + 1);
+        }
+        compute(buf, s);
     }
 
+    // Plain outputs of 16 bits: two lanes with neighbouring column quarters exchange halves, so that each stores eight columns.
+    const uint32_t nw = n0 + wn * (BN / WN);
+    if (!EXACT && p.plain && NT % 2 == 0 && nw + BN / WN <= p.n) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const uint32_t r = wm * (BM / WM) + 16 * i + col;
+            const bool there = r < t.rows;
+            const bool none = there && p.a_rows && (uint32_t)p.a_rows[t.first + r] >= p.a_row_count;
+            uint16_t* const d = (uint16_t*)p.d + (uint64_t)(t.first + r) * p.d_stride + nw + 16 * (kq & 1) + 4 * (kq & 2);
+            const float scale = none ? __builtin_nanf("") : p.ab_scale;
+#pragma unroll
+            for (int j = 0; j < NT; j += 2) {
+                uint32_t h[2][2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        h[u][e] = fp8_pack2(p.d_dt, scale * acc[i][j + u][2 * e], scale * acc[i][j + u][2 * e + 1]);
+                const auto x = __builtin_amdgcn_permlane16_swap(h[0][0], h[1][0], false, false);
+                const auto y = __builtin_amdgcn_permlane16_swap(h[0][1], h[1][1], false, false);
+                if (there) *(u32x4*)(d + 16 * j) = u32x4{x[0], y[0], x[1], y[1]};
+            }
+        }
+        return;
+    }
     const void* bias = p.bias ? (const uint8_t*)p.bias + t.expert * p.bias_expert * (p.d_dt == STARK_QMM_F32 ? 4 : 2) : nullptr;
     // Outputs go through LDS, a row block at a time in the wave's own part, so that whole rows are stored.
     constexpr int C = BN / WN, P = C / 4 + 1;  // columns of the wave; pieces of a row, one more than it has: rows start on other banks
@@ -172,22 +220,19 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN>& l
 
 template <int BM, int BN, int WM, int WN, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN) void fp8_tiles(Fp8Product p) {
-    __shared__ TileLds<BM, BN> lds;
+    __shared__ TileLds<BM, BN, WM * WN> lds;
+    const uint32_t columns = (p.n + BN - 1) / BN;
     const Fp8Groups<BM> groups(p);
-    const uint32_t columns = (p.n + BN - 1) / BN, tiles = groups.total * columns;
-    for (uint32_t i = blockIdx.x; i < (tiles + 7) / 8 * 8; i += gridDim.x) {
-        const uint32_t t = fp8::tile_of(i, tiles);
-        if (t >= tiles) continue;
-        const Fp8Tile rows = groups.tile(p, t / columns);
-        if (rows.rows) fp8_tile<BM, BN, WM, WN, EXACT>(p, lds, rows, (t % columns) * BN);
-    }
+    const fp8::Place at = fp8::place(fp8::tile_of(blockIdx.x, groups.total * columns), groups.total, columns);
+    const Fp8Tile rows = groups.tile(p, at.row);
+    if (rows.rows) fp8_tile<BM, BN, WM, WN, EXACT>(p, lds, rows, at.column * BN);
 }
 
 template <int BM, int BN, int WM, int WN, bool EXACT>
 stark_qmm_status launch(const Fp8Product& p, hipStream_t stream) {
     const uint64_t tiles = (uint64_t)fp8::row_tiles(p.m, p.experts, BM) * ((p.n + BN - 1) / BN);
-    const uint32_t grid = (uint32_t)std::min<uint64_t>((tiles + 7) / 8 * 8, 1u << 20);
-    hipLaunchKernelGGL((fp8_tiles<BM, BN, WM, WN, EXACT>), dim3(grid), dim3(64 * WM * WN), 0, stream, p);
+    if (tiles >= 1u << 24) return STARK_QMM_UNSUPPORTED;
+    hipLaunchKernelGGL((fp8_tiles<BM, BN, WM, WN, EXACT>), dim3((uint32_t)((tiles + 7) / 8 * 8)), dim3(64 * WM * WN), 0, stream, p);
     QMM_HIP_CHECK(hipGetLastError());
     return STARK_QMM_OK;
 }
@@ -195,7 +240,9 @@ stark_qmm_status launch(const Fp8Product& p, hipStream_t stream) {
 }  // namespace
 
 stark_qmm_status launch_fp8_tiles(const Fp8Product& p, hipStream_t stream) {
-    return p.d_dt == STARK_QMM_F32 ? launch<128, 128, 2, 2, true>(p, stream) : launch<128, 128, 2, 2, false>(p, stream);
+    if (p.d_dt == STARK_QMM_F32) return launch<128, 128, 2, 2, true>(p, stream);
+    if (fp8::wide_tiles(p.m, p.experts, p.n)) return launch<256, 256, 4, 2, false>(p, stream);
+    return launch<128, 128, 2, 2, false>(p, stream);
 }
 
 }  // namespace qmm

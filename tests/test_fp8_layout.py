@@ -22,6 +22,8 @@ void group(int32_t a, int32_t b, uint32_t n, uint32_t* r) { const fp8::Range x =
 uint32_t row_tiles(uint32_t rows, uint32_t groups, uint32_t tile) { return fp8::row_tiles(rows, groups, tile); }
 uint32_t tile_of(uint32_t i, uint32_t tiles) { return fp8::tile_of(i, tiles); }
 void row_share(uint64_t t, uint32_t n, uint32_t k, uint32_t* r) { const fp8::RowShare x = fp8::row_share(t, n, k); r[0] = x.strips; r[1] = x.waves; }
+void place(uint32_t i, uint32_t rows, uint32_t columns, uint32_t* r) { const fp8::Place x = fp8::place(i, rows, columns); r[0] = x.row; r[1] = x.column; }
+int wide_tiles(uint32_t rows, uint32_t groups, uint32_t n) { return fp8::wide_tiles(rows, groups, n); }
 void split(uint32_t i, uint32_t b, uint32_t* r) { const fp8::Split x = fp8::split(i, b, fp8::inverse(b)); r[0] = x.row; r[1] = x.block; }
 }
 """
@@ -66,6 +68,22 @@ def test_every_tile_has_one_workgroup():
         assert sorted(t for t in got if t < tiles) == list(range(tiles))
 
 
+def test_every_tile_has_one_place():
+    """Workgroups past the last tile have none: neither a row tile nor a column tile of theirs is there."""
+    L = rules()
+    for rows, columns in ((0, 3), (1, 1), (1, 5), (2, 9), (7, 1), (8, 3), (9, 4), (16, 48), (61, 7)):
+        tiles = rows * columns
+        seen = []
+        for i in range((tiles + 7) // 8 * 8 + 8):
+            row, column = _pair(L.place, L.tile_of(i, tiles), rows, columns)
+            if row < rows:
+                assert column < columns
+                seen.append((row, column))
+            else:
+                assert row == rows
+        assert sorted(seen) == [(r, c) for r in range(rows) for c in range(columns)]
+
+
 def test_items_split_into_rows_and_blocks():
     L, r = rules(), random.Random(4)
     for blocks in (1, 2, 3, 6, 7, 31, 32, 96, 8191, 8192):
@@ -79,6 +97,12 @@ def test_row_shares_fill_the_gpu_and_no_more():
     assert _pair(L.row_share, 1, 12288, 4096) == (1, 4) and _pair(L.row_share, 1, 4096, 12288) == (1, 8)
     assert _pair(L.row_share, 128, 1536, 2048) == (2, 4) and _pair(L.row_share, 1, 16, 65536) == (1, 16)
     assert _pair(L.row_share, 1, 16, 100) == (1, 2) and _pair(L.row_share, 2 ** 20, 2 ** 24, 128) == (2, 4)
+
+
+def test_wide_tiles_need_rows_and_tiles():
+    L = rules()
+    assert L.wide_tiles(4096, 1, 12288) and L.wide_tiles(65536, 128, 1536)
+    assert not L.wide_tiles(333, 1, 1001) and not L.wide_tiles(1024, 128, 1536) and not L.wide_tiles(255, 1, 1 << 20)
 
 
 def test_plain_codes_are_the_nearest():
