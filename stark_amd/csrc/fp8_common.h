@@ -25,6 +25,9 @@ struct Fp8Product {
     float ab_scale, soft_cap;
     uint32_t vec;    // four outputs of a row may be stored at once
     uint32_t plain;  // eight 16-bit ones, that are the scaled sums
+    uint32_t parts;  // runs of the inner axis, whose sums meet in `partial` [parts, m, partial_stride]
+    float* partial;
+    uint64_t partial_stride;
 };
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -100,11 +103,9 @@ QMM_DEVICE void fp8_store4(const Fp8Product& p, f32x4 sum, uint32_t row, uint32_
     const size_t at = (size_t)row * p.d_stride + n;
     if (n >= p.n) return;
     if (!p.vec || n + 4 > p.n) {
-#pragma unroll 1
-        for (uint32_t e = 0; e < 4 && n + e < p.n; ++e) {
-            const float x = e == 0 ? sum[0] : e == 1 ? sum[1] : e == 2 ? sum[2] : sum[3];
-            store_from_f32(p.d, p.d_dt, at + e, fp8_finish(p, x, at + e, bias, n + e));
-        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (n + e < p.n) store_from_f32(p.d, p.d_dt, at + e, fp8_finish(p, sum[e], at + e, bias, n + e));
         return;
     }
     float v[4];
@@ -187,7 +188,7 @@ struct Fp8Groups {
     }
 };
 
-stark_qmm_status launch_fp8_rows(const Fp8Product& p, hipStream_t stream);
-stark_qmm_status launch_fp8_tiles(const Fp8Product& p, hipStream_t stream);
+stark_qmm_status launch_fp8_rows(const Fp8Product& p, uint32_t rows, hipStream_t stream);
+stark_qmm_status launch_fp8_tiles(const Fp8Product& p, uint32_t tile, hipStream_t stream);
 
 }  // namespace qmm

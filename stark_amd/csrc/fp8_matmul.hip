@@ -24,7 +24,7 @@ stark_qmm_status check_sizes(const stark_qmm_fp8_matmul_args& q, const Groups& g
     if (q.d_ops.rht_factors) return STARK_QMM_UNSUPPORTED_D_OP;
     if (q.m > (1u << 24) || q.n > (1u << 24) || q.k == 0 || q.k > (1u << 20)) return STARK_QMM_INVALID_ARGUMENT;
     if (g.experts == 0 || g.experts > 1024) return STARK_QMM_INVALID_ARGUMENT;
-    const uint64_t a_rows = g.gathered ? g.a_row_count : q.m, blocks = fp8::blocks(q.k);
+    const uint64_t a_rows = g.gathered ? g.a_row_count : q.m;
     if (g.gathered && (g.a_row_count == 0 || g.a_row_count > 0x7fffffffu)) return STARK_QMM_INVALID_ARGUMENT;
     if (!code_rows(a_rows, q.a_row_stride, q.k) || !code_rows(q.n, q.b_row_stride, q.k)) return STARK_QMM_INVALID_ARGUMENT;
     if (q.a_scale_row_stride > kScaleStride || q.a_scale_block_stride >> 32 || q.b_scale_row_stride >> 32 || q.b_scale_block_stride >> 32 ||
@@ -45,8 +45,20 @@ stark_qmm_status check_sizes(const stark_qmm_fp8_matmul_args& q, const Groups& g
     // a gathered row's place is a 32-bit offset from the first
     if (g.gathered && (fp8_span(a_rows, p->a_stride, (q.k + 15) / 16 * 16) >> 32 || fp8_span(a_rows, 4 * p->as_row, 4) >> 32))
         return STARK_QMM_UNSUPPORTED;
-    (void)blocks;
     return STARK_QMM_OK;
+}
+
+fp8::Choice choice(const Fp8Product& p, bool grouped) { return fp8::choose(p.m, p.n, p.k, p.experts, grouped, p.d_dt == STARK_QMM_F32); }
+
+// The parts' sums: rows of whole 16-byte pieces.
+uint64_t partial_stride(const Fp8Product& p) { return (p.n + 3ull) / 4 * 4; }
+uint64_t workspace_of(const Fp8Product& p, fp8::Choice c) { return c.parts > 1 ? 4ull * c.parts * p.m * partial_stride(p) : 0; }
+
+stark_qmm_status size_of(const stark_qmm_fp8_matmul_args& q, const Groups& g, bool grouped, uint64_t* bytes) {
+    Fp8Product p{};
+    const stark_qmm_status st = check_sizes(q, g, &p);
+    if (st == STARK_QMM_OK) *bytes = p.m && p.n ? workspace_of(p, choice(p, grouped)) : 0;
+    return st;
 }
 
 stark_qmm_status run(const stark_qmm_fp8_matmul_args& q, const Groups& g, const int32_t* start, const int32_t* rows, hipStream_t stream) {
@@ -72,8 +84,16 @@ stark_qmm_status run(const stark_qmm_fp8_matmul_args& q, const Groups& g, const 
     p.group_start = start, p.a_rows = rows;
     p.vec = fp8_aligned(q.d, 4 * e) && p.d_stride % 4 == 0;
     p.plain = e == 2 && !p.flags && !p.bias && fp8_aligned(q.d, 16) && p.d_stride % 8 == 0;
-    if (p.m <= 16ull * p.experts || p.k < fp8::kBlock) return launch_fp8_rows(p, stream);
-    return launch_fp8_tiles(p, stream);
+    const fp8::Choice c = choice(p, start != nullptr);
+    p.parts = c.parts;
+    const uint64_t need = workspace_of(p, c);
+    if (need) {
+        if (!q.workspace || !fp8_aligned(q.workspace, 16)) return STARK_QMM_INVALID_ARGUMENT;
+        if (need > q.workspace_size) return STARK_QMM_WORKSPACE_TOO_SMALL;
+        if (fp8_overlap(q.workspace, need, q.d, dn)) return STARK_QMM_INVALID_ARGUMENT;
+        p.partial = (float*)q.workspace, p.partial_stride = partial_stride(p);
+    }
+    return c.tile ? launch_fp8_tiles(p, c.tile, stream) : launch_fp8_rows(p, c.rows, stream);
 }
 
 stark_qmm_status groups_of(const stark_qmm_fp8_grouped_args* a, Groups* g) {
@@ -90,10 +110,7 @@ extern "C" {
 
 stark_qmm_status stark_qmm_fp8_matmul_workspace_size(const stark_qmm_fp8_matmul_args* args, uint64_t* bytes) {
     if (!args || !bytes) return STARK_QMM_INVALID_ARGUMENT;
-    Fp8Product p{};
-    const stark_qmm_status st = check_sizes(*args, Groups{}, &p);
-    if (st == STARK_QMM_OK) *bytes = 0;
-    return st;
+    return size_of(*args, Groups{}, false, bytes);
 }
 
 stark_qmm_status stark_qmm_fp8_matmul(const stark_qmm_fp8_matmul_args* args, void* stream) {
@@ -104,12 +121,8 @@ stark_qmm_status stark_qmm_fp8_matmul(const stark_qmm_fp8_matmul_args* args, voi
 stark_qmm_status stark_qmm_fp8_grouped_matmul_workspace_size(const stark_qmm_fp8_grouped_args* args, uint64_t* bytes) {
     if (!bytes) return STARK_QMM_INVALID_ARGUMENT;
     Groups g;
-    stark_qmm_status st = groups_of(args, &g);
-    if (st != STARK_QMM_OK) return st;
-    Fp8Product p{};
-    st = check_sizes(args->product, g, &p);
-    if (st == STARK_QMM_OK) *bytes = 0;
-    return st;
+    const stark_qmm_status st = groups_of(args, &g);
+    return st != STARK_QMM_OK ? st : size_of(args->product, g, true, bytes);
 }
 
 stark_qmm_status stark_qmm_fp8_grouped_matmul(const stark_qmm_fp8_grouped_args* args, void* stream) {

@@ -1,7 +1,7 @@
 // Products of 8-bit floating-point codes with few rows, dense or grouped by expert: the weights are read once, from memory
 // straight into registers.
 //
-// A workgroup takes a strip of 16 NT columns and up to 16 MT rows; its W waves share the inner axis, in runs of whole blocks,
+// A workgroup takes a strip of 16 NT columns and up to 16 MT rows (16, or 32 by 32 columns); its W waves share the inner axis, in runs of whole blocks,
 // and their sums meet in LDS, in wave order. HBM bounds it.
 #include "fp8_common.h"
 
@@ -169,8 +169,10 @@ stark_qmm_status launch_waves(const Fp8Product& p, uint32_t waves, hipStream_t s
 
 }  // namespace
 
-stark_qmm_status launch_fp8_rows(const Fp8Product& p, hipStream_t stream) {
-    const fp8::RowShare s = fp8::row_share(fp8::row_tiles(p.m, p.experts, 16), p.n, p.k);
+stark_qmm_status launch_fp8_rows(const Fp8Product& p, uint32_t rows, hipStream_t stream) {
+    const uint64_t tiles = fp8::row_tiles(p.m, p.experts, rows);
+    if (rows == 32) return tiles * ((p.n + 31) / 32) < 256 ? launch<2, 2, 8>(p, stream) : launch<2, 2, 4>(p, stream);
+    const fp8::RowShare s = fp8::row_share(tiles, p.n, p.k);
     return s.strips == 1 ? launch_waves<1>(p, s.waves, stream) : launch_waves<2>(p, s.waves, stream);
 }
 

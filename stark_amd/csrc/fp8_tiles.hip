@@ -21,17 +21,18 @@ constexpr uint32_t kChunk = 8;  // steps whose scales of the rows are staged tog
 // LDS rows of 128 bytes, 16-byte piece c of row r at piece c ^ (r / 2 % 8). Sixteen lanes of an operand read cover the 64 banks
 // once, be they lanes with one piece of sixteen rows or, as a 16-byte read takes them, four lanes each of rows r and r + 12 with
 // piece c and of r + 4 and r + 8 with piece c + 1.
-template <int BM, int BN, int W>
+template <int BM, int BN, int W, int S>
 struct TileLds {
-    u32x4 a[2][BM * 8];
-    u32x4 b[2][BN * 8];
+    u32x4 a[S][BM * 8];
+    u32x4 b[S][BN * 8];
     float sa[2][BM * kChunk];  // [8 rows][step][row] of a chunk
     float sb[2][64];           // [128 columns][step]
 };
 
-// Output tile of BM rows and BN columns by WM x WN waves.
-template <int BM, int BN, int WM, int WN, bool EXACT>
-__device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM * WN>& lds, const Fp8Tile t, uint32_t n0) {
+// Output tile of BM rows and BN columns by WM x WN waves, with the operands of S steps in LDS; the `part`-th of p.parts runs of
+// the steps.
+template <int BM, int BN, int WM, int WN, int S, bool EXACT>
+__device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM * WN, S>& lds, const Fp8Tile t, uint32_t n0, uint32_t part) {
     constexpr int W = WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, LA = BM / 8 / W, LB = BN / 8 / W;
     static_assert(BM % (16 * WM) == 0 && BN % (16 * WN) == 0 && BM % (8 * W) == 0 && BN % (8 * W) == 0, "whole pieces a wave");
     static_assert(BN <= 128 || BN / WN <= 128, "one weight scale a wave and step");
@@ -40,7 +41,8 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t wm = wave / WN, wn = wave % WN, col = lane & 15, kq = lane >> 4;
     const uint32_t steps = p.k / kStep, tail = p.k % kStep;
-    const uint32_t before = tail ? 1 : 0, total = steps + before;  // a short last block is the first step
+    const uint32_t before = tail ? 1 : 0, all = steps + before;  // a short last block is the first step
+    const uint32_t from = part * all / p.parts, total = (part + 1) * all / p.parts;
 
     // staging: a wave's i-th load takes rows 8 (i W + wave) .. + 7; rows past the tile's last are read from it
     const uint32_t srow = lane >> 3, piece = (lane & 7) ^ ((4 * wave + (srow >> 1)) & 7);
@@ -93,7 +95,7 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
     for (int i = 0; i < LA; ++i) so[i] = a_row(8 * (i * W + wave) + (lane & 7)) * (uint32_t)p.as_row;
     const auto load_scales = [&](uint32_t chunk) {
         const auto block = [&](uint32_t in) {
-            const uint32_t s = min(chunk * kChunk + in, total - 1);
+            const uint32_t s = min(from + chunk * kChunk + in, total - 1);
             return s < before ? steps : s - before;
         };
         const uint32_t s = block(lane >> 3);
@@ -117,7 +119,7 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
         return Fp8Operand<EXACT>(i32x8{(int)x[0], (int)x[1], (int)x[2], (int)x[3], (int)y[0], (int)y[1], (int)y[2], (int)y[3]});
     };
     const auto compute = [&](int buf, uint32_t s) {
-        const uint32_t in = s % kChunk, cb = s / kChunk & 1;
+        const uint32_t in = (s - from) % kChunk, cb = (s - from) / kChunk & 1;
         const float sb = lds.sb[cb][8 * (wn * (BN / WN) / kStep) + in];
         Fp8Operand<EXACT> x[MT];
         float c[MT];
@@ -149,23 +151,53 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
         }
     };
 
-    // A step's loads are issued a step ahead and waited for at its start: where a wave passes the barrier, all waves' pieces
-    // are in LDS and none still reads the other buffer.
-    if (tail) load_tail(0);
-    else load(0, 0);
+    // A step's loads are issued S - 1 steps ahead and waited for at its start, while those of the steps between stay in flight:
+    // where a wave passes the barrier, all waves' pieces are in LDS and none still reads the buffer that is loaded next. (No
+    // fence here: one would wait for all loads.)
+    constexpr int F = (S - 2) * (LA + LB);  // loads of the steps between
+    const auto arrive = [&](bool between) {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        if (S > 2 && between) __builtin_amdgcn_s_waitcnt(0x0070 | (F & 15) | (F >> 4 << 14));  // vmcnt(F), lgkmcnt(0)
+        else __builtin_amdgcn_s_waitcnt(0x0070);
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+    };
     load_scales(0);
+#pragma unroll
+    for (int i = 0; i < S - 1; ++i)
+        if (from + i < total) {
+            if (from + i < before) load_tail(i);
+            else load(from + i, i);
+        }
+    int buf = 0;
 #pragma unroll 1
-    for (uint32_t s = 0; s < total; ++s) {
-        const int buf = s & 1;
-        __builtin_amdgcn_s_waitcnt(0xf70);  // vmcnt(0)
-        __syncthreads();
-        if (s + 1 < total) {
-            load(s + 1, buf ^ 1);
-            if (s % kChunk == kChunk - 1) load_scales(s / kChunk + 1);
+    for (uint32_t s = from; s < total; ++s) {
+        arrive(s + S - 2 < total);
+        if (s + S - 1 < total) {
+            const uint32_t next = s + S - 1 - from;
+            if (next % kChunk == 0) load_scales(next / kChunk);
+            load(s + S - 1, buf ? buf - 1 : S - 1);
         }
         compute(buf, s);
+        buf = buf + 1 < S ? buf + 1 : 0;
     }
 
+    // A part's sums go to the workspace as they are.
+    if (p.parts > 1) {
+        float* const w = p.partial + (uint64_t)part * p.m * p.partial_stride;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            const uint32_t r = wm * (BM / WM) + 16 * i + col;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                const uint32_t n = n0 + wn * (BN / WN) + 16 * j + 4 * kq;
+                if (r < t.rows && n < p.n) *(f32x4*)(w + (uint64_t)(t.first + r) * p.partial_stride + n) = acc[i][j];
+            }
+        }
+        return;
+    }
     // Plain outputs of 16 bits: two lanes with neighbouring column quarters exchange halves, so that each stores eight columns.
     const uint32_t nw = n0 + wn * (BN / WN);
     if (!EXACT && p.plain && NT % 2 == 0 && nw + BN / WN <= p.n) {
@@ -194,7 +226,7 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
     const void* bias = p.bias ? (const uint8_t*)p.bias + t.expert * p.bias_expert * (p.d_dt == STARK_QMM_F32 ? 4 : 2) : nullptr;
     // Outputs go through LDS, a row block at a time in the wave's own part, so that whole rows are stored.
     constexpr int C = BN / WN, P = C / 4 + 1;  // columns of the wave; pieces of a row, one more than it has: rows start on other banks
-    static_assert(W * 16 * P <= 2 * 8 * (BM + BN), "the outputs' rows fit the operands' place");
+    static_assert(W * 16 * P <= S * 8 * (BM + BN), "the outputs' rows fit the operands' place");
     f32x4* const out = (f32x4*)&lds + wave * 16 * P;
     __syncthreads();
 #pragma unroll 1
@@ -206,43 +238,105 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
                 for (int j = 0; j < NT; ++j) out[col * P + 4 * j + kq] = acc[k][j];
             }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const auto missing = [&](uint32_t r) { return p.a_rows && (uint32_t)p.a_rows[t.first + r] >= p.a_row_count; };
+        if (p.vec) {
+#pragma unroll 2
+            for (int j = 0; j < NT; ++j) {
+                const uint32_t row = (64 * j + lane) / (C / 4), c = (64 * j + lane) % (C / 4), r = wm * (BM / WM) + 16 * i + row;
+                if (r >= t.rows) continue;
+                f32x4 v = out[row * P + c];
+                if (missing(r)) v = f32x4{1, 1, 1, 1} * __builtin_nanf("");
+                fp8_store4(p, v, t.first + r, n0 + wn * C + 4 * c, bias);
+            }
+        } else {  // rows that start anywhere: a column a lane, four at a time
 #pragma unroll 1
-        for (int j = 0; j < NT; ++j) {
-            const uint32_t row = (64 * j + lane) / (C / 4), c = (64 * j + lane) % (C / 4), r = wm * (BM / WM) + 16 * i + row;
-            if (r >= t.rows) continue;
-            f32x4 v = out[row * P + c];
-            if (p.a_rows && (uint32_t)p.a_rows[t.first + r] >= p.a_row_count) v = f32x4{1, 1, 1, 1} * __builtin_nanf("");
-            fp8_store4(p, v, t.first + r, n0 + wn * C + 4 * c, bias);
+            for (int j0 = 0; j0 < 4 * NT; j0 += 4) {
+                float v[4];
+                uint32_t r[4], n[4];
+                bool there[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    // a row is the same in every lane where it has 64 columns or more
+                    const uint32_t row = C >= 64 ? (j0 + u) / (C / 64 ? C / 64 : 1) : (j0 + u) * (64 / C) + lane / C;
+                    const uint32_t c = C >= 64 ? lane + 64 * ((j0 + u) % (C / 64 ? C / 64 : 1)) : lane % C;
+                    r[u] = wm * (BM / WM) + 16 * i + row, n[u] = n0 + wn * C + c;
+                    there[u] = r[u] < t.rows && n[u] < p.n;
+                    v[u] = ((const float*)(out + row * P))[c];
+                    if (there[u] && missing(r[u])) v[u] = __builtin_nanf("");
+                }
+                if (!p.flags) {
+                    float add[4] = {0, 0, 0, 0};
+                    if (bias) {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) add[u] = load_as_f32(bias, p.d_dt, min(n[u], p.n - 1));
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) v[u] = p.ab_scale * v[u] + add[u];
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (there[u]) v[u] = fp8_finish(p, v[u], (size_t)(t.first + r[u]) * p.d_stride + n[u], bias, n[u]);
+                }
+                if (p.d_dt == STARK_QMM_F32) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (there[u]) ((float*)p.d + (uint64_t)(t.first + r[u]) * p.d_stride)[n[u]] = v[u];
+                } else {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (there[u]) ((uint16_t*)p.d + (uint64_t)(t.first + r[u]) * p.d_stride)[n[u]] = (uint16_t)fp8_pack2(p.d_dt, v[u], 0.0f);
+                }
+            }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
 }
 
-template <int BM, int BN, int WM, int WN, bool EXACT>
+template <int BM, int BN, int WM, int WN, int S, bool EXACT>
 __global__ __launch_bounds__(64 * WM * WN) void fp8_tiles(Fp8Product p) {
-    __shared__ TileLds<BM, BN, WM * WN> lds;
+    __shared__ TileLds<BM, BN, WM * WN, S> lds;
     const uint32_t columns = (p.n + BN - 1) / BN;
     const Fp8Groups<BM> groups(p);
     const fp8::Place at = fp8::place(fp8::tile_of(blockIdx.x, groups.total * columns), groups.total, columns);
     const Fp8Tile rows = groups.tile(p, at.row);
-    if (rows.rows) fp8_tile<BM, BN, WM, WN, EXACT>(p, lds, rows, at.column * BN);
+    if (rows.rows) fp8_tile<BM, BN, WM, WN, S, EXACT>(p, lds, rows, at.column * BN, blockIdx.y);
 }
 
-template <int BM, int BN, int WM, int WN, bool EXACT>
+// The parts' sums, in their order, four columns a thread.
+__global__ __launch_bounds__(256) void fp8_join(Fp8Product p) {
+    const uint32_t quarters = (p.n + 3) / 4, i = blockIdx.x * 256 + threadIdx.x, row = i / quarters, n = 4 * (i % quarters);
+    if (row >= p.m) return;
+    const float* w = p.partial + (uint64_t)row * p.partial_stride + n;
+    f32x4 v = *(const f32x4*)w;
+    for (uint32_t part = 1; part < p.parts; ++part) v += *(const f32x4*)(w + (uint64_t)part * p.m * p.partial_stride);
+    fp8_store4(p, v, row, n, p.bias);
+}
+
+template <int BM, int BN, int WM, int WN, int S, bool EXACT>
 stark_qmm_status launch(const Fp8Product& p, hipStream_t stream) {
     const uint64_t tiles = (uint64_t)fp8::row_tiles(p.m, p.experts, BM) * ((p.n + BN - 1) / BN);
     if (tiles >= 1u << 24) return STARK_QMM_UNSUPPORTED;
-    hipLaunchKernelGGL((fp8_tiles<BM, BN, WM, WN, EXACT>), dim3((uint32_t)((tiles + 7) / 8 * 8)), dim3(64 * WM * WN), 0, stream, p);
+    hipLaunchKernelGGL((fp8_tiles<BM, BN, WM, WN, S, EXACT>), dim3((uint32_t)((tiles + 7) / 8 * 8), p.parts), dim3(64 * WM * WN), 0, stream, p);
     QMM_HIP_CHECK(hipGetLastError());
     return STARK_QMM_OK;
 }
 
+template <bool EXACT>
+stark_qmm_status launch_size(const Fp8Product& p, uint32_t tile, hipStream_t stream) {
+    if (tile == 64) return launch<64, 64, 2, 2, 3, EXACT>(p, stream);
+    if constexpr (!EXACT)
+        if (tile == 256) return launch<256, 256, 4, 2, 2, EXACT>(p, stream);
+    return launch<128, 128, 2, 2, 2, EXACT>(p, stream);
+}
+
 }  // namespace
 
-stark_qmm_status launch_fp8_tiles(const Fp8Product& p, hipStream_t stream) {
-    if (p.d_dt == STARK_QMM_F32) return launch<128, 128, 2, 2, true>(p, stream);
-    if (fp8::wide_tiles(p.m, p.experts, p.n)) return launch<256, 256, 4, 2, false>(p, stream);
-    return launch<128, 128, 2, 2, false>(p, stream);
+stark_qmm_status launch_fp8_tiles(const Fp8Product& p, uint32_t tile, hipStream_t stream) {
+    stark_qmm_status st = p.d_dt == STARK_QMM_F32 ? launch_size<true>(p, tile, stream) : launch_size<false>(p, tile, stream);
+    if (st != STARK_QMM_OK || p.parts == 1) return st;
+    hipLaunchKernelGGL(fp8_join, dim3((uint32_t)(((uint64_t)p.m * ((p.n + 3) / 4) + 255) / 256)), dim3(256), 0, stream, p);
+    QMM_HIP_CHECK(hipGetLastError());
+    return STARK_QMM_OK;
 }
 
 }  // namespace qmm

@@ -23,7 +23,9 @@ uint32_t row_tiles(uint32_t rows, uint32_t groups, uint32_t tile) { return fp8::
 uint32_t tile_of(uint32_t i, uint32_t tiles) { return fp8::tile_of(i, tiles); }
 void row_share(uint64_t t, uint32_t n, uint32_t k, uint32_t* r) { const fp8::RowShare x = fp8::row_share(t, n, k); r[0] = x.strips; r[1] = x.waves; }
 void place(uint32_t i, uint32_t rows, uint32_t columns, uint32_t* r) { const fp8::Place x = fp8::place(i, rows, columns); r[0] = x.row; r[1] = x.column; }
-int wide_tiles(uint32_t rows, uint32_t groups, uint32_t n) { return fp8::wide_tiles(rows, groups, n); }
+void choose(uint32_t m, uint32_t n, uint32_t k, uint32_t g, int grouped, int exact, uint32_t* r) {
+    const fp8::Choice c = fp8::choose(m, n, k, g, grouped, exact); r[0] = c.tile; r[1] = c.rows; r[2] = c.parts;
+}
 void split(uint32_t i, uint32_t b, uint32_t* r) { const fp8::Split x = fp8::split(i, b, fp8::inverse(b)); r[0] = x.row; r[1] = x.block; }
 }
 """
@@ -96,13 +98,37 @@ def test_row_shares_fill_the_gpu_and_no_more():
     L.row_share.argtypes = [C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p]
     assert _pair(L.row_share, 1, 12288, 4096) == (1, 4) and _pair(L.row_share, 1, 4096, 12288) == (1, 8)
     assert _pair(L.row_share, 128, 1536, 2048) == (2, 4) and _pair(L.row_share, 1, 16, 65536) == (1, 16)
-    assert _pair(L.row_share, 1, 16, 100) == (1, 2) and _pair(L.row_share, 2 ** 20, 2 ** 24, 128) == (2, 4)
+    assert _pair(L.row_share, 1, 4096, 4096) == (1, 4) and _pair(L.row_share, 1, 16, 100) == (1, 2) and _pair(L.row_share, 2 ** 20, 2 ** 24, 128) == (2, 4)
 
 
-def test_wide_tiles_need_rows_and_tiles():
-    L = rules()
-    assert L.wide_tiles(4096, 1, 12288) and L.wide_tiles(65536, 128, 1536)
-    assert not L.wide_tiles(333, 1, 1001) and not L.wide_tiles(1024, 128, 1536) and not L.wide_tiles(255, 1, 1 << 20)
+def _choose(m, n, k, groups=1, grouped=False, exact=False):
+    r = (C.c_uint32 * 3)()
+    rules().choose(m, n, k, groups, int(grouped), int(exact), r)
+    return tuple(r)
+
+
+def test_each_kernel_takes_its_calls():
+    """(tile, rows of the few-rows kernel, parts of the inner axis)."""
+    assert _choose(1, 12288, 4096) == (0, 16, 1) and _choose(5, 4096, 12288) == (0, 16, 1) and _choose(4096, 12288, 4096) == (256, 0, 1)
+    assert _choose(32, 12288, 4096)[0] == 64 and _choose(64, 4096, 12288) == (64, 0, 4) and _choose(16, 256, 16384)[2] == 8 and _choose(512, 4096, 4096) == (64, 0, 1)
+    assert _choose(128, 1001, 2000) == (0, 32, 1) and _choose(1024, 4096, 4096) == (128, 0, 1)
+    for tokens, want in ((16, 0), (64, 0), (256, 64), (2048, 128), (8192, 256)):
+        assert _choose(8 * tokens, 1536, 2048, 128, True)[0] == want
+
+
+def test_choices_are_what_the_kernels_take():
+    """Blocks of fewer than 128 codes go to the few-rows kernel; parts are of calls without groups and have four steps each."""
+    r = random.Random(8)
+    for _ in range(3000):
+        m, n, k = (int(2 ** r.uniform(0, e)) for e in (24, 24, 20))
+        grouped = r.random() < 0.5
+        groups = int(2 ** r.uniform(0, 10)) if grouped else 1
+        exact = r.random() < 0.5
+        tile, rows, parts = _choose(m, n, k, groups, grouped, exact)
+        assert (tile, rows) in ((0, 16), (0, 32), (64, 0), (128, 0), (256, 0)) and not (exact and tile == 256)
+        assert parts == 1 or (not grouped and tile and 4 * parts <= -(-k // 128))
+        if k < 128:
+            assert tile == 0
 
 
 def test_plain_codes_are_the_nearest():
@@ -194,6 +220,15 @@ def test_matmul_refusals():
     assert go(m=0) == go(n=0) == go(m=0, a=None, d=None) == Q.OK
     for bad in BAD_PRODUCTS:
         assert go(**bad) == Q.INVALID_ARGUMENT, bad
+    # a call in parts: 64 rows, N 4096, K 12288
+    parts = dict(m=64, n=4096, k=12288, a_row_stride=12288, b_row_stride=12288, d_row_stride=4096, d=FAKE + 2 ** 28, b=FAKE + 2 ** 22,
+                 a_scales=FAKE + 2 ** 21, b_scales=FAKE + 2 ** 27, a_scale_row_stride=96, b_scale_row_stride=96)
+    assert lib.stark_qmm_fp8_matmul_workspace_size(C.byref(_struct(F._MatmulArgs, PRODUCT, parts)), C.byref(n)) == Q.OK
+    assert n.value == 4 * 4 * 64 * 4096
+    assert go(**parts) == go(**parts, workspace=FAKE + 2 ** 29 + 8, workspace_size=n.value) == Q.INVALID_ARGUMENT
+    assert go(**parts, workspace=FAKE + 2 ** 28 + 16, workspace_size=n.value) == Q.INVALID_ARGUMENT
+    assert go(**parts, workspace=FAKE + 2 ** 29, workspace_size=n.value - 1) == Q.WORKSPACE_TOO_SMALL
+    assert lib.stark_qmm_fp8_matmul_workspace_size(C.byref(_struct(F._MatmulArgs, PRODUCT, {})), C.byref(n)) == Q.OK and n.value == 0
 
 
 def test_grouped_refusals():

@@ -242,6 +242,76 @@ def test_matmul_epilogue_and_strides(F, dtype, m, n, k, ab, accumulate, bias, ca
     _near(_np(d), want, tol, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m,n,k", [(64, 1024, 8192), (70, 1001, 6000), (17, 300, 16384), (130, 516, 8200)])
+def test_matmul_in_parts(F, dtype, m, n, k):
+    """Products whose inner axis is shared by workgroups, with a bias and another operator's call between two on one workspace."""
+    r = np.random.default_rng(m + n)
+    a, sa, b, sb = _operands(r, m, n, k)
+    bias = _held(r.normal(0, 1, n), dtype)
+    x = [_padded(a), _dev(sa), _padded(b), _dev(sb)]
+    d, e = (torch.full((m, n), 7.0, dtype=DT[dtype], device="cuda") for _ in range(2))
+    first = F.Fp8Matmul(*x, d, bias=_dev(bias, DT[dtype]))
+    assert first.workspace_bytes > 0
+    second = F.Fp8Matmul(*x, e, ab_scale=2.0, workspace=first.workspace)
+    for op in (first, second, first):
+        op.encode()
+    torch.cuda.synchronize()
+    want, mag, cut = R.product(a, sa, b, sb)
+    for t, ab, bi in ((d, 1.0, bias), (e, 2.0, None)):
+        w, tol = _epilogue(want, R.bound(want, mag, cut, k, dtype, ab), ab, None, bi, None)
+        _near(_np(t), w, tol, dtype)
+
+
+def test_captured_products_in_parts(F):
+    """Two captured calls with workspaces of their own replay on other rows."""
+    r = np.random.default_rng(14)
+    m, n, k = 64, 512, 8192
+    a, sa, b, sb = _operands(r, m, n, k)
+    sets = []
+    for _ in range(2):
+        x = [_padded(a), _dev(sa), _padded(b), _dev(sb), torch.zeros(m, n, dtype=torch.bfloat16, device="cuda")]
+        op = F.Fp8Matmul(*x)
+        assert op.workspace_bytes > 0
+        op.encode()
+        sets.append((x, op))
+    torch.cuda.synchronize()
+    graphs, stream = [], torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    for _, op in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            op.encode()
+        graphs.append(g)
+    for _ in range(3):
+        wants = []
+        for x, _ in sets:
+            a = R.nearest(r.normal(0, 110, (m, k)))
+            x[0].copy_(_dev(a))
+            wants.append(R.product(a, sa, b, sb))
+        torch.cuda.synchronize()
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for (x, _), (want, mag, cut) in zip(sets, wants):
+            _near(_np(x[4]), want, R.bound(want, mag, cut, k, "bf16"), "bf16")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("m,n,k", [(300, 3000, 1160), (1500, 4100, 136), (1501, 4103, 1160), (3000, 8200, 136), (3001, 8203, 136), (2500, 8200, 2304)])
+def test_matmul_wide_tiles(F, dtype, m, n, k):
+    """Calls of tiles of 64, 128 and 256, their last row and column tiles cut, odd strides among them; some rows are compared."""
+    r = np.random.default_rng(m)
+    a, sa, b, sb = _operands(r, m, n, k)
+    d = torch.full((m, n), 7.0, dtype=DT[dtype], device="cuda")
+    F.Fp8Matmul(_padded(a), _dev(sa), _padded(b), _dev(sb), d).encode()
+    torch.cuda.synchronize()
+    assert not (d == 7).all(1).any()
+    at = np.unique(np.concatenate([np.arange(0, m, max(7, m // 60)), [m - 1]]))
+    want, mag, cut = R.product(a[at], sa[at], b, sb)
+    _near(_np(d)[at], want, R.bound(want, mag, cut, k, dtype), dtype)
+
+
 @pytest.mark.parametrize("m,n,k", [(1, 130, 512), (5, 64, 256), (150, 200, 384)])
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_matmul_not_a_number(F, dtype, m, n, k):
@@ -286,7 +356,7 @@ def test_matmul_large_scales(F):
 
 # ---------------------------------------------------------------- grouped products
 
-def _grouped(F, r, sizes, n, k, dtype, gather, spare=0, lead_rows=0, bias=False, tokens=50):
+def _grouped(F, r, sizes, n, k, dtype, gather, spare=0, lead_rows=0, bias=False, tokens=50, every=1):
     E, total = len(sizes), sum(sizes)
     m = lead_rows + total + spare
     start = lead_rows + np.concatenate([[0], np.cumsum(sizes)])
@@ -306,10 +376,12 @@ def _grouped(F, r, sizes, n, k, dtype, gather, spare=0, lead_rows=0, bias=False,
         live[at] = True
         if sizes[e] == 0:
             continue
-        which = rows[at] if gather else np.arange(m)[at]
+        some = np.unique(np.concatenate([np.arange(start[e], start[e + 1], every), [start[e + 1] - 1]]))
+        which = rows[some] if gather else some
         want, mag, cut = R.product(a[which], sa[which], b[e], sb[e])
         want, tol = _epilogue(want, R.bound(want, mag, cut, k, dtype), 1.0, None, bi[e] if bias else None, None)
-        _near(got[at], want, tol, dtype, f"expert {e}")
+        _near(got[some], want, tol, dtype, f"expert {e}")
+        assert not (got[at] == 3).all(1).any()
     assert (got[~live] == 3).all(), "rows of no group were written"
 
 
@@ -319,6 +391,11 @@ def _grouped(F, r, sizes, n, k, dtype, gather, spare=0, lead_rows=0, bias=False,
                                        ([130, 1, 0, 260], 200, 272), ([40, 200, 7], 300, 512), ([0, 0], 64, 128)])
 def test_grouped(F, dtype, gather, sizes, n, k):
     _grouped(F, np.random.default_rng(sum(sizes) + n), sizes, n, k, dtype, gather)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_grouped_wide_tiles(F, dtype):
+    _grouped(F, np.random.default_rng(15), [900, 0, 1030, 513, 257, 1, 2300], 4100, 136, dtype, True, spare=9, tokens=300, every=23)
 
 
 @pytest.mark.parametrize("gather", [False, True])
