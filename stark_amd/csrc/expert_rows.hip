@@ -10,8 +10,12 @@ namespace {
 // id, a lane's rank is the wave's count of that expert so far and the lower lanes among them. So positions do not depend on
 // the order in which anything runs. A workgroup's sixteen waves take consecutive runs of its routes; a call of more than one
 // workgroup counts first (plan_count), and each workgroup adds up what the ones before it have (plan_place).
+// Latency bounds it, so a wave has as few turns as 256 workgroups allow.
 constexpr int kPlanThreads = 1024, kPlanWaves = kPlanThreads / 64;
-constexpr uint32_t kMaxExperts = 1024, kGroupRoutes = 4096;  // routes of a workgroup where there are several
+constexpr uint32_t kMaxExperts = 1024;
+// Routes that one workgroup takes without counting first (2048 routes 5.8 us, with a count 7.4; 4096 routes 8.9 and 7.6; 65536
+// routes 17.6 us with 4096 to a workgroup, 10.0 with 1024).
+constexpr uint32_t kOneGroup = 2048;
 
 struct Plan {
     const uint32_t* ids;
@@ -19,7 +23,7 @@ struct Plan {
     int32_t* tokens;
     int32_t* slots;
     uint32_t* counts;  // [workgroups, experts]
-    uint32_t routes, active, experts, first, groups, bits;
+    uint32_t routes, active, experts, first, groups, per_group, bits;
 };
 
 // Lanes of the wave whose key is this lane's.
@@ -41,9 +45,8 @@ QMM_DEVICE uint32_t route_key(const Plan& p, uint32_t r, uint32_t end) {
 
 // Routes of this wave: [begin, end), whole 64s but the last.
 QMM_DEVICE void wave_routes(const Plan& p, uint32_t wave, uint32_t* begin, uint32_t* end) {
-    const uint32_t per_group = p.groups > 1 ? kGroupRoutes : (p.routes + 63) / 64 * 64;
-    const uint32_t g0 = blockIdx.x * per_group, g1 = min(g0 + per_group, p.routes);
-    const uint32_t per_wave = (per_group / 64 + kPlanWaves - 1) / kPlanWaves * 64;
+    const uint32_t g0 = blockIdx.x * p.per_group, g1 = min(g0 + p.per_group, p.routes);
+    const uint32_t per_wave = (p.per_group / 64 + kPlanWaves - 1) / kPlanWaves * 64;
     *begin = min(g0 + wave * per_wave, g1);
     *end = min(*begin + per_wave, g1);
 }
@@ -82,7 +85,7 @@ __global__ __launch_bounds__(kPlanThreads) void plan_count(Plan p) {
 
 __global__ __launch_bounds__(kPlanThreads) void plan_place(Plan p) {
     __shared__ uint32_t cnt[kPlanWaves][kMaxExperts];
-    __shared__ uint32_t sums[kPlanWaves];
+    __shared__ uint32_t sums[kPlanWaves], part[2][kPlanThreads];
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     for (uint32_t e = lane; e < p.experts; e += 64) cnt[wave][e] = 0;
     uint32_t begin, end;
@@ -91,16 +94,24 @@ __global__ __launch_bounds__(kPlanThreads) void plan_place(Plan p) {
     __syncthreads();
     // thread e: the routes of expert e in all, before this workgroup, and in its waves
     uint32_t before = 0, all = 0;
-    if (tid < p.experts) {
-        if (p.groups > 1) {
-            for (uint32_t g = 0; g < p.groups; ++g) {
-                const uint32_t n = p.counts[(size_t)g * p.experts + tid];
+    if (p.groups > 1) {
+        // slices of the threads take every so many groups' counts, all loads in flight
+        const uint32_t wide = (p.experts + 63) / 64 * 64, slices = kPlanThreads / wide, slice = tid / wide, e = tid % wide;
+        if (slice < slices && e < p.experts) {
+#pragma unroll 8
+            for (uint32_t g = slice; g < p.groups; g += slices) {
+                const uint32_t n = p.counts[(size_t)g * p.experts + e];
                 all += n;
                 before += g < blockIdx.x ? n : 0;
             }
-        } else {
-            for (int w = 0; w < kPlanWaves; ++w) all += cnt[w][tid];
         }
+        part[0][tid] = all, part[1][tid] = before;
+        __syncthreads();
+        all = before = 0;
+        if (tid < p.experts)
+            for (uint32_t i = 0; i < slices; ++i) all += part[0][i * wide + tid], before += part[1][i * wide + tid];
+    } else if (tid < p.experts) {
+        for (int w = 0; w < kPlanWaves; ++w) all += cnt[w][tid];
     }
     uint32_t start = all;  // inclusive scan over the experts
 #pragma unroll
@@ -137,7 +148,9 @@ __global__ __launch_bounds__(kPlanThreads) void plan_place(Plan p) {
     });
 }
 
-uint32_t plan_groups(uint32_t routes) { return routes <= 2 * kGroupRoutes ? 1 : (routes + kGroupRoutes - 1) / kGroupRoutes; }
+// Routes of a workgroup: whole turns of its waves, and at most 256 workgroups.
+uint32_t plan_routes(uint32_t routes) { return routes <= kOneGroup ? (routes + 63) / 64 * 64 : std::max(1u, (routes + 262143) / 262144) * 1024; }
+uint32_t plan_groups(uint32_t routes) { return routes <= kOneGroup ? 1 : (routes + plan_routes(routes) - 1) / plan_routes(routes); }
 
 stark_qmm_status check_plan(const stark_qmm_expert_plan_args* a, uint64_t* bytes) {
     if (!a || !bytes) return STARK_QMM_INVALID_ARGUMENT;
@@ -246,7 +259,7 @@ stark_qmm_status stark_qmm_expert_plan(const stark_qmm_expert_plan_args* a, void
     if (need && (!a->workspace || !fp8_aligned(a->workspace, 16))) return STARK_QMM_INVALID_ARGUMENT;
     if (need > a->workspace_size) return STARK_QMM_WORKSPACE_TOO_SMALL;
     Plan p{a->ids, a->group_start, a->tokens_out, a->slots, (uint32_t*)a->workspace, routes, a->active, a->experts, a->first,
-           plan_groups(routes), 0};
+           plan_groups(routes), plan_routes(routes), 0};
     while ((1u << p.bits) <= a->experts) ++p.bits;  // keys are 0 .. experts
     if (p.groups > 1) {
         hipLaunchKernelGGL(plan_count, dim3(p.groups), dim3(kPlanThreads), 0, (hipStream_t)stream, p);

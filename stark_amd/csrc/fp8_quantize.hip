@@ -43,12 +43,12 @@ QMM_DEVICE void load8(const void* x, uint64_t at, uint32_t c, uint32_t end, floa
     for (int e = 0; e < 8; ++e) v[e] = c + e < end ? load_as_f32(x, DT, at + c + e) : 0.0f;
 }
 
-// v * g / (1 + exp(-g)); exp(-g) = 2^t with the product's rounding error carried into the result.
+// v * g / (1 + exp(-g)), the reciprocal to its last place; exp(-g) = 2^t with the product's rounding error carried into the result.
 QMM_DEVICE float gate(float v, float g) {
     constexpr float kHi = 0x1.715476p+0f, kLo = 0x1.4ae0c0p-26f, kLn2 = 0x1.62e430p-1f;  // log2(e) in two parts
     const float t = -g * kHi, r = fmaf(-g, kLo, fmaf(-g, kHi, -t));
     const float p = __builtin_amdgcn_exp2f(t), ex = fabsf(t) < 128.0f ? fmaf(p, r * kLn2, p) : p;
-    return v * (g / (1.0f + ex));
+    return v * (g * __builtin_amdgcn_rcpf(1.0f + ex));
 }
 
 // e4m3 codes of x[0] / s and x[1] / s in the low 16 bits; i is within a few ulp of 1 / s. Where the quotient is so near the
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(kThreads) void fp8_quantize(Quantize q) {
     for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
     top = group_max<kLanes>(top);
     const bool bad = top >= 0x7f800000u;
-    const float s = fmaxf(__uint_as_float(bad ? 0 : top) / 448.0f, 0x1p-126f), i = 1.0f / s;
+    const float s = fmaxf(__uint_as_float(bad ? 0 : top) / 448.0f, 0x1p-126f), i = __builtin_amdgcn_rcpf(s);
     uint32_t w[2] = {0, 0};
     if (!bad) {
 #pragma unroll

@@ -64,7 +64,8 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
         const uint32_t k0 = __builtin_amdgcn_readfirstlane((s - before) * kStep);
 #pragma unroll
         for (int i = 0; i < LA; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)&lds.a[buf][64 * (i * W + wave)], 16, ao[i], k0, 0, 0);
+            if (S > 2 || 8 * (i * W + wave) < t.rows)  // (with S > 2 a wave's loads of a step are counted)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)&lds.a[buf][64 * (i * W + wave)], 16, ao[i], k0, 0, 0);
 #pragma unroll
         for (int i = 0; i < LB; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void*)&lds.b[buf][64 * (i * W + wave)], 16, bo[i], k0, 0, 0);
@@ -180,7 +181,7 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
             if (next % kChunk == 0) load_scales(next / kChunk);
             load(s + S - 1, buf ? buf - 1 : S - 1);
         }
-        compute(buf, s);
+        if (wm * (BM / WM) < t.rows) compute(buf, s);  // (a wave whose rows a group's last tile has not)
         buf = buf + 1 < S ? buf + 1 : 0;
     }
 
