@@ -162,8 +162,9 @@ stark_qmm_status check_plan(const stark_qmm_expert_plan_args* a, uint64_t* bytes
     return STARK_QMM_OK;
 }
 
-// ---- combine: a workgroup takes a token and 2048 values of its row (1024 in f32); a thread 16 bytes of every route's row.
-constexpr int kSumThreads = 256;
+// ---- combine: a workgroup takes a token and 2048 values of its row (1024 in f32, or where rows start anywhere). A thread has 16
+// bytes of a row, or four values 256 apart; the rows of four routes are loaded together. HBM bounds it.
+constexpr int kSumThreads = 256, kSumRoutes = 4;
 
 struct Combine {
     const void* x;
@@ -175,58 +176,80 @@ struct Combine {
 };
 
 template <uint32_t DT, bool VEC>
-__global__ __launch_bounds__(kSumThreads) void expert_combine(Combine q) {
-    constexpr int E = VEC ? (DT == STARK_QMM_F32 ? 4 : 8) : 1;
-    const uint32_t token = blockIdx.x, c = (blockIdx.y * kSumThreads + threadIdx.x) * E;
-    if (c >= q.width) return;
-    float sum[E];
-    const auto add = [&](const void* p, size_t at, float w, bool first) {
-        float v[E];
+struct SumValues {
+    static constexpr int kCount = VEC && DT != STARK_QMM_F32 ? 8 : 4;
+    float v[kCount];
+    // values of a row from column c on
+    QMM_DEVICE void load(const void* p, size_t row, uint32_t c, uint32_t width) {
         if constexpr (!VEC) {
-            v[0] = load_as_f32(p, DT, at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = load_as_f32(p, DT, row + min(c + e * kSumThreads, width - 1));
         } else if constexpr (DT == STARK_QMM_F32) {
-            const f32x4 t = *(const f32x4*)((const float*)p + at);
+            const f32x4 t = *(const f32x4*)((const float*)p + row + c);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] = t[e];
         } else {
-            const u32x4 t = *(const u32x4*)((const uint16_t*)p + at);
+            const u32x4 t = *(const u32x4*)((const uint16_t*)p + row + c);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 v[2 * e] = DT == STARK_QMM_BF16 ? __uint_as_float(t[e] << 16) : f16_bits_to_f32(t[e] & 0xffffu);
                 v[2 * e + 1] = DT == STARK_QMM_BF16 ? __uint_as_float(t[e] & 0xffff0000u) : f16_bits_to_f32(t[e] >> 16);
             }
         }
-#pragma unroll
-        for (int e = 0; e < E; ++e) sum[e] = first ? v[e] : fmaf(w, v[e], sum[e]);
-    };
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum[e] = 0.0f;
-    const size_t out_at = (size_t)token * q.out_stride + c;
-    if (q.accumulate) add(q.out, out_at, 1.0f, true);
-    for (uint32_t j = 0; j < q.active; ++j) {
-        const uint32_t slot = (uint32_t)q.slots[(size_t)token * q.active + j];
-        const float w = q.weights[(size_t)token * q.active + j];
-        if (slot < q.rows) add(q.x, (size_t)slot * q.x_stride + c, w, false);
     }
-    if constexpr (!VEC) {
-        store_from_f32(q.out, DT, out_at, sum[0]);
-    } else if constexpr (DT == STARK_QMM_F32) {
-        *(f32x4*)((float*)q.out + out_at) = f32x4{sum[0], sum[1], sum[2], sum[3]};
-    } else {
-        u32x4 t;
+    QMM_DEVICE void store(void* p, size_t row, uint32_t c, uint32_t width) const {
+        if constexpr (!VEC) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t lo = DT == STARK_QMM_BF16 ? f32_to_bf16_bits(sum[2 * e]) : f32_to_f16_bits(sum[2 * e]);
-            const uint32_t hi = DT == STARK_QMM_BF16 ? f32_to_bf16_bits(sum[2 * e + 1]) : f32_to_f16_bits(sum[2 * e + 1]);
-            t[e] = lo | (hi << 16);
+            for (int e = 0; e < 4; ++e)
+                if (c + e * kSumThreads < width) store_from_f32(p, DT, row + c + e * kSumThreads, v[e]);
+        } else if constexpr (DT == STARK_QMM_F32) {
+            *(f32x4*)((float*)p + row + c) = f32x4{v[0], v[1], v[2], v[3]};
+        } else {
+            u32x4 t;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) t[e] = fp8_pack2(DT, v[2 * e], v[2 * e + 1]);
+            *(u32x4*)((uint16_t*)p + row + c) = t;
         }
-        *(u32x4*)((uint16_t*)q.out + out_at) = t;
     }
+};
+
+template <uint32_t DT, bool VEC>
+__global__ __launch_bounds__(kSumThreads) void expert_combine(Combine q) {
+    using Values = SumValues<DT, VEC>;
+    constexpr int E = Values::kCount;
+    const uint32_t token = blockIdx.x, c = blockIdx.y * kSumThreads * E + threadIdx.x * (VEC ? E : 1);
+    if (c >= q.width) return;
+    Values sum;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum.v[e] = 0.0f;
+    const size_t out = (size_t)token * q.out_stride, route = (size_t)token * q.active;
+    if (q.accumulate) sum.load(q.out, out, c, q.width);
+    for (uint32_t j = 0; j < q.active; j += kSumRoutes) {
+        uint32_t slot[kSumRoutes];
+        float w[kSumRoutes];
+        Values x[kSumRoutes];
+#pragma unroll
+        for (int u = 0; u < kSumRoutes; ++u) {
+            const size_t at = route + min(j + u, q.active - 1);
+            slot[u] = j + u < q.active ? (uint32_t)q.slots[at] : q.rows;
+            w[u] = q.weights[at];
+        }
+#pragma unroll
+        for (int u = 0; u < kSumRoutes; ++u)
+            if (slot[u] < q.rows) x[u].load(q.x, (size_t)slot[u] * q.x_stride, c, q.width);
+#pragma unroll
+        for (int u = 0; u < kSumRoutes; ++u)
+            if (slot[u] < q.rows) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) sum.v[e] = fmaf(w[u], x[u].v[e], sum.v[e]);
+            }
+    }
+    sum.store(q.out, out, c, q.width);
 }
 
 template <uint32_t DT>
 void launch_combine(const Combine& q, uint32_t tokens, bool vec, hipStream_t s) {
-    const uint32_t each = kSumThreads * (vec ? (DT == STARK_QMM_F32 ? 4 : 8) : 1);
+    const uint32_t each = kSumThreads * (vec && DT != STARK_QMM_F32 ? 8 : 4);
     const dim3 grid(tokens, (q.width + each - 1) / each);
     if (vec) hipLaunchKernelGGL((expert_combine<DT, true>), grid, dim3(kSumThreads), 0, s, q);
     else hipLaunchKernelGGL((expert_combine<DT, false>), grid, dim3(kSumThreads), 0, s, q);
