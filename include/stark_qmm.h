@@ -710,7 +710,7 @@ typedef struct stark_qmm_fp8_quantize_args {
     uint64_t code_row_stride;    /* bytes, a multiple of 16 */
     float* scales;               /* [rows, ceil(columns / 128)] */
     uint64_t scale_row_stride, scale_block_stride; /* elements */
-    uint32_t rows, columns;
+    uint32_t rows, columns;      /* at most 2^24 and 2^20; of 2^28 blocks and more in all: UNSUPPORTED */
     uint32_t gated;              /* x = value * gate / (1 + exp(-gate)), in f32 */
     const int32_t* row_count;    /* device: rows from here on stay as they were (at most `rows`), or NULL */
 } stark_qmm_fp8_quantize_args;
@@ -742,7 +742,12 @@ typedef struct stark_qmm_fp8_matmul_args {
 
 /* d[m, n] = ab_scale * sum over blocks of (a_scale * b_scale) * (sum of a * b in
  * the block), then the other d_ops in the order of stark_qmm_encode. The two
- * scales are multiplied first, in f32; sums are f32. d may not overlap an input. */
+ * scales are multiplied first, in f32; sums are f32. Outputs of F16 and BF16 may
+ * come from matrix instructions that add eight neighbouring products at a time and
+ * cut each off below 2^-13 of the largest one's binade (off by 1.5e-5 of their size
+ * for normally distributed codes); F32 ones do not. Which kernel takes a call goes
+ * by its sizes, and so do the last bits of its sums; a call repeated gives the same
+ * bits. d may not overlap an input. */
 STARK_QMM_API stark_qmm_status stark_qmm_fp8_matmul(const stark_qmm_fp8_matmul_args* args, void* stream);
 /* 0 where the call needs none (workspace may then be NULL). */
 STARK_QMM_API stark_qmm_status stark_qmm_fp8_matmul_workspace_size(const stark_qmm_fp8_matmul_args* args, uint64_t* bytes);
@@ -796,7 +801,7 @@ typedef struct stark_qmm_expert_combine_args {
     const float* weights;        /* [tokens, active] */
     void* out;                   /* [tokens, width] */
     uint64_t x_row_stride, out_row_stride; /* elements */
-    uint32_t tokens, active, rows, width;  /* active 1 .. 1024 */
+    uint32_t tokens, active, rows, width;  /* tokens below 2^24, active 1 .. 1024 */
     uint32_t accumulate;         /* out += instead of out = */
 } stark_qmm_expert_combine_args;
 

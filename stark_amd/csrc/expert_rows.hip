@@ -298,7 +298,7 @@ stark_qmm_status stark_qmm_expert_combine(const stark_qmm_expert_combine_args* a
     if (!a) return STARK_QMM_INVALID_ARGUMENT;
     if (a->struct_size != sizeof(*a)) return STARK_QMM_ABI_MISMATCH;
     if (!fp8_type(a->data_type)) return STARK_QMM_UNSUPPORTED_DATA_TYPE;
-    if (a->active == 0 || a->active > 1024 || a->tokens > (1u << 24) || a->width > (1u << 24) || a->rows > 0x7fffffffu)
+    if (a->active == 0 || a->active > 1024 || a->tokens >= (1u << 24) || a->width > (1u << 24) || a->rows > 0x7fffffffu)
         return STARK_QMM_INVALID_ARGUMENT;
     if (a->tokens == 0 || a->width == 0) return STARK_QMM_OK;
     const uint64_t e = fp8_element(a->data_type), routes = (uint64_t)a->tokens * a->active;

@@ -39,6 +39,8 @@ inline bool fp8_overlap(const void* p, uint64_t pn, const void* q, uint64_t qn) 
     return p && q && pn && qn && (uintptr_t)p < (uintptr_t)q + qn && (uintptr_t)q < (uintptr_t)p + pn;
 }
 inline uint64_t fp8_span(uint64_t rows, uint64_t stride, uint64_t width) { return rows ? (rows - 1) * stride + width : 0; }
+// Workgroups of a launch whose threads 32 bits count.
+inline bool fp8_launches(uint64_t groups, uint32_t threads) { return groups * threads < 1ull << 32; }
 inline bool fp8_aligned(const void* p, uint64_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 inline uint64_t fp8_element(uint32_t dt) { return dt == STARK_QMM_F32 ? 4 : 2; }
 inline bool fp8_type(uint32_t dt) { return dt == STARK_QMM_F32 || dt == STARK_QMM_F16 || dt == STARK_QMM_BF16; }

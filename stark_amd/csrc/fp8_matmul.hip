@@ -72,13 +72,12 @@ stark_qmm_status run(const stark_qmm_fp8_matmul_args& q, const Groups& g, const 
         !fp8_aligned(q.d, e) || !fp8_aligned(q.d_ops.bias, e) || !fp8_aligned(start, 4) || !fp8_aligned(rows, 4))
         return STARK_QMM_INVALID_ARGUMENT;
     // what d must not meet
-    const uint64_t dn = e * fp8_span(q.m, p.d_stride, q.n), last = g.experts - 1;
-    if (fp8_overlap(q.d, dn, q.a, fp8_span(p.a_row_count, p.a_stride, wide)) ||
-        fp8_overlap(q.d, dn, q.a_scales, 4 * (fp8_span(p.a_row_count, p.as_row, 1) + (kb - 1) * p.as_block)) ||
-        fp8_overlap(q.d, dn, q.b, last * g.b_expert + fp8_span(q.n, p.b_stride, wide)) ||
-        fp8_overlap(q.d, dn, q.b_scales, 4 * (last * g.bs_expert + fp8_span(nb, p.bs_row, 1) + (kb - 1) * p.bs_block)) ||
-        fp8_overlap(q.d, dn, q.d_ops.bias, e * (last * g.bias_expert + q.n)) || fp8_overlap(q.d, dn, start, 4ull * (g.experts + 1)) ||
-        fp8_overlap(q.d, dn, rows, 4ull * q.m))
+    const uint64_t last = g.experts - 1, dn = e * fp8_span(q.m, p.d_stride, q.n), an = fp8_span(p.a_row_count, p.a_stride, wide),
+                   asn = 4 * (fp8_span(p.a_row_count, p.as_row, 1) + (kb - 1) * p.as_block), bn = last * g.b_expert + fp8_span(q.n, p.b_stride, wide),
+                   bsn = 4 * (last * g.bs_expert + fp8_span(nb, p.bs_row, 1) + (kb - 1) * p.bs_block);
+    if (fp8_overlap(q.d, dn, q.a, an) || fp8_overlap(q.d, dn, q.a_scales, asn) || fp8_overlap(q.d, dn, q.b, bn) ||
+        fp8_overlap(q.d, dn, q.b_scales, bsn) || fp8_overlap(q.d, dn, q.d_ops.bias, e * (last * g.bias_expert + q.n)) ||
+        fp8_overlap(q.d, dn, start, 4ull * (g.experts + 1)) || fp8_overlap(q.d, dn, rows, 4ull * q.m))
         return STARK_QMM_INVALID_ARGUMENT;
     p.a = q.a, p.b = q.b, p.as = q.a_scales, p.bs = q.b_scales, p.d = q.d, p.bias = q.d_ops.bias;
     p.group_start = start, p.a_rows = rows;
@@ -90,7 +89,10 @@ stark_qmm_status run(const stark_qmm_fp8_matmul_args& q, const Groups& g, const 
     if (need) {
         if (!q.workspace || !fp8_aligned(q.workspace, 16)) return STARK_QMM_INVALID_ARGUMENT;
         if (need > q.workspace_size) return STARK_QMM_WORKSPACE_TOO_SMALL;
-        if (fp8_overlap(q.workspace, need, q.d, dn)) return STARK_QMM_INVALID_ARGUMENT;
+        if (fp8_overlap(q.workspace, need, q.d, dn) || fp8_overlap(q.workspace, need, q.a, an) || fp8_overlap(q.workspace, need, q.b, bn) ||
+            fp8_overlap(q.workspace, need, q.a_scales, asn) || fp8_overlap(q.workspace, need, q.b_scales, bsn) ||
+            fp8_overlap(q.workspace, need, q.d_ops.bias, e * q.n))
+            return STARK_QMM_INVALID_ARGUMENT;
         p.partial = (float*)q.workspace, p.partial_stride = partial_stride(p);
     }
     return c.tile ? launch_fp8_tiles(p, c.tile, stream) : launch_fp8_rows(p, c.rows, stream);

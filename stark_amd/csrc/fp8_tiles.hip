@@ -2,8 +2,19 @@
 //   D[m, n] = sum_b (as[m, b] * bs[n / 128, b]) * sum_{k in b} A[m, k] B[n, k].
 //
 // A step is one block of 128 codes of the inner axis, whose sum of 16 x 16 outputs (fp8_block) starts at zero, is scaled in f32
-// and added to the accumulator. The weights are the matrix instruction's rows, so that
-// a lane's outputs are four consecutive columns of one row of D, and share one scale product.
+// and added to the accumulator. The weights are the matrix instruction's rows, so that a lane's outputs are four consecutive
+// columns of one row of D, and share one scale product. Operands go from memory into LDS without registers between.
+//
+// 256 x 256 outputs by eight waves (64 x 128 each): 64 rows and 128 columns of a wave are 24 LDS reads for 32 matrix instructions,
+// so that LDS is busy for half of their time, and the tile reads half of what 128 x 128 tiles read. 4096 rows, N 12288, K 4096 take
+// 190 us (2170 TFLOP/s; a large product with one scale a tensor reaches 2660 on this card). The matrix instructions bound it
+// (82 us at their peak), with the starts of steps, where two waves a SIMD wait for their operands out of LDS, and the start and
+// the stores of a tile, some 8 us that nothing hides: one workgroup to a CU. (A version of 222 us took 97 with its loads alone,
+// 141 with its products alone and 173 without its stores.) 65536 rows of 128 experts, N 1536, K 2048, whose tiles have 16 steps:
+// 292 us. Steps on the way to it, for the first call: 128 x 128 tiles with a lane's scales loaded each step 382 us; 256 x 256 274;
+// scales staged 228; LDS pieces without conflicts 223; outputs from registers 203; a scalar step offset and the order of the
+// products held 188. 128 x 128 by four waves (two workgroups to a CU) takes smaller calls, 64 x 64 with three steps in LDS the
+// smallest, where each step is latency (0.35 us).
 #include "fp8_common.h"
 
 namespace qmm {
@@ -53,23 +64,33 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
         r = min(r, t.rows - 1);
         return p.a_rows ? min((uint32_t)p.a_rows[t.first + r], p.a_row_count - 1) : r;
     };
-    uint32_t ao[LA], bo[LB];
+    // (rows and scales first: gathered ones are loads of their own, which the weights' first loads need not wait for)
+    uint32_t ao[LA], bo[LB], so[LA];
 #pragma unroll
-    for (int i = 0; i < LA; ++i) ao[i] = a_row(8 * (i * W + wave) + srow) * (uint32_t)p.a_stride + 16 * piece;
+    for (int i = 0; i < LA; ++i) ao[i] = a_row(8 * (i * W + wave) + srow);
+#pragma unroll
+    for (int i = 0; i < LA; ++i) so[i] = a_row(8 * (i * W + wave) + (lane & 7));
 #pragma unroll
     for (int i = 0; i < LB; ++i) bo[i] = min(8 * (i * W + wave) + srow, nlast) * (uint32_t)p.b_stride + 16 * piece;
 
     const __amdgpu_buffer_rsrc_t ra = everything(abase), rb = everything(bbase);
-    const auto load = [&](uint32_t s, int buf) {  // a step that is not the short one
+    const auto load_b = [&](uint32_t s, int buf) {  // a step that is not the short one
+        const uint32_t k0 = __builtin_amdgcn_readfirstlane((s - before) * kStep);
+#pragma unroll
+        for (int i = 0; i < LB; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void*)&lds.b[buf][64 * (i * W + wave)], 16, bo[i], k0, 0, 0);
+    };
+    const auto load_a = [&](uint32_t s, int buf) {
         const uint32_t k0 = __builtin_amdgcn_readfirstlane((s - before) * kStep);
 #pragma unroll
         for (int i = 0; i < LA; ++i)
             if (S > 2 || 8 * (i * W + wave) < t.rows)  // (with S > 2 a wave's loads of a step are counted)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)&lds.a[buf][64 * (i * W + wave)], 16, ao[i], k0, 0, 0);
-#pragma unroll
-        for (int i = 0; i < LB; ++i)
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void*)&lds.b[buf][64 * (i * W + wave)], 16, bo[i], k0, 0, 0);
     };
+    if (from >= before && from < total) load_b(from, 0);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < LA; ++i) ao[i] = ao[i] * (uint32_t)p.a_stride + 16 * piece, so[i] *= (uint32_t)p.as_row;
     // The last, short block: pieces past the row's end are not read, codes past it in its last piece are cleared.
     const auto load_tail = [&](int buf) {
         const uint32_t have = min(16u, tail > 16 * piece ? tail - 16 * piece : 0u);
@@ -91,9 +112,6 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
     // Scales of a chunk of steps: a load takes eight rows' (one line each where a row's scales are contiguous).
     const float* asbase = p.a_rows ? p.as : p.as + (uint64_t)t.first * p.as_row;
     const float* bsbase = p.bs + t.expert * p.bs_expert;
-    uint32_t so[LA];
-#pragma unroll
-    for (int i = 0; i < LA; ++i) so[i] = a_row(8 * (i * W + wave) + (lane & 7)) * (uint32_t)p.as_row;
     const auto load_scales = [&](uint32_t chunk) {
         const auto block = [&](uint32_t in) {
             const uint32_t s = min(from + chunk * kChunk + in, total - 1);
@@ -169,8 +187,12 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
 #pragma unroll
     for (int i = 0; i < S - 1; ++i)
         if (from + i < total) {
-            if (from + i < before) load_tail(i);
-            else load(from + i, i);
+            if (from + i < before) {
+                load_tail(i);
+            } else {
+                load_a(from + i, i);
+                if (i > 0) load_b(from + i, i);
+            }
         }
     int buf = 0;
 #pragma unroll 1
@@ -179,7 +201,8 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
         if (s + S - 1 < total) {
             const uint32_t next = s + S - 1 - from;
             if (next % kChunk == 0) load_scales(next / kChunk);
-            load(s + S - 1, buf ? buf - 1 : S - 1);
+            load_a(s + S - 1, buf ? buf - 1 : S - 1);
+            load_b(s + S - 1, buf ? buf - 1 : S - 1);
         }
         if (wm * (BM / WM) < t.rows) compute(buf, s);  // (a wave whose rows a group's last tile has not)
         buf = buf + 1 < S ? buf + 1 : 0;
@@ -316,7 +339,7 @@ __global__ __launch_bounds__(256) void fp8_join(Fp8Product p) {
 template <int BM, int BN, int WM, int WN, int S, bool EXACT>
 stark_qmm_status launch(const Fp8Product& p, hipStream_t stream) {
     const uint64_t tiles = (uint64_t)fp8::row_tiles(p.m, p.experts, BM) * ((p.n + BN - 1) / BN);
-    if (tiles >= 1u << 24) return STARK_QMM_UNSUPPORTED;
+    if (!fp8_launches(tiles + 7, 64 * WM * WN)) return STARK_QMM_UNSUPPORTED;
     hipLaunchKernelGGL((fp8_tiles<BM, BN, WM, WN, S, EXACT>), dim3((uint32_t)((tiles + 7) / 8 * 8), p.parts), dim3(64 * WM * WN), 0, stream, p);
     QMM_HIP_CHECK(hipGetLastError());
     return STARK_QMM_OK;

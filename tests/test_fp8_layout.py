@@ -182,6 +182,7 @@ def test_quantize_refusals():
     assert go(struct_size=4) == Q.ABI_MISMATCH
     assert go(data_type=Q.U8) == Q.UNSUPPORTED_DATA_TYPE
     assert go(rows=0) == go(columns=0) == Q.OK
+    assert go(rows=2 ** 24, columns=2 ** 11) == Q.UNSUPPORTED  # more blocks than a launch has threads for
     for bad in (dict(rows=2 ** 24 + 1), dict(columns=2 ** 20 + 1), dict(x=None), dict(codes=None), dict(scales=None), dict(x=FAKE + 1),
                 dict(codes=FAKE + 2 ** 16 + 8), dict(scales=FAKE + 2 ** 17 + 2), dict(x_row_stride=511), dict(code_row_stride=504),
                 dict(code_row_stride=520), dict(gated=1), dict(scale_row_stride=3), dict(scale_row_stride=0), dict(scale_block_stride=0),
@@ -226,7 +227,8 @@ def test_matmul_refusals():
     assert lib.stark_qmm_fp8_matmul_workspace_size(C.byref(_struct(F._MatmulArgs, PRODUCT, parts)), C.byref(n)) == Q.OK
     assert n.value == 4 * 4 * 64 * 4096
     assert go(**parts) == go(**parts, workspace=FAKE + 2 ** 29 + 8, workspace_size=n.value) == Q.INVALID_ARGUMENT
-    assert go(**parts, workspace=FAKE + 2 ** 28 + 16, workspace_size=n.value) == Q.INVALID_ARGUMENT
+    for meets in (parts["d"] + 16, FAKE, parts["b"] + 16, parts["a_scales"], parts["b_scales"] + 16):
+        assert go(**parts, workspace=meets, workspace_size=n.value) == Q.INVALID_ARGUMENT
     assert go(**parts, workspace=FAKE + 2 ** 29, workspace_size=n.value - 1) == Q.WORKSPACE_TOO_SMALL
     assert lib.stark_qmm_fp8_matmul_workspace_size(C.byref(_struct(F._MatmulArgs, PRODUCT, {})), C.byref(n)) == Q.OK and n.value == 0
 
@@ -304,7 +306,7 @@ def test_combine_refusals():
     assert go(struct_size=4) == Q.ABI_MISMATCH
     assert go(data_type=Q.U8) == Q.UNSUPPORTED_DATA_TYPE
     assert go(tokens=0) == go(width=0) == Q.OK
-    for bad in (dict(active=0), dict(active=1025), dict(tokens=2 ** 24 + 1), dict(width=2 ** 24 + 1), dict(rows=2 ** 31), dict(x=None),
+    for bad in (dict(active=0), dict(active=1025), dict(tokens=2 ** 24), dict(width=2 ** 24 + 1), dict(rows=2 ** 31), dict(x=None),
                 dict(slots=None), dict(weights=None), dict(out=None), dict(x=FAKE + 1), dict(weights=FAKE + 2 ** 18 + 2), dict(x_row_stride=63),
                 dict(out_row_stride=63), dict(out=FAKE), dict(out=FAKE + 2 ** 17), dict(out=FAKE + 2 ** 18 + 4)):
         assert go(**bad) == Q.INVALID_ARGUMENT, bad
