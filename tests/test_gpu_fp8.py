@@ -612,6 +612,76 @@ def test_calls_on_two_streams(F):
         assert torch.equal(s["out"], was)
 
 
+def test_calls_of_nothing(F):
+    """No rows, no columns, no tokens: nothing is launched or written, and a plan's starts are zeros."""
+    w, ws = F.new_rows(8, 200)
+    ws = torch.zeros(1, 2, device="cuda")
+    c0, s0 = F.new_rows(0, 200)
+    F.Fp8Matmul(c0, s0, w, ws, torch.zeros(0, 8, device="cuda")).encode()
+    c, s = F.new_rows(5, 200)
+    F.Fp8Matmul(c, s, w[:0], torch.zeros(0, 2, device="cuda"), torch.zeros(5, 0, device="cuda")).encode()
+    F.Fp8GroupedMatmul(c0, s0, w[None], ws[None], torch.zeros(0, 8, device="cuda"), _ints([0, 0])).encode()
+    F.Fp8Quantize(torch.zeros(0, 200, device="cuda"), c0, s0).encode()
+    plan = F.ExpertPlan(torch.zeros(0, 2, dtype=torch.int32, device="cuda"), 3)
+    plan.group_start.fill_(-1)
+    plan.encode()
+    F.ExpertCombine(torch.zeros(0, 8, device="cuda"), torch.zeros(0, 2, dtype=torch.int32, device="cuda"), torch.zeros(0, 2, device="cuda"),
+                    torch.zeros(0, 8, device="cuda")).encode()
+    torch.cuda.synchronize()
+    assert plan.group_start.tolist() == [0, 0, 0, 0]
+
+
+def _far(F, shape):
+    """Codes of more than 4 GiB, and their values' rows as float64 on the device."""
+    c = torch.randint(0, 0x7f, shape, dtype=torch.uint8, device="cuda")
+    c[:, ::2] |= 0x80
+    return c, lambda rows: torch.from_numpy(R.VALUES).cuda()[c[rows].long()]
+
+
+@pytest.mark.parametrize("m", [3, 40])
+def test_matmul_places_past_32_bits(F, m):
+    """Weights of 5.4 GB: the first and the last columns, in each kernel."""
+    n, k = 41000, 131072
+    c, values = _far(F, (n, k))
+    a, sa = R.nearest(np.random.default_rng(1).normal(0, 110, (m, k))), np.full((m, k // 128), 1e-3, np.float32)
+    d = torch.zeros(m, n, device="cuda")
+    F.Fp8Matmul(_padded(a), _dev(sa), c, torch.full((R.blocks(n), k // 128), 1e-3, device="cuda"), d).encode()
+    torch.cuda.synchronize()
+    at = torch.tensor([0, 1, 20000, n - 33, n - 1], device="cuda")
+    x = torch.from_numpy(R.VALUES[a]).cuda()
+    scale = float(np.float32(1e-3)) ** 2
+    want, mag = x @ values(at).t() * scale, x.abs() @ values(at).abs().t() * scale
+    tol = R.bound(None, mag, 0, k, "f32")
+    assert ((d[:, at].double() - want).abs() <= tol + 2.0 ** -24 * want.abs()).all()
+
+
+def test_rows_past_32_bits(F):
+    """Rows of more than 4 GiB in and out of the quantizer, the products and the sums: the last ones."""
+    rows, k = 1100000, 4096
+    x = torch.zeros(rows, k, dtype=torch.bfloat16, device="cuda")
+    r = np.random.default_rng(2)
+    last = _held(r.normal(0, 1, (40, k)), "bf16")
+    x[-40:] = _dev(last, torch.bfloat16)
+    codes, scales = F.new_rows(rows, k)
+    F.Fp8Quantize(x, codes, scales).encode()
+    torch.cuda.synchronize()
+    want = R.quantize(last)
+    _check_codes((codes[-40:].view(torch.uint8).cpu().numpy(), scales[-40:].cpu().numpy()), want)
+    _, _, b, sb = _operands(r, 1, 4100, k)
+    d = torch.zeros(rows, 4100, dtype=torch.bfloat16, device="cuda")
+    F.Fp8Matmul(codes, scales, _padded(b), _dev(sb), d).encode()
+    torch.cuda.synchronize()
+    w, mag, cut = R.product(*want, b, sb)
+    _near(_np(d[-40:]), w, R.bound(w, mag, cut, k, "bf16"), "bf16")
+    out = torch.zeros(3, k, dtype=torch.bfloat16, device="cuda")
+    slots = np.array([[rows - 1, 0], [rows - 40, rows - 2], [5, rows]])
+    F.ExpertCombine(x, _ints(slots), _dev(np.ones((3, 2), np.float32)), out).encode()
+    torch.cuda.synchronize()
+    z = np.concatenate([last, np.zeros((1, k))])
+    s, m = R.combine(z, np.array([[39, 40], [0, 38], [40, 41]]), np.ones((3, 2)))
+    _near(_np(out), s, m * 3 * 2.0 ** -24, "bf16")
+
+
 def test_python_refusals(F, qmm):
     codes, scales = F.new_rows(4, 200)
     w, ws = F.new_rows(6, 200)
