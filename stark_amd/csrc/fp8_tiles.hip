@@ -139,27 +139,34 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
     };
     const auto compute = [&](int buf, uint32_t s) {
         const uint32_t in = (s - from) % kChunk, cb = (s - from) / kChunk & 1;
-        const float sb = lds.sb[cb][8 * (wn * (BN / WN) / kStep) + in];
-        Fp8Operand<EXACT> x[MT];
+        // A matrix instruction's result takes some twelve issue slots: each sum is scaled two instructions later, and the
+        // columns' codes are read two column blocks ahead. The order is held as it is written: the first instruction waits for its
+        // own operands only, the scales come last.
+        constexpr int D = 2, Q = MT * NT;
+        f32x4 v[D + 1];
+        Fp8Operand<EXACT> w[2], x[MT];
         float c[MT];
+        const auto columns = [&](int j) { return operand(lds.b[buf] + 8 * (wn * (BN / WN) + 16 * j)); };
+        w[0] = columns(0);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             x[i] = operand(lds.a[buf] + 8 * (wm * (BM / WM) + 16 * i));
-            c[i] = lds.sa[cb][8 * (wm * (BM / WM) + 16 * i) + 64 * (col >> 3) + 8 * in + (col & 7)] * sb;
+            if (!EXACT) __builtin_amdgcn_sched_barrier(0);
         }
-        // A matrix instruction's result takes some twelve issue slots: each sum is scaled two instructions later, and the
-        // columns' codes are read two column blocks ahead. The order is held as it is written.
-        constexpr int D = 2, Q = MT * NT;
-        f32x4 v[D + 1];
-        Fp8Operand<EXACT> w[2];
-        const auto columns = [&](int j) { return operand(lds.b[buf] + 8 * (wn * (BN / WN) + 16 * j)); };
-        w[0] = columns(0);
         if (NT > 1) w[1] = columns(1);
+        if (!EXACT) __builtin_amdgcn_sched_barrier(0);
+        const float sb = lds.sb[cb][8 * (wn * (BN / WN) / kStep) + in];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) c[i] = lds.sa[cb][8 * (wm * (BM / WM) + 16 * i) + 64 * (col >> 3) + 8 * in + (col & 7)];
         if (!EXACT) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int q = 0; q < Q + D; ++q) {
             if (q < Q) v[q % (D + 1)] = fp8_block(w[q / MT % 2], x[q % MT]);
             if (!EXACT) __builtin_amdgcn_sched_barrier(0);
+            if (q == D - 1) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) c[i] *= sb;
+            }
             if (q >= D) {
                 const int i = (q - D) % MT, j = (q - D) / MT;
 #pragma unroll
