@@ -44,9 +44,15 @@ QMM_DEVICE void load8(const void* x, uint64_t at, uint32_t c, uint32_t end, floa
 }
 
 // v * g / (1 + exp(-g)), the reciprocal to its last place; exp(-g) = 2^t with the product's rounding error carried into the result.
+// From -87 on 1 + exp(-g) nears f32's end, where its reciprocal is subnormal (v_rcp_f32 gives zero) and then exp(-g) infinite:
+// there the sigmoid is exp(g), as four equal factors, so that nothing but the product itself leaves the normal range.
 QMM_DEVICE float gate(float v, float g) {
     constexpr float kHi = 0x1.715476p+0f, kLo = 0x1.4ae0c0p-26f, kLn2 = 0x1.62e430p-1f;  // log2(e) in two parts
     const float t = -g * kHi, r = fmaf(-g, kLo, fmaf(-g, kHi, -t));
+    if (g < -87.0f) {
+        const float q = __builtin_amdgcn_exp2f(-0.25f * t);
+        return v * q * q * q * (g * q) * (t < 512.0f ? fmaf(-r, kLn2, 1.0f) : 1.0f);
+    }
     const float p = __builtin_amdgcn_exp2f(t), ex = fabsf(t) < 128.0f ? fmaf(p, r * kLn2, p) : p;
     return v * (g * __builtin_amdgcn_rcpf(1.0f + ex));
 }
