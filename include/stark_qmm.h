@@ -742,10 +742,10 @@ typedef struct stark_qmm_fp8_matmul_args {
 
 /* d[m, n] = ab_scale * sum over blocks of (a_scale * b_scale) * (sum of a * b in
  * the block), then the other d_ops in the order of stark_qmm_encode. The two
- * scales are multiplied first, in f32; sums are f32. Outputs of F16 and BF16 may
+ * scales are multiplied first, in f32; sums are f32. Outputs of BF16 may
  * come from matrix instructions that add eight neighbouring products at a time and
- * cut each off below 2^-13 of the largest one's binade (off by 1.5e-5 of their size
- * for normally distributed codes); F32 ones do not. Which kernel takes a call goes
+ * cut each off below 2^-13 of the largest one's binade (off by 1.5e-5 of the outputs'
+ * norm for normally distributed codes); F16 and F32 ones do not. Which kernel takes a call goes
  * by its sizes, and so do the last bits of its sums; a call repeated gives the same
  * bits. d may not overlap an input. */
 STARK_QMM_API stark_qmm_status stark_qmm_fp8_matmul(const stark_qmm_fp8_matmul_args* args, void* stream);

@@ -43,6 +43,7 @@ inline uint64_t fp8_span(uint64_t rows, uint64_t stride, uint64_t width) { retur
 inline bool fp8_launches(uint64_t groups, uint32_t threads) { return groups * threads < 1ull << 32; }
 inline bool fp8_aligned(const void* p, uint64_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 inline uint64_t fp8_element(uint32_t dt) { return dt == STARK_QMM_F32 ? 4 : 2; }
+inline bool fp8_exact(uint32_t d_dt) { return d_dt != STARK_QMM_BF16; }  // sums of f32 (Fp8Operand)
 inline bool fp8_type(uint32_t dt) { return dt == STARK_QMM_F32 || dt == STARK_QMM_F16 || dt == STARK_QMM_BF16; }
 
 // A 16 x 16 block of A B over 128 codes, from zero: lane l has row (column) l % 16 of A (B) and 32 of its codes (which 32 does
@@ -50,9 +51,9 @@ inline bool fp8_type(uint32_t dt) { return dt == STARK_QMM_F32 || dt == STARK_QM
 //
 // v_mfma_f32_16x16x128_f8f6f4 takes codes as they are. It adds products in groups of eight neighbouring codes, and what a
 // product has below 2^-13 of the largest product's binade in its group is cut off before the sum (measured; sums of groups are
-// f32): outputs of normally distributed codes are off by 1.5e-5 of their size, which one of 8 or 11 bits does not show
-// (1.7e-3 and 2e-4 by its own rounding). f32 outputs would: their codes are widened to bf16 first, exactly, and
-// v_mfma_f32_16x16x32_bf16 adds in f32 (1e-8), at half the rate.
+// f32): outputs of normally distributed codes are off by 1.5e-5 of the outputs' norm. bf16 outputs take it, whose own rounding is
+// off by 1.7e-3. f16 and f32 ones would show it (an f16 output of a tenth of the norm is rounded by 2e-5 of it): their codes are
+// widened to bf16 first, exactly, and v_mfma_f32_16x16x32_bf16 adds in f32 (1e-8), at half the rate.
 typedef __bf16 fp8_bf16x8 __attribute__((ext_vector_type(8)));
 template <bool EXACT>
 struct Fp8Operand {

@@ -48,7 +48,7 @@ stark_qmm_status check_sizes(const stark_qmm_fp8_matmul_args& q, const Groups& g
     return STARK_QMM_OK;
 }
 
-fp8::Choice choice(const Fp8Product& p, bool grouped) { return fp8::choose(p.m, p.n, p.k, p.experts, grouped, p.d_dt == STARK_QMM_F32); }
+fp8::Choice choice(const Fp8Product& p, bool grouped) { return fp8::choose(p.m, p.n, p.k, p.experts, grouped, fp8_exact(p.d_dt)); }
 
 // The parts' sums: rows of whole 16-byte pieces.
 uint64_t partial_stride(const Fp8Product& p) { return (p.n + 3ull) / 4 * 4; }

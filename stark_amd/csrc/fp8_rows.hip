@@ -156,7 +156,7 @@ stark_qmm_status launch(const Fp8Product& p, hipStream_t stream) {
     const uint64_t tiles = (uint64_t)fp8::row_tiles(p.m, p.experts, 16 * MT) * ((p.n + 16 * NT - 1) / (16 * NT));
     if (!fp8_launches(tiles, 64 * W)) return STARK_QMM_UNSUPPORTED;
     const dim3 grid((uint32_t)tiles), block(64 * W);
-    if (p.d_dt == STARK_QMM_F32) hipLaunchKernelGGL((fp8_rows<MT, NT, W, true>), grid, block, 0, stream, p);
+    if (fp8_exact(p.d_dt)) hipLaunchKernelGGL((fp8_rows<MT, NT, W, true>), grid, block, 0, stream, p);
     else hipLaunchKernelGGL((fp8_rows<MT, NT, W, false>), grid, block, 0, stream, p);
     QMM_HIP_CHECK(hipGetLastError());
     return STARK_QMM_OK;

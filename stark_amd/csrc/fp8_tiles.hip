@@ -231,7 +231,7 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
     }
     // Plain outputs of 16 bits: two lanes with neighbouring column quarters exchange halves, so that each stores eight columns.
     const uint32_t nw = n0 + wn * (BN / WN);
-    if (!EXACT && p.plain && NT % 2 == 0 && nw + BN / WN <= p.n) {
+    if (p.plain && NT % 2 == 0 && nw + BN / WN <= p.n) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             const uint32_t r = wm * (BM / WM) + 16 * i + col;
@@ -363,7 +363,7 @@ stark_qmm_status launch_size(const Fp8Product& p, uint32_t tile, hipStream_t str
 }  // namespace
 
 stark_qmm_status launch_fp8_tiles(const Fp8Product& p, uint32_t tile, hipStream_t stream) {
-    stark_qmm_status st = p.d_dt == STARK_QMM_F32 ? launch_size<true>(p, tile, stream) : launch_size<false>(p, tile, stream);
+    stark_qmm_status st = fp8_exact(p.d_dt) ? launch_size<true>(p, tile, stream) : launch_size<false>(p, tile, stream);
     if (st != STARK_QMM_OK || p.parts == 1) return st;
     hipLaunchKernelGGL(fp8_join, dim3((uint32_t)(((uint64_t)p.m * ((p.n + 3) / 4) + 255) / 256)), dim3(256), 0, stream, p);
     QMM_HIP_CHECK(hipGetLastError());

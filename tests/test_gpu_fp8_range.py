@@ -1,9 +1,10 @@
 """Operators of 8-bit floating-point codes on the GPU at the ends of their range, against the plain 64-bit forms of tests/fp8_ref.py."""
 import numpy as np
 import pytest
+import torch
 
 from tests import fp8_ref as R
-from tests.test_gpu_fp8 import F, _held, _quantize  # noqa: F401 (F is a fixture)
+from tests.test_gpu_fp8 import DT, F, _held, _ints, _np, _padded, _quantize  # noqa: F401 (F is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +40,49 @@ def test_quantize_gates_without_end(F):
     codes, scales = _quantize(F, x.astype(np.float32).astype(np.float64), "f32", gated=True)
     assert (R.VALUES[codes[:3]] == 0).all() and (scales[:3] == np.float32(R.SMALLEST_SCALE)).all()
     assert np.isnan(scales[3]).tolist() == [True, False] and (codes[3, :128] == 0).all()
+
+
+# ---------------------------------------------------------------- products
+
+def _whole(r, m, n, k):
+    """Codes of whole numbers with the scale 1: in each eight neighbours one product of 448 * 448, which the next eight take away,
+    and seven of -2 .. 2. Sums of any of a block's are whole and below 2^24 and the blocks' sums are small, so that sums in f32 are
+    exact in every order; the results stay below 2^11: exact in f16 too. (Products cut off below 2^-13 of a neighbour's would be
+    gone.)"""
+    a, b = np.ones((m, k)), r.integers(-2, 3, (n, k)).astype(np.float64)
+    large = np.arange(0, k, 8)
+    large = large[:large.size // 2 * 2]
+    a[:, large] = 448.0
+    b[:, large[0::2]], b[:, large[1::2]] = 448.0, -448.0
+    return a, b
+
+
+WHOLE = [(1, 300, 1024), (16, 96, 2048), (33, 96, 2048), (64, 1024, 8192), (300, 3000, 1160), (1500, 4100, 136), (2000, 4104, 512)]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("m,n,k", WHOLE)
+def test_sums_are_f32(F, dtype, m, n, k):
+    """Outputs of more bits than bf16's come from sums of f32, in every kernel."""
+    a, b = _whole(np.random.default_rng(m), m, n, k)
+    d = torch.full((m, n), 7.0, dtype=DT[dtype], device="cuda")
+    x = [_padded(R.nearest(a)), torch.ones(m, R.blocks(k), device="cuda"), _padded(R.nearest(b)), torch.ones(R.blocks(n), R.blocks(k), device="cuda")]
+    F.Fp8Matmul(*x, d).encode()
+    torch.cuda.synchronize()
+    assert np.array_equal(_np(d), a @ b.T)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("sizes,n,k", [([1, 2, 0, 9], 100, 1024), ([40, 7, 200], 1536, 272), ([900, 0, 1030, 513], 4100, 136)])
+def test_grouped_sums_are_f32(F, dtype, sizes, n, k):
+    r = np.random.default_rng(n)
+    m, experts = sum(sizes), len(sizes)
+    a, _ = _whole(r, m, 1, k)
+    b = np.stack([_whole(r, 1, n, k)[1] for _ in sizes])
+    start = np.concatenate([[0], np.cumsum(sizes)])
+    d = torch.full((m, n), 7.0, dtype=DT[dtype], device="cuda")
+    x = [_padded(R.nearest(a)), torch.ones(m, R.blocks(k), device="cuda"), _padded(R.nearest(b)),
+         torch.ones(experts, R.blocks(n), R.blocks(k), device="cuda")]
+    F.Fp8GroupedMatmul(*x, d, _ints(start)).encode()
+    torch.cuda.synchronize()
+    assert np.array_equal(_np(d), np.concatenate([a[start[e]:start[e + 1]] @ b[e].T for e in range(experts)]))
