@@ -44,17 +44,19 @@ QMM_DEVICE void load8(const void* x, uint64_t at, uint32_t c, uint32_t end, floa
 }
 
 // v * g / (1 + exp(-g)), the reciprocal to its last place; exp(-g) = 2^t with the product's rounding error carried into the result.
-// From -87 on 1 + exp(-g) nears f32's end, where its reciprocal is subnormal (v_rcp_f32 gives zero) and then exp(-g) infinite:
-// there the sigmoid is exp(g), as four equal factors, so that nothing but the product itself leaves the normal range.
+constexpr float kLog2e = 0x1.715476p+0f, kLog2eLow = 0x1.4ae0c0p-26f, kLn2 = 0x1.62e430p-1f;
 QMM_DEVICE float gate(float v, float g) {
-    constexpr float kHi = 0x1.715476p+0f, kLo = 0x1.4ae0c0p-26f, kLn2 = 0x1.62e430p-1f;  // log2(e) in two parts
-    const float t = -g * kHi, r = fmaf(-g, kLo, fmaf(-g, kHi, -t));
-    if (g < -87.0f) {
-        const float q = __builtin_amdgcn_exp2f(-0.25f * t);
-        return v * q * q * q * (g * q) * (t < 512.0f ? fmaf(-r, kLn2, 1.0f) : 1.0f);
-    }
+    const float t = -g * kLog2e, r = fmaf(-g, kLog2eLow, fmaf(-g, kLog2e, -t));
     const float p = __builtin_amdgcn_exp2f(t), ex = fabsf(t) < 128.0f ? fmaf(p, r * kLn2, p) : p;
     return v * (g * __builtin_amdgcn_rcpf(1.0f + ex));
+}
+
+// The same below kFarGate, where 1 + exp(-g) nears f32's end, its reciprocal is subnormal (v_rcp_f32 gives zero) and then exp(-g)
+// infinite: the sigmoid is exp(g), as four equal factors, so that nothing but the product itself leaves the normal range.
+constexpr float kFarGate = -87.0f;
+QMM_DEVICE float gate_far(float v, float g) {
+    const float t = g * kLog2e, r = fmaf(g, kLog2eLow, fmaf(g, kLog2e, -t)), q = __builtin_amdgcn_exp2f(0.25f * t);
+    return v * q * q * q * (g * q) * (t > -512.0f ? fmaf(r, kLn2, 1.0f) : 1.0f);
 }
 
 // e4m3 codes of x[0] / s and x[1] / s in the low 16 bits; i is within a few ulp of 1 / s. Where the quotient is so near the
@@ -94,8 +96,16 @@ __global__ __launch_bounds__(kThreads) void fp8_quantize(Quantize q) {
     if constexpr (GATED) {
         float g[8];
         load8<DT, VEC>(q.x, x_at + q.columns, c, q.columns, g);
+        float low = g[0];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = gate(v[e], g[e]);
+        for (int e = 0; e < 8; ++e) low = fminf(low, g[e]);
+        if (low < kFarGate) {  // (a branch around the eight: 65536 rows of 768 in bf16 47.9 us, with a choice for each value 49.4)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = g[e] < kFarGate ? gate_far(v[e], g[e]) : gate(v[e], g[e]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = gate(v[e], g[e]);
+        }
     }
     uint32_t top = 0;  // the largest magnitude's bits: those of a NaN are above an infinity's, and these above the rest
 #pragma unroll
