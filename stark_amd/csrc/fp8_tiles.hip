@@ -229,9 +229,10 @@ __device__ __forceinline__ void fp8_tile(const Fp8Product& p, TileLds<BM, BN, WM
         }
         return;
     }
-    // Plain outputs of 16 bits: two lanes with neighbouring column quarters exchange halves, so that each stores eight columns.
-    const uint32_t nw = n0 + wn * (BN / WN);
-    if (p.plain && NT % 2 == 0 && nw + BN / WN <= p.n) {
+    // Plain outputs of 16 bits: two lanes with neighbouring column quarters exchange halves, so that each stores eight columns. (A
+    // tile that ends past the last column takes the other way with all its waves: there is a barrier on it.)
+    if (p.plain && NT % 2 == 0 && n0 + BN <= p.n) {
+        const uint32_t nw = n0 + wn * (BN / WN);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
             const uint32_t r = wm * (BM / WM) + 16 * i + col;
