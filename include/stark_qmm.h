@@ -735,7 +735,8 @@ typedef struct stark_qmm_fp8_matmul_args {
     void* d;                     /* [m, n] */
     uint64_t d_row_stride;       /* elements */
     stark_qmm_d_ops d_ops;       /* bias in d_type; rht_factors: STARK_QMM_UNSUPPORTED_D_OP */
-    uint32_t m, n, k;            /* at most 2^24, 2^24 and 2^20; k at least 1 */
+    uint32_t m, n, k;            /* at most 2^24, 2^24 and 2^20; k at least 1; of 2^32 - 8 workgroups and more, which no
+                                  * m * n below 2^40 has: UNSUPPORTED */
     void* workspace;             /* device, 16-byte aligned, >= the size query's bytes */
     uint64_t workspace_size;     /* its contents do not survive the call; calls that may overlap need their own */
 } stark_qmm_fp8_matmul_args;

@@ -120,6 +120,18 @@ FP8_BOTH Choice choose(uint32_t m, uint32_t n, uint32_t k, uint32_t groups, bool
     return best;
 }
 
+// Workgroups of a call's product (without those of the join), and how many a call may have: 32 bits count them. No call whose m * n
+// is at most 2^40 has more.
+constexpr uint64_t kMostGroups = (1ull << 32) - 8;
+FP8_BOTH uint64_t workgroups(Choice c, uint32_t m, uint32_t n, uint32_t k, uint32_t groups) {
+    const uint32_t rows = row_tiles(m, groups, c.tile ? c.tile : c.rows);
+    const uint32_t columns = c.tile ? c.tile : c.rows == 32 ? 32 : 16 * row_share(rows, n, k).strips;
+    return (uint64_t)rows * ((n + columns - 1) / columns);
+}
+
+// A launch holds fewer than 2^32 threads; a call of more workgroups is several launches of whole eights of them.
+FP8_BOTH uint32_t launch_groups(uint32_t threads) { return 0xffffffffu / threads / 8 * 8; }
+
 // item / blocks by the inverse floor(2^32 / blocks) (0xffffffff for 1): the estimate is at most one short.
 struct Split {
     uint32_t row, block;

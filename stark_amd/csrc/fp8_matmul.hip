@@ -48,7 +48,11 @@ stark_qmm_status check_sizes(const stark_qmm_fp8_matmul_args& q, const Groups& g
     return STARK_QMM_OK;
 }
 
-fp8::Choice choice(const Fp8Product& p, bool grouped) { return fp8::choose(p.m, p.n, p.k, p.experts, grouped, fp8_exact(p.d_dt)); }
+// Which kernel takes a call of some outputs.
+stark_qmm_status choice(const Fp8Product& p, bool grouped, fp8::Choice* c) {
+    *c = fp8::choose(p.m, p.n, p.k, p.experts, grouped, fp8_exact(p.d_dt));
+    return fp8::workgroups(*c, p.m, p.n, p.k, p.experts) > fp8::kMostGroups ? STARK_QMM_UNSUPPORTED : STARK_QMM_OK;
+}
 
 // The parts' sums: rows of whole 16-byte pieces.
 uint64_t partial_stride(const Fp8Product& p) { return (p.n + 3ull) / 4 * 4; }
@@ -56,16 +60,21 @@ uint64_t workspace_of(const Fp8Product& p, fp8::Choice c) { return c.parts > 1 ?
 
 stark_qmm_status size_of(const stark_qmm_fp8_matmul_args& q, const Groups& g, bool grouped, uint64_t* bytes) {
     Fp8Product p{};
-    const stark_qmm_status st = check_sizes(q, g, &p);
-    if (st == STARK_QMM_OK) *bytes = p.m && p.n ? workspace_of(p, choice(p, grouped)) : 0;
+    fp8::Choice c{0, 16, 1};
+    stark_qmm_status st = check_sizes(q, g, &p);
+    if (st == STARK_QMM_OK && p.m && p.n) st = choice(p, grouped, &c);
+    if (st == STARK_QMM_OK) *bytes = workspace_of(p, c);
     return st;
 }
 
 stark_qmm_status run(const stark_qmm_fp8_matmul_args& q, const Groups& g, const int32_t* start, const int32_t* rows, hipStream_t stream) {
     Fp8Product p{};
-    const stark_qmm_status st = check_sizes(q, g, &p);
+    stark_qmm_status st = check_sizes(q, g, &p);
     if (st != STARK_QMM_OK) return st;
     if (q.m == 0 || q.n == 0) return STARK_QMM_OK;
+    fp8::Choice c;
+    st = choice(p, start != nullptr, &c);
+    if (st != STARK_QMM_OK) return st;
     const uint64_t e = fp8_element(q.d_type), wide = ((uint64_t)q.k + 15) / 16 * 16, kb = fp8::blocks(q.k), nb = fp8::blocks(q.n);
     if (!q.a || !q.a_scales || !q.b || !q.b_scales || !q.d) return STARK_QMM_INVALID_ARGUMENT;
     if (!fp8_aligned(q.a, 16) || !fp8_aligned(q.b, 16) || !fp8_aligned(q.a_scales, 4) || !fp8_aligned(q.b_scales, 4) ||
@@ -83,7 +92,6 @@ stark_qmm_status run(const stark_qmm_fp8_matmul_args& q, const Groups& g, const 
     p.group_start = start, p.a_rows = rows;
     p.vec = fp8_aligned(q.d, 4 * e) && p.d_stride % 4 == 0;
     p.plain = e == 2 && !p.flags && !p.bias && fp8_aligned(q.d, 16) && p.d_stride % 8 == 0;
-    const fp8::Choice c = choice(p, start != nullptr);
     p.parts = c.parts;
     const uint64_t need = workspace_of(p, c);
     if (need) {

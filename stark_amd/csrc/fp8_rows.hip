@@ -29,9 +29,10 @@ __global__ __launch_bounds__(64 * W) void fp8_rows(Fp8Product p) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t strips = (p.n + 16 * NT - 1) / (16 * NT), blocks = fp8::blocks(p.k);
     const uint32_t each = (blocks + W - 1) / W, b0 = min(wave * each, blocks), b1 = min(b0 + each, blocks);
-    const Fp8Tile t = Fp8Groups<16 * MT>(p).tile(p, blockIdx.x / strips);
+    const uint32_t group = p.first_group + blockIdx.x;
+    const Fp8Tile t = Fp8Groups<16 * MT>(p).tile(p, group / strips);
     if (!t.rows) return;
-    const uint32_t n0 = (blockIdx.x % strips) * 16 * NT;
+    const uint32_t n0 = (group % strips) * 16 * NT;
 
     uint32_t ar[MT];
 #pragma unroll
@@ -154,12 +155,10 @@ __global__ __launch_bounds__(64 * W) void fp8_rows(Fp8Product p) {
 template <int MT, int NT, int W>
 stark_qmm_status launch(const Fp8Product& p, hipStream_t stream) {
     const uint64_t tiles = (uint64_t)fp8::row_tiles(p.m, p.experts, 16 * MT) * ((p.n + 16 * NT - 1) / (16 * NT));
-    if (!fp8_launches(tiles, 64 * W)) return STARK_QMM_UNSUPPORTED;
-    const dim3 grid((uint32_t)tiles), block(64 * W);
-    if (fp8_exact(p.d_dt)) hipLaunchKernelGGL((fp8_rows<MT, NT, W, true>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL((fp8_rows<MT, NT, W, false>), grid, block, 0, stream, p);
-    QMM_HIP_CHECK(hipGetLastError());
-    return STARK_QMM_OK;
+    return fp8_launch(p, tiles, 64 * W, [&](const Fp8Product& part, uint32_t groups) {
+        if (fp8_exact(p.d_dt)) hipLaunchKernelGGL((fp8_rows<MT, NT, W, true>), dim3(groups), dim3(64 * W), 0, stream, part);
+        else hipLaunchKernelGGL((fp8_rows<MT, NT, W, false>), dim3(groups), dim3(64 * W), 0, stream, part);
+    });
 }
 
 template <int NT>

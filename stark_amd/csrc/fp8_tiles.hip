@@ -329,7 +329,7 @@ __global__ __launch_bounds__(64 * WM * WN) void fp8_tiles(Fp8Product p) {
     __shared__ TileLds<BM, BN, WM * WN, S> lds;
     const uint32_t columns = (p.n + BN - 1) / BN;
     const Fp8Groups<BM> groups(p);
-    const fp8::Place at = fp8::place(fp8::tile_of(blockIdx.x, groups.total * columns), groups.total, columns);
+    const fp8::Place at = fp8::place(fp8::tile_of(p.first_group + blockIdx.x, groups.total * columns), groups.total, columns);
     const Fp8Tile rows = groups.tile(p, at.row);
     if (rows.rows) fp8_tile<BM, BN, WM, WN, S, EXACT>(p, lds, rows, at.column * BN, blockIdx.y);
 }
@@ -347,10 +347,9 @@ __global__ __launch_bounds__(256) void fp8_join(Fp8Product p) {
 template <int BM, int BN, int WM, int WN, int S, bool EXACT>
 stark_qmm_status launch(const Fp8Product& p, hipStream_t stream) {
     const uint64_t tiles = (uint64_t)fp8::row_tiles(p.m, p.experts, BM) * ((p.n + BN - 1) / BN);
-    if (!fp8_launches(tiles + 7, 64 * WM * WN)) return STARK_QMM_UNSUPPORTED;
-    hipLaunchKernelGGL((fp8_tiles<BM, BN, WM, WN, S, EXACT>), dim3((uint32_t)((tiles + 7) / 8 * 8), p.parts), dim3(64 * WM * WN), 0, stream, p);
-    QMM_HIP_CHECK(hipGetLastError());
-    return STARK_QMM_OK;
+    return fp8_launch(p, (tiles + 7) / 8 * 8, 64 * WM * WN, [&](const Fp8Product& part, uint32_t groups) {
+        hipLaunchKernelGGL((fp8_tiles<BM, BN, WM, WN, S, EXACT>), dim3(groups, p.parts), dim3(64 * WM * WN), 0, stream, part);
+    });
 }
 
 template <bool EXACT>

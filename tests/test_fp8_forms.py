@@ -1,10 +1,15 @@
 """The rules that choose a kernel (csrc/fp8_layout.h, compiled for the CPU) against the forms that the GPU tests name."""
 import ctypes as C
+import functools
+import os
+import random
+import subprocess
+import tempfile
 
 import pytest
 
 from tests import fp8_forms as K
-from tests.test_fp8_layout import _choose, _pair, rules
+from tests.test_fp8_layout import CSRC, PRODUCT, _choose, _pair, _struct, rules
 
 
 def form(m, n, k, groups=1, grouped=False, exact=False):
@@ -28,3 +33,56 @@ def held(want, exact):
 @pytest.mark.parametrize("size,want", K.CUT_TILES)
 def test_cut_tiles(size, want, exact):
     assert form(*size, exact=exact) == held(want, exact)
+
+
+_COUNT = """
+#include "fp8_layout.h"
+extern "C" uint64_t workgroups(uint32_t m, uint32_t n, uint32_t k, uint32_t groups, int grouped, int exact) {
+    return fp8::workgroups(fp8::choose(m, n, k, groups, grouped, exact), m, n, k, groups);
+}
+extern "C" uint32_t launch_groups(uint32_t threads) { return fp8::launch_groups(threads); }
+"""
+
+
+@functools.lru_cache(None)
+def _counts():
+    with tempfile.TemporaryDirectory() as d:
+        src, lib = os.path.join(d, "count.cpp"), os.path.join(d, "count.so")
+        with open(src, "w") as f:
+            f.write(_COUNT)
+        subprocess.run(["g++", "-std=c++17", "-O1", "-shared", "-fPIC", "-I", CSRC, src, "-o", lib], check=True)
+        L = C.CDLL(lib)
+        L.workgroups.restype = C.c_uint64
+        return L
+
+
+def test_launches_hold_every_call():
+    """Workgroups of a call of at most 2^40 outputs are counted by 32 bits, those of a launch have fewer than 2^32 threads, and the
+    sums of parts one thread for four."""
+    L, r = _counts(), random.Random(2)
+    sizes = [(2 ** 22, 4096, 64, 1, False), (2 ** 24, 2 ** 16, 100, 1, False), (2 ** 16, 2 ** 24, 1, 1024, True), (2 ** 20, 2 ** 20, 2 ** 20, 1, False)]
+    while len(sizes) < 3000:
+        m, n, k = (int(2 ** r.uniform(0, e)) for e in (24, 24, 20))
+        grouped = r.random() < 0.5
+        if m * n <= 2 ** 40:
+            sizes.append((m, n, k, int(2 ** r.uniform(0, 10)) if grouped else 1, grouped))
+    for m, n, k, groups, grouped in sizes:
+        for exact in (False, True):
+            assert 0 < L.workgroups(m, n, k, groups, int(grouped), int(exact)) <= 2 ** 32 - 8
+            parts = _choose(m, n, k, groups, grouped, exact)[2]
+            assert parts == 1 or m * -(-n // 4) + 255 < 2 ** 32
+    for threads in (128, 256, 512, 1024):
+        each = L.launch_groups(threads)
+        assert each % 8 == 0 and 2 ** 32 - 16 * threads < each * threads < 2 ** 32
+
+
+def test_calls_of_too_many_workgroups_are_refused():
+    """By the size query too."""
+    from stark_amd import fp8 as P, qmm as Q
+    lib, n = Q.lib(), C.c_uint64(77)
+    size = dict(m=2 ** 24, n=2 ** 24, d_row_stride=2 ** 24)
+    call = C.byref(_struct(P._MatmulArgs, PRODUCT, size))
+    assert lib.stark_qmm_fp8_matmul_workspace_size(call, C.byref(n)) == lib.stark_qmm_fp8_matmul(call, None) == Q.UNSUPPORTED
+    # 34 GB of outputs in the few-rows kernel: more threads than a launch holds
+    ok = C.byref(_struct(P._MatmulArgs, PRODUCT, dict(m=2 ** 22, n=4096, k=64, d_row_stride=4096)))
+    assert lib.stark_qmm_fp8_matmul_workspace_size(ok, C.byref(n)) == Q.OK and n.value == 0

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests import fp8_ref as R
-from tests.test_gpu_fp8 import DT, F, _held, _ints, _np, _padded, _quantize  # noqa: F401 (F is a fixture)
+from tests.test_gpu_fp8 import DT, F, _dev, _held, _ints, _near, _np, _padded, _quantize  # noqa: F401 (F is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +86,20 @@ def test_grouped_sums_are_f32(F, dtype, sizes, n, k):
     F.Fp8GroupedMatmul(*x, d, _ints(start)).encode()
     torch.cuda.synchronize()
     assert np.array_equal(_np(d), np.concatenate([a[start[e]:start[e + 1]] @ b[e].T for e in range(experts)]))
+
+
+def test_more_workgroups_than_a_launch_holds(F):
+    """2^22 rows, N 4096, K 64: 2^24 workgroups of 256 threads, in two launches. Rows on both sides of where the second one
+    begins (the last row tile), and no row left out."""
+    m, n, k = 2 ** 22, 4096, 64
+    r = np.random.default_rng(5)
+    a = torch.randint(0, 0x7f, (m, k), dtype=torch.uint8, device="cuda")
+    sa = torch.rand(m, 1, device="cuda") + 0.5
+    b, sb = R.nearest(r.normal(0, 110, (n, k))), r.random((32, 1)).astype(np.float32)
+    d = torch.full((m, n), 7.0, dtype=torch.bfloat16, device="cuda")
+    F.Fp8Matmul(a, sa, _padded(b), _dev(sb), d).encode()
+    torch.cuda.synchronize()
+    assert not any((part == 7).all(1).any() for part in d.split(m // 16))
+    at = torch.tensor([0, 1, 2 ** 21, m - 65, m - 33, m - 32, m - 31, m - 1], device="cuda")
+    want, mag, cut = R.product(a[at].cpu().numpy(), sa[at].cpu().numpy(), b, sb)
+    _near(_np(d[at]), want, R.bound(want, mag, cut, k, "bf16"), "bf16")
