@@ -710,7 +710,7 @@ typedef struct stark_qmm_fp8_quantize_args {
     uint64_t code_row_stride;    /* bytes, a multiple of 16 */
     float* scales;               /* [rows, ceil(columns / 128)] */
     uint64_t scale_row_stride, scale_block_stride; /* elements */
-    uint32_t rows, columns;      /* at most 2^24 and 2^20; of 2^28 blocks and more in all: UNSUPPORTED */
+    uint32_t rows, columns;      /* at most 2^24 and 2^20; of more than 2^28 - 16 blocks in all: UNSUPPORTED */
     uint32_t gated;              /* x = value * gate / (1 + exp(-gate)), in f32, off by 2^-20 of itself at most */
     const int32_t* row_count;    /* device: rows from here on stay as they were (at most `rows`), or NULL */
 } stark_qmm_fp8_quantize_args;

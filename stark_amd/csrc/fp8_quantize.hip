@@ -153,7 +153,8 @@ extern "C" stark_qmm_status stark_qmm_fp8_quantize(const stark_qmm_fp8_quantize_
     if (a->rows == 0 || a->columns == 0) return STARK_QMM_OK;
     const uint64_t e = fp8_element(a->data_type), wide = (uint64_t)a->columns * (a->gated ? 2 : 1), rows = a->rows;
     const uint32_t blocks = fp8::blocks(a->columns);
-    if (rows * blocks >= 1ull << 28) return STARK_QMM_UNSUPPORTED;  // 32 bits of threads in a launch, sixteen to a block
+    // a launch has fewer than 2^32 threads, whole workgroups of them: sixteen blocks each
+    if (rows * blocks > (1ull << 28) - kThreads / kLanes) return STARK_QMM_UNSUPPORTED;
     if (!a->x || !a->codes || !a->scales || !fp8_aligned(a->x, e) || !fp8_aligned(a->codes, 16) || !fp8_aligned(a->scales, 4) ||
         !fp8_aligned(a->row_count, 4))
         return STARK_QMM_INVALID_ARGUMENT;

@@ -9,7 +9,7 @@ import tempfile
 import pytest
 
 from tests import fp8_forms as K
-from tests.test_fp8_layout import CSRC, PRODUCT, _choose, _pair, _struct, rules
+from tests.test_fp8_layout import CSRC, PRODUCT, QUANTIZE, _choose, _pair, _struct, rules
 
 
 def form(m, n, k, groups=1, grouped=False, exact=False):
@@ -86,3 +86,15 @@ def test_calls_of_too_many_workgroups_are_refused():
     # 34 GB of outputs in the few-rows kernel: more threads than a launch holds
     ok = C.byref(_struct(P._MatmulArgs, PRODUCT, dict(m=2 ** 22, n=4096, k=64, d_row_stride=4096)))
     assert lib.stark_qmm_fp8_matmul_workspace_size(ok, C.byref(n)) == Q.OK and n.value == 0
+
+
+def test_a_quantizer_launch_holds_its_blocks():
+    """2^28 - 1 blocks have 2^32 threads in whole workgroups."""
+    from stark_amd import fp8 as P, qmm as Q
+
+    def go(rows, columns):
+        return Q.lib().stark_qmm_fp8_quantize(C.byref(_struct(P._QuantizeArgs, QUANTIZE, dict(rows=rows, columns=columns, x=None))), None)
+
+    assert 49155 * 5461 == 2 ** 28 - 1 and 2 ** 12 * (2 ** 16 - 1) < 2 ** 28 - 16
+    assert go(49155, 5461 * 128) == Q.UNSUPPORTED
+    assert go(2 ** 16 - 1, 2 ** 12 * 128) == Q.INVALID_ARGUMENT  # no x
