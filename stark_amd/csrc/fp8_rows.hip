@@ -161,20 +161,16 @@ stark_qmm_status launch(const Fp8Product& p, hipStream_t stream) {
     });
 }
 
-template <int NT>
-stark_qmm_status launch_waves(const Fp8Product& p, uint32_t waves, hipStream_t stream) {
-    if (waves <= 2) return launch<1, NT, 2>(p, stream);
-    if (waves <= 4) return launch<1, NT, 4>(p, stream);
-    return waves <= 8 ? launch<1, NT, 8>(p, stream) : launch<1, NT, 16>(p, stream);
-}
-
 }  // namespace
 
 stark_qmm_status launch_fp8_rows(const Fp8Product& p, uint32_t rows, hipStream_t stream) {
     const uint64_t tiles = fp8::row_tiles(p.m, p.experts, rows);
     if (rows == 32) return tiles * ((p.n + 31) / 32) < 256 ? launch<2, 2, 8>(p, stream) : launch<2, 2, 4>(p, stream);
     const fp8::RowShare s = fp8::row_share(tiles, p.n, p.k);
-    return s.strips == 1 ? launch_waves<1>(p, s.waves, stream) : launch_waves<2>(p, s.waves, stream);
+    if (s.strips == 2) return launch<1, 2, 4>(p, stream);
+    if (s.waves <= 2) return launch<1, 1, 2>(p, stream);
+    if (s.waves <= 4) return launch<1, 1, 4>(p, stream);
+    return s.waves <= 8 ? launch<1, 1, 8>(p, stream) : launch<1, 1, 16>(p, stream);
 }
 
 }  // namespace qmm

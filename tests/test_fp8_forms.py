@@ -98,3 +98,11 @@ def test_a_quantizer_launch_holds_its_blocks():
     assert 49155 * 5461 == 2 ** 28 - 1 and 2 ** 12 * (2 ** 16 - 1) < 2 ** 28 - 16
     assert go(49155, 5461 * 128) == Q.UNSUPPORTED
     assert go(2 ** 16 - 1, 2 ** 12 * 128) == Q.INVALID_ARGUMENT  # no x
+
+
+def test_row_shares_are_the_kernels_there_are():
+    """Two strips with four waves, one with 2, 4, 8 or 16."""
+    r, L = random.Random(7), rules()
+    L.row_share.argtypes = [C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p]
+    seen = {_pair(L.row_share, int(2 ** r.uniform(0, 20)), int(2 ** r.uniform(0, 24)), int(2 ** r.uniform(0, 20))) for _ in range(20000)}
+    assert seen == {(2, 4), (1, 2), (1, 4), (1, 8), (1, 16)}
