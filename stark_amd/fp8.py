@@ -14,8 +14,8 @@ whose 8-bit weights are integers), and what routed experts need around them:
 Codes are torch.float8_e4m3fn or uint8 tensors whose rows start on 16-byte boundaries, scales float32: one for each row and
 128 values of activations, one for each 128 x 128 values of weights. Arguments are marshalled once, when an operator is made:
 it keeps the tensors it was given, and every encode() reads what they hold then. encode() is asynchronous on its stream (the
-current one by default) and may be captured in a graph. Tensors are GPU tensors; errors are MatmulError with the library's
-status.
+current one by default) and may be captured in a graph. An operator outlives the graphs that hold its calls, and its calls on a
+stream that is given as a bare handle. Tensors are GPU tensors; errors are MatmulError with the library's status.
 """
 from __future__ import annotations
 
@@ -153,6 +153,7 @@ class _Product(_Operator):
         self.workspace_bytes = need.value
         if workspace is None and need.value:
             workspace = torch.empty(need.value, dtype=torch.uint8, device=self.device)
+            self._make(workspace)
         if workspace is not None:
             product.workspace, product.workspace_size = Q._ptr(workspace), Q._nbytes(workspace)
         self.workspace = workspace
@@ -219,6 +220,7 @@ class ExpertPlan(_Operator):
         self.group_start, self.tokens, self.slots = new(experts + 1), new(ids.numel()), new(*ids.shape)
         self.count = self.group_start[experts:]
         self._keep(ids, self.group_start, self.tokens, self.slots, workspace)
+        self._make(self.group_start, self.tokens, self.slots)
         s = _PlanArgs()
         s.struct_size = C.sizeof(s)
         s.ids, s.group_start, s.tokens_out, s.slots = (Q._ptr(t) for t in (ids, self.group_start, self.tokens, self.slots))
@@ -228,6 +230,7 @@ class ExpertPlan(_Operator):
         self.workspace_bytes = need.value
         if workspace is None and need.value:
             workspace = torch.empty(need.value, dtype=torch.uint8, device=ids.device)
+            self._make(workspace)
         if workspace is not None:
             s.workspace, s.workspace_size = Q._ptr(workspace), Q._nbytes(workspace)
         self.workspace = workspace

@@ -8,7 +8,8 @@ caches hold 16-bit rows of one session): the calls of a serving loop's step.
 
 Arguments are marshalled once, when an operator is made: it keeps the tensors it was given, and every encode() reads
 what they hold then. encode() is asynchronous on its stream (the current one by default) and may be captured in a
-graph. Tensors are GPU tensors; errors are MatmulError with the library's status.
+graph. An operator outlives the graphs that hold its calls, and its calls on a stream that is given as a bare handle.
+Tensors are GPU tensors; errors are MatmulError with the library's status.
 """
 from __future__ import annotations
 
@@ -105,6 +106,11 @@ class _Operator:
         devices = {t.device for t in self._tensors}
         _require(len(devices) == 1, f"{type(self).__name__}: tensors on {sorted(map(str, devices))}")
         self.device = devices.pop()
+        self._made, self._streams = [], {_current_stream(self.device.index)}
+
+    def _make(self, *tensors):
+        """Tensors that the operator made itself: dropped with it, their memory waits for the streams that it was called on."""
+        self._made += [t for t in tensors if t is not None]
 
     def _begin(self, args):
         args.struct_size = C.sizeof(args)
@@ -115,13 +121,26 @@ class _Operator:
 
     def encode(self, stream=None) -> None:
         # (torch's own accessors of the current device and stream without their wrappers: 2 us less a call)
+        handle = _current_stream(self._index) if stream is None else Q._stream(stream)
         if _current_device() == self._index:
-            status = self._call(self._address, _current_stream(self._index) if stream is None else Q._stream(stream))
+            status = self._call(self._address, handle)
         else:
             with torch.cuda.device(self.device):
-                status = self._call(self._address, _current_stream(self._index) if stream is None else Q._stream(stream))
+                status = self._call(self._address, handle)
+        if handle not in self._streams:
+            self._follow(stream, handle)
         if status != Q.OK:
             raise Q.MatmulError(status, type(self).__name__)
+
+    def _follow(self, stream, handle) -> None:
+        """The first call on a stream: torch's allocator keeps what the operator made until that stream is done with it. (Of a
+        stream that is a bare handle torch knows nothing, its life included.)"""
+        self._streams.add(handle)
+        if stream is None:
+            stream = torch.cuda.current_stream(self.device)
+        if isinstance(stream, torch.cuda.Stream):
+            for t in self._made:
+                t.record_stream(stream)
 
 
 class KvCache:
@@ -158,6 +177,7 @@ class KvPlan(_Operator):
         self.free_left, self.status = new(1), new(1)
         self._keep(cached, added, free_pages, free_count, block_table, self.query_start, self.kv_lengths, self.slots,
                    self.positions, self.free_left, self.status)
+        self._make(self.query_start, self.kv_lengths, self.slots, self.positions, self.free_left, self.status)
         s = _PlanArgs()
         s.cached, s.added = Q._ptr(_ints(cached, batch, "cached")), Q._ptr(_ints(added, batch, "added"))
         s.free_pages = Q._ptr(_ints(free_pages, 0, "free_pages"))
@@ -274,6 +294,7 @@ class KvAttention(_Operator):
         self.workspace_bytes = need.value
         if workspace is None and need.value:
             workspace = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+            self._make(workspace)
         if workspace is not None:
             s.workspace, s.workspace_size = Q._ptr(workspace), Q._nbytes(workspace)
         self.workspace = workspace
