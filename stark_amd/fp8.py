@@ -76,8 +76,14 @@ def new_rows(rows: int, columns: int, device="cuda") -> Tuple[torch.Tensor, torc
     return codes, torch.zeros(rows, blocks(columns), dtype=torch.float32, device=device)
 
 
+def _counts(what: str, *n: int):
+    """Sizes that the library's 32 bits hold (its own limits are lower; ctypes would cut what is above)."""
+    _require(all(0 <= x < 1 << 32 for x in n), f"{what}: {n} are no sizes")
+
+
 def _matrix(t: torch.Tensor, rows: int, columns: int, what: str):
     """Pointer and row stride of [rows, columns] whose rows are contiguous."""
+    _counts(what, rows, columns)
     _require(tuple(t.shape) == (rows, columns), f"{what}: {tuple(t.shape)} is not {(rows, columns)}")
     _require(columns <= 1 or t.stride(1) == 1 or t.numel() == 0, f"{what}: the values of a row must be contiguous")
     return Q._ptr(t), t.stride(0) if rows > 1 else columns
@@ -190,6 +196,7 @@ class Fp8GroupedMatmul(_Product):
         _require(bias is None or (bias.dim() == 2 and bias.shape[0] == b.shape[0]), "bias: [experts, n]")
         self._keep(a, a_scales, b, b_scales, d, group_start, a_rows, bias, workspace)
         _codes(b, "b")
+        _counts("experts", b.shape[0])
         s, m = _GroupedArgs(), d.shape[0]
         s.product = self._product(a, a_scales, b[0], b_scales[0], d, m, a.shape[0] if a_rows is not None else m,
                                   None if bias is None else bias[0], ab_scale, accumulate, soft_cap)
@@ -213,6 +220,7 @@ class ExpertPlan(_Operator):
     def __init__(self, ids: torch.Tensor, experts: int, first: int = 0, workspace: Optional[torch.Tensor] = None):
         _require(ids.dim() == 2 and ids.dtype == torch.int32 and ids.is_contiguous(), "ids: int32 [tokens, active], contiguous")
         _require(experts >= 1 and first >= 0, "experts: 1 or more, from 0 on")
+        _counts("ids, experts and the first", *ids.shape, experts, first)
 
         def new(*n):
             return torch.empty(*n, dtype=torch.int32, device=ids.device)
@@ -245,6 +253,7 @@ class ExpertCombine(_Operator):
     def __init__(self, x: torch.Tensor, slots: torch.Tensor, weights: torch.Tensor, out: torch.Tensor, accumulate: bool = False):
         _require(x.dim() == 2 and out.dim() == 2 and slots.dim() == 2, "x, out, slots: two axes")
         (tokens, active), (rows, width) = slots.shape, x.shape
+        _counts("slots", tokens, active)
         self._keep(x, slots, weights, out)
         _require(x.dtype == out.dtype, "x and out are of one type")
         _require(weights.dtype == torch.float32 and weights.is_contiguous() and weights.numel() == tokens * active,

@@ -103,3 +103,20 @@ def test_more_workgroups_than_a_launch_holds(F):
     at = torch.tensor([0, 1, 2 ** 21, m - 65, m - 33, m - 32, m - 31, m - 1], device="cuda")
     want, mag, cut = R.product(a[at].cpu().numpy(), sa[at].cpu().numpy(), b, sb)
     _near(_np(d[at]), want, R.bound(want, mag, cut, k, "bf16"), "bf16")
+
+
+def test_sizes_past_32_bits_are_refused(F, qmm):
+    """One row seen 2^32 + 1 times is no call of one row."""
+    many = 2 ** 32 + 1
+    codes, scales = F.new_rows(1, 16)
+    row = torch.zeros(1, 16, device="cuda")
+    for call in (lambda: F.Fp8Quantize(row.expand(many, 16), codes.expand(many, 16), scales.expand(many, 1)),
+                 lambda: F.Fp8Matmul(codes, scales, codes.expand(many, 16), scales.expand(many // 128 + 1, 1), torch.zeros(1, 1, device="cuda").expand(1, many)),
+                 lambda: F.Fp8Matmul(codes.expand(many, 16), scales.expand(many, 1), codes, scales, torch.zeros(1, 1, device="cuda").expand(many, 1)),
+                 lambda: F.Fp8GroupedMatmul(codes.expand(many, 16), scales.expand(many, 1), codes[None], scales[None],
+                                            torch.zeros(1, 1, device="cuda"), _ints([0, 1]), a_rows=_ints([0])),
+                 lambda: F.ExpertPlan(_ints([[0]]), 1, 2 ** 32),
+                 lambda: F.ExpertPlan(_ints([[0]]), 2 ** 32 + 1)):
+        with pytest.raises(qmm.MatmulError) as e:
+            call()
+        assert e.value.status == qmm.INVALID_ARGUMENT
