@@ -106,3 +106,15 @@ def test_row_shares_are_the_kernels_there_are():
     L.row_share.argtypes = [C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p]
     seen = {_pair(L.row_share, int(2 ** r.uniform(0, 20)), int(2 ** r.uniform(0, 24)), int(2 ** r.uniform(0, 20))) for _ in range(20000)}
     assert seen == {(2, 4), (1, 2), (1, 4), (1, 8), (1, 16)}
+
+
+@pytest.mark.parametrize("exact", [False, True])
+def test_calls_named_by_their_kernel(exact):
+    for size, want in K.ROWS:
+        assert form(*size, exact=exact) == want
+    for sizes, n, k, want in K.GROUPED:
+        assert form(sum(sizes) + K.AROUND, n, k, len(sizes), True, exact) == held(want, exact)
+    for tokens, active, _, experts, n, k, want in K.SHARES:
+        assert form(tokens * active, n, k, experts, True, exact) == held(want, exact)
+    for size, want in K.CUT_TILES:  # one group of all rows
+        assert form(*size, 1, True, exact) == held(want, exact)
