@@ -96,10 +96,10 @@ __global__ __launch_bounds__(kThreads) void fp8_quantize(Quantize q) {
     if constexpr (GATED) {
         float g[8];
         load8<DT, VEC>(q.x, x_at + q.columns, c, q.columns, g);
-        float low = g[0];
+        uint32_t low = 0;  // the lowest gate's bits: those of negative values are above the others', and the higher the lower the value
 #pragma unroll
-        for (int e = 0; e < 8; ++e) low = fminf(low, g[e]);
-        if (low < kFarGate) {  // (a branch around the eight: 65536 rows of 768 in bf16 47.9 us, with a choice for each value 49.4)
+        for (int e = 0; e < 8; ++e) low = max(low, __float_as_uint(g[e]));
+        if (low > __float_as_uint(kFarGate)) {  // (a branch around the eight: 65536 rows of 768 in bf16 48.9 us, with a choice for each value 50.6)
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = g[e] < kFarGate ? gate_far(v[e], g[e]) : gate(v[e], g[e]);
         } else {
