@@ -5,7 +5,7 @@ whose 8-bit weights are integers), and what routed experts need around them:
     quantize = Fp8Quantize(x, codes, scales)
     product = Fp8Matmul(codes, scales, weights, weight_scales, y)
 
-    plan = ExpertPlan(ids, experts)                                                          # routed experts
+    plan = ExpertPlan(ids.view(tokens, active), experts)                                     # routed experts
     up = Fp8GroupedMatmul(codes, scales, up_w, up_s, h, plan.group_start, a_rows=plan.tokens)
     gate = Fp8Quantize(h, h_codes, h_scales, gated=True, row_count=plan.count)
     down = Fp8GroupedMatmul(h_codes, h_scales, down_w, down_s, r, plan.group_start)
@@ -212,7 +212,7 @@ class Fp8GroupedMatmul(_Product):
 
 
 class ExpertPlan(_Operator):
-    """stark_qmm_expert_plan: routes ids [tokens, active] (int32, as moe_route writes them) in the order of the experts
+    """stark_qmm_expert_plan: routes ids [tokens, active] (int32; moe_route's, which are flat, as a view) in the order of the experts
     first .. first + experts - 1. group_start [experts + 1], tokens [tokens * active] (-1 behind the last) and slots [tokens,
     active] (-1: another's expert) are made here and rewritten by every encode(); count is group_start's last."""
     _entry = "stark_qmm_expert_plan"
