@@ -135,10 +135,10 @@ class _Operator:
     def _follow(self, stream, handle) -> None:
         """The first call on a stream: torch's allocator keeps what the operator made until that stream is done with it. (Of a
         stream that is a bare handle torch knows nothing, its life included.)"""
-        self._streams.add(handle)
         if stream is None:
             stream = torch.cuda.current_stream(self.device)
         if isinstance(stream, torch.cuda.Stream):
+            self._streams.add(handle)
             for t in self._made:
                 t.record_stream(stream)
 

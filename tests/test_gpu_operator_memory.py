@@ -60,7 +60,7 @@ def _meets(places, busy=lambda: True):
     return any(p < q + m and q < p + n for p, n in places for q, m in _ranges(got[:counted]))
 
 
-@pytest.mark.parametrize("how", ["given", "current"])
+@pytest.mark.parametrize("how", ["given", "current", "handle first"])
 @pytest.mark.parametrize("make", [_product, _plan, _attention, _kv_plan])
 def test_memory_waits_for_the_stream(F, make, how):
     """The call waits behind some tens of ms of other work on its stream; what is allocated meanwhile is not the operator's memory."""
@@ -78,7 +78,9 @@ def test_memory_waits_for_the_stream(F, make, how):
             torch.mm(x, x, out=y)
         if how == "current":
             op.encode()
-    if how == "given":
+    if how == "handle first":  # of which torch knows nothing
+        op.encode(stream=side.cuda_stream)
+    if how != "current":
         op.encode(stream=side)
     del op, made
     assert not _meets(places, lambda: not side.query())
