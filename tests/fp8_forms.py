@@ -12,6 +12,9 @@ ROWS = [((20, 200, 640), (16, 1, 2)), ((16, 256, 4096), (16, 1, 4)), ((6, 2000, 
         ((1, 40, 8192), (16, 1, 8)), ((1, 70000, 128), (16, 2, 4)), ((12, 66000, 200), (16, 2, 4)), ((17, 5000, 384), (32, 2, 8)),
         ((32, 9000, 300), (32, 2, 4))]
 
+# (m, n, k) -> form: the inner axis in parts
+PARTS = [((64, 1024, 8192), (64, 8)), ((70, 1001, 6000), (64, 8)), ((130, 2000, 3000), (64, 4))]
+
 # (rows of each expert, n, k) -> form, with AROUND rows of d more that no expert has
 AROUND = 42
 GROUPED = [([1, 2, 0, 3] * 32, 1100, 384, (16, 2, 4)), ([9, 20, 30, 1] * 8, 600, 384, (32, 2, 4)), ([33, 0, 70, 1] * 16, 1000, 384, (64, 1)),

@@ -110,7 +110,7 @@ def test_row_shares_are_the_kernels_there_are():
 
 @pytest.mark.parametrize("exact", [False, True])
 def test_calls_named_by_their_kernel(exact):
-    for size, want in K.ROWS:
+    for size, want in K.ROWS + K.PARTS:
         assert form(*size, exact=exact) == want
     for sizes, n, k, want in K.GROUPED:
         assert form(sum(sizes) + K.AROUND, n, k, len(sizes), True, exact) == held(want, exact)

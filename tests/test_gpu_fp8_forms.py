@@ -65,7 +65,7 @@ def _d(r, m, n, dtype, before, gap):
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("ab,accumulate,bias,cap,before,gap", EPILOGUES)
-@pytest.mark.parametrize("size,want", K.CUT_TILES + K.ROWS)
+@pytest.mark.parametrize("size,want", K.CUT_TILES + K.ROWS + K.PARTS)
 def test_epilogues(F, dtype, size, want, ab, accumulate, bias, cap, before, gap):
     """The d_ops in every kernel, into rows that can and that cannot be stored in pieces; scales with their blocks outermost."""
     m, n, k = size
